@@ -26,6 +26,11 @@ HCK_OP_MUL_XHALF = 5
 HCK_OP_MAC = 6
 HCK_OP_ADD_SCALAR = 7
 
+HCK_BF16 = 0
+HCK_F16 = 1
+HCK_F32 = 2
+HCK_TOP_MAX = 32   # include/holmes_ckks.h: alternatives of hck_token_scores
+
 # Every symbol include/holmes_ckks.h declares, with (restype, argtypes).
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -106,6 +111,14 @@ SIGNATURES = {
     # the reference sidecar's encode entry (argtypes of bench/cmp/holmes_fast_stage2.py:37)
     "holmes_encode_stage2": (_i, [_vp, _vp, ctypes.c_longlong, _i, ctypes.c_double, _i, _vp, _vp, _vp, _vp, _vp, _vp,
                                   _vp, _i, _i, _i]),
+    "hck_kv4_page_bytes": (_sz, [_i]),
+    "hck_kv4_append": (_i, [_vp, _i64, _i, _i, _i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "hck_kv4_read": (_i, [_vp, _i64, _i, _i, _i, _vp, _i64, _vp, _vp, _vp]),
+    "hck_kv4_attend_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i, _i]),
+    "hck_kv4_attend": (_i, [_vp, _i64, _i, _i, _i, _vp, _i64, _i, _i64, _i64, _vp, _i64, _i, _vp, _vp, _i, _i, _i,
+                            ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "hck_token_scores_workspace_bytes": (_sz, [_i64, _i, _i, _i]),
+    "hck_token_scores": (_i, [_vp, _i, _i64, _i, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,307 @@
+// Log probabilities of given tokens under rows of logits, with the entropy and the top alternatives.
+//
+// For a row x over the vocabulary, in units of log 2 (t_i = x_i log2 e - r with a running reference r
+// close to the row's maximum):  l = sum 2^(t_i),  s = sum 2^(t_i) t_i, then
+//   log p(i) = ln 2 (t_i - log2 l),   H = ln 2 (log2 l - s / l).
+// Every lane keeps its own (r, l, s) over the values that it meets and they are joined at the end, so
+// a row is read once.  The reference enters each t_i through one fused multiply-add and is subtracted
+// again as the same 32-bit number, so its own rounding cancels.
+//
+// The top values: a wave keeps its k best in order, entry i in lane i.  A wave meets its values in
+// rising order of their index, so after the first blocks a block of 64 lanes' values is dismissed by
+// one comparison of the lanes' maxima with the k-th best.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/holmes_ckks.h"
+#include "internal.hpp"
+
+namespace hck {
+namespace {
+
+constexpr int kWaves = 4, kVecs = 4;  // waves of a workgroup, 16-byte pieces of a lane in flight
+constexpr int kMaxTop = 32;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct ScoreArgs {
+  const void* x;
+  const long long* tokens;  // null: no given tokens
+  float *given, *entropy, *top_logs;
+  long long* top_ids;
+  float* part;  // with splits > 1: [row][split] of (r, l, s, 0), then [row][split][top] of (key, index)
+  long long row_stride;
+  int rows, vocab, top, splits;
+};
+
+// Unsigned numbers in the order of the values: NaN above all, -0 as 0, nothing maps to 0.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return x != x ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float(k == 0xffffffffu ? 0x7fc00000u : (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+__device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
+
+// (reference, sum, weighted sum) of a part of a row; r = -inf: no finite value met, sums against 0.
+struct Sums {
+  float r = -INFINITY, l = 0.f, s = 0.f;
+  __device__ __forceinline__ void rebase(float to) {
+    if (to == r) return;
+    const float d = finite_or_zero(r) - finite_or_zero(to);
+    const float f = r == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(d);  // nothing but zeros to scale
+    s = f * (s + (l == 0.f ? 0.f : l * d));
+    l *= f;
+    r = to;
+  }
+  __device__ __forceinline__ void add(Sums o) {
+    const float to = fmaxf(r, o.r);
+    rebase(to);
+    o.rebase(to);
+    l += o.l;
+    s += o.s;
+  }
+};
+
+// A wave's k best: lane i holds the i-th.
+struct Best {
+  uint32_t key = 0, index = 0xffffffffu;
+  uint32_t last_key = 0, last_index = 0xffffffffu;  // the k-th, in every lane
+  __device__ __forceinline__ static bool before(uint32_t ak, uint32_t ai, uint32_t bk, uint32_t bi) {
+    return ak > bk || (ak == bk && ai < bi);
+  }
+  // Offers a value of every lane (key 0: none).
+  __device__ __forceinline__ void offer(uint32_t k, uint32_t i, int top) {
+    const int lane = threadIdx.x & 63;
+    unsigned long long left = __ballot(k != 0 && before(k, i, last_key, last_index));
+    while (left) {
+      const int from = __ffsll((unsigned long long)left) - 1;
+      const uint32_t nk = __builtin_amdgcn_readlane(k, from), ni = __builtin_amdgcn_readlane(i, from);
+      const int at = __popcll(__ballot(before(key, index, nk, ni)));
+      const uint32_t uk = __shfl_up(key, 1), ui = __shfl_up(index, 1);
+      if (lane > at) key = uk, index = ui;
+      if (lane == at) key = nk, index = ni;
+      if (lane >= top) key = 0, index = 0xffffffffu;
+      last_key = __builtin_amdgcn_readlane(key, top - 1);
+      last_index = __builtin_amdgcn_readlane(index, top - 1);
+      left &= left - 1;
+      left &= __ballot(before(k, i, last_key, last_index));
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float element(u32x4 v, int e) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(v[e]);
+  } else if constexpr (__is_same(T, __bf16)) {
+    return __uint_as_float((e & 1) ? v[e / 2] & 0xffff0000u : v[e / 2] << 16);
+  } else {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(v[e / 2] >> (16 * (e & 1))));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const Sums& a, const Best& best) {
+  const int lane = threadIdx.x & 63;
+  const float ref = finite_or_zero(a.r);
+  const float log = a.l == 0.f ? 0.f : __builtin_amdgcn_logf(a.l);  // a row without a finite value
+  if (lane == 0) {
+    A.entropy[row] = (log - (a.l == 0.f ? 0.f : a.s / a.l)) * kLn2;
+    if (A.tokens) {
+      const long long t = A.tokens[row];
+      float lp = 0.f;
+      if (t >= A.vocab) lp = __uint_as_float(0x7fc00000u);
+      else if (t >= 0) lp = (__builtin_fmaf((float)((const T*)A.x)[row * A.row_stride + t], kLog2e, -ref) - log) * kLn2;
+      A.given[row] = lp;
+    }
+  }
+  if (lane < A.top) {
+    A.top_ids[row * A.top + lane] = best.index;
+    A.top_logs[row * A.top + lane] = (__builtin_fmaf(value_of(best.key), kLog2e, -ref) - log) * kLn2;
+  }
+}
+
+__device__ __forceinline__ Sums over_lanes(Sums a) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    Sums o;
+    o.r = __shfl_xor(a.r, d);
+    o.l = __shfl_xor(a.l, d);
+    o.s = __shfl_xor(a.s, d);
+    a.add(o);
+  }
+  return a;
+}
+
+// `N` values of the lane, `live` of them there, the first at `index`, the others in rising order `step(n)`.
+template <int N, typename V, typename I>
+__device__ __forceinline__ void take(Sums& a, Best& best, int top, V value, I index) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < N; ++n) m = fmaxf(m, value(n));
+  const float r = fmaxf(a.r, m * kLog2e);
+  a.rebase(r);
+  const float ref = finite_or_zero(r);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float t = __builtin_fmaf(value(n), kLog2e, -ref);
+    const float e = __builtin_amdgcn_exp2f(t);
+    a.l += e;
+    a.s = __builtin_fmaf(e, fmaxf(t, -1000.f), a.s);  // 2^-inf counts nothing, and 0 * -inf would
+  }
+  if (top > 0 && __any(key_of(m) > best.last_key || a.l != a.l || best.last_key == 0)) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint32_t i = index(n);
+      const uint32_t k = i == 0xffffffffu ? 0 : key_of(value(n));
+      best.offer(k, i, top);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(64 * kWaves) void k_scores(ScoreArgs A) {
+  constexpr int kPer = 16 / sizeof(T);  // values of a 16-byte piece
+  __shared__ float s_sums[kWaves][3];
+  __shared__ uint32_t s_key[kWaves][kMaxTop], s_index[kWaves][kMaxTop];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long row = blockIdx.y + (long long)blockIdx.z * 32768;
+  if (row >= A.rows) return;
+  const T* x = (const T*)A.x + row * A.row_stride;
+  // values before the first 16-byte border, whole pieces, and the rest
+  const int head = min(A.vocab, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
+  const int pieces = (A.vocab - head) / kPer, tail = head + pieces * kPer;
+  const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
+  const int blocks = (pieces + 64 * kVecs - 1) / (64 * kVecs);
+  Sums a;
+  Best best;
+  const int first = blockIdx.x * kWaves + wave;
+  if (first == 0 && head > 0)
+    take<1>(a, best, A.top, [&](int) { return lane < head ? (float)x[lane] : -INFINITY; },
+            [&](int) { return lane < head ? (uint32_t)lane : 0xffffffffu; });
+  for (int bl = first; bl < blocks; bl += A.splits * kWaves) {
+    u32x4 v[kVecs];
+    const int p0 = bl * 64 * kVecs + lane;
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const int p = p0 + 64 * j;
+      if constexpr (sizeof(T) == 4) v[j] = u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
+      else if constexpr (__is_same(T, __bf16)) v[j] = u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+      else v[j] = u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
+      if (p < pieces) v[j] = body[p];
+    }
+    take<kVecs * kPer>(a, best, A.top, [&](int n) { return element<T>(v[n / kPer], n % kPer); },
+                       [&](int n) {
+                         const int p = p0 + 64 * (n / kPer);
+                         return p < pieces ? (uint32_t)(head + p * kPer + n % kPer) : 0xffffffffu;
+                       });
+  }
+  if (first == A.splits * kWaves - 1 && tail < A.vocab)
+    take<1>(a, best, A.top, [&](int) { return tail + lane < A.vocab ? (float)x[tail + lane] : -INFINITY; },
+            [&](int) { return tail + lane < A.vocab ? (uint32_t)(tail + lane) : 0xffffffffu; });
+
+  a = over_lanes(a);
+  if (lane == 0) s_sums[wave][0] = a.r, s_sums[wave][1] = a.l, s_sums[wave][2] = a.s;
+  if (lane < A.top) s_key[wave][lane] = best.key, s_index[wave][lane] = best.index;
+  __syncthreads();
+  if (wave != 0) return;
+  for (int w = 1; w < kWaves; ++w) {
+    Sums o;
+    o.r = s_sums[w][0], o.l = s_sums[w][1], o.s = s_sums[w][2];
+    a.add(o);
+    if (A.top) best.offer(lane < A.top ? s_key[w][lane] : 0, lane < A.top ? s_index[w][lane] : 0, A.top);
+  }
+  if (A.splits == 1) return finish<T>(A, row, a, best);
+  float* sums = A.part + (row * A.splits + blockIdx.x) * 4;
+  uint32_t* tops = (uint32_t*)(A.part + (long long)A.rows * A.splits * 4) + (row * A.splits + blockIdx.x) * A.top * 2;
+  if (lane == 0) sums[0] = a.r, sums[1] = a.l, sums[2] = a.s;
+  if (lane < A.top) tops[2 * lane] = best.key, tops[2 * lane + 1] = best.index;
+}
+
+// Joins the parts of a row: one wave a row.
+template <typename T>
+__global__ __launch_bounds__(64) void k_join(ScoreArgs A) {
+  const long long row = blockIdx.x;
+  const int lane = threadIdx.x;
+  Sums a;
+  for (int s = lane; s < A.splits; s += 64) {
+    const float* p = A.part + (row * A.splits + s) * 4;
+    Sums o;
+    o.r = p[0], o.l = p[1], o.s = p[2];
+    a.add(o);
+  }
+  a = over_lanes(a);
+  Best best;
+  if (A.top) {
+    const uint32_t* tops = (const uint32_t*)(A.part + (long long)A.rows * A.splits * 4) + row * A.splits * A.top * 2;
+    const int all = A.splits * A.top;
+    for (int e = lane; e - lane < all; e += 64)
+      best.offer(e < all ? tops[2 * e] : 0, e < all ? tops[2 * e + 1] : 0, A.top);
+  }
+  finish<T>(A, row, a, best);
+}
+
+// Parts of a row: workgroups for all 256 compute units four times, none with less than one block a wave.
+int splits_of(int64_t rows, int vocab, int size) {
+  const int64_t want = (1024 + rows - 1) / std::max<int64_t>(rows, 1);
+  const int64_t block = (int64_t)64 * kVecs * 16 / size, most = std::max<int64_t>(1, vocab / (block * kWaves));
+  return (int)std::min<int64_t>(std::min<int64_t>(want, most), 64);
+}
+
+int size_of(int type) { return type == HCK_F32 ? 4 : type == HCK_BF16 || type == HCK_F16 ? 2 : 0; }
+
+template <typename T>
+int launch(const ScoreArgs& A, hipStream_t s) {
+  const int gy = std::min(A.rows, 32768), gz = (A.rows + 32767) / 32768;
+  k_scores<T><<<dim3(A.splits, gy, gz), 64 * kWaves, 0, s>>>(A);
+  HCK_CHECK_LAUNCH();
+  if (A.splits > 1) {
+    k_join<T><<<A.rows, 64, 0, s>>>(A);
+    HCK_CHECK_LAUNCH();
+  }
+  return HCK_OK;
+}
+
+}  // namespace
+}  // namespace hck
+
+extern "C" size_t hck_token_scores_workspace_bytes(int64_t rows, int vocab, int type, int top) {
+  if (rows < 1 || rows > (1 << 30) || vocab < 1 || top < 0 || top > hck::kMaxTop || !hck::size_of(type)) return 0;
+  const int splits = hck::splits_of(rows, vocab, hck::size_of(type));
+  return splits == 1 ? 0 : (size_t)rows * splits * (4 + 2 * top) * sizeof(float);
+}
+
+extern "C" int hck_token_scores(const void* logits, int type, int64_t rows, int vocab, int64_t row_stride,
+                                const int64_t* tokens, int top, float* given, float* entropy, int64_t* top_ids,
+                                float* top_logs, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!hck::size_of(type)) return HCK_ERR_UNSUPPORTED;
+  if (rows < 0 || rows > (1 << 30) || vocab < 1 || top < 0 || top > hck::kMaxTop || top > vocab) return HCK_ERR_ARG;
+  if (rows == 0) return HCK_OK;
+  if (!logits || !entropy || (tokens && !given) || (top && (!top_ids || !top_logs))) return HCK_ERR_ARG;
+  if ((uintptr_t)logits % hck::size_of(type)) return HCK_ERR_ARG;
+  const size_t need = hck_token_scores_workspace_bytes(rows, vocab, type, top);
+  if (need > workspace_bytes || (need && !workspace)) return HCK_ERR_WORKSPACE;
+  hck::ScoreArgs A{};
+  A.x = logits;
+  A.tokens = (const long long*)tokens;
+  A.given = given;
+  A.entropy = entropy;
+  A.top_logs = top_logs;
+  A.top_ids = (long long*)top_ids;
+  A.part = (float*)workspace;
+  A.row_stride = row_stride;
+  A.rows = (int)rows;
+  A.vocab = vocab;
+  A.top = top;
+  A.splits = hck::splits_of(rows, vocab, hck::size_of(type));
+  hipStream_t s = (hipStream_t)stream;
+  if (type == HCK_BF16) return hck::launch<__bf16>(A, s);
+  if (type == HCK_F16) return hck::launch<_Float16>(A, s);
+  return hck::launch<float>(A, s);
+}

@@ -422,6 +422,58 @@ int hck_lincomb_rescale(const hck_context* ctx, int level_limbs, int groups, int
                         const uint64_t* weights, uint64_t* const* out, const uint64_t* add, uint64_t add_mask,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- cleartext companions
+ * The cleartext model beside the encrypted layer: its key/value cache in 4 bits, attention over it with
+ * the range of every row's scores (what the encrypted softmax's intervals are taken from), and the
+ * scoring of given tokens.  Types of values are HCK_BF16, HCK_F16 or HCK_F32; head_dim is 64 or 128
+ * (HCK_ERR_UNSUPPORTED otherwise). */
+#define HCK_BF16 0
+#define HCK_F16 1
+#define HCK_F32 2
+#define HCK_TOP_MAX 32
+
+/* Bytes of one page of one key/value head (128 tokens, keys and values); 0: no such head_dim.  A pool is
+ * pages * kv_heads * that, 16-byte aligned and zeroed before its first use. */
+size_t hck_kv4_page_bytes(int head_dim);
+
+/* Quantises `tokens` keys and values into the slots slots[i] (device; page * 128 + place; outside the
+ * pool: the token is left out; a slot named twice holds either token's values).  Token i, head h is at
+ * i * token_stride + h * head_stride elements, its head_dim values contiguous. */
+int hck_kv4_append(void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* keys,
+                   int64_t key_token_stride, int64_t key_head_stride, const void* values, int64_t value_token_stride,
+                   int64_t value_head_stride, const int64_t* slots, int64_t tokens, void* stream);
+
+/* The values that slots[i] hold, into dense [tokens][kv_heads][head_dim] keys and values; zeros for a slot
+ * outside the pool; values above an fp16 output's range become its largest. */
+int hck_kv4_read(const void* pool, int64_t pages, int kv_heads, int head_dim, int type, const int64_t* slots,
+                 int64_t tokens, void* keys, void* values, void* stream);
+
+/* Attention of queries [tokens][kv_heads * group][head_dim] (bf16 or fp16; element strides, the last axis
+ * contiguous) over the pages of their sequences.  Sequence b has the pages table[b * table_stride ..
+ * + table_columns), lengths[b] cached tokens and the queries starts[b] .. starts[b + 1] (starts NULL: the
+ * one query b), which are its last tokens; with `causal` a query sees the tokens up to its own, without it
+ * all of them.  `most` is at least the largest number of queries of a sequence.  table, lengths and starts
+ * are device arrays: a page outside the pool counts as tokens that are not there.  out is dense, of the
+ * queries' type; lse, low and high (both NULL or both given) are [tokens][kv_heads * group] float: log sum
+ * exp and the least and largest of a row's scaled scores.  A row that sees nothing gives 0, -inf, inf, -inf.
+ * A token that no sequence covers is left unwritten. */
+size_t hck_kv4_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim, int most,
+                                      int table_columns);
+int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* queries,
+                   int64_t tokens, int group, int64_t q_token_stride, int64_t q_head_stride, const int32_t* table,
+                   int64_t table_stride, int table_columns, const int32_t* lengths, const int32_t* starts, int seqs,
+                   int most, int causal, float scale, void* out, float* lse, float* low, float* high, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Of `rows` rows of logits over `vocab` tokens (rows row_stride elements apart): given[i] = log p(tokens[i])
+ * (tokens NULL: not asked; a negative token gives 0, one at or above vocab NaN), the entropy in nats, and the
+ * `top` (at most HCK_TOP_MAX and vocab) most likely tokens with their log probabilities, ties to the lowest
+ * token, NaN above all.  A logit of -inf is a token that cannot be; a row of nothing else gives -inf and 0. */
+size_t hck_token_scores_workspace_bytes(int64_t rows, int vocab, int type, int top);
+int hck_token_scores(const void* logits, int type, int64_t rows, int vocab, int64_t row_stride, const int64_t* tokens,
+                     int top, float* given, float* entropy, int64_t* top_ids, float* top_logs, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
