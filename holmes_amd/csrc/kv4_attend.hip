@@ -28,6 +28,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 64;   // tokens that a wave takes at a time: half a page
 constexpr int kWaves = 4;
+constexpr int kFew = 16;    // rows of k_attend's workgroup
+constexpr int kMany = 128;  // rows of k_prompt's
 // Exponentials are taken times 2^24, so that those from 2^-126 to 2^-150 of a row's largest, which the
 // exponential instruction gives as 0, still count where every larger one meets a value of 0.  Sums then
 // stay finite for values up to 2^103 over the number of tokens.
@@ -42,12 +44,128 @@ struct AttendArgs {
   const int* starts;   // null: sequence b has the one query b
   void* out;
   float *lse, *low, *high;  // [token][query head]; low, high nullable
-  float* part;         // with splits > 1: [row][split] of (m, l, low, 0), then [row][split][D] of sums
+  // with `join`: [slot][row] of (m, l, low, -), [slot][row][D] of sums, and [tile][head] of (first slot, slots)
+  float *stat, *sums;
+  int* plan;
   long long q_ts, q_hs, tokens, pages;
   long long table_stride;
-  int cols, heads, group, splits, causal;
+  int cols, heads, group, causal;
+  int seqs, tiles;     // tiles of rows that the longest sequence can have
+  int rows;            // rows of a slot
+  int slots, least;    // workgroups to share the work out to, units that are not worth sharing
+  int join;
   float scale;
 };
+
+// The rows of one sequence: query tokens [q0, q0 + nq), each with `group` heads, row = query * group + head.
+struct Rows {
+  long long q0;
+  int nq, rows, length;
+  __device__ __forceinline__ Rows(const AttendArgs& A, int b) {
+    long long first = b, last = b + 1;
+    if (A.starts) first = A.starts[b], last = A.starts[b + 1];
+    q0 = max(first, 0ll);
+    nq = (int)max(min(last, A.tokens) - q0, 0ll);
+    rows = (int)min((long long)nq * A.group, (long long)A.tiles * (A.rows > kFew ? kMany : kFew));
+    length = (int)min((long long)max(A.lengths[b], 0), (long long)A.cols * kPageTokens);
+  }
+  // tokens that row r sees
+  __device__ __forceinline__ int seen(const AttendArgs& A, int r) const {
+    return A.causal ? max(0, min(length, length - nq + r / A.group + 1)) : length;
+  }
+};
+
+// A workgroup's work: a tile of rows, a key head, and a part of the units of 64 tokens that they see.
+struct Item {
+  int b, tile, h, u0, u1, slot, slots;
+};
+
+// The units of a tile's rows, -1: no rows.
+__device__ __forceinline__ int units_of(const AttendArgs& A, int pair, int size) {
+  const Rows R(A, pair / A.tiles);
+  const int first = (pair % A.tiles) * size;
+  if (first >= R.rows) return -1;
+  return (R.seen(A, min(first + size, R.rows) - 1) + kUnit - 1) / kUnit;
+}
+
+__device__ __forceinline__ long long over_wave(long long x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+  return x;
+}
+__device__ __forceinline__ int over_wave(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+  return x;
+}
+
+constexpr int kPairs = 8;  // tiles of rows that a lane looks through to share the work out
+
+// Which part of the work is workgroup w's.  Lengths are on the device, so every wave works it out: with
+// all tiles' units in its lanes, a share is the smallest for which the parts (whole shares of a tile and
+// its rest) are no more than the workgroups that run at once.  Later tiles, which see more, come first.
+__device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Item& it) {
+  const int pairs = A.seqs * A.tiles, lane = threadIdx.x & 63;
+  it.h = w % A.heads;
+  it.slot = w, it.slots = 1;
+  int r = w / A.heads;
+  if (!A.join) {
+    const int p = pairs - 1 - r;
+    it.b = p / A.tiles, it.tile = p % A.tiles;
+    it.u0 = 0, it.u1 = 0x7fffffff;
+    return true;
+  }
+  const int per = (pairs + 63) / 64;
+  int n[kPairs];
+  long long total = 0;
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    const int p = pairs - 1 - (lane * per + j);
+    n[j] = j < per && p >= 0 ? units_of(A, p, size) : -1;
+    total += max(n[j], 0);
+  }
+  total = over_wave(total) * A.heads;
+  const int base = (int)min(1ll << 26, max((long long)A.least, (total + A.slots - 1) / A.slots));
+  int share = 0, mine = 0;
+#pragma unroll
+  for (int f = 4; f <= 8; ++f) {
+    if (f == 7) continue;
+    const int s = base / 4 * f + (base % 4 * f + 3) / 4;
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) c += n[j] < 0 ? 0 : max(1, (n[j] + s - 1) / s);
+    const bool last = f == 8;
+    if (last || (long long)over_wave(c) * A.heads <= A.slots) {
+      share = s, mine = c;
+      break;
+    }
+  }
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int x = __shfl_up(upto, d);
+    if (lane >= d) upto += x;
+  }
+  const int owner = __popcll(__ballot(upto <= r));  // the lane that holds part r
+  if (owner > 63) return false;
+  int pair = 0, u0 = 0, count = 1, at = upto - mine;
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    const int c = n[j] < 0 ? 0 : max(1, (n[j] + share - 1) / share);
+    if (r >= at && r < at + c) pair = pairs - 1 - (lane * per + j), u0 = (r - at) * share, count = c;
+    at += c;
+  }
+  pair = __builtin_amdgcn_readlane(pair, owner);
+  it.u0 = __builtin_amdgcn_readlane(u0, owner);
+  it.slots = __builtin_amdgcn_readlane(count, owner);
+  it.u1 = it.u0 + share;
+  it.b = pair / A.tiles, it.tile = pair % A.tiles;
+  if (it.u0 == 0 && threadIdx.x == 0) {
+    A.plan[2 * (pair * A.heads + it.h)] = w;
+    A.plan[2 * (pair * A.heads + it.h) + 1] = it.slots;
+  }
+  return true;
+}
 
 // 16 bytes from an address that is a multiple of the elements' two bytes only.
 struct __attribute__((packed, aligned(2))) Loose16 {
@@ -150,33 +268,52 @@ __device__ __forceinline__ float log2_sum(float m, float l) {
   return fabsf(m) == INFINITY ? m + l : __builtin_ceilf(m) + (__builtin_amdgcn_logf(l) - kLift);
 }
 
-// One workgroup: 16 rows of one key head, a share of their tokens; its waves take units in turn.
+// Packs the upper halves of two numbers.
+__device__ __forceinline__ uint32_t heads_of(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float rest_of(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
+
+// A row's results from its sums: maximum m in units of log 2, sum l, `N` values from dim d0.
+template <typename T, int N, bool RANGE>
+__device__ __forceinline__ void store_row(const AttendArgs& A, long long at, int dim, int d0, float m, float l, float low,
+                                          const float* o) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  typedef T vec __attribute__((ext_vector_type(N)));
+  vec x;
+#pragma unroll
+  for (int c = 0; c < N; ++c) x[c] = (T)(o[c] * inv);
+  *reinterpret_cast<vec*>((T*)A.out + at * dim + d0) = x;
+  if (d0 == 0) {
+    const bool bad = l != l;
+    A.lse[at] = log2_sum(m, l) * kLn2;
+    if constexpr (RANGE) A.low[at] = bad ? l : low * kLn2, A.high[at] = bad ? l : m * kLn2;
+  }
+}
+
+// 16 rows of one key head, a part of their tokens; the waves take units in turn.
 template <typename T, int D, bool RANGE>
 __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
   using L = Kv4<D>;
   constexpr int kSteps = D / 32, kDpl = L::kDpl;
   constexpr bool kHalf = __is_same(T, _Float16);
-  __shared__ float s_m[kWaves][16], s_l[kWaves][16], s_low[kWaves][16];
-  __shared__ float s_o[kWaves][16][D + 4];
+  __shared__ float s_m[kWaves][kFew], s_l[kWaves][kFew], s_low[kWaves][kFew];
+  extern __shared__ float s_o[];  // [wave][A.rows][D + 4]
 
+  Item it;
+  if (!locate(A, kFew, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % A.splits, tile = blockIdx.x / A.splits, h = blockIdx.y, b = blockIdx.z;
-  long long q0 = b, q1 = b + 1;
-  if (A.starts) q0 = A.starts[b], q1 = A.starts[b + 1];
-  q0 = max(q0, 0ll);
-  q1 = min(q1, A.tokens);
-  const int nq = (int)max(q1 - q0, 0ll);
-  const int rows = nq * A.group;
-  if (tile * 16 >= rows) return;
-  const int length = (int)min((long long)max(A.lengths[b], 0), (long long)A.cols * kPageTokens);
-  const int row = tile * 16 + m;
+  const int tile = it.tile, h = it.h, b = it.b;
+  const Rows R(A, b);
+  const long long q0 = R.q0;
+  const int rows = R.rows;
+  if (tile * kFew >= rows) return;
+  const int row = tile * kFew + m;
   const bool live = row < rows;
   const int qi = live ? row / A.group : 0, qo = live ? row % A.group : 0;
-  const int seen = !live ? 0 : A.causal ? max(0, min(length, length - nq + qi + 1)) : length;
-  const int last = min(tile * 16 + 15, rows - 1) / A.group;
-  const int most = A.causal ? max(0, min(length, length - nq + last + 1)) : length;
-  const int units = (most + kUnit - 1) / kUnit;
-  const int u0 = (int)((long long)units * split / A.splits), u1 = (int)((long long)units * (split + 1) / A.splits);
+  const int seen = live ? R.seen(A, row) : 0;
+  const int all = R.seen(A, tile * kFew), most = R.seen(A, min(tile * kFew + kFew, rows) - 1);
+  const int u0 = it.u0, u1 = min((most + kUnit - 1) / kUnit, it.u1);
 
   // the lane's part of its row's query: dims D / 4 g + 8 s .. + 7 of step s
   bf16x8 qh[kSteps], ql[kSteps];
@@ -223,43 +360,53 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
         if constexpr (kHalf) c = mfma(kk, ql[s], c);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t[i][k] = c[k] * scale2;
+      for (int k = 0; k < 4; ++k) t[i][k] = c[k];
     }
     const int base = u * kUnit + 4 * g;
+    if (u * kUnit + kUnit > all) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool see = base + 16 * i + k < seen;
+          if constexpr (RANGE) low = see ? fminf(low, t[i][k]) : low;
+          t[i][k] = see ? t[i][k] : -INFINITY;
+        }
+    } else if constexpr (RANGE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) low = fminf(low, t[i][k]);
+    }
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool see = base + 16 * i + k < seen;
-        if constexpr (RANGE) low = see ? fminf(low, t[i][k]) : low;
-        t[i][k] = see ? t[i][k] : -INFINITY;
-        mx = fmaxf(mx, t[i][k]);
-      }
-    mx = fmaxf(top, over_g(mx, fmax2));
+      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[i][k]);
+    mx = fmaxf(top, over_g(mx, fmax2) * scale2);
     const float f = rebase(top, mx);
     top = mx;
     const float ref = reference(mx) - kLift;
-    sum *= f;
+    if (__any(f != 1.f)) {
+      sum *= f;
 #pragma unroll
-    for (int i = 0; i < kDpl; ++i) acc[i] *= f;
+      for (int i = 0; i < kDpl; ++i) acc[i] *= f;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        t[i][k] = __builtin_amdgcn_exp2f(t[i][k] - ref);
+        t[i][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][k], scale2, -ref));
         sum += t[i][k];
       }
 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      bf16x8 ph, pl;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float p = t[2 * i + (k >> 2)][k & 3];
-        ph[k] = (__bf16)p;
-        pl[k] = (__bf16)(p - (float)ph[k]);
-      }
+      const float* p0 = t[2 * i];
+      const float* p1 = t[2 * i + 1];
+      const bf16x8 ph = operand(heads_of(p0[0], p0[1]), heads_of(p0[2], p0[3]), heads_of(p1[0], p1[1]), heads_of(p1[2], p1[3]));
+      const bf16x8 pl = operand(pack(rest_of(p0[0]), rest_of(p0[1])), pack(rest_of(p0[2]), rest_of(p0[3])),
+                                pack(rest_of(p1[0]), rest_of(p1[1])), pack(rest_of(p1[2]), rest_of(p1[3])));
       uint32_t vs[2] = {x.vs[i][0], x.vs[i][1]};
       float sc[8];
       // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  It is taken
@@ -304,16 +451,18 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
 
   // join the waves: lane (m, g) holds dims D / 4 g + kDpl i + d of row m in acc[d][i]
   sum = over_g(sum, [](float a, float c) { return a + c; });
-  if constexpr (RANGE) low = over_g(low, fmin2);
+  if constexpr (RANGE) low = over_g(low, fmin2) * scale2;
   if (g == 0) s_m[wave][m] = top, s_l[wave][m] = sum, s_low[wave][m] = low;
+  if (m < A.rows) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int d = 0; d < kDpl; ++d) s_o[wave][m][g * (D / 4) + kDpl * i + d] = acc[d][i];
+      for (int d = 0; d < kDpl; ++d) s_o[(wave * A.rows + m) * (D + 4) + g * (D / 4) + kDpl * i + d] = acc[d][i];
+  }
   __syncthreads();
   constexpr int kCols = D / 16;  // dims of a thread: 16 threads to a row
   const int r = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * kCols;
-  if (tile * 16 + r >= rows) return;
+  if (r >= A.rows || tile * kFew + r >= rows) return;
   float mm = -INFINITY, ll = 0.f, lo = INFINITY, o[kCols];
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, s_m[w][r]);
@@ -325,74 +474,114 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
     ll += f * s_l[w][r];
     lo = fminf(lo, s_low[w][r]);
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) o[c] += f * s_o[w][r][c0 + c];
+    for (int c = 0; c < kCols; ++c) o[c] += f * s_o[(w * A.rows + r) * (D + 4) + c0 + c];
   }
-  const int qr = (tile * 16 + r) / A.group, qc = (tile * 16 + r) % A.group;
-  const long long at = (q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc;
-  if (A.splits > 1) {
-    float* stat = A.part + (at * A.splits + split) * 4;
-    float* sums = A.part + A.tokens * A.heads * A.group * (long long)A.splits * 4 + (at * A.splits + split) * D + c0;
-    if (c0 == 0) stat[0] = mm, stat[1] = ll, stat[2] = lo;
+  if (it.slots > 1) {
+    const long long at = (long long)it.slot * A.rows + r;
+    if (c0 == 0) *reinterpret_cast<f32x4*>(A.stat + at * 4) = f32x4{mm, ll, lo, 0.f};
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) sums[c] = o[c];
+    for (int c = 0; c < kCols; c += 4)
+      *reinterpret_cast<f32x4*>(A.sums + at * D + c0 + c) = f32x4{o[c], o[c + 1], o[c + 2], o[c + 3]};
     return;
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  T* to = (T*)A.out + at * D + c0;
+  const int qr = (tile * kFew + r) / A.group, qc = (tile * kFew + r) % A.group;
+  store_row<T, kCols, RANGE>(A, (q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, c0, mm, ll, lo, o);
+}
+
+// Joins the slots of a row, where it has more than one.  One workgroup a row of few, its waves taking the
+// slots in turn; of many rows, one workgroup 32 of them and a wave a row, for they have few slots each.
+template <typename T, int D, bool RANGE, bool FEW>
+__global__ __launch_bounds__(64 * kWaves) void k_join(AttendArgs A) {
+  constexpr int kCols = D / 64;
+  __shared__ float s_l[kWaves], s_low[kWaves], s_o[kWaves][D];
+  const int pair = blockIdx.x / A.heads, h = blockIdx.x % A.heads;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Rows R(A, pair / A.tiles);
+  const int first = (pair % A.tiles) * (FEW ? kFew : kMany);
+  if (first >= R.rows) return;
+  const int slot = A.plan[2 * blockIdx.x], slots = A.plan[2 * blockIdx.x + 1];
+  if (slots < 2) return;
+  constexpr int kStep = FEW ? kWaves : 1;
+  const int r0 = FEW ? blockIdx.y : blockIdx.y * 32 + wave, r1 = FEW ? r0 + 1 : min(A.rows, (int)blockIdx.y * 32 + 32);
+  for (int r = r0; r < r1 && first + r < R.rows; r += kWaves) {
+    const float* stat = A.stat + ((long long)slot * A.rows + r) * 4;  // slots of a tile and head: `heads` apart
+    const float* sums = A.sums + ((long long)slot * A.rows + r) * D + lane * kCols;
+    const long long step = (long long)A.heads * A.rows;
+    float top = -INFINITY;
+    for (int s = lane; s < slots; s += 64) top = fmaxf(top, stat[s * step * 4]);
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) to[c] = (T)(o[c] * inv);
-  if (c0 == 0) {
-    const bool bad = ll != ll;
-    A.lse[at] = log2_sum(mm, ll) * kLn2;
-    if constexpr (RANGE) A.low[at] = bad ? ll : lo * kLn2, A.high[at] = bad ? ll : mm * kLn2;
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    float ll = 0.f, lo = INFINITY, o[kCols] = {};
+    int s = FEW ? wave : 0;
+    auto add = [&](auto N) {
+      constexpr int n = decltype(N)::value;
+      f32x4 st[n];
+      float x[n][kCols];
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        st[i] = *reinterpret_cast<const f32x4*>(stat + (s + i * kStep) * step * 4);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) x[i][c] = sums[(s + i * kStep) * step * D + c];
+      }
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float f = rebase(st[i][0], top);
+        ll += f * st[i][1];
+        lo = fminf(lo, st[i][2]);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] += f * x[i][c];
+      }
+    };
+    for (; s + 7 * kStep < slots; s += 8 * kStep) add(std::integral_constant<int, 8>());
+    for (; s < slots; s += kStep) add(std::integral_constant<int, 1>());
+    if constexpr (FEW) {
+      if (lane == 0) s_l[wave] = ll, s_low[wave] = lo;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) s_o[wave][lane * kCols + c] = o[c];
+      __syncthreads();
+      if (wave != 0) return;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        ll += s_l[w];
+        lo = fminf(lo, s_low[w]);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] += s_o[w][lane * kCols + c];
+      }
+    }
+    const int qr = (first + r) / A.group, qc = (first + r) % A.group;
+    store_row<T, kCols, RANGE>(A, (R.q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, lane * kCols, top, ll, lo, o);
   }
 }
 
-// Joins the splits of a row: one wave a row.
+// How a call is run, from what the host knows of it.
+struct Way {
+  bool few, join;
+  int rows, least;
+  int64_t tiles, slots, pairs, items;
+  Way(int64_t tokens, int64_t seqs, int heads, int group, int most, int cols) {
+    const int64_t all = (int64_t)most * group, units = std::max<int64_t>(1, (int64_t)cols * (kPageTokens / kUnit));
+    few = true;
+    const int size = few ? kFew : kMany;
+    tiles = (all + size - 1) / size;
+    rows = (int)std::min<int64_t>(all, size);
+    least = few ? 4 * kWaves : 8;
+    slots = few ? 1024 : 512;
+    pairs = seqs * tiles;
+    join = pairs <= 64 * kPairs && units > least;
+    items = !join ? pairs * heads : std::min(pairs * ((units + least - 1) / least), pairs + (slots + heads - 1) / heads) * heads;
+  }
+  size_t bytes(int heads, int dim) const {
+    return join ? (size_t)items * rows * (4 + dim) * sizeof(float) + (size_t)pairs * heads * 2 * sizeof(int) : 0;
+  }
+};
+
 template <typename T, int D, bool RANGE>
-__global__ __launch_bounds__(256) void k_join(AttendArgs A) {
-  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), all = A.tokens * A.heads * A.group;
-  const int lane = threadIdx.x & 63;
-  if (at >= all) return;
-  const float* stat = A.part + at * A.splits * 4;
-  const float* sums = A.part + all * A.splits * 4 + at * A.splits * D;
-  float mm = -INFINITY, ll = 0.f, lo = INFINITY, o[D / 64];
-  for (int s = 0; s < A.splits; ++s) mm = fmaxf(mm, stat[4 * s]);
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) o[c] = 0.f;
-  for (int s = 0; s < A.splits; ++s) {
-    const float f = rebase(stat[4 * s], mm);
-    ll += f * stat[4 * s + 1];
-    lo = fminf(lo, stat[4 * s + 2]);
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) o[c] += f * sums[s * D + c * 64 + lane];
-  }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  T* to = (T*)A.out + at * D;
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) to[c * 64 + lane] = (T)(o[c] * inv);
-  if (lane == 0) {
-    const bool bad = ll != ll;
-    A.lse[at] = log2_sum(mm, ll) * kLn2;
-    if constexpr (RANGE) A.low[at] = bad ? ll : lo * kLn2, A.high[at] = bad ? ll : mm * kLn2;
-  }
-}
-
-// Splits of a row's tokens: enough workgroups for four on each of the 256 compute units, and no
-// share under two units a wave of the longest table.
-int splits_of(int64_t seqs, int heads, int64_t tiles, int cols) {
-  const int64_t groups = std::max<int64_t>(1, seqs * heads * tiles);
-  const int64_t want = (1024 + groups - 1) / groups, most = std::max(1, cols * (kPageTokens / kUnit) / (2 * kWaves));
-  return (int)std::min<int64_t>(std::min<int64_t>(want, most), 128);
-}
-
-template <typename T, int D, bool RANGE>
-int launch(const AttendArgs& A, int64_t tiles, int seqs, hipStream_t s) {
-  k_attend<T, D, RANGE><<<dim3((unsigned)(tiles * A.splits), A.heads, seqs), 64 * kWaves, 0, s>>>(A);
+int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
+  const size_t lds = kWaves * W.rows * (D + 4) * sizeof(float);
+  k_attend<T, D, RANGE><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
   HCK_CHECK_LAUNCH();
-  if (A.splits > 1) {
-    const long long rows = A.tokens * A.heads * A.group;
-    k_join<T, D, RANGE><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(A);
+  if (W.join) {
+    k_join<T, D, RANGE, true><<<dim3((unsigned)(W.pairs * A.heads), W.rows), 64 * kWaves, 0, s>>>(A);
     HCK_CHECK_LAUNCH();
   }
   return HCK_OK;
@@ -410,9 +599,7 @@ bool shape_ok(int64_t tokens, int seqs, int kv_heads, int group, int most, int c
 extern "C" size_t hck_kv4_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim,
                                                  int most, int table_columns) {
   if (!hck::shape_ok(tokens, seqs, kv_heads, group, most, table_columns)) return 0;
-  const int64_t tiles = ((int64_t)most * group + 15) / 16;
-  const int splits = hck::splits_of(seqs, kv_heads, tiles, table_columns);
-  return splits == 1 ? 0 : (size_t)(tokens * kv_heads * group) * splits * (4 + head_dim) * sizeof(float);
+  return hck::Way(tokens, seqs, kv_heads, group, most, table_columns).bytes(kv_heads, head_dim);
 }
 
 extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int head_dim, int type,
@@ -427,7 +614,11 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
   if (tokens == 0 || seqs == 0 || most == 0) return HCK_OK;
   if (!queries || !lengths || (!table && table_columns > 0) || !out || !lse) return HCK_ERR_ARG;
   if (!starts && tokens < seqs) return HCK_ERR_ARG;
-  const int64_t tiles = ((int64_t)most * group + 15) / 16;
+  if (((uintptr_t)pool | (uintptr_t)out | (uintptr_t)workspace) % 16) return HCK_ERR_ARG;
+  const hck::Way W(tokens, seqs, kv_heads, group, most, table_columns);
+  const size_t need = W.bytes(kv_heads, head_dim);
+  if (W.items > 0x7fffffff || W.pairs > 0x7fffffff) return HCK_ERR_ARG;
+  if (need > workspace_bytes || (need && !workspace)) return HCK_ERR_WORKSPACE;
   hck::AttendArgs A{};
   A.pool = (const uint8_t*)pool;
   A.q = queries;
@@ -438,7 +629,11 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
   A.lse = lse;
   A.low = low;
   A.high = high;
-  A.part = (float*)workspace;
+  if (W.join) {
+    A.stat = (float*)workspace;
+    A.sums = A.stat + W.items * W.rows * 4;
+    A.plan = (int*)(A.sums + W.items * W.rows * head_dim);
+  }
   A.q_ts = q_token_stride;
   A.q_hs = q_head_stride;
   A.tokens = tokens;
@@ -447,18 +642,20 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
   A.cols = table_columns;
   A.heads = kv_heads;
   A.group = group;
-  A.splits = hck::splits_of(seqs, kv_heads, tiles, table_columns);
   A.causal = causal;
+  A.seqs = seqs;
+  A.tiles = (int)W.tiles;
+  A.rows = W.rows;
+  A.slots = (int)W.slots;
+  A.least = W.least;
+  A.join = W.join;
   A.scale = scale;
-  if (tiles * A.splits > 0x7fffffff) return HCK_ERR_ARG;
-  const size_t need = hck_kv4_attend_workspace_bytes(tokens, seqs, kv_heads, group, head_dim, most, table_columns);
-  if (need > workspace_bytes || (need && !workspace)) return HCK_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   const bool range = low != nullptr;
   if (head_dim == 128) {
-    if (type == HCK_BF16) return range ? hck::launch<__bf16, 128, true>(A, tiles, seqs, s) : hck::launch<__bf16, 128, false>(A, tiles, seqs, s);
-    return range ? hck::launch<_Float16, 128, true>(A, tiles, seqs, s) : hck::launch<_Float16, 128, false>(A, tiles, seqs, s);
+    if (type == HCK_BF16) return range ? hck::launch<__bf16, 128, true>(A, W, s) : hck::launch<__bf16, 128, false>(A, W, s);
+    return range ? hck::launch<_Float16, 128, true>(A, W, s) : hck::launch<_Float16, 128, false>(A, W, s);
   }
-  if (type == HCK_BF16) return range ? hck::launch<__bf16, 64, true>(A, tiles, seqs, s) : hck::launch<__bf16, 64, false>(A, tiles, seqs, s);
-  return range ? hck::launch<_Float16, 64, true>(A, tiles, seqs, s) : hck::launch<_Float16, 64, false>(A, tiles, seqs, s);
+  if (type == HCK_BF16) return range ? hck::launch<__bf16, 64, true>(A, W, s) : hck::launch<__bf16, 64, false>(A, W, s);
+  return range ? hck::launch<_Float16, 64, true>(A, W, s) : hck::launch<_Float16, 64, false>(A, W, s);
 }
