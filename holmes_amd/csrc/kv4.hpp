@@ -3,12 +3,13 @@
 // A page holds 128 tokens; the pool is [page][kv head][kBytes].  Values are e2m1 codes (0, .5, 1,
 // 1.5, 2, 3, 4, 6 and their negatives) times 2^(b - 127), one byte b for each run of 32 values along
 // the head dimension.  One head's part of a page is
-//   key codes    [token][D / 2 bytes], as the matrix product's left operand takes a token's dims
-//   value codes  [32-token block][g < 4][c < 16][j < 8][D / 16 codes]: the product over tokens wants a
-//                lane to hold one dim of 8 tokens, so lane (c, g) finds its 8 tokens' dims
-//                c D/16 .. (c + 1) D/16 - 1 in one piece of memory; tokens 4 g + j (j < 4) and
-//                16 + 4 g + j - 4 are the ones whose scores that lane holds after the first product
-//   key scales   [run][token % 16][token / 16]: the bytes of a lane's token in all eight 16-token tiles
+//   key codes    [16-token tile][g < 4][token % 16][D / 8 bytes]: lane (token % 16, g) of a matrix product's
+//                left operand holds dims g D/4 .. (g + 1) D/4 - 1, so a wave loads a tile as it lies
+//   value codes  [32-token block][piece][g < 4][c < 16][16 bytes]: the product over tokens wants a lane to
+//                hold one dim of 8 tokens, so lane (c, g) finds dims c D/16 .. (c + 1) D/16 - 1 of its tokens
+//                j < 8 there, D/32 bytes each, 4 to a piece at D = 128 and all 8 at D = 64; tokens 4 g + j
+//                (j < 4) and 16 + 4 g + j - 4 are the ones whose scores that lane holds after the first product
+//   key scales   [64 tokens][run][token % 16][token / 16 % 4]: the bytes of a lane's token in four tiles
 //   value scales [32-token block][g][run][j]: the bytes of a lane's 8 tokens
 // A token owns every byte that it writes, so appends never read.
 #pragma once
@@ -29,12 +30,17 @@ struct Kv4 {
   static constexpr int kScales = kPageTokens * kRuns;
   static constexpr int kVCodes = kCodes, kKScales = 2 * kCodes, kVScales = kKScales + kScales;
   static constexpr int kBytes = 2 * (kCodes + kScales);
-  __device__ static int key_code(int t, int d) { return t * (D / 2) + d / 2; }
-  __device__ static int key_scale(int t, int run) { return kKScales + run * kPageTokens + (t & 15) * 8 + (t >> 4); }
+  __device__ static int key_code(int t, int d) {
+    return (t >> 4) * (8 * D) + (d / (D / 4) * 16 + (t & 15)) * (D / 8) + d % (D / 4) / 2;
+  }
+  __device__ static int key_scale(int t, int run) {
+    return kKScales + (t >> 6) * (64 * kRuns) + run * 64 + (t & 15) * 4 + ((t >> 4) & 3);
+  }
   __device__ static int value_j(int t) { return ((t >> 4) & 1) * 4 + (t & 3); }
   __device__ static int value_g(int t) { return (t >> 2) & 3; }
   __device__ static int value_code(int t, int c) {
-    return kVCodes + (t >> 5) * (16 * D) + ((value_g(t) * 16 + c) * 8 + value_j(t)) * (kDpl / 2);
+    const int at = value_j(t) * (kDpl / 2);
+    return kVCodes + (t >> 5) * (16 * D) + (at >> 4) * 1024 + (value_g(t) * 16 + c) * 16 + (at & 15);
   }
   __device__ static int value_scale(int t, int run) {
     return kVScales + (t >> 5) * (32 * kRuns) + (value_g(t) * kRuns + run) * 8 + value_j(t);

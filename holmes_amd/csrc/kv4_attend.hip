@@ -28,6 +28,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 64;   // tokens that a wave takes at a time: half a page
 constexpr int kWaves = 4;
+constexpr int kComputeUnits = 256;
 constexpr int kFew = 16;    // rows of k_attend's workgroup
 constexpr int kMany = 128;  // rows of k_prompt's
 // Exponentials are taken times 2^24, so that those from 2^-126 to 2^-150 of a row's largest, which the
@@ -198,21 +199,24 @@ __device__ __forceinline__ bool has_nan(uint32_t w) {  // a byte of 255 among th
 template <int D>
 struct Unit {
   uint32_t k[4][D / 32], ks, v[2][D / 16], vs[2][2];
-  __device__ __forceinline__ void load(const uint8_t* page, int half, int m, int g) {
+  __device__ __forceinline__ void load_keys(const uint8_t* page, int half, int m, int g) {
     using L = Kv4<D>;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t* p = page + (64 * half + 16 * i + m) * (D / 2) + g * (D / 8);
+      const uint8_t* p = page + (4 * half + i) * (8 * D) + (g * 16 + m) * (D / 8);
       if constexpr (D == 128) *reinterpret_cast<u32x4*>(k[i]) = *reinterpret_cast<const u32x4*>(p);
       else *reinterpret_cast<u32x2*>(k[i]) = *reinterpret_cast<const u32x2*>(p);
     }
     ks = *reinterpret_cast<const uint32_t*>(page + L::key_scale(64 * half + m, g * (D / 4) / kRun));
+  }
+  __device__ __forceinline__ void load_values(const uint8_t* page, int half, int m, int g) {
+    using L = Kv4<D>;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint8_t* p = page + L::kVCodes + (2 * half + i) * (16 * D) + (g * 16 + m) * (D / 4);
+      const uint8_t* p = page + L::kVCodes + (2 * half + i) * (16 * D) + (g * 16 + m) * 16;
 #pragma unroll
       for (int w = 0; w < D / 64; ++w)
-        reinterpret_cast<u32x4*>(v[i])[w] = reinterpret_cast<const u32x4*>(p)[w];
+        reinterpret_cast<u32x4*>(v[i])[w] = *reinterpret_cast<const u32x4*>(p + 1024 * w);
       *reinterpret_cast<u32x2*>(vs[i]) = *reinterpret_cast<const u32x2*>(
           page + L::kVScales + (2 * half + i) * (32 * L::kRuns) + (g * L::kRuns + m * L::kDpl / kRun) * 8);
     }
@@ -291,10 +295,33 @@ __device__ __forceinline__ void store_row(const AttendArgs& A, long long at, int
   }
 }
 
-// 16 rows of one key head, a part of their tokens; the waves take units in turn.
-template <typename T, int D, bool RANGE>
-__global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
+// A lane's neighbours 4 and 8 on, of the 16 that share g.
+template <int N>
+__device__ __forceinline__ float turn(float x) {
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x120 + N, 0xf, 0xf, true));
+}
+template <int R, typename F>
+__device__ __forceinline__ float over_row(float x, F f) {
+  if constexpr (R <= 8) x = f(x, turn<8>(x));
+  if constexpr (R <= 4) x = f(x, turn<4>(x));
+  return over_g(x, f);
+}
+
+// Waves of k_attend on a SIMD, which the registers of its dims and query parts set.
+constexpr int waves_of(int dim, bool half) { return dim == 64 ? 4 : half ? 2 : 3; }
+
+// R rows of one key head, a part of their tokens; the waves take units in turn.
+//
+// With R < 16 the product's 16 columns hold the rows 16 / R times.  Each copy keeps the scores of its own
+// share of the 64 tokens, so that no exponential is taken for an empty column, and goes into the second
+// product with zeros for the other copies' tokens; the copies' sums are added at the end.
+//
+// Keys of the next unit are loaded as soon as the first product is done with this one's, its values after the
+// second, so that loads are in flight throughout without registers of their own.
+template <typename T, int D, bool RANGE, int R>
+__global__ __launch_bounds__(64 * kWaves, waves_of(D, __is_same(T, _Float16))) void k_attend(AttendArgs A) {
   using L = Kv4<D>;
+  constexpr int kTiles = R / 4;  // 16-token tiles of a lane's scores
   constexpr int kSteps = D / 32, kDpl = L::kDpl;
   constexpr bool kHalf = __is_same(T, _Float16);
   __shared__ float s_m[kWaves][kFew], s_l[kWaves][kFew], s_low[kWaves][kFew];
@@ -302,17 +329,17 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
 
   Item it;
   if (!locate(A, kFew, blockIdx.x, it)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-  const int tile = it.tile, h = it.h, b = it.b;
-  const Rows R(A, b);
-  const long long q0 = R.q0;
-  const int rows = R.rows;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
+  const int copy = m / R, tile = it.tile, h = it.h, b = it.b;
+  const Rows S(A, b);
+  const long long q0 = S.q0;
+  const int rows = S.rows;
   if (tile * kFew >= rows) return;
-  const int row = tile * kFew + m;
+  const int row = tile * kFew + m % R;
   const bool live = row < rows;
   const int qi = live ? row / A.group : 0, qo = live ? row % A.group : 0;
-  const int seen = live ? R.seen(A, row) : 0;
-  const int all = R.seen(A, tile * kFew), most = R.seen(A, min(tile * kFew + kFew, rows) - 1);
+  const int seen = live ? S.seen(A, row) : 0;
+  const int all = S.seen(A, tile * kFew), most = S.seen(A, min(tile * kFew + R, rows) - 1);
   const int u0 = it.u0, u1 = min((most + kUnit - 1) / kUnit, it.u1);
 
   // the lane's part of its row's query: dims D / 4 g + 8 s .. + 7 of step s
@@ -341,13 +368,28 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
   float top = -INFINITY, sum = 0.f, low = INFINITY;
   const float scale2 = A.scale * kLog2e;
 
-  for (int u = u0 + wave; u < u1; u += kWaves) {
-    const int pg = A.table[b * A.table_stride + (u >> 1)];
-    if (pg < 0 || pg >= A.pages) continue;  // no such page: its tokens are not there
-    Unit<D> x;
-    x.load(A.pool + ((long long)pg * A.heads + h) * L::kBytes, u & 1, m, g);
+  // a page number that is not in the pool is read as page 0, and its tokens are left out
+  const int* table = A.table + b * A.table_stride;
+  auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + h) * L::kBytes; };
+  int u = u0 + wave, pg = 0, next = 0;
+  Unit<D> x;
+  if (u < u1) {
+    pg = table[u >> 1];
+    x.load_keys(page_of(pg), u & 1, m, g);
+    x.load_values(page_of(pg), u & 1, m, g);
+    if (u + kWaves < u1) next = table[(u + kWaves) >> 1];
+  }
+  for (; u < u1; u += kWaves) {
+    const bool there = pg >= 0 && pg < A.pages, more = u + kWaves < u1;
+    pg = next;
+    if (u + 2 * kWaves < u1) next = table[(u + 2 * kWaves) >> 1];
+    const uint8_t* page = page_of(pg);
+    if (!there) {
+      if (more) x.load_keys(page, u & 1, m, g), x.load_values(page, u & 1, m, g);
+      continue;
+    }
 
-    float t[4][4];
+    float t[kTiles][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f32x4 c = {0.f, 0.f, 0.f, 0.f};
@@ -360,30 +402,31 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
         if constexpr (kHalf) c = mfma(kk, ql[s], c);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t[i][k] = c[k];
+      for (int k = 0; k < 4; ++k) t[i % kTiles][k] = i < kTiles || copy == i / kTiles ? c[k] : t[i % kTiles][k];
     }
-    const int base = u * kUnit + 4 * g;
+    if (more) x.load_keys(page, u & 1, m, g);
+    const int base = u * kUnit + 4 * g, own = base + 16 * kTiles * copy;
     if (u * kUnit + kUnit > all) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < kTiles; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const bool see = base + 16 * i + k < seen;
+          const bool see = own + 16 * i + k < seen;
           if constexpr (RANGE) low = see ? fminf(low, t[i][k]) : low;
           t[i][k] = see ? t[i][k] : -INFINITY;
         }
     } else if constexpr (RANGE) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < kTiles; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) low = fminf(low, t[i][k]);
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[i][k]);
-    mx = fmaxf(top, over_g(mx, fmax2) * scale2);
+    mx = fmaxf(top, over_row<R>(mx, fmax2) * scale2);
     const float f = rebase(top, mx);
     top = mx;
     const float ref = reference(mx) - kLift;
@@ -392,21 +435,30 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
 #pragma unroll
       for (int i = 0; i < kDpl; ++i) acc[i] *= f;
     }
+    u32x2 hi[kTiles], lo[kTiles];  // the probabilities in two bf16 parts
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         t[i][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][k], scale2, -ref));
         sum += t[i][k];
       }
+      hi[i] = u32x2{heads_of(t[i][0], t[i][1]), heads_of(t[i][2], t[i][3])};
+      lo[i] = u32x2{pack(rest_of(t[i][0]), rest_of(t[i][1])), pack(rest_of(t[i][2]), rest_of(t[i][3]))};
+    }
 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float* p0 = t[2 * i];
-      const float* p1 = t[2 * i + 1];
-      const bf16x8 ph = operand(heads_of(p0[0], p0[1]), heads_of(p0[2], p0[3]), heads_of(p1[0], p1[1]), heads_of(p1[2], p1[3]));
-      const bf16x8 pl = operand(pack(rest_of(p0[0]), rest_of(p0[1])), pack(rest_of(p0[2]), rest_of(p0[3])),
-                                pack(rest_of(p1[0]), rest_of(p1[1])), pack(rest_of(p1[2]), rest_of(p1[3])));
+      auto part = [&](const u32x2* p) {
+        u32x2 w[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const bool mine = copy == (2 * i + n) / kTiles;
+          w[n] = kTiles == 4 ? p[(2 * i + n) % kTiles] : u32x2{mine ? p[n % kTiles][0] : 0u, mine ? p[n % kTiles][1] : 0u};
+        }
+        return operand(w[0][0], w[0][1], w[1][0], w[1][1]);
+      };
+      const bf16x8 ph = part(hi), pl = part(lo);
       uint32_t vs[2] = {x.vs[i][0], x.vs[i][1]};
       float sc[8];
       // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  It is taken
@@ -447,13 +499,21 @@ __global__ __launch_bounds__(64 * kWaves) void k_attend(AttendArgs A) {
         step(std::integral_constant<int, 3>());
       }
     }
+    if (more) x.load_values(page, u & 1, m, g);
   }
 
   // join the waves: lane (m, g) holds dims D / 4 g + kDpl i + d of row m in acc[d][i]
-  sum = over_g(sum, [](float a, float c) { return a + c; });
-  if constexpr (RANGE) low = over_g(low, fmin2) * scale2;
-  if (g == 0) s_m[wave][m] = top, s_l[wave][m] = sum, s_low[wave][m] = low;
-  if (m < A.rows) {
+  sum = over_row<R>(sum, [](float a, float c) { return a + c; });
+  if constexpr (RANGE) low = over_row<R>(low, fmin2) * scale2;
+#pragma unroll
+  for (int d = 0; d < kDpl; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (R <= 8) acc[d][i] += turn<8>(acc[d][i]);
+      if constexpr (R <= 4) acc[d][i] += turn<4>(acc[d][i]);
+    }
+  if (lane < R) s_m[wave][m] = top, s_l[wave][m] = sum, s_low[wave][m] = low;
+  if (m < R && m < A.rows) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -558,14 +618,14 @@ struct Way {
   bool few, join;
   int rows, least;
   int64_t tiles, slots, pairs, items;
-  Way(int64_t tokens, int64_t seqs, int heads, int group, int most, int cols) {
+  Way(int64_t seqs, int heads, int group, int dim, bool half, int most, int cols) {
     const int64_t all = (int64_t)most * group, units = std::max<int64_t>(1, (int64_t)cols * (kPageTokens / kUnit));
     few = true;
     const int size = few ? kFew : kMany;
     tiles = (all + size - 1) / size;
     rows = (int)std::min<int64_t>(all, size);
     least = few ? 4 * kWaves : 8;
-    slots = few ? 1024 : 512;
+    slots = kComputeUnits * (few ? waves_of(dim, half) : 2);
     pairs = seqs * tiles;
     join = pairs <= 64 * kPairs && units > least;
     items = !join ? pairs * heads : std::min(pairs * ((units + least - 1) / least), pairs + (slots + heads - 1) / heads) * heads;
@@ -578,7 +638,9 @@ struct Way {
 template <typename T, int D, bool RANGE>
 int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
   const size_t lds = kWaves * W.rows * (D + 4) * sizeof(float);
-  k_attend<T, D, RANGE><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
+  if (W.rows <= 4) k_attend<T, D, RANGE, 4><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
+  else if (W.rows <= 8) k_attend<T, D, RANGE, 8><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
+  else k_attend<T, D, RANGE, 16><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
   HCK_CHECK_LAUNCH();
   if (W.join) {
     k_join<T, D, RANGE, true><<<dim3((unsigned)(W.pairs * A.heads), W.rows), 64 * kWaves, 0, s>>>(A);
@@ -599,7 +661,11 @@ bool shape_ok(int64_t tokens, int seqs, int kv_heads, int group, int most, int c
 extern "C" size_t hck_kv4_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim,
                                                  int most, int table_columns) {
   if (!hck::shape_ok(tokens, seqs, kv_heads, group, most, table_columns)) return 0;
-  return hck::Way(tokens, seqs, kv_heads, group, most, table_columns).bytes(kv_heads, head_dim);
+  // the type is not known here: the most that either needs
+  size_t most_bytes = 0;
+  for (bool half : {false, true})
+    most_bytes = std::max(most_bytes, hck::Way(seqs, kv_heads, group, head_dim, half, most, table_columns).bytes(kv_heads, head_dim));
+  return most_bytes;
 }
 
 extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int head_dim, int type,
@@ -615,7 +681,7 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
   if (!queries || !lengths || (!table && table_columns > 0) || !out || !lse) return HCK_ERR_ARG;
   if (!starts && tokens < seqs) return HCK_ERR_ARG;
   if (((uintptr_t)pool | (uintptr_t)out | (uintptr_t)workspace) % 16) return HCK_ERR_ARG;
-  const hck::Way W(tokens, seqs, kv_heads, group, most, table_columns);
+  const hck::Way W(seqs, kv_heads, group, head_dim, type == HCK_F16, most, table_columns);
   const size_t need = W.bytes(kv_heads, head_dim);
   if (W.items > 0x7fffffff || W.pairs > 0x7fffffff) return HCK_ERR_ARG;
   if (need > workspace_bytes || (need && !workspace)) return HCK_ERR_WORKSPACE;
