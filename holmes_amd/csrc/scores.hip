@@ -7,9 +7,12 @@
 // a row is read once.  The reference enters each t_i through one fused multiply-add and is subtracted
 // again as the same 32-bit number, so its own rounding cancels.
 //
-// The top values: a wave keeps its k best in order, entry i in lane i.  A wave meets its values in
-// rising order of their index, so after the first blocks a block of 64 lanes' values is dismissed by
-// one comparison of the lanes' maxima with the k-th best.
+// The top values: every lane keeps the maximum of what it met.  The k-th largest T of a workgroup's 256
+// maxima is no more than the k-th largest value, and only lanes whose maximum reaches T can hold a value
+// that does: hardly more than k of them, whose values are read again.  What reaches T goes into a list
+// and is put in order by counting.  If the list runs over (many values alike), every wave keeps its k best
+// in order, entry i in lane i, and goes through its values once more; they come in rising order of their
+// index, so most blocks are dismissed by one comparison.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -22,7 +25,7 @@ namespace hck {
 namespace {
 
 constexpr int kWaves = 4, kVecs = 4;  // waves of a workgroup, 16-byte pieces of a lane in flight
-constexpr int kMaxTop = 32;
+constexpr int kMaxTop = 32, kMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -32,7 +35,7 @@ struct ScoreArgs {
   const long long* tokens;  // null: no given tokens
   float *given, *entropy, *top_logs;
   long long* top_ids;
-  float* part;  // with splits > 1: [row][split] of (r, l, s, 0), then [row][split][top] of (key, index)
+  float* part;  // with splits > 1: [row][split] of (r, l, s, 0), then [row][split][top] of keys and indexes, 64 bits each
   long long row_stride;
   int rows, vocab, top, splits;
 };
@@ -107,7 +110,7 @@ __device__ __forceinline__ float element(u32x4 v, int e) {
 }
 
 template <typename T>
-__device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const Sums& a, const Best& best) {
+__device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const Sums& a, unsigned long long best) {
   const int lane = threadIdx.x & 63;
   const float ref = finite_or_zero(a.r);
   const float log = a.l == 0.f ? 0.f : __builtin_amdgcn_logf(a.l);  // a row without a finite value
@@ -122,8 +125,8 @@ __device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const 
     }
   }
   if (lane < A.top) {
-    A.top_ids[row * A.top + lane] = best.index;
-    A.top_logs[row * A.top + lane] = (__builtin_fmaf(value_of(best.key), kLog2e, -ref) - log) * kLn2;
+    A.top_ids[row * A.top + lane] = 0xffffffffu - (uint32_t)best;
+    A.top_logs[row * A.top + lane] = (__builtin_fmaf(value_of((uint32_t)(best >> 32)), kLog2e, -ref) - log) * kLn2;
   }
 }
 
@@ -139,12 +142,13 @@ __device__ __forceinline__ Sums over_lanes(Sums a) {
   return a;
 }
 
-// `N` values of the lane, `live` of them there, the first at `index`, the others in rising order `step(n)`.
-template <int N, typename V, typename I>
-__device__ __forceinline__ void take(Sums& a, Best& best, int top, V value, I index) {
+// `N` values of the lane into its sums and maximum.
+template <int N, typename V>
+__device__ __forceinline__ void take(Sums& a, float& top, V value) {
   float m = -INFINITY;
 #pragma unroll
   for (int n = 0; n < N; ++n) m = fmaxf(m, value(n));
+  top = fmaxf(top, m);
   const float r = fmaxf(a.r, m * kLog2e);
   a.rebase(r);
   const float ref = finite_or_zero(r);
@@ -155,21 +159,82 @@ __device__ __forceinline__ void take(Sums& a, Best& best, int top, V value, I in
     a.l += e;
     a.s = __builtin_fmaf(e, fmaxf(t, -1000.f), a.s);  // 2^-inf counts nothing, and 0 * -inf would
   }
-  if (top > 0 && __any(key_of(m) > best.last_key || a.l != a.l || best.last_key == 0)) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const uint32_t i = index(n);
-      const uint32_t k = i == 0xffffffffu ? 0 : key_of(value(n));
-      best.offer(k, i, top);
-    }
+}
+
+constexpr int kThreads = 64 * kWaves, kList = 256;
+
+// The candidates of a workgroup for the top values.
+struct Candidates {
+  uint32_t most[kThreads];             // every thread's largest key
+  unsigned long long list[kList], best[kMaxTop];
+  int count, hot[64];
+  __device__ __forceinline__ static unsigned long long order(uint32_t key, uint32_t index) {
+    return (unsigned long long)key << 32 | (0xffffffffu - index);  // larger: before
   }
+  __device__ __forceinline__ static uint32_t key(unsigned long long o) { return (uint32_t)(o >> 32); }
+  __device__ __forceinline__ static uint32_t index(unsigned long long o) { return 0xffffffffu - (uint32_t)o; }
+
+  // A key that `top` threads' largest reach, as large as a few more allow, and how many do.
+  __device__ __forceinline__ uint32_t reach(uint32_t mine, int top, int& threads) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    most[threadIdx.x] = mine;
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    uint32_t k[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) k[w] = most[64 * w + lane];
+    uint32_t t = 0;
+    threads = kThreads;
+    for (uint32_t bit = 0x80000000u; bit != 0 && threads > top + 3; bit >>= 1) {
+      int n = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) n += __popcll(__ballot(k[w] >= (t | bit)));
+      if (n >= top) t |= bit, threads = n;
+    }
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      if (w < wave) before += __popcll(__ballot(k[w] >= t));
+    const unsigned long long here = __ballot(mine >= t);
+    const int at = before + __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0));
+    if (mine >= t && at < 64) hot[at] = threadIdx.x;
+    __syncthreads();
+    return t;
+  }
+  __device__ __forceinline__ void offer(uint32_t k, uint32_t i, uint32_t least) {
+    if (k < least) return;
+    const int at = atomicAdd(&count, 1);
+    if (at < kList) list[at] = order(k, i);
+  }
+  // The list's first `top` in order; false: it does not hold them.
+  __device__ __forceinline__ bool sort(int top) {
+    __syncthreads();
+    const int n = count;
+    if (n < top || n > kList) return false;
+    if ((int)threadIdx.x < n) {
+      const unsigned long long mine = list[threadIdx.x];
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += list[i] > mine;
+      if (rank < top) best[rank] = mine;
+    }
+    __syncthreads();
+    return true;
+  }
+};
+static_assert(kList <= kThreads, "a thread an entry");
+
+template <typename T>
+__device__ __forceinline__ u32x4 nothing() {
+  if constexpr (sizeof(T) == 4) return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
+  else if constexpr (__is_same(T, __bf16)) return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+  else return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
 }
 
 template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void k_scores(ScoreArgs A) {
+__global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
   constexpr int kPer = 16 / sizeof(T);  // values of a 16-byte piece
   __shared__ float s_sums[kWaves][3];
-  __shared__ uint32_t s_key[kWaves][kMaxTop], s_index[kWaves][kMaxTop];
+  __shared__ Candidates C;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long row = blockIdx.y + (long long)blockIdx.z * 32768;
   if (row >= A.rows) return;
@@ -179,79 +244,132 @@ __global__ __launch_bounds__(64 * kWaves) void k_scores(ScoreArgs A) {
   const int pieces = (A.vocab - head) / kPer, tail = head + pieces * kPer;
   const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   const int blocks = (pieces + 64 * kVecs - 1) / (64 * kVecs);
+  const int first = blockIdx.x * kWaves + wave, stride = A.splits * kWaves;
+  const bool heads = first == 0 && head > 0, tails = first == stride - 1 && tail < A.vocab;
   Sums a;
-  Best best;
-  const int first = blockIdx.x * kWaves + wave;
-  if (first == 0 && head > 0)
-    take<1>(a, best, A.top, [&](int) { return lane < head ? (float)x[lane] : -INFINITY; },
-            [&](int) { return lane < head ? (uint32_t)lane : 0xffffffffu; });
-  for (int bl = first; bl < blocks; bl += A.splits * kWaves) {
+  float top = -INFINITY;
+  if (heads) take<1>(a, top, [&](int) { return lane < head ? (float)x[lane] : -INFINITY; });
+  for (int bl = first; bl < blocks; bl += stride) {
     u32x4 v[kVecs];
     const int p0 = bl * 64 * kVecs + lane;
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
       const int p = p0 + 64 * j;
-      if constexpr (sizeof(T) == 4) v[j] = u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
-      else if constexpr (__is_same(T, __bf16)) v[j] = u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
-      else v[j] = u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
+      v[j] = nothing<T>();
       if (p < pieces) v[j] = body[p];
     }
-    take<kVecs * kPer>(a, best, A.top, [&](int n) { return element<T>(v[n / kPer], n % kPer); },
-                       [&](int n) {
-                         const int p = p0 + 64 * (n / kPer);
-                         return p < pieces ? (uint32_t)(head + p * kPer + n % kPer) : 0xffffffffu;
-                       });
+    take<kVecs * kPer>(a, top, [&](int n) { return element<T>(v[n / kPer], n % kPer); });
   }
-  if (first == A.splits * kWaves - 1 && tail < A.vocab)
-    take<1>(a, best, A.top, [&](int) { return tail + lane < A.vocab ? (float)x[tail + lane] : -INFINITY; },
-            [&](int) { return tail + lane < A.vocab ? (uint32_t)(tail + lane) : 0xffffffffu; });
+  if (tails) take<1>(a, top, [&](int) { return tail + lane < A.vocab ? (float)x[tail + lane] : -INFINITY; });
 
+  bool listed = true;
+  if (A.top > 0) {
+    int threads;
+    const uint32_t least = C.reach(a.l != a.l ? 0xffffffffu : key_of(top), A.top, threads);
+    listed = threads <= 64;
+    if (listed) {
+      // the pieces of the threads that reach it, one a thread; a wave of the workgroup has `per` of them a lane
+      const int per = (blocks - (int)blockIdx.x * kWaves + stride - 1) / stride * kVecs;
+      for (int i = threadIdx.x; i < threads * per; i += kThreads) {
+        const int t = C.hot[i / per], n = i % per;
+        const int p = ((int)blockIdx.x * kWaves + (t >> 6) + n / kVecs * stride) * 64 * kVecs + (t & 63) + 64 * (n % kVecs);
+        if (p >= pieces) continue;
+        const u32x4 v = body[p];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) C.offer(key_of(element<T>(v, e)), (uint32_t)(head + p * kPer + e), least);
+      }
+      if (heads && lane < head) C.offer(key_of((float)x[lane]), (uint32_t)lane, least);
+      if (tails && tail + lane < A.vocab) C.offer(key_of((float)x[tail + lane]), (uint32_t)(tail + lane), least);
+      listed = C.sort(A.top);
+    }
+  }
+  if (!listed) {  // the same for all threads
+    __syncthreads();
+    Best best;
+    auto offer = [&](bool there, float value, int index) { best.offer(there ? key_of(value) : 0, (uint32_t)index, A.top); };
+    if (heads) offer(lane < head, lane < head ? (float)x[lane] : 0.f, lane);
+    for (int bl = first; bl < blocks; bl += stride)
+      for (int j = 0; j < kVecs; ++j) {
+        const int p = bl * 64 * kVecs + lane + 64 * j;
+        const u32x4 v = p < pieces ? body[p] : nothing<T>();
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) offer(p < pieces, element<T>(v, e), head + p * kPer + e);
+      }
+    if (tails) offer(tail + lane < A.vocab, tail + lane < A.vocab ? (float)x[tail + lane] : 0.f, tail + lane);
+    static_assert(kWaves * kMaxTop <= kList, "the waves' lists");
+    if (lane < A.top) C.list[wave * kMaxTop + lane] = Candidates::order(best.key, best.index);
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < kWaves; ++w) {
+        const unsigned long long o = lane < A.top ? C.list[w * kMaxTop + lane] : 0;
+        best.offer(Candidates::key(o), Candidates::index(o), A.top);
+      }
+      if (lane < A.top) C.best[lane] = Candidates::order(best.key, best.index);
+    }
+  }
   a = over_lanes(a);
   if (lane == 0) s_sums[wave][0] = a.r, s_sums[wave][1] = a.l, s_sums[wave][2] = a.s;
-  if (lane < A.top) s_key[wave][lane] = best.key, s_index[wave][lane] = best.index;
   __syncthreads();
   if (wave != 0) return;
   for (int w = 1; w < kWaves; ++w) {
     Sums o;
     o.r = s_sums[w][0], o.l = s_sums[w][1], o.s = s_sums[w][2];
     a.add(o);
-    if (A.top) best.offer(lane < A.top ? s_key[w][lane] : 0, lane < A.top ? s_index[w][lane] : 0, A.top);
   }
-  if (A.splits == 1) return finish<T>(A, row, a, best);
-  float* sums = A.part + (row * A.splits + blockIdx.x) * 4;
-  uint32_t* tops = (uint32_t*)(A.part + (long long)A.rows * A.splits * 4) + (row * A.splits + blockIdx.x) * A.top * 2;
+  if (A.splits == 1) return finish<T>(A, row, a, lane < A.top ? C.best[lane] : 0);
+  const long long part = row * A.splits + blockIdx.x;
+  float* sums = A.part + part * 4;
+  unsigned long long* tops = (unsigned long long*)(A.part + (long long)A.rows * A.splits * 4) + part * A.top;
   if (lane == 0) sums[0] = a.r, sums[1] = a.l, sums[2] = a.s;
-  if (lane < A.top) tops[2 * lane] = best.key, tops[2 * lane + 1] = best.index;
+  if (lane < A.top) tops[lane] = C.best[lane];
 }
 
-// Joins the parts of a row: one wave a row.
+// Joins the parts of a row, one workgroup a row.
 template <typename T>
-__global__ __launch_bounds__(64) void k_join(ScoreArgs A) {
+__global__ __launch_bounds__(kThreads) void k_join(ScoreArgs A) {
+  __shared__ Candidates C;
   const long long row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const unsigned long long* tops = (const unsigned long long*)(A.part + (long long)A.rows * A.splits * 4) + row * A.splits * A.top;
   Sums a;
-  for (int s = lane; s < A.splits; s += 64) {
-    const float* p = A.part + (row * A.splits + s) * 4;
-    Sums o;
-    o.r = p[0], o.l = p[1], o.s = p[2];
-    a.add(o);
+  if (lane < A.splits) {
+    const float* p = A.part + (row * A.splits + lane) * 4;
+    a.r = p[0], a.l = p[1], a.s = p[2];
   }
-  a = over_lanes(a);
-  Best best;
-  if (A.top) {
-    const uint32_t* tops = (const uint32_t*)(A.part + (long long)A.rows * A.splits * 4) + row * A.splits * A.top * 2;
+  if (A.top > 0) {
+    constexpr int kMost = kMaxSplits * kMaxTop / kThreads;
     const int all = A.splits * A.top;
-    for (int e = lane; e - lane < all; e += 64)
-      best.offer(e < all ? tops[2 * e] : 0, e < all ? tops[2 * e + 1] : 0, A.top);
+    unsigned long long o[kMost], most = 0;
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+      const int e = threadIdx.x + kThreads * j;
+      o[j] = e < all ? tops[e] : 0;
+      most = o[j] > most ? o[j] : most;
+    }
+    int threads;
+    const uint32_t least = max(1u, C.reach(Candidates::key(most), A.top, threads));
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) C.offer(Candidates::key(o[j]), Candidates::index(o[j]), least);
+    if (!C.sort(A.top)) {
+      Best best;
+      if (threadIdx.x < 64) {
+        for (int e = lane; e - lane < all; e += 64) {
+          const unsigned long long n = e < all ? tops[e] : 0;
+          best.offer(Candidates::key(n), Candidates::index(n), A.top);
+        }
+        if (lane < A.top) C.best[lane] = Candidates::order(best.key, best.index);
+      }
+    }
   }
-  finish<T>(A, row, a, best);
+  if (threadIdx.x >= 64) return;
+  finish<T>(A, row, over_lanes(a), lane < A.top ? C.best[lane] : 0);
 }
 
 // Parts of a row: workgroups for all 256 compute units four times, none with less than one block a wave.
 int splits_of(int64_t rows, int vocab, int size) {
   const int64_t want = (1024 + rows - 1) / std::max<int64_t>(rows, 1);
   const int64_t block = (int64_t)64 * kVecs * 16 / size, most = std::max<int64_t>(1, vocab / (block * kWaves));
-  return (int)std::min<int64_t>(std::min<int64_t>(want, most), 64);
+  return (int)std::min<int64_t>(std::min<int64_t>(want, most), kMaxSplits);
 }
 
 int size_of(int type) { return type == HCK_F32 ? 4 : type == HCK_BF16 || type == HCK_F16 ? 2 : 0; }
@@ -259,10 +377,10 @@ int size_of(int type) { return type == HCK_F32 ? 4 : type == HCK_BF16 || type ==
 template <typename T>
 int launch(const ScoreArgs& A, hipStream_t s) {
   const int gy = std::min(A.rows, 32768), gz = (A.rows + 32767) / 32768;
-  k_scores<T><<<dim3(A.splits, gy, gz), 64 * kWaves, 0, s>>>(A);
+  k_scores<T><<<dim3(A.splits, gy, gz), kThreads, 0, s>>>(A);
   HCK_CHECK_LAUNCH();
   if (A.splits > 1) {
-    k_join<T><<<A.rows, 64, 0, s>>>(A);
+    k_join<T><<<A.rows, kThreads, 0, s>>>(A);
     HCK_CHECK_LAUNCH();
   }
   return HCK_OK;
@@ -284,7 +402,7 @@ extern "C" int hck_token_scores(const void* logits, int type, int64_t rows, int 
   if (rows < 0 || rows > (1 << 30) || vocab < 1 || top < 0 || top > hck::kMaxTop || top > vocab) return HCK_ERR_ARG;
   if (rows == 0) return HCK_OK;
   if (!logits || !entropy || (tokens && !given) || (top && (!top_ids || !top_logs))) return HCK_ERR_ARG;
-  if ((uintptr_t)logits % hck::size_of(type)) return HCK_ERR_ARG;
+  if ((uintptr_t)logits % hck::size_of(type) || (uintptr_t)workspace % 16) return HCK_ERR_ARG;
   const size_t need = hck_token_scores_workspace_bytes(rows, vocab, type, top);
   if (need > workspace_bytes || (need && !workspace)) return HCK_ERR_WORKSPACE;
   hck::ScoreArgs A{};
