@@ -66,19 +66,14 @@ class SoftmaxRanges(NamedTuple):
     rsqrt_interval: tuple
 
 
-def _type(dtype: torch.dtype, allowed, what: str) -> int:
-    if dtype not in allowed:
-        raise ValueError(f"{what} must be {', '.join(str(d).replace('torch.', '') for d in allowed)}, not {dtype}")
-    return _TYPES[dtype]
-
-
-def _check(cond: bool, message: str) -> None:
-    if not cond:
-        raise ValueError(message)
+# A call on a few tokens costs what the host does for it, so checks are plain conditions and messages are
+# put together only where one fails.
+def _no_type(dtype: torch.dtype, allowed, what: str):
+    return ValueError(f"{what} must be {', '.join(str(d).replace('torch.', '') for d in allowed)}, not {dtype}")
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # torch.cuda.current_stream without its object
 
 
 class ClearKVPages:
@@ -107,8 +102,8 @@ class ClearKVPages:
         return int(self.buf.numel())
 
     def _slots(self, slots) -> torch.Tensor:
-        _check(slots.dim() == 1 and slots.dtype == torch.int64 and slots.device == self.buf.device,
-               "slots must be a 1-d int64 tensor on the pool's device")
+        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != self.buf.device:
+            raise ValueError("slots must be a 1-d int64 tensor on the pool's device")
         return slots if slots.is_contiguous() else slots.contiguous()
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor) -> None:
@@ -116,28 +111,37 @@ class ClearKVPages:
         the last axis contiguous) into ``slots`` [tokens].  A slot outside the pool, as -1 for padding, leaves
         its token out; the slots of one call must differ."""
 
-        slots = self._slots(slots)
-        shape = (slots.numel(), self.kv_heads, self.head_dim)
-        kind = _type(keys.dtype, _TYPES, "keys")
-        for name, x in (("keys", keys), ("values", values)):
-            _check(x.shape == shape and x.dtype == keys.dtype and x.device == self.buf.device and x.stride(2) == 1,
-                   f"{name} must be {list(shape)}, contiguous along the last axis, in one type on the pool's device")
-        nat.check(self._lib.hck_kv4_append(
-            self.buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, kind, keys.data_ptr(), keys.stride(0),
-            keys.stride(1), values.data_ptr(), values.stride(0), values.stride(1), slots.data_ptr(), shape[0],
-            _stream(self.buf.device)), "hck_kv4_append")
+        buf, slots = self.buf, self._slots(slots)
+        shape, dtype, device = (slots.numel(), self.kv_heads, self.head_dim), keys.dtype, buf.device
+        kind = _TYPES.get(dtype)
+        if kind is None:
+            raise _no_type(dtype, _TYPES, "keys")
+        k_token, k_head, k_dim = keys.stride() if keys.dim() == 3 else (0, 0, 0)
+        v_token, v_head, v_dim = values.stride() if values.dim() == 3 else (0, 0, 0)
+        for name, x, last in (("keys", keys, k_dim), ("values", values, v_dim)):
+            if x.shape != shape or x.dtype != dtype or x.device != device or last != 1:
+                raise ValueError(f"{name} must be {list(shape)}, contiguous along the last axis, in one type on the "
+                                 "pool's device")
+        err = self._lib.hck_kv4_append(buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, kind, keys.data_ptr(),
+                                       k_token, k_head, values.data_ptr(), v_token, v_head, slots.data_ptr(), shape[0],
+                                       _stream(device))
+        if err:
+            nat.check(err, "hck_kv4_append")
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> tuple:
         """What ``slots`` hold, as ``(keys, values)`` [tokens][kv_heads][head_dim] in ``dtype``: exact in bf16
         and fp32; in fp16 rounded, with its largest value for any above.  Zeros for a slot outside the pool."""
 
-        slots = self._slots(slots)
-        kind = _type(dtype, _TYPES, "dtype")
-        keys = torch.empty((slots.numel(), self.kv_heads, self.head_dim), dtype=dtype, device=self.buf.device)
+        buf, slots = self.buf, self._slots(slots)
+        kind, tokens = _TYPES.get(dtype), slots.numel()
+        if kind is None:
+            raise _no_type(dtype, _TYPES, "dtype")
+        keys = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=buf.device)
         values = torch.empty_like(keys)
-        nat.check(self._lib.hck_kv4_read(
-            self.buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, kind, slots.data_ptr(), slots.numel(),
-            keys.data_ptr(), values.data_ptr(), _stream(self.buf.device)), "hck_kv4_read")
+        err = self._lib.hck_kv4_read(buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, kind, slots.data_ptr(),
+                                     tokens, keys.data_ptr(), values.data_ptr(), _stream(buf.device))
+        if err:
+            nat.check(err, "hck_kv4_read")
         return keys, values
 
     def attend(self, queries: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
@@ -154,37 +158,47 @@ class ClearKVPages:
         sequence covers.  A page outside the pool counts as tokens that are not there.  ``scale`` multiplies
         the scores (default head_dim^-1/2); ``ranges`` asks for their least and largest."""
 
-        _check(queries.dim() == 3 and queries.shape[2] == self.head_dim and queries.stride(2) == 1,
-               f"queries must be [tokens][query heads][{self.head_dim}], contiguous along the last axis")
-        kind = _type(queries.dtype, (torch.bfloat16, torch.float16), "queries")
-        tokens, heads = int(queries.shape[0]), int(queries.shape[1])
-        _check(heads > 0 and heads % self.kv_heads == 0, f"query heads must be a multiple of {self.kv_heads}")
-        _check(table.dim() == 2 and lengths.dim() == 1 and table.shape[0] == lengths.shape[0],
-               "table must be [sequences][columns] and lengths [sequences]")
-        seqs = int(lengths.shape[0])
-        _check(starts.shape == (seqs + 1,) if starts is not None else tokens == seqs,
-               "starts must be [sequences + 1], or there is one query for each sequence")
-        dev = self.buf.device
+        dim, kv_heads, dev, lib = self.head_dim, self.kv_heads, self.buf.device, self._lib
+        if queries.dim() != 3 or queries.shape[2] != dim or queries.stride(2) != 1 or queries.device != dev:
+            raise ValueError(f"queries must be [tokens][query heads][{dim}], contiguous along the last axis, on the "
+                             "pool's device")
+        kind = _TYPES.get(queries.dtype)
+        if kind is None or kind == nat.HCK_F32:
+            raise _no_type(queries.dtype, (torch.bfloat16, torch.float16), "queries")
+        tokens, heads, _ = queries.shape
+        if heads == 0 or heads % kv_heads:
+            raise ValueError(f"query heads must be a multiple of {kv_heads}")
+        if table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != lengths.shape[0]:
+            raise ValueError("table must be [sequences][columns] and lengths [sequences]")
+        seqs, cols = table.shape
+        if starts.shape != (seqs + 1,) if starts is not None else tokens != seqs:
+            raise ValueError("starts must be [sequences + 1], or there is one query for each sequence")
         for name, x in (("table", table), ("lengths", lengths), ("starts", starts)):
-            _check(x is None or (x.dtype == torch.int32 and x.device == dev and (x.numel() == 0 or x.stride(-1) == 1)),
-                   f"{name} must be int32 on the pool's device, contiguous along the last axis")
-        _check(queries.device == dev, "queries must be on the pool's device")
+            if x is not None and (x.dtype != torch.int32 or x.device != dev or (x.stride(-1) != 1 and x.numel() != 0)):
+                raise ValueError(f"{name} must be int32 on the pool's device, contiguous along the last axis")
         most = (1 if starts is None else tokens) if most is None else min(int(most), tokens)
-        _check(most >= 0, "most must not be negative")
-        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        _check(0.0 < scale < math.inf, "scale must be positive and finite")
-        out = torch.empty((tokens, heads, self.head_dim), dtype=queries.dtype, device=dev)
-        sums = torch.empty((3 if ranges else 1, tokens, heads), dtype=torch.float32, device=dev)
-        group, cols = heads // self.kv_heads, int(table.shape[1])
-        need = self._lib.hck_kv4_attend_workspace_bytes(tokens, seqs, self.kv_heads, group, self.head_dim, most, cols)
+        if most < 0:
+            raise ValueError("most must not be negative")
+        scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+        if not 0.0 < scale < math.inf:
+            raise ValueError("scale must be positive and finite")
+        group = heads // kv_heads
+        out = torch.empty((tokens, heads, dim), dtype=queries.dtype, device=dev)
+        if ranges:
+            lse, low, high = torch.empty((3, tokens, heads), dtype=torch.float32, device=dev).unbind(0)
+        else:
+            lse, low, high = torch.empty((tokens, heads), dtype=torch.float32, device=dev), None, None
+        need = lib.hck_kv4_attend_workspace_bytes(tokens, seqs, kv_heads, group, dim, most, cols)
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        at = [sums[i].data_ptr() if i < len(sums) else None for i in range(3)]
-        nat.check(self._lib.hck_kv4_attend(
-            self.buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, kind, queries.data_ptr(), tokens, group,
-            queries.stride(0), queries.stride(1), table.data_ptr(), table.stride(0), cols, lengths.data_ptr(),
-            None if starts is None else starts.data_ptr(), seqs, most, int(causal), scale, out.data_ptr(), at[0], at[1],
-            at[2], None if work is None else work.data_ptr(), need, _stream(dev)), "hck_kv4_attend")
-        return Attended(out, sums[0], *((sums[1], sums[2]) if ranges else (None, None)))
+        err = lib.hck_kv4_attend(
+            self.buf.data_ptr(), self.pages, kv_heads, dim, kind, queries.data_ptr(), tokens, group, queries.stride(0),
+            queries.stride(1), table.data_ptr(), table.stride(0), cols, lengths.data_ptr(),
+            None if starts is None else starts.data_ptr(), seqs, most, int(causal), scale, out.data_ptr(),
+            lse.data_ptr(), low.data_ptr() if ranges else None, high.data_ptr() if ranges else None,
+            work.data_ptr() if need else None, need, _stream(dev))
+        if err:
+            nat.check(err, "hck_kv4_attend")
+        return Attended(out, lse, low, high)
 
 
 def softmax_ranges(low: torch.Tensor, high: torch.Tensor, lse: torch.Tensor, margin: float = 0.05) -> SoftmaxRanges:
@@ -210,25 +224,33 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     NaN), the entropies, and the ``top`` (up to 32) most likely tokens, int64 and log probabilities.  A logit
     of -inf is a token that cannot be; a row of nothing else gives -inf, and 0 for the entropy."""
 
-    kind = _type(logits.dtype, _TYPES, "logits")
-    _check(logits.dim() == 2 and logits.shape[1] >= 1 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-           "logits must be [rows][vocabulary], contiguous along the last axis")
-    rows, vocab = int(logits.shape[0]), int(logits.shape[1])
-    _check(0 <= top <= min(nat.HCK_TOP_MAX, vocab), f"top must be in 0..{min(nat.HCK_TOP_MAX, vocab)}")
+    kind = _TYPES.get(logits.dtype)
+    if kind is None:
+        raise _no_type(logits.dtype, _TYPES, "logits")
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] != 1):
+        raise ValueError("logits must be [rows][vocabulary], contiguous along the last axis")
+    rows, vocab = logits.shape
+    if not 0 <= top <= min(nat.HCK_TOP_MAX, vocab):
+        raise ValueError(f"top must be in 0..{min(nat.HCK_TOP_MAX, vocab)}")
+    dev = logits.device
     if tokens is not None:
-        _check(tokens.shape == (rows,) and tokens.dtype == torch.int64 and tokens.device == logits.device,
-               "tokens must be [rows] int64 on the logits' device")
+        if tokens.shape != (rows,) or tokens.dtype != torch.int64 or tokens.device != dev:
+            raise ValueError("tokens must be [rows] int64 on the logits' device")
         tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    if logits.device.type != "cuda":
+    if dev.type != "cuda":
         raise RuntimeError("token scores run on a GPU: there is no CPU path")
-    dev, lib = logits.device, nat.lib()
-    floats = torch.empty((2 + top, rows), dtype=torch.float32, device=dev)
-    logs = floats[2:].view(rows, top)
-    ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    lib = nat.lib()
+    given, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+    ids = logs = None
+    if top:
+        ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        logs = torch.empty((rows, top), dtype=torch.float32, device=dev)
     need = lib.hck_token_scores_workspace_bytes(rows, vocab, kind, top)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    nat.check(lib.hck_token_scores(
+    err = lib.hck_token_scores(
         logits.data_ptr(), kind, rows, vocab, logits.stride(0), None if tokens is None else tokens.data_ptr(), top,
-        floats[0].data_ptr(), floats[1].data_ptr(), ids.data_ptr(), logs.data_ptr(),
-        None if work is None else work.data_ptr(), need, _stream(dev)), "hck_token_scores")
-    return TokenScores(None if tokens is None else floats[0], floats[1], ids if top else None, logs if top else None)
+        given.data_ptr(), entropy.data_ptr(), ids.data_ptr() if top else None, logs.data_ptr() if top else None,
+        work.data_ptr() if need else None, need, _stream(dev))
+    if err:
+        nat.check(err, "hck_token_scores")
+    return TokenScores(None if tokens is None else given, entropy, ids, logs)
