@@ -12,187 +12,10 @@
 // fp16 query goes in as two bf16 parts (16 bits).  Scores, maxima, sums and outputs are held in 32
 // bits.  The probabilities go in as two bf16 parts as well, which leaves 2^-17 of each, far below the
 // rounding of the output; the sum l takes the unrounded ones.
-#include "kv4.hpp"
-
-#include "../../include/holmes_ckks.h"
-#include "internal.hpp"
+#include "kv4_attend.hpp"
 
 namespace hck {
 namespace {
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kUnit = 64;   // tokens that a wave takes at a time: half a page
-constexpr int kWaves = 4;
-constexpr int kComputeUnits = 256;
-constexpr int kFew = 16;    // rows of k_attend's workgroup
-constexpr int kMany = 128;  // rows of k_prompt's
-// Exponentials are taken times 2^24, so that those from 2^-126 to 2^-150 of a row's largest, which the
-// exponential instruction gives as 0, still count where every larger one meets a value of 0.  Sums then
-// stay finite for values up to 2^103 over the number of tokens.
-constexpr float kLift = 24.f;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-struct AttendArgs {
-  const uint8_t* pool;
-  const void* q;
-  const int* table;
-  const int* lengths;
-  const int* starts;   // null: sequence b has the one query b
-  void* out;
-  float *lse, *low, *high;  // [token][query head]; low, high nullable
-  // with `join`: [slot][row] of (m, l, low, -), [slot][row][D] of sums, and [tile][head] of (first slot, slots)
-  float *stat, *sums;
-  int* plan;
-  long long q_ts, q_hs, tokens, pages;
-  long long table_stride;
-  int cols, heads, group, causal;
-  int seqs, tiles;     // tiles of rows that the longest sequence can have
-  int rows;            // rows of a slot
-  int slots, least;    // workgroups to share the work out to, units that are not worth sharing
-  int join;
-  float scale;
-};
-
-// The rows of one sequence: query tokens [q0, q0 + nq), each with `group` heads, row = query * group + head.
-struct Rows {
-  long long q0;
-  int nq, rows, length;
-  __device__ __forceinline__ Rows(const AttendArgs& A, int b) {
-    long long first = b, last = b + 1;
-    if (A.starts) first = A.starts[b], last = A.starts[b + 1];
-    q0 = max(first, 0ll);
-    nq = (int)max(min(last, A.tokens) - q0, 0ll);
-    rows = (int)min((long long)nq * A.group, (long long)A.tiles * (A.rows > kFew ? kMany : kFew));
-    length = (int)min((long long)max(A.lengths[b], 0), (long long)A.cols * kPageTokens);
-  }
-  // tokens that row r sees
-  __device__ __forceinline__ int seen(const AttendArgs& A, int r) const {
-    return A.causal ? max(0, min(length, length - nq + r / A.group + 1)) : length;
-  }
-};
-
-// A workgroup's work: a tile of rows, a key head, and a part of the units of 64 tokens that they see.
-struct Item {
-  int b, tile, h, u0, u1, slot, slots;
-};
-
-// The units of a tile's rows, -1: no rows.
-__device__ __forceinline__ int units_of(const AttendArgs& A, int pair, int size) {
-  const Rows R(A, pair / A.tiles);
-  const int first = (pair % A.tiles) * size;
-  if (first >= R.rows) return -1;
-  return (R.seen(A, min(first + size, R.rows) - 1) + kUnit - 1) / kUnit;
-}
-
-__device__ __forceinline__ long long over_wave(long long x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-  return x;
-}
-__device__ __forceinline__ int over_wave(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-  return x;
-}
-
-constexpr int kPairs = 8;  // tiles of rows that a lane looks through to share the work out
-
-// Which part of the work is workgroup w's.  Lengths are on the device, so every wave works it out: with
-// all tiles' units in its lanes, a share is the smallest for which the parts (whole shares of a tile and
-// its rest) are no more than the workgroups that run at once.  Later tiles, which see more, come first.
-__device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Item& it) {
-  const int pairs = A.seqs * A.tiles, lane = threadIdx.x & 63;
-  it.h = w % A.heads;
-  it.slot = w, it.slots = 1;
-  int r = w / A.heads;
-  if (!A.join) {
-    const int p = pairs - 1 - r;
-    it.b = p / A.tiles, it.tile = p % A.tiles;
-    it.u0 = 0, it.u1 = 0x7fffffff;
-    return true;
-  }
-  const int per = (pairs + 63) / 64;
-  int n[kPairs];
-  long long total = 0;
-#pragma unroll
-  for (int j = 0; j < kPairs; ++j) {
-    const int p = pairs - 1 - (lane * per + j);
-    n[j] = j < per && p >= 0 ? units_of(A, p, size) : -1;
-    total += max(n[j], 0);
-  }
-  total = over_wave(total) * A.heads;
-  const int base = (int)min(1ll << 26, max((long long)A.least, (total + A.slots - 1) / A.slots));
-  int share = 0, mine = 0;
-#pragma unroll
-  for (int f = 4; f <= 8; ++f) {
-    if (f == 7) continue;
-    const int s = base / 4 * f + (base % 4 * f + 3) / 4;
-    int c = 0;
-#pragma unroll
-    for (int j = 0; j < kPairs; ++j) c += n[j] < 0 ? 0 : max(1, (n[j] + s - 1) / s);
-    const bool last = f == 8;
-    if (last || (long long)over_wave(c) * A.heads <= A.slots) {
-      share = s, mine = c;
-      break;
-    }
-  }
-  int upto = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int x = __shfl_up(upto, d);
-    if (lane >= d) upto += x;
-  }
-  const int owner = __popcll(__ballot(upto <= r));  // the lane that holds part r
-  if (owner > 63) return false;
-  int pair = 0, u0 = 0, count = 1, at = upto - mine;
-#pragma unroll
-  for (int j = 0; j < kPairs; ++j) {
-    const int c = n[j] < 0 ? 0 : max(1, (n[j] + share - 1) / share);
-    if (r >= at && r < at + c) pair = pairs - 1 - (lane * per + j), u0 = (r - at) * share, count = c;
-    at += c;
-  }
-  pair = __builtin_amdgcn_readlane(pair, owner);
-  it.u0 = __builtin_amdgcn_readlane(u0, owner);
-  it.slots = __builtin_amdgcn_readlane(count, owner);
-  it.u1 = it.u0 + share;
-  it.b = pair / A.tiles, it.tile = pair % A.tiles;
-  if (it.u0 == 0 && threadIdx.x == 0) {
-    A.plan[2 * (pair * A.heads + it.h)] = w;
-    A.plan[2 * (pair * A.heads + it.h) + 1] = it.slots;
-  }
-  return true;
-}
-
-// 16 bytes from an address that is a multiple of the elements' two bytes only.
-struct __attribute__((packed, aligned(2))) Loose16 {
-  u32x4 v;
-};
-
-__device__ __forceinline__ float scale_of(uint32_t word, int byte) {
-  return __uint_as_float(((word >> (8 * byte)) & 0xffu) << 23);
-}
-
-template <int B>
-__device__ __forceinline__ uint32_t cvt(uint32_t codes, float scale) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, B));
-}
-
-__device__ __forceinline__ bf16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __builtin_bit_cast(bf16x8, u32x4{a, b, c, d});
-}
-
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
-}
-
-__device__ __forceinline__ bool has_nan(uint32_t w) {  // a byte of 255 among the four
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u;
-}
 
 // What a lane holds of 64 tokens: lane (m, g) = (lane % 16, lane / 16) has D / 4 dims from D / 4 * g of
 // token m of every 16-token tile, and D / 16 dims from D / 16 * m of the 8 tokens (g, j) of each 32.
@@ -246,55 +69,6 @@ struct Unit {
   }
 };
 
-__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// A reduction over the four lanes that share a row.
-template <typename F>
-__device__ __forceinline__ float over_g(float x, F f) {
-  x = f(x, __shfl_xor(x, 16));
-  return f(x, __shfl_xor(x, 32));
-}
-
-__device__ __forceinline__ float fmax2(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ float fmin2(float a, float b) { return fminf(a, b); }
-
-// Sums are taken against the whole number at or above a row's running maximum, so that going over to
-// another reference is an exact power of two.  The factor of sums against the maximum a, now against b:
-// 1 where nothing changed, also while nothing was seen (both -inf).
-__device__ __forceinline__ float rebase(float a, float b) {
-  return a == b ? 1.f : __builtin_ldexpf(1.f, (int)(__builtin_ceilf(a) - __builtin_ceilf(b)));
-}
-__device__ __forceinline__ float reference(float m) { return fabsf(m) == INFINITY ? 0.f : __builtin_ceilf(m); }
-// log2 of a row's sum, against its reference.
-__device__ __forceinline__ float log2_sum(float m, float l) {
-  return fabsf(m) == INFINITY ? m + l : __builtin_ceilf(m) + (__builtin_amdgcn_logf(l) - kLift);
-}
-
-// Packs the upper halves of two numbers.
-__device__ __forceinline__ uint32_t heads_of(float a, float b) {
-  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-}
-__device__ __forceinline__ float rest_of(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
-
-// A row's results from its sums: maximum m in units of log 2, sum l, `N` values from dim d0.
-template <typename T, int N, bool RANGE>
-__device__ __forceinline__ void store_row(const AttendArgs& A, long long at, int dim, int d0, float m, float l, float low,
-                                          const float* o) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  typedef T vec __attribute__((ext_vector_type(N)));
-  vec x;
-#pragma unroll
-  for (int c = 0; c < N; ++c) x[c] = (T)(o[c] * inv);
-  *reinterpret_cast<vec*>((T*)A.out + at * dim + d0) = x;
-  if (d0 == 0) {
-    const bool bad = l != l;
-    A.lse[at] = log2_sum(m, l) * kLn2;
-    if constexpr (RANGE) A.low[at] = bad ? l : low * kLn2, A.high[at] = bad ? l : m * kLn2;
-  }
-}
-
 // A lane's neighbours 4 and 8 on, of the 16 that share g.
 template <int N>
 __device__ __forceinline__ float turn(float x) {
@@ -307,9 +81,6 @@ __device__ __forceinline__ float over_row(float x, F f) {
   return over_g(x, f);
 }
 
-// Waves of k_attend on a SIMD, which the registers of its dims and query parts set.
-constexpr int waves_of(int dim, bool half) { return dim == 64 ? 4 : half ? 2 : 3; }
-
 // R rows of one key head, a part of their tokens; the waves take units in turn.
 //
 // With R < 16 the product's 16 columns hold the rows 16 / R times.  Each copy keeps the scores of its own
@@ -319,7 +90,7 @@ constexpr int waves_of(int dim, bool half) { return dim == 64 ? 4 : half ? 2 : 3
 // Keys of the next unit are loaded as soon as the first product is done with this one's, its values after the
 // second, so that loads are in flight throughout without registers of their own.
 template <typename T, int D, bool RANGE, int R>
-__global__ __launch_bounds__(64 * kWaves, waves_of(D, __is_same(T, _Float16))) void k_attend(AttendArgs A) {
+__global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16))) void k_attend(AttendArgs A) {
   using L = Kv4<D>;
   constexpr int kTiles = R / 4;  // 16-token tiles of a lane's scores
   constexpr int kSteps = D / 32, kDpl = L::kDpl;
@@ -349,17 +120,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(D, __is_same(T, _Float16))) v
   for (int s = 0; s < kSteps; ++s) {
     u32x4 raw = {0, 0, 0, 0};
     if (live) raw = reinterpret_cast<const Loose16*>(qp + 8 * s)->v;
-    if constexpr (kHalf) {
-      typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-      const f16x8 x = __builtin_bit_cast(f16x8, raw);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        qh[s][k] = (__bf16)(float)x[k];
-        ql[s][k] = (__bf16)((float)x[k] - (float)qh[s][k]);
-      }
-    } else {
-      qh[s] = __builtin_bit_cast(bf16x8, raw);
-    }
+    query_parts<T>(raw, qh[s], ql[s]);
   }
 
   f32x4 acc[kDpl];
@@ -613,37 +374,25 @@ __global__ __launch_bounds__(64 * kWaves) void k_join(AttendArgs A) {
   }
 }
 
-// How a call is run, from what the host knows of it.
-struct Way {
-  bool few, join;
-  int rows, least;
-  int64_t tiles, slots, pairs, items;
-  Way(int64_t seqs, int heads, int group, int dim, bool half, int most, int cols) {
-    const int64_t all = (int64_t)most * group, units = std::max<int64_t>(1, (int64_t)cols * (kPageTokens / kUnit));
-    few = true;
-    const int size = few ? kFew : kMany;
-    tiles = (all + size - 1) / size;
-    rows = (int)std::min<int64_t>(all, size);
-    least = few ? 4 * kWaves : 8;
-    slots = kComputeUnits * (few ? waves_of(dim, half) : 2);
-    pairs = seqs * tiles;
-    join = pairs <= 64 * kPairs && units > least;
-    items = !join ? pairs * heads : std::min(pairs * ((units + least - 1) / least), pairs + (slots + heads - 1) / heads) * heads;
-  }
-  size_t bytes(int heads, int dim) const {
-    return join ? (size_t)items * rows * (4 + dim) * sizeof(float) + (size_t)pairs * heads * 2 * sizeof(int) : 0;
-  }
-};
 
 template <typename T, int D, bool RANGE>
 int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
+  const dim3 grid((unsigned)W.items);
   const size_t lds = kWaves * W.rows * (D + 4) * sizeof(float);
-  if (W.rows <= 4) k_attend<T, D, RANGE, 4><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
-  else if (W.rows <= 8) k_attend<T, D, RANGE, 8><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
-  else k_attend<T, D, RANGE, 16><<<dim3((unsigned)W.items), 64 * kWaves, lds, s>>>(A);
+  if (!W.few) {
+    if (const int err = launch_prompt(A, W, D, __is_same(T, _Float16) ? HCK_F16 : HCK_BF16, s)) return err;
+  } else if (W.rows <= 4) {
+    k_attend<T, D, RANGE, 4><<<grid, 64 * kWaves, lds, s>>>(A);
+  } else if (W.rows <= 8) {
+    k_attend<T, D, RANGE, 8><<<grid, 64 * kWaves, lds, s>>>(A);
+  } else {
+    k_attend<T, D, RANGE, 16><<<grid, 64 * kWaves, lds, s>>>(A);
+  }
   HCK_CHECK_LAUNCH();
   if (W.join) {
-    k_join<T, D, RANGE, true><<<dim3((unsigned)(W.pairs * A.heads), W.rows), 64 * kWaves, 0, s>>>(A);
+    const unsigned pairs = (unsigned)(W.pairs * A.heads);
+    if (W.few) k_join<T, D, RANGE, true><<<dim3(pairs, W.rows), 64 * kWaves, 0, s>>>(A);
+    else k_join<T, D, RANGE, false><<<dim3(pairs, (W.rows + 31) / 32), 64 * kWaves, 0, s>>>(A);
     HCK_CHECK_LAUNCH();
   }
   return HCK_OK;
