@@ -100,9 +100,10 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
 
   Item it;
   if (!locate(A, kFew, blockIdx.x, it)) return;
+  it.uniform();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const int copy = m / R, tile = it.tile, h = it.h, b = it.b;
-  const Rows S(A, b);
+  const Rows S = Rows(A, b).uniform();
   const long long q0 = S.q0;
   const int rows = S.rows;
   if (tile * kFew >= rows) return;
@@ -135,14 +136,14 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   int u = u0 + wave, pg = 0, next = 0;
   Unit<D> x;
   if (u < u1) {
-    pg = table[u >> 1];
+    pg = __builtin_amdgcn_readfirstlane(table[u >> 1]);
     x.load_keys(page_of(pg), u & 1, m, g);
     x.load_values(page_of(pg), u & 1, m, g);
     if (u + kWaves < u1) next = table[(u + kWaves) >> 1];
   }
   for (; u < u1; u += kWaves) {
     const bool there = pg >= 0 && pg < A.pages, more = u + kWaves < u1;
-    pg = next;
+    pg = __builtin_amdgcn_readfirstlane(next);
     if (u + 2 * kWaves < u1) next = table[(u + 2 * kWaves) >> 1];
     const uint8_t* page = page_of(pg);
     if (!there) {
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
     }
     if (more) x.load_keys(page, u & 1, m, g);
     const int base = u * kUnit + 4 * g, own = base + 16 * kTiles * copy;
-    if (u * kUnit + kUnit > all) {
+    if (__builtin_amdgcn_readfirstlane(u * kUnit) + kUnit > all) {
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
 #pragma unroll
@@ -180,13 +181,13 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) low = fminf(low, t[i][k]);
+        for (int k = 0; k < 4; ++k) low = smaller(low, t[i][k]);
     }
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[i][k]);
+      for (int k = 0; k < 4; ++k) mx = larger(mx, t[i][k]);
     mx = fmaxf(top, over_row<R>(mx, fmax2) * scale2);
     const float f = rebase(top, mx);
     top = mx;
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
         sum += t[i][k];
       }
       hi[i] = u32x2{heads_of(t[i][0], t[i][1]), heads_of(t[i][2], t[i][3])};
-      lo[i] = u32x2{pack(rest_of(t[i][0]), rest_of(t[i][1])), pack(rest_of(t[i][2]), rest_of(t[i][3]))};
+      lo[i] = u32x2{rests_of(t[i][0], t[i][1], hi[i][0]), rests_of(t[i][2], t[i][3], hi[i][1])};
     }
 
 #pragma unroll
@@ -263,6 +264,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
     if (more) x.load_values(page, u & 1, m, g);
   }
 
+  publish(A, it);
   // join the waves: lane (m, g) holds dims D / 4 g + kDpl i + d of row m in acc[d][i]
   sum = over_row<R>(sum, [](float a, float c) { return a + c; });
   if constexpr (RANGE) low = over_row<R>(low, fmin2) * scale2;

@@ -60,6 +60,16 @@ struct Rows {
     rows = (int)min((long long)nq * A.group, (long long)A.tiles * (A.rows > kFew ? kMany : kFew));
     length = (int)min((long long)max(A.lengths[b], 0), (long long)A.cols * kPageTokens);
   }
+  // the same for all lanes, where b is
+  __device__ __forceinline__ Rows uniform() const {
+    Rows r = *this;
+    r.q0 = (long long)(((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(q0 >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)q0));
+    r.nq = __builtin_amdgcn_readfirstlane(nq);
+    r.rows = __builtin_amdgcn_readfirstlane(rows);
+    r.length = __builtin_amdgcn_readfirstlane(length);
+    return r;
+  }
   // tokens that row r sees
   __device__ __forceinline__ int seen(const AttendArgs& A, int r) const {
     return A.causal ? max(0, min(length, length - nq + r / A.group + 1)) : length;
@@ -69,6 +79,12 @@ struct Rows {
 // A workgroup's work: a tile of rows, a key head, and a part of the units of 64 tokens that they see.
 struct Item {
   int b, tile, h, u0, u1, slot, slots;
+  // into scalar registers
+  __device__ __forceinline__ void uniform() {
+    b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile), h = __builtin_amdgcn_readfirstlane(h);
+    u0 = __builtin_amdgcn_readfirstlane(u0), u1 = __builtin_amdgcn_readfirstlane(u1);
+    slot = __builtin_amdgcn_readfirstlane(slot), slots = __builtin_amdgcn_readfirstlane(slots);
+  }
 };
 
 // The units of a tile's rows, -1: no rows.
@@ -87,7 +103,14 @@ __device__ __forceinline__ long long over_wave(long long x) {
 __device__ __forceinline__ int over_wave(int x) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-  return x;
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// Where the join finds the slots of a tile and head, from the workgroup that has their first.
+__device__ __forceinline__ void publish(const AttendArgs& A, const Item& it) {
+  if (!A.join || it.u0 != 0 || threadIdx.x != 0) return;
+  int* to = A.plan + 2 * ((long long)(it.b * A.tiles + it.tile) * A.heads + it.h);
+  to[0] = it.slot, to[1] = it.slots;
 }
 
 constexpr int kPairs = 8;  // tiles of rows that a lane looks through to share the work out
@@ -116,7 +139,7 @@ __device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Ite
     total += max(n[j], 0);
   }
   total = over_wave(total) * A.heads;
-  const int base = (int)min(1ll << 26, max((long long)A.least, (total + A.slots - 1) / A.slots));
+  const int base = __builtin_amdgcn_readfirstlane((int)min(1ll << 26, max((long long)A.least, (total + A.slots - 1) / A.slots)));
   int share = 0, mine = 0;
 #pragma unroll
   for (int f = 4; f <= 8; ++f) {
@@ -151,10 +174,6 @@ __device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Ite
   it.slots = __builtin_amdgcn_readlane(count, owner);
   it.u1 = it.u0 + share;
   it.b = pair / A.tiles, it.tile = pair % A.tiles;
-  if (it.u0 == 0 && threadIdx.x == 0) {
-    A.plan[2 * (pair * A.heads + it.h)] = w;
-    A.plan[2 * (pair * A.heads + it.h) + 1] = it.slots;
-  }
   return true;
 }
 
@@ -213,6 +232,10 @@ __device__ __forceinline__ float over_g(float x, F f) {
 
 __device__ __forceinline__ float fmax2(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float fmin2(float a, float b) { return fminf(a, b); }
+// The larger and the smaller of two in one instruction (fmaxf of a matrix product's result takes another to make
+// a number of it first).  Of a NaN and b: b, and -inf, which a row with a NaN never shows.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+__device__ __forceinline__ float smaller(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, -INFINITY); }
 
 // Sums are taken against the whole number at or above a row's running maximum, so that going over to
 // another reference is an exact power of two.  The factor of sums against the maximum a, now against b:
@@ -230,7 +253,16 @@ __device__ __forceinline__ float log2_sum(float m, float l) {
 __device__ __forceinline__ uint32_t heads_of(float a, float b) {
   return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
-__device__ __forceinline__ float rest_of(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
+// What they leave: a0 - h0 and a1 - h1 for h of two such halves, each in one instruction (times 1 and 0: exact).
+// The factors (-1, 0) and (0, -1) come out of registers: as constants the compiler makes them one inline -1.0.
+__device__ __forceinline__ uint32_t rests_of(float a0, float a1, uint32_t h) {
+  uint32_t low, high;
+  asm("s_mov_b32 %0, 0x0000bf80" : "=s"(low));
+  asm("s_mov_b32 %0, 0xbf800000" : "=s"(high));
+  const bf16x2 x = __builtin_bit_cast(bf16x2, h);
+  return pack(__builtin_amdgcn_fdot2_f32_bf16(x, __builtin_bit_cast(bf16x2, low), a0, false),
+              __builtin_amdgcn_fdot2_f32_bf16(x, __builtin_bit_cast(bf16x2, high), a1, false));
+}
 
 // A row's results from its sums: maximum m in units of log 2, sum l, `N` values from dim d0.
 template <typename T, int N, bool RANGE>

@@ -83,9 +83,10 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
 
   Item it;
   if (!locate(A, kMany, blockIdx.x, it)) return;
+  it.uniform();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const int h = it.h;
-  const Rows S(A, it.b);
+  const Rows S = Rows(A, it.b).uniform();
   const int rows = S.rows, first = it.tile * kMany;
   if (first >= rows) return;
   const int most = S.seen(A, min(first + kMany, rows) - 1);
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
   int pg = 0, next = 0;
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   if (u0 < u1) {
-    pg = table[u0 >> 1];
+    pg = __builtin_amdgcn_readfirstlane(table[u0 >> 1]);
     x.load(page_of(pg), u0 & 1, wave, lane);
     if (u0 + 1 < u1) next = table[(u0 + 1) >> 1];
   }
@@ -138,11 +139,13 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
     if (store(o, x, wave, lane)) s_odd[u & 1] = u + 1;
     const bool there = pg >= 0 && pg < A.pages;
     const uint8_t* page = page_of(pg);
-    pg = next;
+    pg = __builtin_amdgcn_readfirstlane(next);
     if (u + 1 < u1) x.load(page_of(pg), (u + 1) & 1, wave, lane);
     if (u + 2 < u1) next = table[(u + 2) >> 1];
     __syncthreads();
-    if (!there || u * kUnit >= last) continue;
+    const int here = __builtin_amdgcn_readfirstlane(u * kUnit);
+    if (!there || here >= last) continue;
+    const bool full = here + kUnit <= least;  // every row sees every token
 
     f32x4 t[kTiles][4];
 #pragma unroll
@@ -160,7 +163,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
     u32x2 hi[kTiles][4], lo[kTiles][4];  // the probabilities in two bf16 parts
 #pragma unroll
     for (int r = 0; r < kTiles; ++r) {
-      if (u * kUnit + kUnit > least) {
+      if (!full) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -173,13 +176,13 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) low[r] = fminf(low[r], t[r][i][k]);
+          for (int k = 0; k < 4; ++k) low[r] = smaller(low[r], t[r][i][k]);
       }
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[r][i][k]);
+        for (int k = 0; k < 4; ++k) mx = larger(mx, t[r][i][k]);
       mx = fmaxf(top[r], over_g(mx, fmax2) * scale2);
       const float f = rebase(top[r], mx);
       top[r] = mx;
@@ -196,7 +199,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
         for (int k = 0; k < 4; ++k) t[r][i][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[r][i][k], scale2, -ref));
         part[i] = (t[r][i][0] + t[r][i][1]) + (t[r][i][2] + t[r][i][3]);
         hi[r][i] = u32x2{heads_of(t[r][i][0], t[r][i][1]), heads_of(t[r][i][2], t[r][i][3])};
-        lo[r][i] = u32x2{pack(rest_of(t[r][i][0]), rest_of(t[r][i][1])), pack(rest_of(t[r][i][2]), rest_of(t[r][i][3]))};
+        lo[r][i] = u32x2{rests_of(t[r][i][0], t[r][i][1], hi[r][i][0]), rests_of(t[r][i][2], t[r][i][3], hi[r][i][1])};
       }
       sum[r] += (part[0] + part[1]) + (part[2] + part[3]);
     }
@@ -238,6 +241,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
       }
   }
 
+  publish(A, it);
   // lane (m, g) holds dims D / 4 g + kDpl i + d of row m in acc[d][i]
 #pragma unroll
   for (int r = 0; r < kTiles; ++r) {
