@@ -152,20 +152,26 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
     }
 
     float t[kTiles][4];
+    f32x4 c[4];
+    float sc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f32x4 c = {0.f, 0.f, 0.f, 0.f};
       const uint32_t byte = (x.ks >> (8 * i)) & 0xffu;
-      const float sc = __uint_as_float(byte << 23);
+      sc[i] = byte == kNanByte ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+      c[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const bf16x8 kk = x.key(i, s, byte == kNanByte ? __uint_as_float(0x7fc00000u) : sc);
-        c = mfma(kk, qh[s], c);
-        if constexpr (kHalf) c = mfma(kk, ql[s], c);
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bf16x8 kk = x.key(i, s, sc[i]);
+        c[i] = mfma(kk, qh[s], c[i]);
+        if constexpr (kHalf) c[i] = mfma(kk, ql[s], c[i]);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t[i % kTiles][k] = i < kTiles || copy == i / kTiles ? c[k] : t[i % kTiles][k];
-    }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[i % kTiles][k] = i < kTiles || copy == i / kTiles ? c[i][k] : t[i % kTiles][k];
     if (more) x.load_keys(page, u & 1, m, g);
     const int base = u * kUnit + 4 * g, own = base + 16 * kTiles * copy;
     if (__builtin_amdgcn_readfirstlane(u * kUnit) + kUnit > all) {
@@ -250,8 +256,8 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
         constexpr int kB = decltype(B)::value;
         x.template value<kB>(i, sc, e, o);
         acc[2 * kB] = mfma(e, ph, acc[2 * kB]);
-        acc[2 * kB] = mfma(e, pl, acc[2 * kB]);
         acc[2 * kB + 1] = mfma(o, ph, acc[2 * kB + 1]);
+        acc[2 * kB] = mfma(e, pl, acc[2 * kB]);
         acc[2 * kB + 1] = mfma(o, pl, acc[2 * kB + 1]);
       };
       step(std::integral_constant<int, 0>());

@@ -223,11 +223,19 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// A reduction over the four lanes that share a row.
+// Reductions over the two and the four lanes that share a row: each swap leaves one operand's halves (of 32
+// lanes, of 16) side by side with the other's.
+template <typename F>
+__device__ __forceinline__ float over_half(float x, F f) {
+  const uint32_t a = __float_as_uint(x);
+  const auto p = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
 template <typename F>
 __device__ __forceinline__ float over_g(float x, F f) {
-  x = f(x, __shfl_xor(x, 16));
-  return f(x, __shfl_xor(x, 32));
+  const uint32_t a = __float_as_uint(x);
+  const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  return over_half(f(__uint_as_float(p[0]), __uint_as_float(p[1])), f);
 }
 
 __device__ __forceinline__ float fmax2(float a, float b) { return fmaxf(a, b); }

@@ -1,10 +1,11 @@
 // Attention of many rows over 4-bit pages: the mathematics of kv4_attend.hip, with 128 rows to a workgroup.
 //
-// Per 64 tokens and 16 rows the products take 48 matrix instructions of 16 cycles (D = 128: 16 for the scores,
-// 32 for the two parts of the probabilities) and the softmax some 150 vector instructions of 4; making operands
-// of the codes would take 190 more.  So it is done once for 128 rows: the four waves each make a quarter of 64
-// tokens' operands, in the lanes' order, in LDS (keys and values 32 KB, twice, so that one barrier a unit is
-// enough), and each takes all of them for its own 32 rows.  Codes of the next unit are in flight meanwhile.
+// Here a tile is 32 by 32: a lane has one row's scores of half of 64 tokens, and a matrix instruction keeps the
+// vector unit from issuing for 8 cycles of its 32, where two of 16 by 16 do for 20 (measured), which counts where
+// both are busy.  Making operands of the codes takes some 190 vector instructions per 64 tokens, as many as the
+// softmax of 32 rows; so it is done once for 128 rows: the four waves each make a quarter of them, in the lanes'
+// order, in LDS (keys and values 32 KB, twice, so that one barrier a unit is enough), and each takes all of them
+// for its own 32 rows.  Codes of the next unit are in flight meanwhile.
 #include "kv4_attend.hpp"
 
 namespace hck {
@@ -28,19 +29,28 @@ struct Share {
   }
 };
 
+// The left operands of 64 tokens.  Keys: lane (token % 32, h) of step s has dims 8 of the D / 4 that follow
+// (2 (s / (D / 32)) + h) D / 4.  Values: lane (i, h) of tile d has dim i / 2 kDpl + 2 d + i % 2 of the tokens
+// 16 j + 4 h + 0..3 and 8 on, whose scores a lane with that h holds.
 template <int D>
 struct Operands {
-  u32x4 k[4][D / 32][64];            // [16-token tile][step][lane]
-  u32x2 v[2][Kv4<D>::kDpl][64][2];   // [32-token block][dim of the lane][lane][4 tokens]
+  u32x4 k[2][D / 16][64];       // [32-token tile][step][lane]
+  u32x2 v[4][D / 32][64][2];    // [16 tokens][32-dim tile][lane][4 tokens]
 };
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
 
 // Writes the thread's share; whether it holds a run of NaN among the values, which are taken as zeros.
 template <int D>
 __device__ __forceinline__ bool store(Operands<D>& o, const Share<D>& x, int wave, int lane) {
   const float sc = x.ks == kNanByte ? __uint_as_float(0x7fc00000u) : __uint_as_float(x.ks << 23);
+  const int m = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int s = 0; s < D / 32; ++s)
-    o.k[wave][s][lane] = u32x4{cvt<0>(x.k[s], sc), cvt<1>(x.k[s], sc), cvt<2>(x.k[s], sc), cvt<3>(x.k[s], sc)};
+    o.k[wave >> 1][(g >> 1) * (D / 32) + s][(g & 1) * 32 + (wave & 1) * 16 + m] = u32x4{cvt<0>(x.k[s], sc), cvt<1>(x.k[s], sc), cvt<2>(x.k[s], sc), cvt<3>(x.k[s], sc)};
   uint32_t vs = x.vs;
   const bool odd = has_nan(vs);
   if (odd) {
@@ -59,9 +69,10 @@ __device__ __forceinline__ bool store(Operands<D>& o, const Share<D>& x, int wav
       if constexpr (D == 128) y[j] = cvt<b>(x.v[j], f[j]);
       else y[j] = (j & 1) ? cvt<(b & 1) + 2>(x.v[j / 2], f[j]) : cvt<(b & 1)>(x.v[j / 2], f[j]);
     }
-    o.v[wave >> 1][2 * b][lane][wave & 1] =
+    u32x2(*to)[2] = &o.v[wave][b][(g & 1) * 32 + 2 * m];
+    to[0][g >> 1] =
         u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x05040100u), __builtin_amdgcn_perm(y[3], y[2], 0x05040100u)};
-    o.v[wave >> 1][2 * b + 1][lane][wave & 1] =
+    to[1][g >> 1] =
         u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x07060302u), __builtin_amdgcn_perm(y[3], y[2], 0x07060302u)};
   };
   pair(std::integral_constant<int, 0>());
@@ -76,55 +87,47 @@ __device__ __forceinline__ bool store(Operands<D>& o, const Share<D>& x, int wav
 template <typename T, int D, bool RANGE>
 __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(AttendArgs A) {
   using L = Kv4<D>;
-  constexpr int kSteps = D / 32, kDpl = L::kDpl, kTiles = kMany / (16 * kWaves);  // 16-row tiles of a wave
+  constexpr int kSteps = D / 16, kTiles = D / 32, kDpl = L::kDpl;
   constexpr bool kHalf = __is_same(T, _Float16);
+  static_assert(kMany == 32 * kWaves, "32 rows a wave");
   __shared__ Operands<D> s_x[2];
   __shared__ int s_odd[2];  // 1 + the unit whose values hold a run of NaN
 
   Item it;
   if (!locate(A, kMany, blockIdx.x, it)) return;
   it.uniform();
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
-  const int h = it.h;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const Rows S = Rows(A, it.b).uniform();
   const int rows = S.rows, first = it.tile * kMany;
   if (first >= rows) return;
   const int most = S.seen(A, min(first + kMany, rows) - 1);
   const int u0 = it.u0, u1 = min((most + kUnit - 1) / kUnit, it.u1);
-  const int mine = first + 16 * kTiles * wave;  // the wave's rows
-  const int least = mine < rows ? S.seen(A, mine) : 0, last = mine < rows ? S.seen(A, min(mine + 16 * kTiles, rows) - 1) : 0;
+  const int mine = first + 32 * wave;  // the wave's rows
+  const int least = mine < rows ? S.seen(A, mine) : 0, last = mine < rows ? S.seen(A, min(mine + 32, rows) - 1) : 0;
+  const int row = mine + (lane & 31);
+  const bool live = row < rows;
+  const int qi = live ? row / A.group : 0, qo = live ? row % A.group : 0;
+  const int seen = live ? S.seen(A, row) : 0;
 
-  // the lane's part of its rows' queries: dims D / 4 g + 8 s .. + 7 of step s
-  bf16x8 qh[kTiles][kSteps], ql[kTiles][kSteps];
-  int seen[kTiles];
+  bf16x8 qh[kSteps], ql[kSteps];
+  const T* qp = (const T*)A.q + (S.q0 + qi) * A.q_ts + (long long)(it.h * A.group + qo) * A.q_hs + h * (D / 4);
 #pragma unroll
-  for (int r = 0; r < kTiles; ++r) {
-    const int row = mine + 16 * r + m;
-    const bool live = row < rows;
-    const int qi = live ? row / A.group : 0, qo = live ? row % A.group : 0;
-    seen[r] = live ? S.seen(A, row) : 0;
-    const T* qp = (const T*)A.q + (S.q0 + qi) * A.q_ts + (long long)(h * A.group + qo) * A.q_hs + g * (D / 4);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      u32x4 raw = {0, 0, 0, 0};
-      if (live) raw = reinterpret_cast<const Loose16*>(qp + 8 * s)->v;
-      query_parts<T>(raw, qh[r][s], ql[r][s]);
-    }
+  for (int s = 0; s < kSteps; ++s) {
+    u32x4 raw = {0, 0, 0, 0};
+    if (live) raw = reinterpret_cast<const Loose16*>(qp + s / (D / 32) * (D / 2) + s % (D / 32) * 8)->v;
+    query_parts<T>(raw, qh[s], ql[s]);
   }
 
-  f32x4 acc[kTiles][kDpl];
-  float top[kTiles], sum[kTiles], low[kTiles];
+  f32x16 acc[kTiles];
 #pragma unroll
-  for (int r = 0; r < kTiles; ++r) {
-    top[r] = -INFINITY, sum[r] = 0.f, low[r] = INFINITY;
+  for (int d = 0; d < kTiles; ++d)
 #pragma unroll
-    for (int d = 0; d < kDpl; ++d) acc[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  float top = -INFINITY, sum = 0.f, low = INFINITY;
   const float scale2 = A.scale * kLog2e;
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
   const int* table = A.table + it.b * A.table_stride;
-  auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + h) * L::kBytes; };
+  auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + it.h) * L::kBytes; };
   Share<D> x;
   int pg = 0, next = 0;
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
@@ -145,128 +148,123 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
     __syncthreads();
     const int here = __builtin_amdgcn_readfirstlane(u * kUnit);
     if (!there || here >= last) continue;
-    const bool full = here + kUnit <= least;  // every row sees every token
 
-    f32x4 t[kTiles][4];
+    f32x16 t[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[0][i] = t[1][i] = 0.f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bf16x8 kk = __builtin_bit_cast(bf16x8, o.k[i][s][lane]);
+      for (int n = 0; n < 2; ++n) {
+        const bf16x8 kk = __builtin_bit_cast(bf16x8, o.k[n][s][lane]);
+        t[n] = mfma32(kk, qh[s], t[n]);
+        if constexpr (kHalf) t[n] = mfma32(kk, ql[s], t[n]);
+      }
+    const int base = here + 4 * h;  // of the lane's tokens base + 32 n + 8 (i / 4) + i % 4
+    if (here + kUnit > least) {
 #pragma unroll
-        for (int r = 0; r < kTiles; ++r) {
-          t[r][i] = mfma(kk, qh[r][s], s == 0 ? zero : t[r][i]);
-          if constexpr (kHalf) t[r][i] = mfma(kk, ql[r][s], t[r][i]);
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool see = base + 32 * n + 8 * (i >> 2) + (i & 3) < seen;
+          if constexpr (RANGE) low = see ? fminf(low, t[n][i]) : low;
+          t[n][i] = see ? t[n][i] : -INFINITY;
         }
-      }
-    const int base = u * kUnit + 4 * g;
-    u32x2 hi[kTiles][4], lo[kTiles][4];  // the probabilities in two bf16 parts
+    } else if constexpr (RANGE) {
 #pragma unroll
-    for (int r = 0; r < kTiles; ++r) {
-      if (!full) {
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 16; ++i) low = smaller(low, t[n][i]);
+    }
+    float mx = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bool see = base + 16 * i + k < seen[r];
-            if constexpr (RANGE) low[r] = see ? fminf(low[r], t[r][i][k]) : low[r];
-            t[r][i][k] = see ? t[r][i][k] : -INFINITY;
-          }
-      } else if constexpr (RANGE) {
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 16; ++i) mx = larger(mx, t[n][i]);
+    mx = fmaxf(top, over_half(mx, fmax2) * scale2);
+    const float f = rebase(top, mx);
+    top = mx;
+    const float ref = reference(mx) - kLift;
+    if (__any(f != 1.f)) {
+      sum *= f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) low[r] = smaller(low[r], t[r][i][k]);
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mx = larger(mx, t[r][i][k]);
-      mx = fmaxf(top[r], over_g(mx, fmax2) * scale2);
-      const float f = rebase(top[r], mx);
-      top[r] = mx;
-      const float ref = reference(mx) - kLift;
-      if (__any(f != 1.f)) {
-        sum[r] *= f;
-#pragma unroll
-        for (int d = 0; d < kDpl; ++d) acc[r][d] *= f;
-      }
-      float part[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) t[r][i][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[r][i][k], scale2, -ref));
-        part[i] = (t[r][i][0] + t[r][i][1]) + (t[r][i][2] + t[r][i][3]);
-        hi[r][i] = u32x2{heads_of(t[r][i][0], t[r][i][1]), heads_of(t[r][i][2], t[r][i][3])};
-        lo[r][i] = u32x2{rests_of(t[r][i][0], t[r][i][1], hi[r][i][0]), rests_of(t[r][i][2], t[r][i][3], hi[r][i][1])};
-      }
-      sum[r] += (part[0] + part[1]) + (part[2] + part[3]);
+      for (int d = 0; d < kTiles; ++d) acc[d] *= f;
     }
 
     if (s_odd[u & 1] == u + 1) {
       // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  Its values are
       // zeros here, and it is counted for the rows that see it by a product of truth values.
 #pragma unroll 1
-      for (int i = 0; i < 2; ++i) {
-        const u32x2 vs = *reinterpret_cast<const u32x2*>(page + L::kVScales + (2 * (u & 1) + i) * (32 * L::kRuns) +
-                                                         (g * L::kRuns + m * L::kDpl / kRun) * 8);
-        bf16x8 bad;
+      for (int j = 0; j < 4; ++j) {
+        bf16x8 bad, see;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) bad[k] = (__bf16)(((vs[k >> 2] >> (8 * (k & 3))) & 0xffu) == kNanByte ? 1.f : 0.f);
+        for (int p = 0; p < 2; ++p) {
+          const uint32_t vs = *reinterpret_cast<const uint32_t*>(
+              page + L::kVScales + (2 * (u & 1) + (j >> 1)) * (32 * L::kRuns) +
+              ((2 * p + h) * L::kRuns + (lane & 31) / 2 * kDpl / kRun) * 8 + 4 * (j & 1));
 #pragma unroll
-        for (int r = 0; r < kTiles; ++r) {
-          bf16x8 see;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) see[k] = (__bf16)(base + 32 * i + 16 * (k >> 2) + (k & 3) < seen[r] ? 1.f : 0.f);
-          const f32x4 n = mfma(bad, see, zero);
-#pragma unroll
-          for (int d = 0; d < kDpl; ++d)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (n[k] > 0.f) acc[r][d][k] = __uint_as_float(0x7fc00000u);
+          for (int k = 0; k < 4; ++k) {
+            bad[4 * p + k] = (__bf16)(((vs >> (8 * k)) & 0xffu) == kNanByte ? 1.f : 0.f);
+            see[4 * p + k] = (__bf16)(base + 16 * j + 8 * p + k < seen ? 1.f : 0.f);
+          }
         }
+        f32x16 n;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) n[i] = 0.f;
+        n = mfma32(bad, see, n);
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (n[i] > 0.f) acc[d][i] = __uint_as_float(0x7fc00000u);
       }
     }
+
+    float part[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 4; ++j) {
+      float p[8];
+      uint32_t hi[4], lo[4];  // the probabilities in two bf16 parts
 #pragma unroll
-      for (int d = 0; d < kDpl; ++d) {
-        const bf16x8 vv = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(o.v[i][d][lane]));
+      for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[j >> 1][8 * (j & 1) + e], scale2, -ref));
 #pragma unroll
-        for (int r = 0; r < kTiles; ++r) {
-          acc[r][d] = mfma(vv, operand(hi[r][2 * i][0], hi[r][2 * i][1], hi[r][2 * i + 1][0], hi[r][2 * i + 1][1]), acc[r][d]);
-          acc[r][d] = mfma(vv, operand(lo[r][2 * i][0], lo[r][2 * i][1], lo[r][2 * i + 1][0], lo[r][2 * i + 1][1]), acc[r][d]);
-        }
+      for (int e = 0; e < 4; ++e) {
+        hi[e] = heads_of(p[2 * e], p[2 * e + 1]);
+        lo[e] = rests_of(p[2 * e], p[2 * e + 1], hi[e]);
+        part[e & 1] += p[2 * e] + p[2 * e + 1];
       }
+      const bf16x8 ph = operand(hi[0], hi[1], hi[2], hi[3]), pl = operand(lo[0], lo[1], lo[2], lo[3]);
+      bf16x8 vv[kTiles];
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) vv[d] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(o.v[j][d][lane]));
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(vv[d], ph, acc[d]);
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(vv[d], pl, acc[d]);
+    }
+    sum += part[0] + part[1];
   }
 
   publish(A, it);
-  // lane (m, g) holds dims D / 4 g + kDpl i + d of row m in acc[d][i]
+  sum = over_half(sum, [](float a, float c) { return a + c; });
+  if constexpr (RANGE) low = over_half(low, fmin2) * scale2;
+  if (row >= rows || row - first >= A.rows) return;
+  const int qr = row / A.group, qc = row % A.group;
+  const long long out = (S.q0 + qr) * (long long)(A.heads * A.group) + it.h * A.group + qc;
+  const long long at = (long long)it.slot * A.rows + (row - first);
+  if (it.slots > 1 && h == 0) *reinterpret_cast<f32x4*>(A.stat + at * 4) = f32x4{top, sum, low, 0.f};
+  // registers 4 q + 2 p + b of tile d: dim (2 h + 4 q + p) kDpl + 2 d + b of the lane's row
 #pragma unroll
-  for (int r = 0; r < kTiles; ++r) {
-    sum[r] = over_g(sum[r], [](float a, float c) { return a + c; });
-    if constexpr (RANGE) low[r] = over_g(low[r], fmin2) * scale2;
-    const int row = mine + 16 * r + m;
-    if (row >= rows || row - first >= A.rows) continue;
+  for (int i = 0; i < 8; ++i) {
+    const int d0 = (2 * h + 4 * (i >> 1) + (i & 1)) * kDpl;
+    float v[kDpl];
+#pragma unroll
+    for (int d = 0; d < kDpl; ++d) v[d] = acc[d >> 1][2 * i + (d & 1)];
     if (it.slots > 1) {
-      const long long at = (long long)it.slot * A.rows + (row - first);
-      if (g == 0) *reinterpret_cast<f32x4*>(A.stat + at * 4) = f32x4{top[r], sum[r], low[r], 0.f};
-      float* to = A.sums + at * D + g * (D / 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int d = 0; d < kDpl; d += 4)
-          *reinterpret_cast<f32x4*>(to + kDpl * i + d) = f32x4{acc[r][d][i], acc[r][d + 1][i], acc[r][d + 2][i], acc[r][d + 3][i]};
+      for (int d = 0; d < kDpl; d += 4) *reinterpret_cast<f32x4*>(A.sums + at * D + d0 + d) = f32x4{v[d], v[d + 1], v[d + 2], v[d + 3]};
     } else {
-      float v[D / 4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int d = 0; d < kDpl; ++d) v[kDpl * i + d] = acc[r][d][i];
-      const int qr = row / A.group, qc = row % A.group;
-      store_row<T, D / 4, RANGE>(A, (S.q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, g * (D / 4), top[r],
-                                 sum[r], low[r], v);
+      store_row<T, kDpl, RANGE>(A, out, D, d0, top, sum, low, v);
     }
   }
 }
