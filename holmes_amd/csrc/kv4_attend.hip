@@ -317,71 +317,108 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   store_row<T, kCols, RANGE>(A, (q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, c0, mm, ll, lo, o);
 }
 
-// Joins the slots of a row, where it has more than one.  One workgroup a row of few, its waves taking the
-// slots in turn; of many rows, one workgroup 32 of them and a wave a row, for they have few slots each.
-template <typename T, int D, bool RANGE, bool FEW>
-__global__ __launch_bounds__(64 * kWaves) void k_join(AttendArgs A) {
-  constexpr int kCols = D / 64;
-  __shared__ float s_l[kWaves], s_low[kWaves], s_o[kWaves][D];
+// Joins the slots of a row of few, where it has more than one: one workgroup a row, its W waves taking 8 slots
+// at a time.  What bounds it is the trips to memory one after another: where the slots are, and then everything
+// in them at once.  (Slots of a tile and head lie `heads` apart.)
+template <typename T, int D, bool RANGE, int W>
+__global__ __launch_bounds__(64 * W) void k_join_few(AttendArgs A) {
+  constexpr int kCols = D / 64, kBatch = 8;
+  __shared__ float s_m[W], s_l[W], s_low[W], s_o[W][D];
   const int pair = blockIdx.x / A.heads, h = blockIdx.x % A.heads;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slot = A.plan[2 * blockIdx.x], slots = A.plan[2 * blockIdx.x + 1];  // nothing there, if no rows
   const Rows R(A, pair / A.tiles);
-  const int first = (pair % A.tiles) * (FEW ? kFew : kMany);
-  if (first >= R.rows) return;
-  const int slot = A.plan[2 * blockIdx.x], slots = A.plan[2 * blockIdx.x + 1];
-  if (slots < 2) return;
-  constexpr int kStep = FEW ? kWaves : 1;
-  const int r0 = FEW ? blockIdx.y : blockIdx.y * 32 + wave, r1 = FEW ? r0 + 1 : min(A.rows, (int)blockIdx.y * 32 + 32);
-  for (int r = r0; r < r1 && first + r < R.rows; r += kWaves) {
-    const float* stat = A.stat + ((long long)slot * A.rows + r) * 4;  // slots of a tile and head: `heads` apart
-    const float* sums = A.sums + ((long long)slot * A.rows + r) * D + lane * kCols;
-    const long long step = (long long)A.heads * A.rows;
-    float top = -INFINITY;
-    for (int s = lane; s < slots; s += 64) top = fmaxf(top, stat[s * step * 4]);
+  const int row = (pair % A.tiles) * kFew + blockIdx.y;
+  if (row >= R.rows || slots < 2) return;
+  const long long step = (long long)A.heads * A.rows, at = (long long)slot * A.rows + blockIdx.y;
+  const float* stat = A.stat + at * 4;
+  const float* sums = A.sums + at * D + lane * kCols;
+  float top = -INFINITY, ll = 0.f, lo = INFINITY, o[kCols] = {};
+  for (int s0 = wave; s0 < slots; s0 += kBatch * W) {
+    f32x4 st[kBatch];
+    float x[kBatch][kCols];
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    float ll = 0.f, lo = INFINITY, o[kCols] = {};
-    int s = FEW ? wave : 0;
-    auto add = [&](auto N) {
-      constexpr int n = decltype(N)::value;
-      f32x4 st[n];
-      float x[n][kCols];
+    for (int i = 0; i < kBatch; ++i) {
+      const long long s = min(s0 + i * W, slots - 1);
+      st[i] = *reinterpret_cast<const f32x4*>(stat + s * step * 4);
 #pragma unroll
-      for (int i = 0; i < n; ++i) {
-        st[i] = *reinterpret_cast<const f32x4*>(stat + (s + i * kStep) * step * 4);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) x[i][c] = sums[(s + i * kStep) * step * D + c];
-      }
-#pragma unroll
-      for (int i = 0; i < n; ++i) {
-        const float f = rebase(st[i][0], top);
-        ll += f * st[i][1];
-        lo = fminf(lo, st[i][2]);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) o[c] += f * x[i][c];
-      }
-    };
-    for (; s + 7 * kStep < slots; s += 8 * kStep) add(std::integral_constant<int, 8>());
-    for (; s < slots; s += kStep) add(std::integral_constant<int, 1>());
-    if constexpr (FEW) {
-      if (lane == 0) s_l[wave] = ll, s_low[wave] = lo;
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) s_o[wave][lane * kCols + c] = o[c];
-      __syncthreads();
-      if (wave != 0) return;
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) {
-        ll += s_l[w];
-        lo = fminf(lo, s_low[w]);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) o[c] += s_o[w][lane * kCols + c];
-      }
+      for (int c = 0; c < kCols; ++c) x[i][c] = sums[s * step * D + c];
     }
-    const int qr = (first + r) / A.group, qc = (first + r) % A.group;
-    store_row<T, kCols, RANGE>(A, (R.q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, lane * kCols, top, ll, lo, o);
+    float m = top;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) m = fmaxf(m, st[i][0]);
+    const float f = rebase(top, m);
+    top = m;
+    ll *= f;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) o[c] *= f;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (s0 + i * W >= slots) break;
+      const float e = rebase(st[i][0], m);
+      ll += e * st[i][1];
+      lo = fminf(lo, st[i][2]);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) o[c] += e * x[i][c];
+    }
   }
+  if (lane == 0) s_m[wave] = top, s_l[wave] = ll, s_low[wave] = lo;
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) s_o[wave][lane * kCols + c] = o[c];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < W; ++w) top = fmaxf(top, s_m[w]);
+  ll = 0.f;
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) o[c] = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float f = rebase(s_m[w], top);
+    ll += f * s_l[w];
+    lo = fminf(lo, s_low[w]);
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) o[c] += f * s_o[w][lane * kCols + c];
+  }
+  store_row<T, kCols, RANGE>(A, (R.q0 + row / A.group) * (long long)(A.heads * A.group) + h * A.group + row % A.group, D,
+                             lane * kCols, top, ll, lo, o);
 }
 
+// The same of many rows, which have few slots each: D / 4 threads a row, a workgroup a quarter of a tile's (where
+// nothing was split, each costs a launch for nothing).
+constexpr int kQuarters = 4;
+template <typename T, int D, bool RANGE>
+__global__ __launch_bounds__(64 * kWaves) void k_join_many(AttendArgs A) {
+  constexpr int kThreads = D / 4, kRows = 64 * kWaves / kThreads;
+  const int pair = blockIdx.x / A.heads, h = blockIdx.x % A.heads;
+  const int slot = A.plan[2 * blockIdx.x], slots = A.plan[2 * blockIdx.x + 1];  // nothing there, if no rows
+  const Rows R(A, pair / A.tiles);
+  const int first = (pair % A.tiles) * kMany, c0 = threadIdx.x % kThreads * 4;
+  if (first >= R.rows || slots < 2) return;
+  const int end = min(min(A.rows, R.rows - first), (int)(blockIdx.y + 1) * (kMany / kQuarters));
+  const long long step = (long long)A.heads * A.rows;
+  for (int r = blockIdx.y * (kMany / kQuarters) + threadIdx.x / kThreads; r < end; r += kRows) {
+    const long long at = (long long)slot * A.rows + r;
+    const float* stat = A.stat + at * 4;
+    const float* sums = A.sums + at * D + c0;
+    float top = -INFINITY, ll = 0.f, lo = INFINITY;
+#pragma unroll 4
+    for (int s = 0; s < slots; ++s) top = fmaxf(top, stat[s * step * 4]);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < slots; ++s) {
+      const f32x4 st = *reinterpret_cast<const f32x4*>(stat + s * step * 4);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(sums + s * step * D);
+      const float f = rebase(st[0], top);
+      ll += f * st[1];
+      lo = fminf(lo, st[2]);
+      o += f * x;
+    }
+    const float v[4] = {o[0], o[1], o[2], o[3]};
+    const int qr = (first + r) / A.group, qc = (first + r) % A.group;
+    store_row<T, 4, RANGE>(A, (R.q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, c0, top, ll, lo, v);
+  }
+}
 
 template <typename T, int D, bool RANGE>
 int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
@@ -399,8 +436,9 @@ int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
   HCK_CHECK_LAUNCH();
   if (W.join) {
     const unsigned pairs = (unsigned)(W.pairs * A.heads);
-    if (W.few) k_join<T, D, RANGE, true><<<dim3(pairs, W.rows), 64 * kWaves, 0, s>>>(A);
-    else k_join<T, D, RANGE, false><<<dim3(pairs, (W.rows + 31) / 32), 64 * kWaves, 0, s>>>(A);
+    if (!W.few) k_join_many<T, D, RANGE><<<dim3(pairs, kQuarters), 64 * kWaves, 0, s>>>(A);
+    else if (W.most_slots > 32) k_join_few<T, D, RANGE, 16><<<dim3(pairs, W.rows), 64 * 16, 0, s>>>(A);
+    else k_join_few<T, D, RANGE, 4><<<dim3(pairs, W.rows), 64 * 4, 0, s>>>(A);
     HCK_CHECK_LAUNCH();
   }
   return HCK_OK;

@@ -95,16 +95,17 @@ __device__ __forceinline__ int units_of(const AttendArgs& A, int pair, int size)
   return (R.seen(A, min(first + size, R.rows) - 1) + kUnit - 1) / kUnit;
 }
 
-__device__ __forceinline__ long long over_wave(long long x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+// Sums of the lanes up to each: by 1, 2, 4 and 8 within 16, then the 16s' last lanes onwards.
+__device__ __forceinline__ int upto_lane(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
   return x;
 }
-__device__ __forceinline__ int over_wave(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
-  return __builtin_amdgcn_readfirstlane(x);
-}
+__device__ __forceinline__ int over_wave(int x) { return __builtin_amdgcn_readlane(upto_lane(x), 63); }
 
 // Where the join finds the slots of a tile and head, from the workgroup that has their first.
 __device__ __forceinline__ void publish(const AttendArgs& A, const Item& it) {
@@ -115,15 +116,20 @@ __device__ __forceinline__ void publish(const AttendArgs& A, const Item& it) {
 
 constexpr int kPairs = 8;  // tiles of rows that a lane looks through to share the work out
 
+__device__ __forceinline__ int ceil_div(int n, int d) { return (int)(((uint32_t)n + (uint32_t)d - 1) / (uint32_t)d); }
+
 // Which part of the work is workgroup w's.  Lengths are on the device, so every wave works it out: with
-// all tiles' units in its lanes, a share is the smallest for which the parts (whole shares of a tile and
-// its rest) are no more than the workgroups that run at once.  Later tiles, which see more, come first.
+// all tiles' units in its lanes, a share is the smallest (to a sixteenth) for which the parts, whole shares
+// of a tile and its rest, are no more than the workgroups that run at once.  Later tiles, which see more,
+// come first.  (A key head's workgroups lie `heads` apart: with 8 heads each XCD has one, and its cache that
+// head's keys and values.  The heads of a page side by side on one XCD, for the address translation, won 2 % of
+// 48 long histories and lost 20 % of 32 uneven ones.)
 __device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Item& it) {
   const int pairs = A.seqs * A.tiles, lane = threadIdx.x & 63;
-  it.h = w % A.heads;
-  it.slot = w, it.slots = 1;
-  int r = w / A.heads;
   if (!A.join) {
+    const int r = w / A.heads;
+    it.h = w % A.heads;
+    it.slot = w, it.slots = 1;
     const int p = pairs - 1 - r;
     it.b = p / A.tiles, it.tile = p % A.tiles;
     it.u0 = 0, it.u1 = 0x7fffffff;
@@ -131,41 +137,39 @@ __device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Ite
   }
   const int per = (pairs + 63) / 64;
   int n[kPairs];
-  long long total = 0;
+  int whole = 0, rest = 0;  // the units' sum, by 2^15: a wave's lengths may pass 31 bits
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
-    const int p = pairs - 1 - (lane * per + j);
-    n[j] = j < per && p >= 0 ? units_of(A, p, size) : -1;
-    total += max(n[j], 0);
-  }
-  total = over_wave(total) * A.heads;
-  const int base = __builtin_amdgcn_readfirstlane((int)min(1ll << 26, max((long long)A.least, (total + A.slots - 1) / A.slots)));
-  int share = 0, mine = 0;
-#pragma unroll
-  for (int f = 4; f <= 8; ++f) {
-    if (f == 7) continue;
-    const int s = base / 4 * f + (base % 4 * f + 3) / 4;
-    int c = 0;
-#pragma unroll
-    for (int j = 0; j < kPairs; ++j) c += n[j] < 0 ? 0 : max(1, (n[j] + s - 1) / s);
-    const bool last = f == 8;
-    if (last || (long long)over_wave(c) * A.heads <= A.slots) {
-      share = s, mine = c;
-      break;
+    n[j] = -1;
+    if (j < per) {
+      const int p = pairs - 1 - (lane * per + j);
+      if (p >= 0) n[j] = units_of(A, p, size);
+      whole += max(n[j], 0) >> 15, rest += max(n[j], 0) & 0x7fff;
     }
   }
-  int upto = mine;
+  const long long total = (((long long)over_wave(whole) << 15) + over_wave(rest)) * A.heads;
+  const int base = (int)min(1ll << 26, max((long long)A.least, (total + A.slots - 1) / A.slots));
+  const int fit = A.slots / A.heads;
+  int share = base, mine = 0;
+  for (int f = 16;; ++f) {
+    share = (int)(((long long)base * f + 15) / 16);
+    mine = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int x = __shfl_up(upto, d);
-    if (lane >= d) upto += x;
+    for (int j = 0; j < kPairs; ++j)
+      if (j < per) mine += n[j] < 0 ? 0 : max(1, ceil_div(n[j], share));
+    if (f == 32 || over_wave(mine) <= fit) break;
   }
+  const int upto = upto_lane(mine), all = __builtin_amdgcn_readlane(upto, 63) * A.heads;
+  if (w >= all) return false;
+  const int r = w / A.heads;
+  it.h = w % A.heads;
+  it.slot = w;
   const int owner = __popcll(__ballot(upto <= r));  // the lane that holds part r
-  if (owner > 63) return false;
   int pair = 0, u0 = 0, count = 1, at = upto - mine;
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
-    const int c = n[j] < 0 ? 0 : max(1, (n[j] + share - 1) / share);
+    if (j >= per) break;
+    const int c = n[j] < 0 ? 0 : max(1, ceil_div(n[j], share));
     if (r >= at && r < at + c) pair = pairs - 1 - (lane * per + j), u0 = (r - at) * share, count = c;
     at += c;
   }
@@ -297,7 +301,7 @@ constexpr int waves_of_many(int dim) { return dim == 64 ? 3 : 2; }
 struct Way {
   bool few, join;
   int rows, least;
-  int64_t tiles, slots, pairs, items;
+  int64_t tiles, slots, pairs, items, most_slots;  // most_slots: of one tile and head
   Way(int64_t seqs, int heads, int group, int dim, bool half, int most, int cols) {
     const int64_t all = (int64_t)most * group, units = std::max<int64_t>(1, (int64_t)cols * (kPageTokens / kUnit));
     few = all <= 32;
@@ -308,6 +312,7 @@ struct Way {
     slots = kComputeUnits * (few ? waves_of_few(dim, half) : waves_of_many(dim));
     pairs = seqs * tiles;
     join = pairs <= 64 * kPairs && units > least;
+    most_slots = std::min((units + least - 1) / least, slots / heads + 1);
     items = !join ? pairs * heads : std::min(pairs * ((units + least - 1) / least), pairs + (slots + heads - 1) / heads) * heads;
   }
   size_t bytes(int heads, int dim) const {
