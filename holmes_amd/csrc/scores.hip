@@ -114,19 +114,21 @@ __device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const 
   const int lane = threadIdx.x & 63;
   const float ref = finite_or_zero(a.r);
   const float log = a.l == 0.f ? 0.f : __builtin_amdgcn_logf(a.l);  // a row without a finite value
+  // No probability is above 1 and no entropy below 0, though their last bits might say so (NaN stays).
+  auto most0 = [](float x) { return x > 0.f ? 0.f : x; };
   if (lane == 0) {
-    A.entropy[row] = (log - (a.l == 0.f ? 0.f : a.s / a.l)) * kLn2;
+    A.entropy[row] = -most0(((a.l == 0.f ? 0.f : a.s / a.l) - log) * kLn2);
     if (A.tokens) {
       const long long t = A.tokens[row];
       float lp = 0.f;
       if (t >= A.vocab) lp = __uint_as_float(0x7fc00000u);
-      else if (t >= 0) lp = (__builtin_fmaf((float)((const T*)A.x)[row * A.row_stride + t], kLog2e, -ref) - log) * kLn2;
+      else if (t >= 0) lp = most0((__builtin_fmaf((float)((const T*)A.x)[row * A.row_stride + t], kLog2e, -ref) - log) * kLn2);
       A.given[row] = lp;
     }
   }
   if (lane < A.top) {
     A.top_ids[row * A.top + lane] = 0xffffffffu - (uint32_t)best;
-    A.top_logs[row * A.top + lane] = (__builtin_fmaf(value_of((uint32_t)(best >> 32)), kLog2e, -ref) - log) * kLn2;
+    A.top_logs[row * A.top + lane] = most0((__builtin_fmaf(value_of((uint32_t)(best >> 32)), kLog2e, -ref) - log) * kLn2);
   }
 }
 
