@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   extern __shared__ float s_o[];  // [wave][A.rows][D + 4]
 
   Item it;
-  if (!locate(A, kFew, blockIdx.x, it)) return;
+  if (!locate(A, blockIdx.x, it)) return;
   it.uniform();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const int copy = m / R, tile = it.tile, h = it.h, b = it.b;
@@ -393,11 +393,11 @@ __global__ __launch_bounds__(64 * kWaves) void k_join_many(AttendArgs A) {
   const int pair = blockIdx.x / A.heads, h = blockIdx.x % A.heads;
   const int slot = A.plan[2 * blockIdx.x], slots = A.plan[2 * blockIdx.x + 1];  // nothing there, if no rows
   const Rows R(A, pair / A.tiles);
-  const int first = (pair % A.tiles) * kMany, c0 = threadIdx.x % kThreads * 4;
+  const int first = (pair % A.tiles) * A.size, c0 = threadIdx.x % kThreads * 4;
   if (first >= R.rows || slots < 2) return;
-  const int end = min(min(A.rows, R.rows - first), (int)(blockIdx.y + 1) * (kMany / kQuarters));
+  const int end = min(min(A.rows, R.rows - first), (int)(blockIdx.y + 1) * (A.size / kQuarters));
   const long long step = (long long)A.heads * A.rows;
-  for (int r = blockIdx.y * (kMany / kQuarters) + threadIdx.x / kThreads; r < end; r += kRows) {
+  for (int r = blockIdx.y * (A.size / kQuarters) + threadIdx.x / kThreads; r < end; r += kRows) {
     const long long at = (long long)slot * A.rows + r;
     const float* stat = A.stat + at * 4;
     const float* sums = A.sums + at * D + c0;
@@ -506,6 +506,7 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
   A.causal = causal;
   A.seqs = seqs;
   A.tiles = (int)W.tiles;
+  A.size = W.size;
   A.rows = W.rows;
   A.slots = (int)W.slots;
   A.least = W.least;

@@ -1,6 +1,9 @@
 // What the two kernels of attention over 4-bit pages share (kv4_attend.hip: few rows, kv4_prompt.hip: many):
 // their arguments, the sharing out of the work, and the arithmetic of a softmax in one pass.
 #pragma once
+#ifndef BIG
+#define BIG 1024
+#endif
 #include "kv4.hpp"
 
 #include <algorithm>
@@ -20,7 +23,6 @@ constexpr int kUnit = 64;   // tokens that a wave takes at a time: half a page
 constexpr int kWaves = 4;
 constexpr int kComputeUnits = 256;
 constexpr int kFew = 16;    // rows of k_attend's workgroup
-constexpr int kMany = 128;  // rows of k_prompt's
 // Exponentials are taken times 2^24, so that those from 2^-126 to 2^-150 of a row's largest, which the
 // exponential instruction gives as 0, still count where every larger one meets a value of 0.  Sums then
 // stay finite for values up to 2^103 over the number of tokens.
@@ -42,7 +44,7 @@ struct AttendArgs {
   long long table_stride;
   int cols, heads, group, causal;
   int seqs, tiles;     // tiles of rows that the longest sequence can have
-  int rows;            // rows of a slot
+  int size, rows;      // rows of a tile, and of a slot
   int slots, least;    // workgroups to share the work out to, units that are not worth sharing
   int join;
   float scale;
@@ -57,7 +59,7 @@ struct Rows {
     if (A.starts) first = A.starts[b], last = A.starts[b + 1];
     q0 = max(first, 0ll);
     nq = (int)max(min(last, A.tokens) - q0, 0ll);
-    rows = (int)min((long long)nq * A.group, (long long)A.tiles * (A.rows > kFew ? kMany : kFew));
+    rows = (int)min((long long)nq * A.group, (long long)A.tiles * A.size);
     length = (int)min((long long)max(A.lengths[b], 0), (long long)A.cols * kPageTokens);
   }
   // the same for all lanes, where b is
@@ -88,11 +90,11 @@ struct Item {
 };
 
 // The units of a tile's rows, -1: no rows.
-__device__ __forceinline__ int units_of(const AttendArgs& A, int pair, int size) {
+__device__ __forceinline__ int units_of(const AttendArgs& A, int pair) {
   const Rows R(A, pair / A.tiles);
-  const int first = (pair % A.tiles) * size;
+  const int first = (pair % A.tiles) * A.size;
   if (first >= R.rows) return -1;
-  return (R.seen(A, min(first + size, R.rows) - 1) + kUnit - 1) / kUnit;
+  return (R.seen(A, min(first + A.size, R.rows) - 1) + kUnit - 1) / kUnit;
 }
 
 // Sums of the lanes up to each: by 1, 2, 4 and 8 within 16, then the 16s' last lanes onwards.
@@ -124,7 +126,7 @@ __device__ __forceinline__ int ceil_div(int n, int d) { return (int)(((uint32_t)
 // come first.  (A key head's workgroups lie `heads` apart: with 8 heads each XCD has one, and its cache that
 // head's keys and values.  The heads of a page side by side on one XCD, for the address translation, won 2 % of
 // 48 long histories and lost 20 % of 32 uneven ones.)
-__device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Item& it) {
+__device__ __forceinline__ bool locate(const AttendArgs& A, int w, Item& it) {
   const int pairs = A.seqs * A.tiles, lane = threadIdx.x & 63;
   if (!A.join) {
     const int r = w / A.heads;
@@ -143,7 +145,7 @@ __device__ __forceinline__ bool locate(const AttendArgs& A, int size, int w, Ite
     n[j] = -1;
     if (j < per) {
       const int p = pairs - 1 - (lane * per + j);
-      if (p >= 0) n[j] = units_of(A, p, size);
+      if (p >= 0) n[j] = units_of(A, p);
       whole += max(n[j], 0) >> 15, rest += max(n[j], 0) & 0x7fff;
     }
   }
@@ -249,16 +251,17 @@ __device__ __forceinline__ float fmin2(float a, float b) { return fminf(a, b); }
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
 __device__ __forceinline__ float smaller(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, -INFINITY); }
 
-// Sums are taken against the whole number at or above a row's running maximum, so that going over to
-// another reference is an exact power of two.  The factor of sums against the maximum a, now against b:
-// 1 where nothing changed, also while nothing was seen (both -inf).
+// Sums are taken against the multiple of 8 at or above a row's running maximum: going over to another
+// reference is an exact power of two, and seldom needed.  The factor of sums against the maximum a, now
+// against b: 1 where nothing changed, also while nothing was seen (both -inf).
+__device__ __forceinline__ float above(float m) { return 8.f * __builtin_ceilf(0.125f * m); }
 __device__ __forceinline__ float rebase(float a, float b) {
-  return a == b ? 1.f : __builtin_ldexpf(1.f, (int)(__builtin_ceilf(a) - __builtin_ceilf(b)));
+  return a == b ? 1.f : __builtin_ldexpf(1.f, (int)(above(a) - above(b)));
 }
-__device__ __forceinline__ float reference(float m) { return fabsf(m) == INFINITY ? 0.f : __builtin_ceilf(m); }
+__device__ __forceinline__ float reference(float m) { return fabsf(m) == INFINITY ? 0.f : above(m); }
 // log2 of a row's sum, against its reference.
 __device__ __forceinline__ float log2_sum(float m, float l) {
-  return fabsf(m) == INFINITY ? m + l : __builtin_ceilf(m) + (__builtin_amdgcn_logf(l) - kLift);
+  return fabsf(m) == INFINITY ? m + l : above(m) + (__builtin_amdgcn_logf(l) - kLift);
 }
 
 // Packs the upper halves of two numbers.
@@ -300,16 +303,16 @@ constexpr int waves_of_many(int dim) { return dim == 64 ? 3 : 2; }
 // How a call is run, from what the host knows of it.
 struct Way {
   bool few, join;
-  int rows, least;
+  int size, rows, least;
   int64_t tiles, slots, pairs, items, most_slots;  // most_slots: of one tile and head
   Way(int64_t seqs, int heads, int group, int dim, bool half, int most, int cols) {
     const int64_t all = (int64_t)most * group, units = std::max<int64_t>(1, (int64_t)cols * (kPageTokens / kUnit));
     few = all <= 32;
-    const int size = few ? kFew : kMany;
+    size = few ? kFew : dim == 128 && all >= BIG ? 256 : 128;
     tiles = (all + size - 1) / size;
     rows = (int)std::min<int64_t>(all, size);
     least = few ? 4 * kWaves : 8;
-    slots = kComputeUnits * (few ? waves_of_few(dim, half) : waves_of_many(dim));
+    slots = kComputeUnits * (few ? waves_of_few(dim, half) : waves_of_many(dim) * 128 / size);
     pairs = seqs * tiles;
     join = pairs <= 64 * kPairs && units > least;
     most_slots = std::min((units + least - 1) / least, slots / heads + 1);

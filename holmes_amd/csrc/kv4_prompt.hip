@@ -11,18 +11,21 @@
 namespace hck {
 namespace {
 
-// One thread's quarter-wave share of 64 tokens: 32 dims (D = 64: 16) of one token's keys, and 8 (4) dims of 4
-// tokens' values.
-template <int D>
+// One thread's share of 64 tokens, with W waves: of one token's keys 32 dims (D = 64: 16), and of 4 tokens' values
+// 8 (4) dims; with 8 waves half of these, which half by the wave.
+template <int D, int W>
 struct Share {
-  uint32_t k[D / 32], v[D / 32], ks, vs;
+  static constexpr int kWords = D / 8 / W;
+  uint32_t k[kWords], v[D / 32], ks, vs;
   __device__ __forceinline__ void load(const uint8_t* page, int half, int wave, int lane) {
     using L = Kv4<D>;
-    typedef uint32_t words __attribute__((ext_vector_type(D / 32)));
-    const int m = lane & 15, g = lane >> 4, block = 2 * half + (wave >> 1), piece = wave & 1;
-    *reinterpret_cast<words*>(k) = *reinterpret_cast<const words*>(page + (4 * half + wave) * (8 * D) + lane * (D / 8));
-    ks = page[L::kKScales + half * (64 * L::kRuns) + g * (D / 4) / kRun * 64 + m * 4 + wave];
-    *reinterpret_cast<words*>(v) = *reinterpret_cast<const words*>(
+    typedef uint32_t kwords __attribute__((ext_vector_type(kWords)));
+    typedef uint32_t vwords __attribute__((ext_vector_type(D / 32)));
+    const int m = lane & 15, g = lane >> 4, quarter = wave & 3, block = 2 * half + (quarter >> 1), piece = quarter & 1;
+    *reinterpret_cast<kwords*>(k) =
+        *reinterpret_cast<const kwords*>(page + (4 * half + quarter) * (8 * D) + lane * (D / 8) + (wave >> 2) * (4 * kWords));
+    ks = page[L::kKScales + half * (64 * L::kRuns) + g * (D / 4) / kRun * 64 + m * 4 + quarter];
+    *reinterpret_cast<vwords*>(v) = *reinterpret_cast<const vwords*>(
         page + L::kVCodes + block * (16 * D) + (D == 128 ? piece * 1024 + lane * 16 : lane * 16 + piece * 8));
     vs = *reinterpret_cast<const uint32_t*>(page + L::kVScales + block * (32 * L::kRuns) +
                                             (g * L::kRuns + m * L::kDpl / kRun) * 8 + 4 * piece);
@@ -44,13 +47,15 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 
 // Writes the thread's share; whether it holds a run of NaN among the values, which are taken as zeros.
-template <int D>
-__device__ __forceinline__ bool store(Operands<D>& o, const Share<D>& x, int wave, int lane) {
+template <int D, int W>
+__device__ __forceinline__ bool store(Operands<D>& o, const Share<D, W>& x, int wave, int lane) {
+  constexpr int kWords = Share<D, W>::kWords;
+  const int m = lane & 15, g = lane >> 4, quarter = wave & 3, part = (wave >> 2) * kWords;
   const float sc = x.ks == kNanByte ? __uint_as_float(0x7fc00000u) : __uint_as_float(x.ks << 23);
-  const int m = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s)
-    o.k[wave >> 1][(g >> 1) * (D / 32) + s][(g & 1) * 32 + (wave & 1) * 16 + m] = u32x4{cvt<0>(x.k[s], sc), cvt<1>(x.k[s], sc), cvt<2>(x.k[s], sc), cvt<3>(x.k[s], sc)};
+  for (int s = 0; s < kWords; ++s)
+    o.k[quarter >> 1][(g >> 1) * (D / 32) + part + s][(g & 1) * 32 + (quarter & 1) * 16 + m] =
+        u32x4{cvt<0>(x.k[s], sc), cvt<1>(x.k[s], sc), cvt<2>(x.k[s], sc), cvt<3>(x.k[s], sc)};
   uint32_t vs = x.vs;
   const bool odd = has_nan(vs);
   if (odd) {
@@ -59,48 +64,48 @@ __device__ __forceinline__ bool store(Operands<D>& o, const Share<D>& x, int wav
       if (((vs >> (8 * j)) & 0xffu) == kNanByte) vs &= ~(0xffu << (8 * j));
   }
   float f[4];
+  uint32_t v[D / 32];
 #pragma unroll
   for (int j = 0; j < 4; ++j) f[j] = scale_of(vs, j);
-  auto pair = [&](auto B) {
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) v[j] = W == 4 ? x.v[j] : x.v[j] >> (8 * part);
+  auto pair = [&](auto B) {  // dims 2 b, 2 b + 1 of the thread's
     constexpr int b = decltype(B)::value;
     uint32_t y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if constexpr (D == 128) y[j] = cvt<b>(x.v[j], f[j]);
-      else y[j] = (j & 1) ? cvt<(b & 1) + 2>(x.v[j / 2], f[j]) : cvt<(b & 1)>(x.v[j / 2], f[j]);
+      if constexpr (D == 128) y[j] = cvt<b>(v[j], f[j]);
+      else y[j] = (j & 1) ? cvt<(b & 1) + 2>(v[j / 2], f[j]) : cvt<(b & 1)>(v[j / 2], f[j]);
     }
-    u32x2(*to)[2] = &o.v[wave][b][(g & 1) * 32 + 2 * m];
-    to[0][g >> 1] =
-        u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x05040100u), __builtin_amdgcn_perm(y[3], y[2], 0x05040100u)};
-    to[1][g >> 1] =
-        u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x07060302u), __builtin_amdgcn_perm(y[3], y[2], 0x07060302u)};
+    u32x2(*to)[2] = &o.v[quarter][part + b][(g & 1) * 32 + 2 * m];
+    to[0][g >> 1] = u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x05040100u), __builtin_amdgcn_perm(y[3], y[2], 0x05040100u)};
+    to[1][g >> 1] = u32x2{__builtin_amdgcn_perm(y[1], y[0], 0x07060302u), __builtin_amdgcn_perm(y[3], y[2], 0x07060302u)};
   };
   pair(std::integral_constant<int, 0>());
-  pair(std::integral_constant<int, 1>());
-  if constexpr (D == 128) {
+  if constexpr (kWords >= 2) pair(std::integral_constant<int, 1>());
+  if constexpr (kWords >= 4) {
     pair(std::integral_constant<int, 2>());
     pair(std::integral_constant<int, 3>());
   }
   return odd;
 }
 
-template <typename T, int D, bool RANGE>
-__global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(AttendArgs A) {
+template <typename T, int D, bool RANGE, int W>
+__global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs A) {
   using L = Kv4<D>;
   constexpr int kSteps = D / 16, kTiles = D / 32, kDpl = L::kDpl;
   constexpr bool kHalf = __is_same(T, _Float16);
-  static_assert(kMany == 32 * kWaves, "32 rows a wave");
   __shared__ Operands<D> s_x[2];
   __shared__ int s_odd[2];  // 1 + the unit whose values hold a run of NaN
 
   Item it;
-  if (!locate(A, kMany, blockIdx.x, it)) return;
+  if (!locate(A, blockIdx.x, it)) return;
   it.uniform();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const Rows S = Rows(A, it.b).uniform();
-  const int rows = S.rows, first = it.tile * kMany;
+  const int rows = S.rows, first = it.tile * (32 * W);
   if (first >= rows) return;
-  const int most = S.seen(A, min(first + kMany, rows) - 1);
+  const int most = S.seen(A, min(first + 32 * W, rows) - 1);
   const int u0 = it.u0, u1 = min((most + kUnit - 1) / kUnit, it.u1);
   const int mine = first + 32 * wave;  // the wave's rows
   const int least = mine < rows ? S.seen(A, mine) : 0, last = mine < rows ? S.seen(A, min(mine + 32, rows) - 1) : 0;
@@ -128,7 +133,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
 
   const int* table = A.table + it.b * A.table_stride;
   auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + it.h) * L::kBytes; };
-  Share<D> x;
+  Share<D, W> x;
   int pg = 0, next = 0;
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   if (u0 < u1) {
@@ -269,10 +274,10 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_many(D)) void k_prompt(Attend
   }
 }
 
-template <typename T, int D>
-int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
-  if (A.low) k_prompt<T, D, true><<<dim3((unsigned)W.items), 64 * kWaves, 0, s>>>(A);
-  else k_prompt<T, D, false><<<dim3((unsigned)W.items), 64 * kWaves, 0, s>>>(A);
+template <typename T, int D, int W>
+int launch(const AttendArgs& A, const Way& way, hipStream_t s) {
+  if (A.low) k_prompt<T, D, true, W><<<dim3((unsigned)way.items), 64 * W, 0, s>>>(A);
+  else k_prompt<T, D, false, W><<<dim3((unsigned)way.items), 64 * W, 0, s>>>(A);
   HCK_CHECK_LAUNCH();
   return HCK_OK;
 }
@@ -280,8 +285,10 @@ int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
 }  // namespace
 
 int launch_prompt(const AttendArgs& A, const Way& W, int head_dim, int type, hipStream_t s) {
-  if (head_dim == 128) return type == HCK_F16 ? launch<_Float16, 128>(A, W, s) : launch<__bf16, 128>(A, W, s);
-  return type == HCK_F16 ? launch<_Float16, 64>(A, W, s) : launch<__bf16, 64>(A, W, s);
+  const bool half = type == HCK_F16;
+  if (head_dim == 64) return half ? launch<_Float16, 64, 4>(A, W, s) : launch<__bf16, 64, 4>(A, W, s);
+  if (W.size == 256) return half ? launch<_Float16, 128, 8>(A, W, s) : launch<__bf16, 128, 8>(A, W, s);
+  return half ? launch<_Float16, 128, 4>(A, W, s) : launch<__bf16, 128, 4>(A, W, s);
 }
 
 }  // namespace hck
