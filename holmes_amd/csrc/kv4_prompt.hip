@@ -17,18 +17,26 @@ template <int D, int W>
 struct Share {
   static constexpr int kWords = D / 8 / W;
   uint32_t k[kWords], v[D / 32], ks, vs;
-  __device__ __forceinline__ void load(const uint8_t* page, int half, int wave, int lane) {
-    using L = Kv4<D>;
+  struct Offsets {  // of a thread's bytes in the first half of a page
+    uint32_t k, v, ks, vs;
+    __device__ __forceinline__ Offsets(int wave, int lane) {
+      using L = Kv4<D>;
+      const int m = lane & 15, g = lane >> 4, quarter = wave & 3, block = quarter >> 1, piece = quarter & 1;
+      k = quarter * (8 * D) + lane * (D / 8) + (wave >> 2) * (4 * kWords);
+      ks = L::kKScales + g * (D / 4) / kRun * 64 + m * 4 + quarter;
+      v = L::kVCodes + block * (16 * D) + (D == 128 ? piece * 1024 + lane * 16 : lane * 16 + piece * 8);
+      vs = L::kVScales + block * (32 * L::kRuns) + (g * L::kRuns + m * L::kDpl / kRun) * 8 + 4 * piece;
+    }
+  };
+  __device__ __forceinline__ void load(const uint8_t* page, int half, const Offsets& at) {
     typedef uint32_t kwords __attribute__((ext_vector_type(kWords)));
     typedef uint32_t vwords __attribute__((ext_vector_type(D / 32)));
-    const int m = lane & 15, g = lane >> 4, quarter = wave & 3, block = 2 * half + (quarter >> 1), piece = quarter & 1;
-    *reinterpret_cast<kwords*>(k) =
-        *reinterpret_cast<const kwords*>(page + (4 * half + quarter) * (8 * D) + lane * (D / 8) + (wave >> 2) * (4 * kWords));
-    ks = page[L::kKScales + half * (64 * L::kRuns) + g * (D / 4) / kRun * 64 + m * 4 + quarter];
-    *reinterpret_cast<vwords*>(v) = *reinterpret_cast<const vwords*>(
-        page + L::kVCodes + block * (16 * D) + (D == 128 ? piece * 1024 + lane * 16 : lane * 16 + piece * 8));
-    vs = *reinterpret_cast<const uint32_t*>(page + L::kVScales + block * (32 * L::kRuns) +
-                                            (g * L::kRuns + m * L::kDpl / kRun) * 8 + 4 * piece);
+    const uint8_t* codes = page + half * (32 * D);
+    const uint8_t* scales = page + half * (64 * Kv4<D>::kRuns);
+    *reinterpret_cast<kwords*>(k) = *reinterpret_cast<const kwords*>(codes + at.k);
+    ks = scales[at.ks];
+    *reinterpret_cast<vwords*>(v) = *reinterpret_cast<const vwords*>(codes + at.v);
+    vs = *reinterpret_cast<const uint32_t*>(scales + at.vs);
   }
 };
 
@@ -95,8 +103,9 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   using L = Kv4<D>;
   constexpr int kSteps = D / 16, kTiles = D / 32, kDpl = L::kDpl;
   constexpr bool kHalf = __is_same(T, _Float16);
-  __shared__ Operands<D> s_x[2];
-  __shared__ int s_odd[2];  // 1 + the unit whose values hold a run of NaN
+  constexpr int kStep = W / 4;  // units between two barriers: a page where the LDS is one workgroup's
+  __shared__ Operands<D> s_x[2][kStep];
+  __shared__ int s_odd[2][kStep];  // 1 + the unit whose values hold a run of NaN
 
   Item it;
   if (!locate(A, blockIdx.x, it)) return;
@@ -132,27 +141,43 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   const float scale2 = A.scale * kLog2e;
 
   const int* table = A.table + it.b * A.table_stride;
-  auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + it.h) * L::kBytes; };
-  Share<D, W> x;
-  int pg = 0, next = 0;
-  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
-  if (u0 < u1) {
-    pg = __builtin_amdgcn_readfirstlane(table[u0 >> 1]);
-    x.load(page_of(pg), u0 & 1, wave, lane);
-    if (u0 + 1 < u1) next = table[(u0 + 1) >> 1];
+  const uint8_t* pool = A.pool + it.h * L::kBytes;
+  const long long each = (long long)A.heads * L::kBytes;
+  auto page_of = [&](int pg) { return pool + (pg < 0 || pg >= A.pages ? 0 : pg) * each; };
+  const typename Share<D, W>::Offsets offsets(wave, lane);
+  Share<D, W> x[kStep];
+  auto load = [&](int pg, int first) {
+    const uint8_t* page = page_of(pg);
+#pragma unroll
+    for (int n = 0; n < kStep; ++n) x[n].load(page, kStep == 2 ? n : first & 1, offsets);
+  };
+  int pg = 0, next = 0, step = u0 / kStep * kStep;
+  if (threadIdx.x < 2 * kStep) s_odd[threadIdx.x / kStep][threadIdx.x % kStep] = 0;
+  if (step < u1) {
+    pg = __builtin_amdgcn_readfirstlane(table[step >> 1]);
+    load(pg, step);
+    if (step + kStep < u1) next = table[(step + kStep) >> 1];
   }
   __syncthreads();
-  for (int u = u0; u < u1; ++u) {
-    Operands<D>& o = s_x[u & 1];
-    if (store(o, x, wave, lane)) s_odd[u & 1] = u + 1;
+  for (int turn = 0; step < u1; step += kStep, turn ^= 1) {
+    Operands<D>(&os)[kStep] = s_x[turn];
+#pragma unroll
+    for (int n = 0; n < kStep; ++n)
+      if (store(os[n], x[n], wave, lane)) s_odd[turn][n] = step + n + 1;
     const bool there = pg >= 0 && pg < A.pages;
     const uint8_t* page = page_of(pg);
     pg = __builtin_amdgcn_readfirstlane(next);
-    if (u + 1 < u1) x.load(page_of(pg), (u + 1) & 1, wave, lane);
-    if (u + 2 < u1) next = table[(u + 2) >> 1];
+    if (step + kStep < u1) load(pg, step + kStep);
+    if (step + 2 * kStep < u1) next = table[(step + 2 * kStep) >> 1];
     __syncthreads();
+    if (!there) continue;
+#pragma unroll 1
+    for (int n = 0; n < kStep; ++n) {
+    const int u = step + n;
     const int here = __builtin_amdgcn_readfirstlane(u * kUnit);
-    if (!there || here >= last) continue;
+    if (here >= last || u < u0 || u >= u1) continue;
+    const Operands<D>& o = os[n];
+    const int odd = s_odd[turn][n];
 
     f32x16 t[2];
 #pragma unroll
@@ -196,7 +221,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
       for (int d = 0; d < kTiles; ++d) acc[d] *= f;
     }
 
-    if (s_odd[u & 1] == u + 1) {
+    if (odd == u + 1) {
       // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  Its values are
       // zeros here, and it is counted for the rows that see it by a product of truth values.
 #pragma unroll 1
@@ -248,6 +273,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
       for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(vv[d], pl, acc[d]);
     }
     sum += part[0] + part[1];
+    }
   }
 
   publish(A, it);
