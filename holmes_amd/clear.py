@@ -66,14 +66,15 @@ class SoftmaxRanges(NamedTuple):
     rsqrt_interval: tuple
 
 
-# A call on a few tokens costs what the host does for it, so checks are plain conditions and messages are
-# put together only where one fails.
+# A call on a few tokens costs what the host does for it: checks are one plain condition, looked at again
+# one by one only where it fails, and tensors are made by the cheapest call.
 def _no_type(dtype: torch.dtype, allowed, what: str):
     return ValueError(f"{what} must be {', '.join(str(d).replace('torch.', '') for d in allowed)}, not {dtype}")
 
 
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)  # torch.cuda.current_stream without its object
+_QUERY_TYPES = {torch.bfloat16: nat.HCK_BF16, torch.float16: nat.HCK_F16}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(index) without its object
+_empty = torch.empty_strided
 
 
 class ClearKVPages:
@@ -92,6 +93,7 @@ class ClearKVPages:
         self._lib = nat.lib()
         self.buf = torch.zeros((self.pages, self.kv_heads, self._lib.hck_kv4_page_bytes(self.head_dim)),
                                dtype=torch.uint8, device=device)
+        self._at, self._device, self._index = self.buf.data_ptr(), self.buf.device, self.buf.device.index
 
     @property
     def device(self) -> torch.device:
@@ -102,7 +104,7 @@ class ClearKVPages:
         return int(self.buf.numel())
 
     def _slots(self, slots) -> torch.Tensor:
-        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != self.buf.device:
+        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != self._device:
             raise ValueError("slots must be a 1-d int64 tensor on the pool's device")
         return slots if slots.is_contiguous() else slots.contiguous()
 
@@ -111,20 +113,20 @@ class ClearKVPages:
         the last axis contiguous) into ``slots`` [tokens].  A slot outside the pool, as -1 for padding, leaves
         its token out; the slots of one call must differ."""
 
-        buf, slots = self.buf, self._slots(slots)
-        shape, dtype, device = (slots.numel(), self.kv_heads, self.head_dim), keys.dtype, buf.device
-        kind = _TYPES.get(dtype)
+        slots = self._slots(slots)
+        tokens, device, dtype = slots.numel(), self._device, keys.dtype
+        shape, kind = (tokens, self.kv_heads, self.head_dim), _TYPES.get(dtype)
         if kind is None:
             raise _no_type(dtype, _TYPES, "keys")
-        k_token, k_head, k_dim = keys.stride() if keys.dim() == 3 else (0, 0, 0)
-        v_token, v_head, v_dim = values.stride() if values.dim() == 3 else (0, 0, 0)
-        for name, x, last in (("keys", keys, k_dim), ("values", values, v_dim)):
-            if x.shape != shape or x.dtype != dtype or x.device != device or last != 1:
-                raise ValueError(f"{name} must be {list(shape)}, contiguous along the last axis, in one type on the "
-                                 "pool's device")
-        err = self._lib.hck_kv4_append(buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, kind, keys.data_ptr(),
-                                       k_token, k_head, values.data_ptr(), v_token, v_head, slots.data_ptr(), shape[0],
-                                       _stream(device))
+        if keys.shape != shape or values.shape != shape or values.dtype != dtype or keys.device != device \
+                or values.device != device or keys.stride(2) != 1 or values.stride(2) != 1:
+            raise ValueError(f"keys and values must be {list(shape)}, contiguous along the last axis, in one type on the "
+                             "pool's device")
+        k_token, k_head, _ = keys.stride()
+        v_token, v_head, _ = values.stride()
+        err = self._lib.hck_kv4_append(self._at, self.pages, self.kv_heads, self.head_dim, kind, keys.data_ptr(), k_token,
+                                       k_head, values.data_ptr(), v_token, v_head, slots.data_ptr(), tokens,
+                                       _raw_stream(self._index))
         if err:
             nat.check(err, "hck_kv4_append")
 
@@ -132,14 +134,14 @@ class ClearKVPages:
         """What ``slots`` hold, as ``(keys, values)`` [tokens][kv_heads][head_dim] in ``dtype``: exact in bf16
         and fp32; in fp16 rounded, with its largest value for any above.  Zeros for a slot outside the pool."""
 
-        buf, slots = self.buf, self._slots(slots)
-        kind, tokens = _TYPES.get(dtype), slots.numel()
+        slots = self._slots(slots)
+        tokens, heads, dim, kind = slots.numel(), self.kv_heads, self.head_dim, _TYPES.get(dtype)
         if kind is None:
             raise _no_type(dtype, _TYPES, "dtype")
-        keys = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=buf.device)
+        keys = _empty((tokens, heads, dim), (heads * dim, dim, 1), dtype=dtype, device=self._device)
         values = torch.empty_like(keys)
-        err = self._lib.hck_kv4_read(buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, kind, slots.data_ptr(),
-                                     tokens, keys.data_ptr(), values.data_ptr(), _stream(buf.device))
+        err = self._lib.hck_kv4_read(self._at, self.pages, heads, dim, kind, slots.data_ptr(), tokens, keys.data_ptr(),
+                                     values.data_ptr(), _raw_stream(self._index))
         if err:
             nat.check(err, "hck_kv4_read")
         return keys, values
@@ -158,44 +160,52 @@ class ClearKVPages:
         sequence covers.  A page outside the pool counts as tokens that are not there.  ``scale`` multiplies
         the scores (default head_dim^-1/2); ``ranges`` asks for their least and largest."""
 
-        dim, kv_heads, dev, lib = self.head_dim, self.kv_heads, self.buf.device, self._lib
+        dim, kv_heads, dev, lib = self.head_dim, self.kv_heads, self._device, self._lib
+        i32, kind = torch.int32, _QUERY_TYPES.get(queries.dtype)
+        if kind is None:
+            raise _no_type(queries.dtype, _QUERY_TYPES, "queries")
         if queries.dim() != 3 or queries.shape[2] != dim or queries.stride(2) != 1 or queries.device != dev:
             raise ValueError(f"queries must be [tokens][query heads][{dim}], contiguous along the last axis, on the "
                              "pool's device")
-        kind = _TYPES.get(queries.dtype)
-        if kind is None or kind == nat.HCK_F32:
-            raise _no_type(queries.dtype, (torch.bfloat16, torch.float16), "queries")
         tokens, heads, _ = queries.shape
         if heads == 0 or heads % kv_heads:
             raise ValueError(f"query heads must be a multiple of {kv_heads}")
         if table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != lengths.shape[0]:
             raise ValueError("table must be [sequences][columns] and lengths [sequences]")
         seqs, cols = table.shape
-        if starts.shape != (seqs + 1,) if starts is not None else tokens != seqs:
-            raise ValueError("starts must be [sequences + 1], or there is one query for each sequence")
-        for name, x in (("table", table), ("lengths", lengths), ("starts", starts)):
-            if x is not None and (x.dtype != torch.int32 or x.device != dev or (x.stride(-1) != 1 and x.numel() != 0)):
-                raise ValueError(f"{name} must be int32 on the pool's device, contiguous along the last axis")
-        most = (1 if starts is None else tokens) if most is None else min(int(most), tokens)
+        if table.dtype != i32 or lengths.dtype != i32 or table.device != dev or lengths.device != dev \
+                or (table.stride(1) != 1 and table.numel()) or (lengths.stride(0) != 1 and seqs):
+            raise ValueError("table and lengths must be int32 on the pool's device, contiguous along the last axis")
+        if starts is None:
+            if tokens != seqs:
+                raise ValueError("starts must be [sequences + 1], or there is one query for each sequence")
+            first, most = None, 1 if most is None else min(int(most), tokens)
+        else:
+            if starts.shape != (seqs + 1,):
+                raise ValueError("starts must be [sequences + 1], or there is one query for each sequence")
+            if starts.dtype != i32 or starts.device != dev or starts.stride(0) != 1:
+                raise ValueError("starts must be int32 on the pool's device, contiguous along the last axis")
+            first, most = starts.data_ptr(), tokens if most is None else min(int(most), tokens)
         if most < 0:
             raise ValueError("most must not be negative")
-        scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+        scale = dim**-0.5 if scale is None else float(scale)
         if not 0.0 < scale < math.inf:
             raise ValueError("scale must be positive and finite")
         group = heads // kv_heads
-        out = torch.empty((tokens, heads, dim), dtype=queries.dtype, device=dev)
+        out = _empty((tokens, heads, dim), (heads * dim, dim, 1), dtype=queries.dtype, device=dev)
+        low = high = low_at = high_at = None
         if ranges:
-            lse, low, high = torch.empty((3, tokens, heads), dtype=torch.float32, device=dev).unbind(0)
+            lse, low, high = _empty((3, tokens, heads), (tokens * heads, heads, 1), dtype=torch.float32, device=dev).unbind(0)
+            low_at, high_at = low.data_ptr(), high.data_ptr()
         else:
-            lse, low, high = torch.empty((tokens, heads), dtype=torch.float32, device=dev), None, None
+            lse = _empty((tokens, heads), (heads, 1), dtype=torch.float32, device=dev)
         need = lib.hck_kv4_attend_workspace_bytes(tokens, seqs, kv_heads, group, dim, most, cols)
-        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        work = _empty((need,), (1,), dtype=torch.uint8, device=dev) if need else None
         err = lib.hck_kv4_attend(
-            self.buf.data_ptr(), self.pages, kv_heads, dim, kind, queries.data_ptr(), tokens, group, queries.stride(0),
-            queries.stride(1), table.data_ptr(), table.stride(0), cols, lengths.data_ptr(),
-            None if starts is None else starts.data_ptr(), seqs, most, int(causal), scale, out.data_ptr(),
-            lse.data_ptr(), low.data_ptr() if ranges else None, high.data_ptr() if ranges else None,
-            work.data_ptr() if need else None, need, _stream(dev))
+            self._at, self.pages, kv_heads, dim, kind, queries.data_ptr(), tokens, group, queries.stride(0),
+            queries.stride(1), table.data_ptr(), table.stride(0), cols, lengths.data_ptr(), first, seqs, most, int(causal),
+            scale, out.data_ptr(), lse.data_ptr(), low_at, high_at, work.data_ptr() if need else None, need,
+            _raw_stream(self._index))
         if err:
             nat.check(err, "hck_kv4_attend")
         return Attended(out, lse, low, high)
@@ -239,18 +249,21 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     if dev.type != "cuda":
         raise RuntimeError("token scores run on a GPU: there is no CPU path")
-    lib = nat.lib()
-    given, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
-    ids = logs = None
+    lib, f32 = nat.lib(), torch.float32
+    entropy = _empty((rows,), (1,), dtype=f32, device=dev)
+    given = given_at = tokens_at = ids = logs = ids_at = logs_at = None
+    if tokens is not None:
+        given = torch.empty_like(entropy)
+        given_at, tokens_at = given.data_ptr(), tokens.data_ptr()
     if top:
-        ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
-        logs = torch.empty((rows, top), dtype=torch.float32, device=dev)
+        ids = _empty((rows, top), (top, 1), dtype=torch.int64, device=dev)
+        logs = _empty((rows, top), (top, 1), dtype=f32, device=dev)
+        ids_at, logs_at = ids.data_ptr(), logs.data_ptr()
     need = lib.hck_token_scores_workspace_bytes(rows, vocab, kind, top)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    err = lib.hck_token_scores(
-        logits.data_ptr(), kind, rows, vocab, logits.stride(0), None if tokens is None else tokens.data_ptr(), top,
-        given.data_ptr(), entropy.data_ptr(), ids.data_ptr() if top else None, logs.data_ptr() if top else None,
-        work.data_ptr() if need else None, need, _stream(dev))
+    work = _empty((need,), (1,), dtype=torch.uint8, device=dev) if need else None
+    err = lib.hck_token_scores(logits.data_ptr(), kind, rows, vocab, logits.stride(0), tokens_at, top, given_at,
+                               entropy.data_ptr(), ids_at, logs_at, work.data_ptr() if need else None, need,
+                               _raw_stream(dev.index))
     if err:
         nat.check(err, "hck_token_scores")
-    return TokenScores(None if tokens is None else given, entropy, ids, logs)
+    return TokenScores(given, entropy, ids, logs)

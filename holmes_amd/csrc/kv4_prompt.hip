@@ -173,106 +173,109 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
     if (!there) continue;
 #pragma unroll 1
     for (int n = 0; n < kStep; ++n) {
-    const int u = step + n;
-    const int here = __builtin_amdgcn_readfirstlane(u * kUnit);
-    if (here >= last || u < u0 || u >= u1) continue;
-    const Operands<D>& o = os[n];
-    const int odd = s_odd[turn][n];
+      const int u = step + n;
+      const int here = __builtin_amdgcn_readfirstlane(u * kUnit);
+      if (here >= last || u < u0 || u >= u1) continue;
+      const Operands<D>& o = os[n];
+      const int odd = s_odd[turn][n];
 
-    f32x16 t[2];
+      f32x16 t[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[0][i] = t[1][i] = 0.f;
+      for (int i = 0; i < 16; ++i) t[0][i] = t[1][i] = 0.f;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const bf16x8 kk = __builtin_bit_cast(bf16x8, o.k[n][s][lane]);
-        t[n] = mfma32(kk, qh[s], t[n]);
-        if constexpr (kHalf) t[n] = mfma32(kk, ql[s], t[n]);
-      }
-    const int base = here + 4 * h;  // of the lane's tokens base + 32 n + 8 (i / 4) + i % 4
-    if (here + kUnit > least) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool see = base + 32 * n + 8 * (i >> 2) + (i & 3) < seen;
-          if constexpr (RANGE) low = see ? fminf(low, t[n][i]) : low;
-          t[n][i] = see ? t[n][i] : -INFINITY;
+        for (int n = 0; n < 2; ++n) {
+          const bf16x8 kk = __builtin_bit_cast(bf16x8, o.k[n][s][lane]);
+          t[n] = mfma32(kk, qh[s], t[n]);
+          if constexpr (kHalf) t[n] = mfma32(kk, ql[s], t[n]);
         }
-    } else if constexpr (RANGE) {
+      const int base = here + 4 * h;  // of the lane's tokens base + 32 n + 8 (i / 4) + i % 4
+      if (here + kUnit > least) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) low = smaller(low, t[n][i]);
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = larger(mx, t[n][i]);
-    mx = fmaxf(top, over_half(mx, fmax2) * scale2);
-    const float f = rebase(top, mx);
-    top = mx;
-    const float ref = reference(mx) - kLift;
-    if (__any(f != 1.f)) {
-      sum *= f;
-#pragma unroll
-      for (int d = 0; d < kTiles; ++d) acc[d] *= f;
-    }
-
-    if (odd == u + 1) {
-      // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  Its values are
-      // zeros here, and it is counted for the rows that see it by a product of truth values.
-#pragma unroll 1
-      for (int j = 0; j < 4; ++j) {
-        bf16x8 bad, see;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const uint32_t vs = *reinterpret_cast<const uint32_t*>(
-              page + L::kVScales + (2 * (u & 1) + (j >> 1)) * (32 * L::kRuns) +
-              ((2 * p + h) * L::kRuns + (lane & 31) / 2 * kDpl / kRun) * 8 + 4 * (j & 1));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            bad[4 * p + k] = (__bf16)(((vs >> (8 * k)) & 0xffu) == kNanByte ? 1.f : 0.f);
-            see[4 * p + k] = (__bf16)(base + 16 * j + 8 * p + k < seen ? 1.f : 0.f);
+          for (int i = 0; i < 16; ++i) {
+            const bool see = base + 32 * n + 8 * (i >> 2) + (i & 3) < seen;
+            if constexpr (RANGE) low = see ? fminf(low, t[n][i]) : low;
+            t[n][i] = see ? t[n][i] : -INFINITY;
           }
-        }
-        f32x16 n;
+      } else if constexpr (RANGE) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) n[i] = 0.f;
-        n = mfma32(bad, see, n);
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int d = 0; d < kTiles; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (n[i] > 0.f) acc[d][i] = __uint_as_float(0x7fc00000u);
+          for (int i = 0; i < 16; ++i) low = smaller(low, t[n][i]);
       }
-    }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = larger(mx, t[n][i]);
+      mx = fmaxf(top, over_half(mx, fmax2) * scale2);
+      const float f = rebase(top, mx);
+      top = mx;
+      const float ref = reference(mx) - kLift;
+      if (__any(f != 1.f)) {
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) acc[d] *= f;
+      }
 
-    float part[2] = {0.f, 0.f};
+      if (odd == u + 1) {
+        // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  Its values are
+        // zeros here, and it is counted for the rows that see it by a product of truth values.
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          bf16x8 bad, see;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float p[8];
-      uint32_t hi[4], lo[4];  // the probabilities in two bf16 parts
+          for (int p = 0; p < 2; ++p) {
+            const uint32_t vs = *reinterpret_cast<const uint32_t*>(
+                page + L::kVScales + (2 * (u & 1) + (j >> 1)) * (32 * L::kRuns) +
+                ((2 * p + h) * L::kRuns + (lane & 31) / 2 * kDpl / kRun) * 8 + 4 * (j & 1));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[j >> 1][8 * (j & 1) + e], scale2, -ref));
+            for (int k = 0; k < 4; ++k) {
+              bad[4 * p + k] = (__bf16)(((vs >> (8 * k)) & 0xffu) == kNanByte ? 1.f : 0.f);
+              see[4 * p + k] = (__bf16)(base + 16 * j + 8 * p + k < seen ? 1.f : 0.f);
+            }
+          }
+          f32x16 n;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        hi[e] = heads_of(p[2 * e], p[2 * e + 1]);
-        lo[e] = rests_of(p[2 * e], p[2 * e + 1], hi[e]);
-        part[e & 1] += p[2 * e] + p[2 * e + 1];
+          for (int i = 0; i < 16; ++i) n[i] = 0.f;
+          n = mfma32(bad, see, n);
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (n[i] > 0.f) acc[d][i] = __uint_as_float(0x7fc00000u);
+        }
       }
-      const bf16x8 ph = operand(hi[0], hi[1], hi[2], hi[3]), pl = operand(lo[0], lo[1], lo[2], lo[3]);
-      bf16x8 vv[kTiles];
+
+      // (a wave in its softmax and second product goes before one in its first, which only waits for the matrix unit)
+      __builtin_amdgcn_s_setprio(1);
+      float part[2] = {0.f, 0.f};
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) vv[d] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(o.v[j][d][lane]));
+      for (int j = 0; j < 4; ++j) {
+        float p[8];
+        uint32_t hi[4], lo[4];  // the probabilities in two bf16 parts
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(vv[d], ph, acc[d]);
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[j >> 1][8 * (j & 1) + e], scale2, -ref));
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(vv[d], pl, acc[d]);
-    }
-    sum += part[0] + part[1];
+        for (int e = 0; e < 4; ++e) {
+          hi[e] = heads_of(p[2 * e], p[2 * e + 1]);
+          lo[e] = rests_of(p[2 * e], p[2 * e + 1], hi[e]);
+          part[e & 1] += p[2 * e] + p[2 * e + 1];
+        }
+        const bf16x8 ph = operand(hi[0], hi[1], hi[2], hi[3]), pl = operand(lo[0], lo[1], lo[2], lo[3]);
+        bf16x8 vv[kTiles];
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) vv[d] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(o.v[j][d][lane]));
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(vv[d], ph, acc[d]);
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(vv[d], pl, acc[d]);
+      }
+      sum += part[0] + part[1];
+      __builtin_amdgcn_s_setprio(0);
     }
   }
 
