@@ -2,7 +2,8 @@
 
 Run ``python -m holmes_amd.build`` (or ``__graft_entry__.build()``).  Each ``.hip`` file is
 compiled to an object in parallel, then linked into one shared library exporting the C ABI of
-``include/holmes_ckks.h``.
+``include/holmes_ckks.h``.  ``csrc/clear_bind.cpp``, the Python side of the cleartext operators, becomes the
+extension module holmes_amd/_lib/_clear.so (host code only, against the installed PyTorch).
 """
 
 from __future__ import annotations
@@ -10,6 +11,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -18,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libholmes_ckks.so"
+CLEAR = OUT_DIR / "_clear.so"
 ARCH = os.environ.get("HOLMES_AMD_ARCH", "gfx950")
 
 SOURCES = ["context.hip", "ntt.hip", "poly.hip", "keyswitch.hip", "ksfused.hip", "bsgs.hip", "encode.hip",
@@ -50,17 +53,47 @@ def _compile(src: str, build_dir: Path) -> Path:
     return obj
 
 
+def _compile_binding(build_dir: Path) -> Path:
+    from torch.utils import cpp_extension
+
+    obj = build_dir / "clear_bind.o"
+    paths = [*cpp_extension.include_paths(), str(Path(HIPCC).resolve().parent.parent / "include"), "/opt/rocm/include",
+             sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1", *(f"-isystem{p}" for p in paths),
+           "-c", str(CSRC / "clear_bind.cpp"), "-o", str(obj)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for clear_bind.cpp:\n{res.stderr}")
+    return obj
+
+
+def _link_binding(obj: Path) -> None:
+    import torch
+
+    tmp = CLEAR.with_suffix(f".so.tmp{os.getpid()}")
+    cmd = ["g++", "-shared", "-o", str(tmp), str(obj), f"-L{OUT_DIR}", f"-l:{LIB.name}",
+           f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link failed:\n{res.stderr}")
+    os.replace(tmp, CLEAR)
+
+
 def build(verbose: bool = False) -> Path:
     build_dir = OUT_DIR / "obj"
     build_dir.mkdir(parents=True, exist_ok=True)
-    with ThreadPoolExecutor(max_workers=min(len(SOURCES), 8)) as pool:
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, 8)) as pool:
+        binding = pool.submit(_compile_binding, build_dir)
         objs = list(pool.map(lambda s: _compile(s, build_dir), SOURCES))
+        binding = binding.result()
     tmp = LIB.with_suffix(f".so.tmp{os.getpid()}")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
+    _link_binding(binding)
     if verbose:
         print(f"built {LIB}")
     return LIB

@@ -22,6 +22,7 @@ Everything runs in libholmes_ckks on the current stream without synchronising; t
 
 from __future__ import annotations
 
+import importlib.util
 import math
 from typing import NamedTuple
 
@@ -33,8 +34,6 @@ __all__ = ["PAGE_TOKENS", "Attended", "ClearKVPages", "SoftmaxRanges", "TokenSco
            "token_logprobs"]
 
 PAGE_TOKENS = 128
-
-_TYPES = {torch.bfloat16: nat.HCK_BF16, torch.float16: nat.HCK_F16, torch.float32: nat.HCK_F32}
 
 
 class Attended(NamedTuple):
@@ -66,15 +65,24 @@ class SoftmaxRanges(NamedTuple):
     rsqrt_interval: tuple
 
 
-# A call on a few tokens costs what the host does for it: checks are one plain condition, looked at again
-# one by one only where it fails, and tensors are made by the cheapest call.
-def _no_type(dtype: torch.dtype, allowed, what: str):
-    return ValueError(f"{what} must be {', '.join(str(d).replace('torch.', '') for d in allowed)}, not {dtype}")
+_binding = None
 
 
-_QUERY_TYPES = {torch.bfloat16: nat.HCK_BF16, torch.float16: nat.HCK_F16}
-_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(index) without its object
-_empty = torch.empty_strided
+def _bound():
+    """The extension module of csrc/clear_bind.cpp: a call on a few tokens costs what the host does for it, so
+    the checks of tensors, the outputs' allocation and the launch are one native call."""
+
+    global _binding
+    if _binding is None:
+        nat.lib()  # the library it calls; raises if it has not been built
+        path = nat.LIB_PATH.with_name("_clear.so")
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build the HIP extension first (python -m holmes_amd.build)")
+        spec = importlib.util.spec_from_file_location("_clear", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
+    return _binding
 
 
 class ClearKVPages:
@@ -93,7 +101,8 @@ class ClearKVPages:
         self._lib = nat.lib()
         self.buf = torch.zeros((self.pages, self.kv_heads, self._lib.hck_kv4_page_bytes(self.head_dim)),
                                dtype=torch.uint8, device=device)
-        self._at, self._device, self._index = self.buf.data_ptr(), self.buf.device, self.buf.device.index
+        self._native = _bound()
+        self._pool = (self.buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, self.buf.device.index)
 
     @property
     def device(self) -> torch.device:
@@ -103,30 +112,12 @@ class ClearKVPages:
     def nbytes(self) -> int:
         return int(self.buf.numel())
 
-    def _slots(self, slots) -> torch.Tensor:
-        if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != self._device:
-            raise ValueError("slots must be a 1-d int64 tensor on the pool's device")
-        return slots if slots.is_contiguous() else slots.contiguous()
-
     def append(self, keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor) -> None:
         """Writes ``keys`` and ``values`` [tokens][kv_heads][head_dim] (bf16, fp16 or fp32, any strides but
         the last axis contiguous) into ``slots`` [tokens].  A slot outside the pool, as -1 for padding, leaves
         its token out; the slots of one call must differ."""
 
-        slots = self._slots(slots)
-        tokens, device, dtype = slots.numel(), self._device, keys.dtype
-        shape, kind = (tokens, self.kv_heads, self.head_dim), _TYPES.get(dtype)
-        if kind is None:
-            raise _no_type(dtype, _TYPES, "keys")
-        if keys.shape != shape or values.shape != shape or values.dtype != dtype or keys.device != device \
-                or values.device != device or keys.stride(2) != 1 or values.stride(2) != 1:
-            raise ValueError(f"keys and values must be {list(shape)}, contiguous along the last axis, in one type on the "
-                             "pool's device")
-        k_token, k_head, _ = keys.stride()
-        v_token, v_head, _ = values.stride()
-        err = self._lib.hck_kv4_append(self._at, self.pages, self.kv_heads, self.head_dim, kind, keys.data_ptr(), k_token,
-                                       k_head, values.data_ptr(), v_token, v_head, slots.data_ptr(), tokens,
-                                       _raw_stream(self._index))
+        err = self._native.append(*self._pool, keys, values, slots)
         if err:
             nat.check(err, "hck_kv4_append")
 
@@ -134,17 +125,10 @@ class ClearKVPages:
         """What ``slots`` hold, as ``(keys, values)`` [tokens][kv_heads][head_dim] in ``dtype``: exact in bf16
         and fp32; in fp16 rounded, with its largest value for any above.  Zeros for a slot outside the pool."""
 
-        slots = self._slots(slots)
-        tokens, heads, dim, kind = slots.numel(), self.kv_heads, self.head_dim, _TYPES.get(dtype)
-        if kind is None:
-            raise _no_type(dtype, _TYPES, "dtype")
-        keys = _empty((tokens, heads, dim), (heads * dim, dim, 1), dtype=dtype, device=self._device)
-        values = torch.empty_like(keys)
-        err = self._lib.hck_kv4_read(self._at, self.pages, heads, dim, kind, slots.data_ptr(), tokens, keys.data_ptr(),
-                                     values.data_ptr(), _raw_stream(self._index))
-        if err:
-            nat.check(err, "hck_kv4_read")
-        return keys, values
+        got = self._native.read(*self._pool, slots, dtype)
+        if type(got) is int:
+            nat.check(got, "hck_kv4_read")
+        return got
 
     def attend(self, queries: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *,
                starts: torch.Tensor | None = None, most: int | None = None, causal: bool = True,
@@ -160,55 +144,10 @@ class ClearKVPages:
         sequence covers.  A page outside the pool counts as tokens that are not there.  ``scale`` multiplies
         the scores (default head_dim^-1/2); ``ranges`` asks for their least and largest."""
 
-        dim, kv_heads, dev, lib = self.head_dim, self.kv_heads, self._device, self._lib
-        i32, kind = torch.int32, _QUERY_TYPES.get(queries.dtype)
-        if kind is None:
-            raise _no_type(queries.dtype, _QUERY_TYPES, "queries")
-        if queries.dim() != 3 or queries.shape[2] != dim or queries.stride(2) != 1 or queries.device != dev:
-            raise ValueError(f"queries must be [tokens][query heads][{dim}], contiguous along the last axis, on the "
-                             "pool's device")
-        tokens, heads, _ = queries.shape
-        if heads == 0 or heads % kv_heads:
-            raise ValueError(f"query heads must be a multiple of {kv_heads}")
-        if table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != lengths.shape[0]:
-            raise ValueError("table must be [sequences][columns] and lengths [sequences]")
-        seqs, cols = table.shape
-        if table.dtype != i32 or lengths.dtype != i32 or table.device != dev or lengths.device != dev \
-                or (table.stride(1) != 1 and table.numel()) or (lengths.stride(0) != 1 and seqs):
-            raise ValueError("table and lengths must be int32 on the pool's device, contiguous along the last axis")
-        if starts is None:
-            if tokens != seqs:
-                raise ValueError("starts must be [sequences + 1], or there is one query for each sequence")
-            first, most = None, 1 if most is None else min(int(most), tokens)
-        else:
-            if starts.shape != (seqs + 1,):
-                raise ValueError("starts must be [sequences + 1], or there is one query for each sequence")
-            if starts.dtype != i32 or starts.device != dev or starts.stride(0) != 1:
-                raise ValueError("starts must be int32 on the pool's device, contiguous along the last axis")
-            first, most = starts.data_ptr(), tokens if most is None else min(int(most), tokens)
-        if most < 0:
-            raise ValueError("most must not be negative")
-        scale = dim**-0.5 if scale is None else float(scale)
-        if not 0.0 < scale < math.inf:
-            raise ValueError("scale must be positive and finite")
-        group = heads // kv_heads
-        out = _empty((tokens, heads, dim), (heads * dim, dim, 1), dtype=queries.dtype, device=dev)
-        low = high = low_at = high_at = None
-        if ranges:
-            lse, low, high = _empty((3, tokens, heads), (tokens * heads, heads, 1), dtype=torch.float32, device=dev).unbind(0)
-            low_at, high_at = low.data_ptr(), high.data_ptr()
-        else:
-            lse = _empty((tokens, heads), (heads, 1), dtype=torch.float32, device=dev)
-        need = lib.hck_kv4_attend_workspace_bytes(tokens, seqs, kv_heads, group, dim, most, cols)
-        work = _empty((need,), (1,), dtype=torch.uint8, device=dev) if need else None
-        err = lib.hck_kv4_attend(
-            self._at, self.pages, kv_heads, dim, kind, queries.data_ptr(), tokens, group, queries.stride(0),
-            queries.stride(1), table.data_ptr(), table.stride(0), cols, lengths.data_ptr(), first, seqs, most, int(causal),
-            scale, out.data_ptr(), lse.data_ptr(), low_at, high_at, work.data_ptr() if need else None, need,
-            _raw_stream(self._index))
-        if err:
-            nat.check(err, "hck_kv4_attend")
-        return Attended(out, lse, low, high)
+        got = self._native.attend(*self._pool, queries, table, lengths, starts, most, causal, scale, ranges)
+        if type(got) is int:
+            nat.check(got, "hck_kv4_attend")
+        return Attended._make(got)
 
 
 def softmax_ranges(low: torch.Tensor, high: torch.Tensor, lse: torch.Tensor, margin: float = 0.05) -> SoftmaxRanges:
@@ -234,36 +173,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     NaN), the entropies, and the ``top`` (up to 32) most likely tokens, int64 and log probabilities.  A logit
     of -inf is a token that cannot be; a row of nothing else gives -inf, and 0 for the entropy."""
 
-    kind = _TYPES.get(logits.dtype)
-    if kind is None:
-        raise _no_type(logits.dtype, _TYPES, "logits")
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] != 1):
-        raise ValueError("logits must be [rows][vocabulary], contiguous along the last axis")
-    rows, vocab = logits.shape
-    if not 0 <= top <= min(nat.HCK_TOP_MAX, vocab):
-        raise ValueError(f"top must be in 0..{min(nat.HCK_TOP_MAX, vocab)}")
-    dev = logits.device
-    if tokens is not None:
-        if tokens.shape != (rows,) or tokens.dtype != torch.int64 or tokens.device != dev:
-            raise ValueError("tokens must be [rows] int64 on the logits' device")
-        tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    if dev.type != "cuda":
-        raise RuntimeError("token scores run on a GPU: there is no CPU path")
-    lib, f32 = nat.lib(), torch.float32
-    entropy = _empty((rows,), (1,), dtype=f32, device=dev)
-    given = given_at = tokens_at = ids = logs = ids_at = logs_at = None
-    if tokens is not None:
-        given = torch.empty_like(entropy)
-        given_at, tokens_at = given.data_ptr(), tokens.data_ptr()
-    if top:
-        ids = _empty((rows, top), (top, 1), dtype=torch.int64, device=dev)
-        logs = _empty((rows, top), (top, 1), dtype=f32, device=dev)
-        ids_at, logs_at = ids.data_ptr(), logs.data_ptr()
-    need = lib.hck_token_scores_workspace_bytes(rows, vocab, kind, top)
-    work = _empty((need,), (1,), dtype=torch.uint8, device=dev) if need else None
-    err = lib.hck_token_scores(logits.data_ptr(), kind, rows, vocab, logits.stride(0), tokens_at, top, given_at,
-                               entropy.data_ptr(), ids_at, logs_at, work.data_ptr() if need else None, need,
-                               _raw_stream(dev.index))
-    if err:
-        nat.check(err, "hck_token_scores")
-    return TokenScores(given, entropy, ids, logs)
+    got = (_binding or _bound()).scores(logits, tokens, top)
+    if type(got) is int:
+        nat.check(got, "hck_token_scores")
+    return TokenScores._make(got)
