@@ -109,8 +109,22 @@ __device__ __forceinline__ float element(u32x4 v, int e) {
   }
 }
 
+// The given token of a row and its logit, asked for before the row's work so that both are there at its end.
 template <typename T>
-__device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const Sums& a, unsigned long long best) {
+struct Given {
+  long long token = -1;
+  float logit = 0.f;
+  __device__ __forceinline__ Given() {}
+  __device__ __forceinline__ Given(const ScoreArgs& A, long long row) {
+    if (!A.tokens) return;
+    token = A.tokens[row];
+    if (token >= 0 && token < A.vocab) logit = (float)((const T*)A.x)[row * A.row_stride + token];
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const Given<T>& given, const Sums& a,
+                                       unsigned long long best) {
   const int lane = threadIdx.x & 63;
   const float ref = finite_or_zero(a.r);
   const float log = a.l == 0.f ? 0.f : __builtin_amdgcn_logf(a.l);  // a row without a finite value
@@ -119,10 +133,9 @@ __device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const 
   if (lane == 0) {
     A.entropy[row] = -most0(((a.l == 0.f ? 0.f : a.s / a.l) - log) * kLn2);
     if (A.tokens) {
-      const long long t = A.tokens[row];
       float lp = 0.f;
-      if (t >= A.vocab) lp = __uint_as_float(0x7fc00000u);
-      else if (t >= 0) lp = most0((__builtin_fmaf((float)((const T*)A.x)[row * A.row_stride + t], kLog2e, -ref) - log) * kLn2);
+      if (given.token >= A.vocab) lp = __uint_as_float(0x7fc00000u);
+      else if (given.token >= 0) lp = most0((__builtin_fmaf(given.logit, kLog2e, -ref) - log) * kLn2);
       A.given[row] = lp;
     }
   }
@@ -132,15 +145,24 @@ __device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const 
   }
 }
 
+// f over the wave's lanes, in every lane: within 16 lanes by turning, then over the 16s.
+template <typename F>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t x, F f) {
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x121, 0xf, 0xf, true));
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x122, 0xf, 0xf, true));
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xf, 0xf, true));
+  x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true));
+  const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f(p[0], p[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(q[0], q[1]);
+}
 __device__ __forceinline__ Sums over_lanes(Sums a) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    Sums o;
-    o.r = __shfl_xor(a.r, d);
-    o.l = __shfl_xor(a.l, d);
-    o.s = __shfl_xor(a.s, d);
-    a.add(o);
-  }
+  auto larger = [](uint32_t x, uint32_t y) { return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y))); };
+  auto plus = [](uint32_t x, uint32_t y) { return __float_as_uint(__uint_as_float(x) + __uint_as_float(y)); };
+  a.rebase(__uint_as_float(over_lanes(__float_as_uint(a.r), larger)));
+  a.l = __uint_as_float(over_lanes(__float_as_uint(a.l), plus));
+  a.s = __uint_as_float(over_lanes(__float_as_uint(a.s), plus));
   return a;
 }
 
@@ -185,9 +207,18 @@ struct Candidates {
     uint32_t k[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) k[w] = most[64 * w + lane];
-    uint32_t t = 0;
+    // the bits that all keys share come first
+    uint32_t most_of = k[0], least_of = k[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) most_of = max(most_of, k[w]), least_of = min(least_of, k[w]);
+    most_of = over_lanes(most_of, [](uint32_t x, uint32_t y) { return max(x, y); });
+    least_of = over_lanes(least_of, [](uint32_t x, uint32_t y) { return min(x, y); });
+    most_of = __builtin_amdgcn_readfirstlane(most_of), least_of = __builtin_amdgcn_readfirstlane(least_of);
+    const uint32_t differ = most_of ^ least_of;
+    uint32_t bit = differ ? 0x80000000u >> __builtin_clz(differ) : 0;
+    uint32_t t = bit ? most_of & ~(2 * bit - 1) : most_of;
     threads = kThreads;
-    for (uint32_t bit = 0x80000000u; bit != 0 && threads > top + 3; bit >>= 1) {
+    for (; bit != 0 && threads > top + 3; bit >>= 1) {
       int n = 0;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) n += __popcll(__ballot(k[w] >= (t | bit)));
@@ -241,6 +272,7 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
   const long long row = blockIdx.y + (long long)blockIdx.z * 32768;
   if (row >= A.rows) return;
   const T* x = (const T*)A.x + row * A.row_stride;
+  const Given<T> given = A.splits == 1 ? Given<T>(A, row) : Given<T>();
   // values before the first 16-byte border, whole pieces, and the rest
   const int head = min(A.vocab, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
   const int pieces = (A.vocab - head) / kPer, tail = head + pieces * kPer;
@@ -318,7 +350,7 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
     o.r = s_sums[w][0], o.l = s_sums[w][1], o.s = s_sums[w][2];
     a.add(o);
   }
-  if (A.splits == 1) return finish<T>(A, row, a, lane < A.top ? C.best[lane] : 0);
+  if (A.splits == 1) return finish<T>(A, row, given, a, lane < A.top ? C.best[lane] : 0);
   const long long part = row * A.splits + blockIdx.x;
   float* sums = A.part + part * 4;
   unsigned long long* tops = (unsigned long long*)(A.part + (long long)A.rows * A.splits * 4) + part * A.top;
@@ -333,6 +365,7 @@ __global__ __launch_bounds__(kThreads) void k_join(ScoreArgs A) {
   const long long row = blockIdx.x;
   const int lane = threadIdx.x & 63;
   const unsigned long long* tops = (const unsigned long long*)(A.part + (long long)A.rows * A.splits * 4) + row * A.splits * A.top;
+  const Given<T> given(A, row);
   Sums a;
   if (lane < A.splits) {
     const float* p = A.part + (row * A.splits + lane) * 4;
@@ -364,7 +397,7 @@ __global__ __launch_bounds__(kThreads) void k_join(ScoreArgs A) {
     }
   }
   if (threadIdx.x >= 64) return;
-  finish<T>(A, row, over_lanes(a), lane < A.top ? C.best[lane] : 0);
+  finish<T>(A, row, given, over_lanes(a), lane < A.top ? C.best[lane] : 0);
 }
 
 // Parts of a row: workgroups for all 256 compute units four times, none with less than one block a wave.
