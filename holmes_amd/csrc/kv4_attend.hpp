@@ -1,9 +1,6 @@
 // What the two kernels of attention over 4-bit pages share (kv4_attend.hip: few rows, kv4_prompt.hip: many):
 // their arguments, the sharing out of the work, and the arithmetic of a softmax in one pass.
 #pragma once
-#ifndef BIG
-#define BIG 1024
-#endif
 #include "kv4.hpp"
 
 #include <algorithm>
@@ -307,8 +304,12 @@ struct Way {
   int64_t tiles, slots, pairs, items, most_slots;  // most_slots: of one tile and head
   Way(int64_t seqs, int heads, int group, int dim, bool half, int most, int cols) {
     const int64_t all = (int64_t)most * group, units = std::max<int64_t>(1, (int64_t)cols * (kPageTokens / kUnit));
-    few = all <= 32;
-    size = few ? kFew : dim == 128 && all >= BIG ? 256 : 128;
+    // Few rows, or so little work that tiles of 16 rows on many compute units come sooner than tiles of 128 on few
+    // (128 tokens, 32 heads of 128: 6.1 us against 9.3; 4 of 500: 38 us against 27).
+    few = all <= 32 || seqs * heads * ((all + 15) / 16) * units <= 24576;
+    // 256 rows make a unit's operands half as often, but one workgroup fills a compute unit: where there is one for
+    // each and a quarter more (376 of them: 271 us against 292 with 128 rows; 256: 98 us against 90).
+    size = few ? kFew : dim == 128 && seqs * heads * ((all + 255) / 256) >= kComputeUnits * 5 / 4 ? 256 : 128;
     tiles = (all + size - 1) / size;
     rows = (int)std::min<int64_t>(all, size);
     least = few ? 4 * kWaves : 8;
