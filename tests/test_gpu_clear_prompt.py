@@ -154,3 +154,49 @@ def test_many_rows_in_a_graph():
         for a, b in zip(got, want):
             bits = torch.int16 if a.dtype == torch.bfloat16 else torch.int32
             assert torch.equal(a.view(bits), b.view(bits)), i
+
+
+def test_offsets_beyond_32_bits():
+    """The last pages of a pool of 4.6 GB hold, read and attend as those of a small one."""
+    from holmes_amd import clear
+
+    print("large pool", flush=True)
+    g = torch.Generator().manual_seed(16)
+    n, heads = 300, 8
+    k, v = (torch.randn((n, heads, 128), generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    q = torch.randn((n, 2 * heads, 128), generator=g).to(torch.bfloat16).cuda()
+    lengths, starts = torch.tensor([n], dtype=torch.int32).cuda(), starts_of([n])
+    got = []
+    for pages in (3, 33000):
+        pool = clear.ClearKVPages(pages, kv_heads=heads)
+        slots = torch.arange(pages * PAGE - n, pages * PAGE).cuda()
+        table = torch.arange(pages - 3, pages, dtype=torch.int32).cuda()[None]
+        first = (pages * PAGE - n) - (pages - 3) * PAGE   # the sequence begins inside its first page
+        pool.append(k, v, slots)
+        zero = torch.zeros((first, heads, 128), dtype=torch.bfloat16, device="cuda")
+        pool.append(zero, zero, torch.arange((pages - 3) * PAGE, pages * PAGE - n).cuda())
+        whole = lengths + first
+        got.append((*pool.read(slots), *pool.attend(q[-1:], table, whole)[:2],
+                    *pool.attend(q, widen(table, 900), whole, starts=starts, ranges=True)))
+        del pool
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_logits_beyond_32_bits():
+    """The last rows of 5 GB of logits score as alone."""
+    from holmes_amd import clear
+
+    print("many logits", flush=True)
+    rows, vocab = 20000, 131072
+    x = torch.zeros((rows, vocab), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(17)
+    last = torch.randn((3, vocab), generator=g, device="cuda").to(torch.bfloat16)
+    x[-3:] = last
+    tokens = torch.arange(rows, device="cuda")
+    got = clear.token_logprobs(x, tokens, top=4)
+    want = clear.token_logprobs(last, tokens[-3:], top=4)
+    assert torch.equal(got.top_ids[-3:], want.top_ids)
+    # the few rows are split, so their sums come in another order
+    for a, b in ((got.logprobs, want.logprobs), (got.entropy, want.entropy), (got.top_logprobs, want.top_logprobs)):
+        assert ((a[-3:] - b).abs() <= 2.0**-24 * (vocab / 64 + 64) + 2.0**-21 * b.abs()).all()
+    assert (got.logprobs[:-3] + math.log(vocab)).abs().max() < 1e-4
