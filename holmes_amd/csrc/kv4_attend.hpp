@@ -312,10 +312,12 @@ struct Way {
     size = few ? kFew : dim == 128 && seqs * heads * ((all + 255) / 256) >= kComputeUnits * 5 / 4 ? 256 : 128;
     tiles = (all + size - 1) / size;
     rows = (int)std::min<int64_t>(all, size);
-    least = few ? 4 * kWaves : 8;
     slots = kComputeUnits * (few ? waves_of_few(dim, half) : waves_of_many(dim) * 128 / size);
     pairs = seqs * tiles;
-    join = pairs <= 64 * kPairs && units > least;
+    // A join costs some 4 us, as much as four units a wave (8 heads, 1000 tokens: 9.0 us whole, 12.0 us in parts);
+    // parts may be half of that where they leave compute units idle (4096 tokens: 12.0 us against 13.6).
+    least = few && pairs * heads >= kComputeUnits ? 4 * kWaves : 8;
+    join = pairs <= 64 * kPairs && units > (few ? 4 * kWaves : 8);
     most_slots = std::min((units + least - 1) / least, slots / heads + 1);
     items = !join ? pairs * heads : std::min(pairs * ((units + least - 1) / least), pairs + (slots + heads - 1) / heads) * heads;
   }
