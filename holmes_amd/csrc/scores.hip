@@ -9,8 +9,10 @@
 //
 // The top values: every lane keeps the maximum of what it met.  The k-th largest T of a workgroup's 256
 // maxima is no more than the k-th largest value, and only lanes whose maximum reaches T can hold a value
-// that does: hardly more than k of them, whose values are read again.  What reaches T goes into a list
-// and is put in order by counting.  If the list runs over (many values alike), every wave keeps its k best
+// that does: hardly more than k of them.  A lane also keeps which block of its values had the maximum and
+// the largest of the others' maxima, so that as a rule one block of it is read again (all of them cost
+// 16 % more traffic at 131072 values and k = 5).  What reaches T goes into a list and is put in order by
+// counting.  If the list runs over (many values alike), every wave keeps its k best
 // in order, entry i in lane i, and goes through its values once more; they come in rising order of their
 // index, so most blocks are dismissed by one comparison.
 #include <hip/hip_runtime.h>
@@ -166,13 +168,28 @@ __device__ __forceinline__ Sums over_lanes(Sums a) {
   return a;
 }
 
-// `N` values of the lane into its sums and maximum.
+// The larger of two in one instruction, b of a NaN and b (fmaxf of bits just shifted into place takes another
+// to make a number of them first).
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
+// A lane's largest value, the block that it is in and the largest value of the other blocks.
+struct Most {
+  float top = -INFINITY, second = -INFINITY;
+  int block = -1;
+  __device__ __forceinline__ void note(float m, int b) {
+    second = fmaxf(second, fminf(top, m));
+    block = m > top ? b : block;
+    top = fmaxf(top, m);
+  }
+};
+
+// `N` values of the lane, all of block b, into its sums and maximum.
 template <int N, typename V>
-__device__ __forceinline__ void take(Sums& a, float& top, V value) {
+__device__ __forceinline__ void take(Sums& a, Most& most, int b, V value) {
   float m = -INFINITY;
 #pragma unroll
-  for (int n = 0; n < N; ++n) m = fmaxf(m, value(n));
-  top = fmaxf(top, m);
+  for (int n = 0; n < N; ++n) m = larger(m, value(n));
+  most.note(m, b);
   const float r = fmaxf(a.r, m * kLog2e);
   a.rebase(r);
   const float ref = finite_or_zero(r);
@@ -191,7 +208,7 @@ constexpr int kThreads = 64 * kWaves, kList = 256;
 struct Candidates {
   uint32_t most[kThreads];             // every thread's largest key
   unsigned long long list[kList], best[kMaxTop];
-  int count, hot[64];
+  int count, hot[64], block[64];       // threads that reach a key, and the block to look through, -2: all
   __device__ __forceinline__ static unsigned long long order(uint32_t key, uint32_t index) {
     return (unsigned long long)key << 32 | (0xffffffffu - index);  // larger: before
   }
@@ -199,7 +216,7 @@ struct Candidates {
   __device__ __forceinline__ static uint32_t index(unsigned long long o) { return 0xffffffffu - (uint32_t)o; }
 
   // A key that `top` threads' largest reach, as large as a few more allow, and how many do.
-  __device__ __forceinline__ uint32_t reach(uint32_t mine, int top, int& threads) {
+  __device__ __forceinline__ uint32_t reach(uint32_t mine, uint32_t second, int where, int top, int& threads) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     most[threadIdx.x] = mine;
     if (threadIdx.x == 0) count = 0;
@@ -230,7 +247,7 @@ struct Candidates {
       if (w < wave) before += __popcll(__ballot(k[w] >= t));
     const unsigned long long here = __ballot(mine >= t);
     const int at = before + __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0));
-    if (mine >= t && at < 64) hot[at] = threadIdx.x;
+    if (mine >= t && at < 64) hot[at] = threadIdx.x, block[at] = second >= t ? -2 : where;
     __syncthreads();
     return t;
   }
@@ -278,39 +295,45 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
   const int pieces = (A.vocab - head) / kPer, tail = head + pieces * kPer;
   const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   const int blocks = (pieces + 64 * kVecs - 1) / (64 * kVecs);
-  const int first = blockIdx.x * kWaves + wave, stride = A.splits * kWaves;
+  const int first = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + wave), stride = A.splits * kWaves;
   const bool heads = first == 0 && head > 0, tails = first == stride - 1 && tail < A.vocab;
   Sums a;
-  float top = -INFINITY;
-  if (heads) take<1>(a, top, [&](int) { return lane < head ? (float)x[lane] : -INFINITY; });
+  Most most;
+  if (heads) take<1>(a, most, -1, [&](int) { return lane < head ? (float)x[lane] : -INFINITY; });
   for (int bl = first; bl < blocks; bl += stride) {
     u32x4 v[kVecs];
     const int p0 = bl * 64 * kVecs + lane;
+    if (bl * 64 * kVecs + 64 * kVecs <= pieces) {
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-      const int p = p0 + 64 * j;
-      v[j] = nothing<T>();
-      if (p < pieces) v[j] = body[p];
+      for (int j = 0; j < kVecs; ++j) v[j] = body[p0 + 64 * j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j) {
+        const int p = p0 + 64 * j;
+        v[j] = nothing<T>();
+        if (p < pieces) v[j] = body[p];
+      }
     }
-    take<kVecs * kPer>(a, top, [&](int n) { return element<T>(v[n / kPer], n % kPer); });
+    take<kVecs * kPer>(a, most, bl, [&](int n) { return element<T>(v[n / kPer], n % kPer); });
   }
-  if (tails) take<1>(a, top, [&](int) { return tail + lane < A.vocab ? (float)x[tail + lane] : -INFINITY; });
+  if (tails) take<1>(a, most, -1, [&](int) { return tail + lane < A.vocab ? (float)x[tail + lane] : -INFINITY; });
 
   bool listed = true;
   if (A.top > 0) {
     int threads;
-    const uint32_t least = C.reach(a.l != a.l ? 0xffffffffu : key_of(top), A.top, threads);
+    const bool nan = a.l != a.l;
+    const uint32_t least = C.reach(nan ? 0xffffffffu : key_of(most.top), nan ? 0xffffffffu : key_of(most.second), most.block,
+                                   A.top, threads);
     listed = threads <= 64;
     if (listed) {
-      // the pieces of the threads that reach it, one a thread; a wave of the workgroup has `per` of them a lane
-      const int per = (blocks - (int)blockIdx.x * kWaves + stride - 1) / stride * kVecs;
+      const int per = (blocks - (int)blockIdx.x * kWaves + stride - 1) / stride * kVecs;  // pieces of a thread, at most
       for (int i = threadIdx.x; i < threads * per; i += kThreads) {
-        const int t = C.hot[i / per], n = i % per;
-        const int p = ((int)blockIdx.x * kWaves + (t >> 6) + n / kVecs * stride) * 64 * kVecs + (t & 63) + 64 * (n % kVecs);
-        if (p >= pieces) continue;
-        const u32x4 v = body[p];
+        const int t = C.hot[i / per], n = i % per, only = C.block[i / per];
+        const int bl = (int)blockIdx.x * kWaves + (t >> 6) + n / kVecs * stride, p = bl * 64 * kVecs + (t & 63) + 64 * (n % kVecs);
+        if ((only != -2 && only != bl) || p >= pieces) continue;
+        const u32x4 x4 = body[p];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) C.offer(key_of(element<T>(v, e)), (uint32_t)(head + p * kPer + e), least);
+        for (int e = 0; e < kPer; ++e) C.offer(key_of(element<T>(x4, e)), (uint32_t)(head + p * kPer + e), least);
       }
       if (heads && lane < head) C.offer(key_of((float)x[lane]), (uint32_t)lane, least);
       if (tails && tail + lane < A.vocab) C.offer(key_of((float)x[tail + lane]), (uint32_t)(tail + lane), least);
@@ -382,7 +405,7 @@ __global__ __launch_bounds__(kThreads) void k_join(ScoreArgs A) {
       most = o[j] > most ? o[j] : most;
     }
     int threads;
-    const uint32_t least = max(1u, C.reach(Candidates::key(most), A.top, threads));
+    const uint32_t least = max(1u, C.reach(Candidates::key(most), 0, -1, A.top, threads));
 #pragma unroll
     for (int j = 0; j < kMost; ++j) C.offer(Candidates::key(o[j]), Candidates::index(o[j]), least);
     if (!C.sort(A.top)) {
