@@ -47,6 +47,8 @@ struct Kv4 {
   }
 };
 
+constexpr int64_t kLastCache = 256 << 20, kL2s = 32 << 20;  // bytes of the card's last cache, of the XCDs' L2s together
+
 // Bytes of one head's part of a page (host side; 0: no such head dimension).
 inline int kv4_bytes(int head_dim) {
   return head_dim == 128 ? Kv4<128>::kBytes : head_dim == 64 ? Kv4<64>::kBytes : 0;

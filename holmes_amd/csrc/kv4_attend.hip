@@ -17,21 +17,30 @@
 namespace hck {
 namespace {
 
+// A load that passes the caches by where nothing is read twice and they could not hold it.
+template <bool ONCE, typename V>
+__device__ __forceinline__ V fetch(const uint8_t* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  else return *reinterpret_cast<const V*>(p);
+}
+
 // What a lane holds of 64 tokens: lane (m, g) = (lane % 16, lane / 16) has D / 4 dims from D / 4 * g of
 // token m of every 16-token tile, and D / 16 dims from D / 16 * m of the 8 tokens (g, j) of each 32.
 template <int D>
 struct Unit {
   uint32_t k[4][D / 32], ks, v[2][D / 16], vs[2][2];
+  template <bool ONCE>
   __device__ __forceinline__ void load_keys(const uint8_t* page, int half, int m, int g) {
     using L = Kv4<D>;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint8_t* p = page + (4 * half + i) * (8 * D) + (g * 16 + m) * (D / 8);
-      if constexpr (D == 128) *reinterpret_cast<u32x4*>(k[i]) = *reinterpret_cast<const u32x4*>(p);
-      else *reinterpret_cast<u32x2*>(k[i]) = *reinterpret_cast<const u32x2*>(p);
+      if constexpr (D == 128) *reinterpret_cast<u32x4*>(k[i]) = fetch<ONCE, u32x4>(p);
+      else *reinterpret_cast<u32x2*>(k[i]) = fetch<ONCE, u32x2>(p);
     }
     ks = *reinterpret_cast<const uint32_t*>(page + L::key_scale(64 * half + m, g * (D / 4) / kRun));
   }
+  template <bool ONCE>
   __device__ __forceinline__ void load_values(const uint8_t* page, int half, int m, int g) {
     using L = Kv4<D>;
 #pragma unroll
@@ -39,7 +48,7 @@ struct Unit {
       const uint8_t* p = page + L::kVCodes + (2 * half + i) * (16 * D) + (g * 16 + m) * 16;
 #pragma unroll
       for (int w = 0; w < D / 64; ++w)
-        reinterpret_cast<u32x4*>(v[i])[w] = *reinterpret_cast<const u32x4*>(p + 1024 * w);
+        reinterpret_cast<u32x4*>(v[i])[w] = fetch<ONCE, u32x4>(p + 1024 * w);
       *reinterpret_cast<u32x2*>(vs[i]) = *reinterpret_cast<const u32x2*>(
           page + L::kVScales + (2 * half + i) * (32 * L::kRuns) + (g * L::kRuns + m * L::kDpl / kRun) * 8);
     }
@@ -87,9 +96,11 @@ __device__ __forceinline__ float over_row(float x, F f) {
 // share of the 64 tokens, so that no exponential is taken for an empty column, and goes into the second
 // product with zeros for the other copies' tokens; the copies' sums are added at the end.
 //
+// ONCE: with loads past the caches (48 sequences of 12000 to 24576 tokens, 917 MB: 187 us through them, 167 us past).
+//
 // Keys of the next unit are loaded as soon as the first product is done with this one's, its values after the
 // second, so that loads are in flight throughout without registers of their own.
-template <typename T, int D, bool RANGE, int R>
+template <typename T, int D, bool RANGE, int R, bool ONCE>
 __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16))) void k_attend(AttendArgs A) {
   using L = Kv4<D>;
   constexpr int kTiles = R / 4;  // 16-token tiles of a lane's scores
@@ -135,10 +146,12 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + h) * L::kBytes; };
   int u = u0 + wave, pg = 0, next = 0;
   Unit<D> x;
+  auto load_keys = [&](const uint8_t* page, int half) { x.template load_keys<ONCE>(page, half, m, g); };
+  auto load_values = [&](const uint8_t* page, int half) { x.template load_values<ONCE>(page, half, m, g); };
   if (u < u1) {
     pg = __builtin_amdgcn_readfirstlane(table[u >> 1]);
-    x.load_keys(page_of(pg), u & 1, m, g);
-    x.load_values(page_of(pg), u & 1, m, g);
+    load_keys(page_of(pg), u & 1);
+    load_values(page_of(pg), u & 1);
     if (u + kWaves < u1) next = table[(u + kWaves) >> 1];
   }
   for (; u < u1; u += kWaves) {
@@ -147,7 +160,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
     if (u + 2 * kWaves < u1) next = table[(u + 2 * kWaves) >> 1];
     const uint8_t* page = page_of(pg);
     if (!there) {
-      if (more) x.load_keys(page, u & 1, m, g), x.load_values(page, u & 1, m, g);
+      if (more) load_keys(page, u & 1), load_values(page, u & 1);
       continue;
     }
 
@@ -172,7 +185,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) t[i % kTiles][k] = i < kTiles || copy == i / kTiles ? c[i][k] : t[i % kTiles][k];
-    if (more) x.load_keys(page, u & 1, m, g);
+    if (more) load_keys(page, u & 1);
     const int base = u * kUnit + 4 * g, own = base + 16 * kTiles * copy;
     if (__builtin_amdgcn_readfirstlane(u * kUnit) + kUnit > all) {
 #pragma unroll
@@ -267,7 +280,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
         step(std::integral_constant<int, 3>());
       }
     }
-    if (more) x.load_values(page, u & 1, m, g);
+    if (more) load_values(page, u & 1);
   }
 
   publish(A, it);
@@ -426,12 +439,16 @@ int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
   const size_t lds = kWaves * W.rows * (D + 4) * sizeof(float);
   if (!W.few) {
     if (const int err = launch_prompt(A, W, D, __is_same(T, _Float16) ? HCK_F16 : HCK_BF16, s)) return err;
-  } else if (W.rows <= 4) {
-    k_attend<T, D, RANGE, 4><<<grid, 64 * kWaves, lds, s>>>(A);
-  } else if (W.rows <= 8) {
-    k_attend<T, D, RANGE, 8><<<grid, 64 * kWaves, lds, s>>>(A);
   } else {
-    k_attend<T, D, RANGE, 16><<<grid, 64 * kWaves, lds, s>>>(A);
+    auto run = [&](auto rows, auto once) {
+      k_attend<T, D, RANGE, decltype(rows)::value, decltype(once)::value><<<grid, 64 * kWaves, lds, s>>>(A);
+    };
+    typedef std::integral_constant<int, 4> Four;
+    typedef std::integral_constant<int, 8> Eight;
+    typedef std::integral_constant<int, 16> Sixteen;
+    if (W.rows <= 4) A.once ? run(Four(), std::true_type()) : run(Four(), std::false_type());
+    else if (W.rows <= 8) A.once ? run(Eight(), std::true_type()) : run(Eight(), std::false_type());
+    else A.once ? run(Sixteen(), std::true_type()) : run(Sixteen(), std::false_type());
   }
   HCK_CHECK_LAUNCH();
   if (W.join) {
@@ -511,6 +528,7 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
   A.slots = (int)W.slots;
   A.least = W.least;
   A.join = W.join;
+  A.once = W.tiles == 1 && (int64_t)seqs * table_columns * kv_heads * hck::kv4_bytes(head_dim) > hck::kLastCache;
   A.scale = scale;
   hipStream_t s = (hipStream_t)stream;
   const bool range = low != nullptr;

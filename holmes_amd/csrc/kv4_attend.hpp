@@ -43,7 +43,7 @@ struct AttendArgs {
   int seqs, tiles;     // tiles of rows that the longest sequence can have
   int size, rows;      // rows of a tile, and of a slot
   int slots, least;    // workgroups to share the work out to, units that are not worth sharing
-  int join;
+  int join, once;      // once: keys and values are read once, and are more than the caches hold
   float scale;
 };
 

@@ -200,3 +200,36 @@ def test_logits_beyond_32_bits():
     for a, b in ((got.logprobs, want.logprobs), (got.entropy, want.entropy), (got.top_logprobs, want.top_logprobs)):
         assert ((a[-3:] - b).abs() <= 2.0**-24 * (vocab / 64 + 64) + 2.0**-21 * b.abs()).all()
     assert (got.logprobs[:-3] + math.log(vocab)).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads,group,dim", [(2, 4, 128), (3, 7, 64), (2, 12, 128)])
+def test_single_tokens_with_room_beyond_the_caches(heads, group, dim, kind):
+    """Tables with room for more than the last cache holds: loads that pass it by."""
+    print("room", heads, group, dim, kind, flush=True)
+    g = torch.Generator().manual_seed(18)
+    seqs = [1, 64, 65, 127, 700, 0, 16, 2100]
+    pool, table, keys, values = build(seqs, heads, dim, g)
+    q = torch.randn((len(seqs), heads * group, dim), generator=g).to(TYPES[kind]).cuda()
+    for columns in (100, 2500):
+        got = pool.attend(q, widen(table, columns), torch.tensor(seqs, dtype=torch.int32).cuda(), ranges=True)
+        check(got, q, keys, values, [1] * len(seqs))
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_a_read_beyond_the_caches(out):
+    from holmes_amd import clear
+    from .test_gpu_clear_pages import held, same
+
+    print("large read", out, flush=True)
+    g = torch.Generator().manual_seed(19)
+    pool = clear.ClearKVPages(70, kv_heads=8)
+    x = torch.randn((2, 8900, 8, 128), generator=g).to(torch.bfloat16)
+    slots = torch.randperm(70 * PAGE, generator=g)[:8900].cuda()
+    slots[5] = -1
+    pool.append(x[0].cuda(), x[1].cuda(), slots)
+    k, v = pool.read(slots, out)
+    assert (k[5] == 0).all() and (v[5] == 0).all()
+    x[:, 5] = 0
+    same(k, held(x[0]))
+    same(v, held(x[1]))
