@@ -317,7 +317,10 @@ struct Way {
     // A join costs some 4 us, as much as four units a wave (8 heads, 1000 tokens: 9.0 us whole, 12.0 us in parts);
     // parts may be half of that where they leave compute units idle (4096 tokens: 12.0 us against 13.6).
     least = few && pairs * heads >= kComputeUnits ? 4 * kWaves : 8;
-    join = pairs <= 64 * kPairs && units > (few ? 4 * kWaves : 8);
+    // One sequence of two tiles or more for every workgroup that runs at once: half of its tiles' units on average, so
+    // that no tile has more than an even share.
+    const bool even = seqs == 1 && pairs * heads >= 2 * slots;
+    join = pairs <= 64 * kPairs && units > (few ? 4 * kWaves : 8) && !even;
     most_slots = std::min((units + least - 1) / least, slots / heads + 1);
     items = !join ? pairs * heads : std::min(pairs * ((units + least - 1) / least), pairs + (slots + heads - 1) / heads) * heads;
   }
