@@ -1,11 +1,16 @@
-// Attention of many rows over 4-bit pages: the mathematics of kv4_attend.hip, with 128 rows to a workgroup.
+// Attention of many rows over 4-bit pages: the mathematics of kv4_attend.hip, with 128 or 256 rows to a workgroup.
 //
 // Here a tile is 32 by 32: a lane has one row's scores of half of 64 tokens, and a matrix instruction keeps the
 // vector unit from issuing for 8 cycles of its 32, where two of 16 by 16 do for 20 (measured), which counts where
 // both are busy.  Making operands of the codes takes some 190 vector instructions per 64 tokens, as many as the
-// softmax of 32 rows; so it is done once for 128 rows: the four waves each make a quarter of them, in the lanes'
-// order, in LDS (keys and values 32 KB, twice, so that one barrier a unit is enough), and each takes all of them
-// for its own 32 rows.  Codes of the next unit are in flight meanwhile.
+// softmax of 32 rows; so it is done once for a workgroup: each of its 4 or 8 waves makes its share of them, in the
+// lanes' order, in LDS (keys and values 32 KB per 64 tokens, twice, so that one barrier is enough; with 8 waves two
+// units to a barrier), and takes all of them for its own 32 rows.  The next codes are in flight meanwhile.
+//
+// What bounds it: per 64 tokens and 32 rows 48 matrix and some 370 vector instructions (D = 128), which two waves of
+// a SIMD issue through one port.  4096 tokens, 32 query heads over 8 key heads of 128: 139 GFLOP in 204 us, or
+// 680 TFLOP/s, and 1.02 PFLOP/s of the products that are done (three for two, by the probabilities' two parts);
+// a bf16 8192^3 product runs at 1.20 PFLOP/s.
 #include "kv4_attend.hpp"
 
 namespace hck {
