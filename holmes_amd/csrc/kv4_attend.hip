@@ -118,7 +118,11 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   it.uniform();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const int copy = m / R, tile = it.tile, h = it.h, b = it.b;
-  const Rows S = Rows(A, b).uniform();
+  // the first page's number, asked for at once (a column of the table, whatever the length)
+  const int* table = A.table + b * A.table_stride;
+  int u = it.u0 + wave;
+  const int begin = (u >> 1) < A.cols ? table[u >> 1] : 0;
+  const Rows S = it.rows;
   const long long q0 = S.q0;
   const int rows = S.rows;
   if (tile * kFew >= rows) return;
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   const int qi = live ? row / A.group : 0, qo = live ? row % A.group : 0;
   const int seen = live ? S.seen(A, row) : 0;
   const int all = S.seen(A, tile * kFew), most = S.seen(A, min(tile * kFew + R, rows) - 1);
-  const int u0 = it.u0, u1 = min((most + kUnit - 1) / kUnit, it.u1);
+  const int u1 = min((most + kUnit - 1) / kUnit, it.u1);
 
   // the lane's part of its row's query: dims D / 4 g + 8 s .. + 7 of step s
   bf16x8 qh[kSteps], ql[kSteps];
@@ -146,14 +150,12 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   const float scale2 = A.scale * kLog2e;
 
   // a page number that is not in the pool is read as page 0, and its tokens are left out
-  const int* table = A.table + b * A.table_stride;
   auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + h) * L::kBytes; };
-  int u = u0 + wave, pg = 0, next = 0;
+  int pg = __builtin_amdgcn_readfirstlane(begin), next = 0;
   Unit<D> x;
   auto load_keys = [&](const uint8_t* page, int half) { x.template load_keys<ONCE>(page, half, m, g); };
   auto load_values = [&](const uint8_t* page, int half) { x.template load_values<ONCE>(page, half, m, g); };
   if (u < u1) {
-    pg = __builtin_amdgcn_readfirstlane(table[u >> 1]);
     load_keys(page_of(pg), u & 1);
     load_values(page_of(pg), u & 1);
     if (u + kWaves < u1) next = table[(u + kWaves) >> 1];

@@ -49,25 +49,26 @@ struct AttendArgs {
 
 // The rows of one sequence: query tokens [q0, q0 + nq), each with `group` heads, row = query * group + head.
 struct Rows {
-  long long q0;
-  int nq, rows, length;
+  int q0, nq, rows, length;
+  Rows() = default;
   __device__ __forceinline__ Rows(const AttendArgs& A, int b) {
     long long first = b, last = b + 1;
     if (A.starts) first = A.starts[b], last = A.starts[b + 1];
-    q0 = max(first, 0ll);
-    nq = (int)max(min(last, A.tokens) - q0, 0ll);
-    rows = (int)min((long long)nq * A.group, (long long)A.tiles * A.size);
+    first = max(first, 0ll);
+    q0 = (int)first;
+    nq = (int)max(min(last, A.tokens) - first, 0ll);
     length = (int)min((long long)max(A.lengths[b], 0), (long long)A.cols * kPageTokens);
+    count(A);
   }
-  // the same for all lanes, where b is
-  __device__ __forceinline__ Rows uniform() const {
-    Rows r = *this;
-    r.q0 = (long long)(((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(q0 >> 32)) << 32) |
-                       (uint32_t)__builtin_amdgcn_readfirstlane((int)q0));
-    r.nq = __builtin_amdgcn_readfirstlane(nq);
-    r.rows = __builtin_amdgcn_readfirstlane(rows);
-    r.length = __builtin_amdgcn_readfirstlane(length);
-    return r;
+  __device__ __forceinline__ void count(const AttendArgs& A) {
+    rows = (int)min((long long)nq * A.group, (long long)A.tiles * A.size);
+  }
+  // those that one lane has, for all
+  __device__ __forceinline__ void of_lane(const AttendArgs& A, int lane) {
+    q0 = __builtin_amdgcn_readlane(q0, lane);
+    nq = __builtin_amdgcn_readlane(nq, lane);
+    length = __builtin_amdgcn_readlane(length, lane);
+    count(A);
   }
   // tokens that row r sees
   __device__ __forceinline__ int seen(const AttendArgs& A, int r) const {
@@ -78,6 +79,7 @@ struct Rows {
 // A workgroup's work: a tile of rows, a key head, and a part of the units of 64 tokens that they see.
 struct Item {
   int b, tile, h, u0, u1, slot, slots;
+  Rows rows;
   // into scalar registers
   __device__ __forceinline__ void uniform() {
     b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile), h = __builtin_amdgcn_readfirstlane(h);
@@ -86,9 +88,8 @@ struct Item {
   }
 };
 
-// The units of a tile's rows, -1: no rows.
-__device__ __forceinline__ int units_of(const AttendArgs& A, int pair) {
-  const Rows R(A, pair / A.tiles);
+// The units that a tile's rows see, -1: no rows.
+__device__ __forceinline__ int units_of(const AttendArgs& A, const Rows& R, int pair) {
   const int first = (pair % A.tiles) * A.size;
   if (first >= R.rows) return -1;
   return (R.seen(A, min(first + A.size, R.rows) - 1) + kUnit - 1) / kUnit;
@@ -132,17 +133,23 @@ __device__ __forceinline__ bool locate(const AttendArgs& A, int w, Item& it) {
     const int p = pairs - 1 - r;
     it.b = p / A.tiles, it.tile = p % A.tiles;
     it.u0 = 0, it.u1 = 0x7fffffff;
+    it.rows = Rows(A, it.b);
+    it.rows.of_lane(A, 0);
     return true;
   }
   const int per = (pairs + 63) / 64;
   int n[kPairs];
+  Rows R[kPairs] = {};
   int whole = 0, rest = 0;  // the units' sum, by 2^15: a wave's lengths may pass 31 bits
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
     n[j] = -1;
     if (j < per) {
       const int p = pairs - 1 - (lane * per + j);
-      if (p >= 0) n[j] = units_of(A, p);
+      if (p >= 0) {
+        R[j] = Rows(A, p / A.tiles);
+        n[j] = units_of(A, R[j], p);
+      }
       whole += max(n[j], 0) >> 15, rest += max(n[j], 0) & 0x7fff;
     }
   }
@@ -165,11 +172,12 @@ __device__ __forceinline__ bool locate(const AttendArgs& A, int w, Item& it) {
   it.slot = w;
   const int owner = __popcll(__ballot(upto <= r));  // the lane that holds part r
   int pair = 0, u0 = 0, count = 1, at = upto - mine;
+  it.rows = R[0];
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
     if (j >= per) break;
     const int c = n[j] < 0 ? 0 : max(1, ceil_div(n[j], share));
-    if (r >= at && r < at + c) pair = pairs - 1 - (lane * per + j), u0 = (r - at) * share, count = c;
+    if (r >= at && r < at + c) pair = pairs - 1 - (lane * per + j), u0 = (r - at) * share, count = c, it.rows = R[j];
     at += c;
   }
   pair = __builtin_amdgcn_readlane(pair, owner);
@@ -177,6 +185,7 @@ __device__ __forceinline__ bool locate(const AttendArgs& A, int w, Item& it) {
   it.slots = __builtin_amdgcn_readlane(count, owner);
   it.u1 = it.u0 + share;
   it.b = pair / A.tiles, it.tile = pair % A.tiles;
+  it.rows.of_lane(A, owner);
   return true;
 }
 

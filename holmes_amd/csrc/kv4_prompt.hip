@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   if (!locate(A, blockIdx.x, it)) return;
   it.uniform();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const Rows S = Rows(A, it.b).uniform();
+  const Rows S = it.rows;
   const int rows = S.rows, first = it.tile * (32 * W);
   if (first >= rows) return;
   const int most = S.seen(A, min(first + 32 * W, rows) - 1);
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   const int seen = live ? S.seen(A, row) : 0;
 
   bf16x8 qh[kSteps], ql[kSteps];
-  const T* qp = (const T*)A.q + (S.q0 + qi) * A.q_ts + (long long)(it.h * A.group + qo) * A.q_hs + h * (D / 4);
+  const T* qp = (const T*)A.q + (long long)(S.q0 + qi) * A.q_ts + (long long)(it.h * A.group + qo) * A.q_hs + h * (D / 4);
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     u32x4 raw = {0, 0, 0, 0};
