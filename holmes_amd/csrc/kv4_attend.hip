@@ -403,9 +403,8 @@ __global__ __launch_bounds__(64 * W) void k_join_few(AttendArgs A) {
                              lane * kCols, top, ll, lo, o);
 }
 
-// The same of many rows, which have few slots each: D / 4 threads a row, a workgroup a quarter of a tile's (where
-// nothing was split, each costs a launch for nothing).
-constexpr int kQuarters = 4;
+// The same of many rows, which have few slots each: D / 4 threads a row, a workgroup a 4th to a 16th of a tile
+// (fewer where there are many tiles, of which most may have nothing to join).
 template <typename T, int D, bool RANGE>
 __global__ __launch_bounds__(64 * kWaves) void k_join_many(AttendArgs A) {
   constexpr int kThreads = D / 4, kRows = 64 * kWaves / kThreads;
@@ -414,9 +413,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_join_many(AttendArgs A) {
   const Rows R(A, pair / A.tiles);
   const int first = (pair % A.tiles) * A.size, c0 = threadIdx.x % kThreads * 4;
   if (first >= R.rows || slots < 2) return;
-  const int end = min(min(A.rows, R.rows - first), (int)(blockIdx.y + 1) * (A.size / kQuarters));
+  const int part = A.size / gridDim.y, end = min(min(A.rows, R.rows - first), (int)(blockIdx.y + 1) * part);
   const long long step = (long long)A.heads * A.rows;
-  for (int r = blockIdx.y * (A.size / kQuarters) + threadIdx.x / kThreads; r < end; r += kRows) {
+  for (int r = blockIdx.y * part + threadIdx.x / kThreads; r < end; r += kRows) {
     const long long at = (long long)slot * A.rows + r;
     const float* stat = A.stat + at * 4;
     const float* sums = A.sums + at * D + c0;
@@ -459,7 +458,7 @@ int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
   HCK_CHECK_LAUNCH();
   if (W.join) {
     const unsigned pairs = (unsigned)(W.pairs * A.heads);
-    if (!W.few) k_join_many<T, D, RANGE><<<dim3(pairs, kQuarters), 64 * kWaves, 0, s>>>(A);
+    if (!W.few) k_join_many<T, D, RANGE><<<dim3(pairs, pairs <= 128 ? 16 : pairs <= 256 ? 8 : 4), 64 * kWaves, 0, s>>>(A);
     else if (W.most_slots > 32) k_join_few<T, D, RANGE, 16><<<dim3(pairs, W.rows), 64 * 16, 0, s>>>(A);
     else k_join_few<T, D, RANGE, 4><<<dim3(pairs, W.rows), 64 * 4, 0, s>>>(A);
     HCK_CHECK_LAUNCH();
