@@ -14,7 +14,7 @@
 // rounding of the output; the sum l takes the unrounded ones.
 //
 // What bounds it (8 key heads of 128, 4 query heads each): over 48 sequences of 12000 to 24576 tokens the bytes,
-// 917 MB in 167 us or 5.5 TB/s (the same loads without arithmetic: 5.9); over 131072 tokens 31 us for 142 MB, of
+// 917 MB in 161 us or 5.7 TB/s (the same loads without arithmetic: 5.9); over 131072 tokens 29 us for 142 MB, of
 // which 5 go by before the first product; over 257 tokens the chain of loads (length, page number, codes), 5 to 7 us.
 #include "kv4_attend.hpp"
 
@@ -100,7 +100,7 @@ __device__ __forceinline__ float over_row(float x, F f) {
 // share of the 64 tokens, so that no exponential is taken for an empty column, and goes into the second
 // product with zeros for the other copies' tokens; the copies' sums are added at the end.
 //
-// ONCE: with loads past the caches (48 sequences of 12000 to 24576 tokens, 917 MB: 187 us through them, 167 us past).
+// ONCE: with loads past the caches (48 sequences of 12000 to 24576 tokens, 917 MB: 187 us through them, 167 us past, then).
 //
 // Keys of the next unit are loaded as soon as the first product is done with this one's, its values after the
 // second, so that loads are in flight throughout without registers of their own.

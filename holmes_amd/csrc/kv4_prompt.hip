@@ -8,8 +8,8 @@
 // units to a barrier), and takes all of them for its own 32 rows.  The next codes are in flight meanwhile.
 //
 // What bounds it: per 64 tokens and 32 rows 48 matrix and some 370 vector instructions (D = 128), which two waves of
-// a SIMD issue through one port.  4096 tokens, 32 query heads over 8 key heads of 128: 139 GFLOP in 204 us, or
-// 680 TFLOP/s, and 1.02 PFLOP/s of the products that are done (three for two, by the probabilities' two parts);
+// a SIMD issue through one port.  4096 tokens, 32 query heads over 8 key heads of 128: 139 GFLOP in 194 us, or
+// 716 TFLOP/s, and 1.07 PFLOP/s of the products that are done (three for two, by the probabilities' two parts);
 // a bf16 8192^3 product runs at 1.20 PFLOP/s.
 #include "kv4_attend.hpp"
 
