@@ -1,11 +1,10 @@
 // Log probabilities of given tokens under rows of logits, with the entropy and the top alternatives.
 //
-// For a row x over the vocabulary, in units of log 2 (t_i = x_i log2 e - r with a running reference r
-// close to the row's maximum):  l = sum 2^(t_i),  s = sum 2^(t_i) t_i, then
-//   log p(i) = ln 2 (t_i - log2 l),   H = ln 2 (log2 l - s / l).
+// For a row x over the vocabulary, in units of log 2 (t_i = (x_i - r) log2 e with a running reference r,
+// the largest value met):  l = sum 2^(t_i),  s = sum 2^(t_i) t_i, then
+//   log p(i) = x_i - r - ln 2 log2 l,   H = ln 2 (log2 l - s / l).
 // Every lane keeps its own (r, l, s) over the values that it meets and they are joined at the end, so
-// a row is read once.  The reference enters each t_i through one fused multiply-add and is subtracted
-// again as the same 32-bit number, so its own rounding cancels.
+// a row is read once.
 //
 // The top values: every lane keeps the maximum of what it met.  The k-th largest T of a workgroup's 256
 // maxima is no more than the k-th largest value, and only lanes whose maximum reaches T can hold a value
@@ -54,12 +53,15 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 
 __device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
 
-// (reference, sum, weighted sum) of a part of a row; r = -inf: no finite value met, sums against 0.
+// (reference, sum, weighted sum) of a part of a row; r = -inf: no finite value met, sums against 0.  The reference is a
+// value of the row and is taken off before log2 e is multiplied in: scaled first, a row of the type's lowest value
+// would overflow, and one product's rounding would be of the values' size and not of their differences'.
 struct Sums {
   float r = -INFINITY, l = 0.f, s = 0.f;
   __device__ __forceinline__ void rebase(float to) {
     if (to == r) return;
-    const float d = finite_or_zero(r) - finite_or_zero(to);
+    // no exponent below -2000, so that l d is a number
+    const float d = fmaxf((finite_or_zero(r) - finite_or_zero(to)) * kLog2e, -2000.f);
     const float f = r == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(d);  // nothing but zeros to scale
     s = f * (s + (l == 0.f ? 0.f : l * d));
     l *= f;
@@ -138,13 +140,13 @@ __device__ __forceinline__ void finish(const ScoreArgs& A, long long row, const 
     if (A.tokens) {
       float lp = 0.f;
       if (given.token >= A.vocab) lp = __uint_as_float(0x7fc00000u);
-      else if (given.token >= 0) lp = most0((__builtin_fmaf(given.logit, kLog2e, -ref) - log) * kLn2);
+      else if (given.token >= 0) lp = most0(__builtin_fmaf(-log, kLn2, given.logit - ref));
       A.given[row] = lp;
     }
   }
   if (lane < A.top) {
     A.top_ids[row * A.top + lane] = 0xffffffffu - (uint32_t)best;
-    A.top_logs[row * A.top + lane] = most0((__builtin_fmaf(value_of((uint32_t)(best >> 32)), kLog2e, -ref) - log) * kLn2);
+    A.top_logs[row * A.top + lane] = most0(__builtin_fmaf(-log, kLn2, value_of((uint32_t)(best >> 32)) - ref));
   }
 }
 
@@ -191,12 +193,11 @@ __device__ __forceinline__ void take(Sums& a, Most& most, int b, V value) {
 #pragma unroll
   for (int n = 0; n < N; ++n) m = larger(m, value(n));
   most.note(m, b);
-  const float r = fmaxf(a.r, m * kLog2e);
-  a.rebase(r);
-  const float ref = finite_or_zero(r);
+  a.rebase(fmaxf(a.r, m));
+  const float ref = finite_or_zero(a.r);
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    const float t = __builtin_fmaf(value(n), kLog2e, -ref);
+    const float t = (value(n) - ref) * kLog2e;
     const float e = __builtin_amdgcn_exp2f(t);
     a.l += e;
     a.s = __builtin_fmaf(e, fmaxf(t, -1000.f), a.s);  // 2^-inf counts nothing, and 0 * -inf would
