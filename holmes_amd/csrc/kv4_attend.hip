@@ -148,6 +148,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   for (int i = 0; i < kDpl; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, sum = 0.f, low = INFINITY;
   const float scale2 = A.scale * kLog2e;
+  float ref = -kLift, factor = scale2;
 
   // a page number that is not in the pool is read as page 0, and its tokens are left out
   auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + h) * L::kBytes; };
@@ -213,11 +214,12 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) mx = larger(mx, t[i][k]);
-    mx = fmaxf(top, over_row<R>(mx, fmax2) * scale2);
+    const float raw = over_row<R>(mx, fmax2);
+    mx = fmaxf(top, raw * scale2);
     const float f = rebase(top, mx);
     top = mx;
-    const float ref = reference(mx) - kLift;
     if (__any(f != 1.f)) {
+      if (f != 1.f) refer(mx, raw, scale2, ref, factor);
       sum *= f;
 #pragma unroll
       for (int i = 0; i < kDpl; ++i) acc[i] *= f;
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
     for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        t[i][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][k], scale2, -ref));
+        t[i][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][k], factor, -ref));
         sum += t[i][k];
       }
       hi[i] = u32x2{heads_of(t[i][0], t[i][1]), heads_of(t[i][2], t[i][3])};

@@ -265,6 +265,17 @@ __device__ __forceinline__ float rebase(float a, float b) {
   return a == b ? 1.f : __builtin_ldexpf(1.f, (int)(above(a) - above(b)));
 }
 __device__ __forceinline__ float reference(float m) { return fabsf(m) == INFINITY ? 0.f : above(m); }
+// What a row's scores are multiplied by and what then comes off: scale log2 e and the reference of its maximum m, whose
+// largest score is `raw`.  Beyond 2^27 a rounding of m is of the exponents' size, and what it took from the largest of
+// scores of 1e10 would be an exponent of 2 in infinite sums.  There the factor is the next power of 2, with which
+// both products are exact; that distances are up to twice theirs is less than the scores' own roundings.
+constexpr float kFar = 1 << 27;
+__device__ __forceinline__ void refer(float m, float raw, float scale2, float& ref, float& factor) {
+  const bool far = fabsf(m) > kFar && fabsf(m) != INFINITY;
+  const float power = __uint_as_float((__float_as_uint(scale2) + 0x7fffffu) & 0xff800000u);
+  factor = far ? power : scale2;
+  ref = (far ? raw * power : reference(m)) - kLift;
+}
 // log2 of a row's sum, against its reference.
 __device__ __forceinline__ float log2_sum(float m, float l) {
   return fabsf(m) == INFINITY ? m + l : above(m) + (__builtin_amdgcn_logf(l) - kLift);

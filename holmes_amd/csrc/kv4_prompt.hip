@@ -144,6 +144,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   float top = -INFINITY, sum = 0.f, low = INFINITY;
   const float scale2 = A.scale * kLog2e;
+  float ref = -kLift, factor = scale2;
 
   const int* table = A.table + it.b * A.table_stride;
   const uint8_t* pool = A.pool + it.h * L::kBytes;
@@ -216,11 +217,12 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = larger(mx, t[n][i]);
-      mx = fmaxf(top, over_half(mx, fmax2) * scale2);
+      const float raw = over_half(mx, fmax2);
+      mx = fmaxf(top, raw * scale2);
       const float f = rebase(top, mx);
       top = mx;
-      const float ref = reference(mx) - kLift;
       if (__any(f != 1.f)) {
+        if (f != 1.f) refer(mx, raw, scale2, ref, factor);
         sum *= f;
 #pragma unroll
         for (int d = 0; d < kTiles; ++d) acc[d] *= f;
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
         float p[8];
         uint32_t hi[4], lo[4];  // the probabilities in two bf16 parts
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[j >> 1][8 * (j & 1) + e], scale2, -ref));
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[j >> 1][8 * (j & 1) + e], factor, -ref));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           hi[e] = heads_of(p[2 * e], p[2 * e + 1]);
