@@ -11,7 +11,8 @@
 // that does: hardly more than k of them.  A lane also keeps which block of its values had the maximum and
 // the largest of the others' maxima, so that as a rule one block of it is read again (all of them cost
 // 16 % more traffic at 131072 values and k = 5).  What reaches T goes into a list and is put in order by
-// counting.  If the list runs over (many values alike), every wave keeps its k best
+// counting.  Where most lanes' maxima are one value (a mask that leaves little), the list takes what is
+// above it and the first places that hold it.  If the list runs over, every wave keeps its k best
 // in order, entry i in lane i, and goes through its values once more; they come in rising order of their
 // index, so most blocks are dismissed by one comparison.
 #include <hip/hip_runtime.h>
@@ -217,8 +218,10 @@ struct Candidates {
   __device__ __forceinline__ static uint32_t key(unsigned long long o) { return (uint32_t)(o >> 32); }
   __device__ __forceinline__ static uint32_t index(unsigned long long o) { return 0xffffffffu - (uint32_t)o; }
 
-  // A key that `top` threads' largest reach, as large as a few more allow, and how many do.
-  __device__ __forceinline__ uint32_t reach(uint32_t mine, uint32_t second, int where, int top, int& threads) {
+  // A key that `top` threads' largest reach, as large as a few more allow, and how many do.  Where many threads' largest
+  // are alike there (a mask that leaves little), the key after it, with `tied`: fewer than `top` threads reach that, and
+  // of the values just below it the first in the row's order are wanted.
+  __device__ __forceinline__ uint32_t reach(uint32_t mine, uint32_t second, int where, int top, int& threads, bool& tied) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     most[threadIdx.x] = mine;
     if (threadIdx.x == 0) count = 0;
@@ -242,6 +245,12 @@ struct Candidates {
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) n += __popcll(__ballot(k[w] >= (t | bit)));
       if (n >= top) t |= bit, threads = n;
+    }
+    tied = threads > 64 && t != 0xffffffffu;
+    if (tied) {
+      ++t, threads = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) threads += __popcll(__ballot(k[w] >= t));
     }
     int before = 0;
 #pragma unroll
@@ -334,9 +343,10 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
     listed = C.sort(A.top);
   } else if (A.top > 0) {
     int threads;
+    bool tied;
     const bool nan = a.l != a.l;
     const uint32_t least = C.reach(nan ? 0xffffffffu : key_of(most.top), nan ? 0xffffffffu : key_of(most.second), most.block,
-                                   A.top, threads);
+                                   A.top, threads, tied);
     listed = threads <= 64;
     if (listed) {
       const int per = (blocks - (int)blockIdx.x * kWaves + stride - 1) / stride * kVecs;  // pieces of a thread, at most
@@ -348,7 +358,14 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
 #pragma unroll
         for (int e = 0; e < kPer; ++e) C.offer(key_of(element<T>(x4, e)), (uint32_t)(head + p * kPer + e), least);
       }
-      if (heads && lane < head) C.offer(key_of((float)x[lane]), (uint32_t)lane, least);
+      if (heads && lane < head) C.offer(key_of((float)x[lane]), (uint32_t)lane, least - tied);
+      if (tied && wave == 0) {  // the workgroup's first 64 values behind the head
+        const int i = head + first * 64 * kVecs * kPer + lane;
+        if (i < tail) {
+          const uint32_t k = key_of((float)x[i]);
+          if (k == least - 1) C.offer(k, (uint32_t)i, k);
+        }
+      }
       if (tails && tail + lane < A.vocab) C.offer(key_of((float)x[tail + lane]), (uint32_t)(tail + lane), least);
       listed = C.sort(A.top);
     }
@@ -418,9 +435,21 @@ __global__ __launch_bounds__(kThreads) void k_join(ScoreArgs A) {
       most = o[j] > most ? o[j] : most;
     }
     int threads;
-    const uint32_t least = max(1u, C.reach(Candidates::key(most), 0, -1, A.top, threads));
+    bool tied;
+    const uint32_t least = max(1u, C.reach(Candidates::key(most), 0, -1, A.top, threads, tied));
+    uint32_t tie = 0, from = 0xffffffffu;  // the key below `least`, and its first places (larger: earlier)
+    if (tied && least > 1) {
+      tie = least - 1;
+      uint32_t place = 0;
 #pragma unroll
-    for (int j = 0; j < kMost; ++j) C.offer(Candidates::key(o[j]), Candidates::index(o[j]), least);
+      for (int j = 0; j < kMost; ++j) place = Candidates::key(o[j]) == tie ? max(place, (uint32_t)o[j]) : place;
+      from = max(1u, C.reach(place, 0, -1, A.top, threads, tied));
+    }
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+      const uint32_t k = Candidates::key(o[j]);
+      C.offer(k, Candidates::index(o[j]), tie && k == tie && (uint32_t)o[j] >= from ? tie : least);
+    }
     if (!C.sort(A.top)) {
       Best best;
       if (threadIdx.x < 64) {
