@@ -111,6 +111,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   constexpr int kSteps = D / 32, kDpl = L::kDpl;
   constexpr bool kHalf = __is_same(T, _Float16);
   __shared__ float s_m[kWaves][kFew], s_l[kWaves][kFew], s_low[kWaves][kFew];
+  __shared__ uint32_t s_large[kWaves];
   extern __shared__ float s_o[];  // [wave][A.rows][D + 4]
 
   Item it;
@@ -149,6 +150,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   float top = -INFINITY, sum = 0.f, low = INFINITY;
   const float scale2 = A.scale * kLog2e;
   float ref = -kLift, factor = scale2;
+  uint32_t large = 0;  // runs whose sums are held times 2^-56
 
   // a page number that is not in the pool is read as page 0, and its tokens are left out
   auto page_of = [&](int pg) { return A.pool + ((long long)(pg < 0 || pg >= A.pages ? 0 : pg) * A.heads + h) * L::kBytes; };
@@ -252,16 +254,35 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
       float sc[8];
       // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  It is taken
       // as zeros here, and counted for the rows that see it by a product of truth values.
-      const bool odd = __any(has_nan(vs[0]) || has_nan(vs[1]));
-      if (odd) {
+      if (__builtin_expect(large || __any(has_large(vs[0]) || has_large(vs[1])), false)) {
         bf16x8 bad, see;
+        bool beyond = false;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const bool is = ((vs[k >> 2] >> (8 * (k & 3))) & 0xffu) == kNanByte;
+          const uint32_t byte = (vs[k >> 2] >> (8 * (k & 3))) & 0xffu;
+          const int token = base + 32 * i + 16 * (k >> 2) + (k & 3);
+          const bool is = byte == kNanByte;
           bad[k] = (__bf16)(is ? 1.f : 0.f);
-          see[k] = (__bf16)(base + 32 * i + 16 * (k >> 2) + (k & 3) < seen ? 1.f : 0.f);
+          see[k] = (__bf16)(token < seen ? 1.f : 0.f);
           if (is) vs[k >> 2] &= ~(0xffu << (8 * (k & 3)));
+          else beyond = beyond || (byte >= kLargeByte && token < most);
         }
+        const unsigned long long all4 = __ballot(beyond);
+        uint32_t lanes = (uint32_t)all4 | (uint32_t)(all4 >> 32), runs = 0;
+        lanes |= lanes >> 16;  // of every g
+#pragma unroll
+        for (int r = 0; r < L::kRuns; ++r)  // a run's lanes: kRun / kDpl neighbours
+          runs |= (lanes >> (r * (kRun / kDpl))) & ((1u << (kRun / kDpl)) - 1) ? 1u << r : 0u;
+        int here = lane;  // (worked out here and not kept from before the loop)
+        asm volatile("" : "+v"(here));
+        if (const uint32_t fresh = runs & ~large) {
+          large |= fresh;
+          if ((fresh >> ((here >> 4) * (D / 4) / kRun)) & 1) {
+#pragma unroll
+            for (int d = 0; d < kDpl; ++d) acc[d] *= kDownBy;
+          }
+        }
+        if ((large >> ((here & 15) * kDpl / kRun)) & 1) vs[0] = down(vs[0]), vs[1] = down(vs[1]);
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
         const f32x4 n = mfma(bad, see, zero);
 #pragma unroll
@@ -303,6 +324,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
       if constexpr (R <= 4) acc[d][i] += turn<4>(acc[d][i]);
     }
   if (lane < R) s_m[wave][m] = top, s_l[wave][m] = sum, s_low[wave][m] = low;
+  if (lane == 0) s_large[wave] = large;
   if (m < R && m < A.rows) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -314,28 +336,31 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
   const int r = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * kCols;
   if (r >= A.rows || tile * kFew + r >= rows) return;
   float mm = -INFINITY, ll = 0.f, lo = INFINITY, o[kCols];
+  uint32_t any = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, s_m[w][r]);
+  for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, s_m[w][r]), any |= s_large[w];
 #pragma unroll
   for (int c = 0; c < kCols; ++c) o[c] = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const float f = rebase(s_m[w][r], mm);
+    float f = rebase(s_m[w][r], mm);
     ll += f * s_l[w][r];
     lo = fminf(lo, s_low[w][r]);
+    f *= to_common(s_large[w], any, c0 / kRun);
 #pragma unroll
     for (int c = 0; c < kCols; ++c) o[c] += f * s_o[(w * A.rows + r) * (D + 4) + c0 + c];
   }
   if (it.slots > 1) {
     const long long at = (long long)it.slot * A.rows + r;
-    if (c0 == 0) *reinterpret_cast<f32x4*>(A.stat + at * 4) = f32x4{mm, ll, lo, 0.f};
+    if (c0 == 0) *reinterpret_cast<f32x4*>(A.stat + at * 4) = f32x4{mm, ll, lo, __uint_as_float(any)};
 #pragma unroll
     for (int c = 0; c < kCols; c += 4)
       *reinterpret_cast<f32x4*>(A.sums + at * D + c0 + c) = f32x4{o[c], o[c + 1], o[c + 2], o[c + 3]};
     return;
   }
   const int qr = (tile * kFew + r) / A.group, qc = (tile * kFew + r) % A.group;
-  store_row<T, kCols, RANGE>(A, (q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, c0, mm, ll, lo, o);
+  store_row<T, kCols, RANGE>(A, (q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, c0, mm, ll, lo, o,
+                             back(any, c0 / kRun));
 }
 
 // Joins the slots of a row of few, where it has more than one: one workgroup a row, its W waves taking 8 slots
@@ -345,6 +370,7 @@ template <typename T, int D, bool RANGE, int W>
 __global__ __launch_bounds__(64 * W) void k_join_few(AttendArgs A) {
   constexpr int kCols = D / 64, kBatch = 8;
   __shared__ float s_m[W], s_l[W], s_low[W], s_o[W][D];
+  __shared__ uint32_t s_large[W];
   const int pair = blockIdx.x / A.heads, h = blockIdx.x % A.heads;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slot = A.plan[2 * blockIdx.x], slots = A.plan[2 * blockIdx.x + 1];  // nothing there, if no rows
@@ -355,6 +381,8 @@ __global__ __launch_bounds__(64 * W) void k_join_few(AttendArgs A) {
   const float* stat = A.stat + at * 4;
   const float* sums = A.sums + at * D + lane * kCols;
   float top = -INFINITY, ll = 0.f, lo = INFINITY, o[kCols] = {};
+  uint32_t large = 0;
+  const int run = lane * kCols / kRun;
   for (int s0 = wave; s0 < slots; s0 += kBatch * W) {
     f32x4 st[kBatch];
     float x[kBatch][kCols];
@@ -366,43 +394,48 @@ __global__ __launch_bounds__(64 * W) void k_join_few(AttendArgs A) {
       for (int c = 0; c < kCols; ++c) x[i][c] = sums[s * step * D + c];
     }
     float m = top;
+    uint32_t any = large;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) m = fmaxf(m, st[i][0]);
-    const float f = rebase(top, m);
+    for (int i = 0; i < kBatch; ++i) m = fmaxf(m, st[i][0]), any |= __float_as_uint(st[i][3]);
+    float f = rebase(top, m);
     top = m;
     ll *= f;
+    f *= to_common(large, any, run);
+    large = any;
 #pragma unroll
     for (int c = 0; c < kCols; ++c) o[c] *= f;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (s0 + i * W >= slots) break;
-      const float e = rebase(st[i][0], m);
+      float e = rebase(st[i][0], m);
       ll += e * st[i][1];
       lo = fminf(lo, st[i][2]);
+      e *= to_common(__float_as_uint(st[i][3]), large, run);
 #pragma unroll
       for (int c = 0; c < kCols; ++c) o[c] += e * x[i][c];
     }
   }
-  if (lane == 0) s_m[wave] = top, s_l[wave] = ll, s_low[wave] = lo;
+  if (lane == 0) s_m[wave] = top, s_l[wave] = ll, s_low[wave] = lo, s_large[wave] = large;
 #pragma unroll
   for (int c = 0; c < kCols; ++c) s_o[wave][lane * kCols + c] = o[c];
   __syncthreads();
   if (wave != 0) return;
 #pragma unroll
-  for (int w = 1; w < W; ++w) top = fmaxf(top, s_m[w]);
+  for (int w = 1; w < W; ++w) top = fmaxf(top, s_m[w]), large |= s_large[w];
   ll = 0.f;
 #pragma unroll
   for (int c = 0; c < kCols; ++c) o[c] = 0.f;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    const float f = rebase(s_m[w], top);
+    float f = rebase(s_m[w], top);
     ll += f * s_l[w];
     lo = fminf(lo, s_low[w]);
+    f *= to_common(s_large[w], large, run);
 #pragma unroll
     for (int c = 0; c < kCols; ++c) o[c] += f * s_o[w][lane * kCols + c];
   }
   store_row<T, kCols, RANGE>(A, (R.q0 + row / A.group) * (long long)(A.heads * A.group) + h * A.group + row % A.group, D,
-                             lane * kCols, top, ll, lo, o);
+                             lane * kCols, top, ll, lo, o, back(large, run));
 }
 
 // The same of many rows, which have few slots each: D / 4 threads a row, a workgroup a 4th to a 16th of a tile
@@ -422,8 +455,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_join_many(AttendArgs A) {
     const float* stat = A.stat + at * 4;
     const float* sums = A.sums + at * D + c0;
     float top = -INFINITY, ll = 0.f, lo = INFINITY;
+    uint32_t large = 0;
 #pragma unroll 4
-    for (int s = 0; s < slots; ++s) top = fmaxf(top, stat[s * step * 4]);
+    for (int s = 0; s < slots; ++s) top = fmaxf(top, stat[s * step * 4]), large |= __float_as_uint(stat[s * step * 4 + 3]);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = 0; s < slots; ++s) {
@@ -432,11 +466,12 @@ __global__ __launch_bounds__(64 * kWaves) void k_join_many(AttendArgs A) {
       const float f = rebase(st[0], top);
       ll += f * st[1];
       lo = fminf(lo, st[2]);
-      o += f * x;
+      o += f * to_common(__float_as_uint(st[3]), large, c0 / kRun) * x;
     }
     const float v[4] = {o[0], o[1], o[2], o[3]};
     const int qr = (first + r) / A.group, qc = (first + r) % A.group;
-    store_row<T, 4, RANGE>(A, (R.q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, c0, top, ll, lo, v);
+    store_row<T, 4, RANGE>(A, (R.q0 + qr) * (long long)(A.heads * A.group) + h * A.group + qc, D, c0, top, ll, lo, v,
+                            back(large, c0 / kRun));
   }
 }
 

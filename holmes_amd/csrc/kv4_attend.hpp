@@ -21,9 +21,14 @@ constexpr int kWaves = 4;
 constexpr int kComputeUnits = 256;
 constexpr int kFew = 16;    // rows of k_attend's workgroup
 // Exponentials are taken times 2^24, so that those from 2^-126 to 2^-150 of a row's largest, which the
-// exponential instruction gives as 0, still count where every larger one meets a value of 0.  Sums then
-// stay finite for values up to 2^103 over the number of tokens.
+// exponential instruction gives as 0, still count where every larger one meets a value of 0.
 constexpr float kLift = 24.f;
+// Sums of such exponentials and values below 6 2^72 stay finite over 2^29 tokens of a wave.  Where a token that is seen
+// has a larger unit (a scale byte of kLargeByte or more; values reach 6 2^125), the sums of its run of 32 dims go over to
+// values times 2^-56, and its scale bytes are that much less from there on (1 at the least: values below 2^-69 no longer
+// count beside those of 2^73).
+constexpr int kLargeByte = 200, kDown = 56;
+constexpr float kDownBy = 0x1p-56f, kUpBy = 0x1p56f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttendArgs {
@@ -34,7 +39,8 @@ struct AttendArgs {
   const int* starts;   // null: sequence b has the one query b
   void* out;
   float *lse, *low, *high;  // [token][query head]; low, high nullable
-  // with `join`: [slot][row] of (m, l, low, -), [slot][row][D] of sums, and [tile][head] of (first slot, slots)
+  // with `join`: [slot][row] of (m, l, low, runs that are summed times 2^-56, a bit each), [slot][row][D] of sums, and
+  // [tile][head] of (first slot, slots)
   float *stat, *sums;
   int* plan;
   long long q_ts, q_hs, tokens, pages;
@@ -215,6 +221,25 @@ __device__ __forceinline__ bool has_nan(uint32_t w) {  // a byte of 255 among th
   return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u;
 }
 
+__device__ __forceinline__ bool has_large(uint32_t w) {  // a byte of kLargeByte or more, 255 among them
+  return ((w & 0x7f7f7f7fu) + (256 - kLargeByte) * 0x01010101u) & w & 0x80808080u;
+}
+// Scale bytes of a run whose sums are held times 2^-56 (0, which stands for a run of NaN here, stays).
+__device__ __forceinline__ uint32_t down(uint32_t w) {
+  uint32_t to = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t b = (w >> (8 * j)) & 0xffu;
+    to |= (b > kDown ? b - kDown : min(b, 1u)) << (8 * j);
+  }
+  return to;
+}
+// What sums of a run are multiplied by before they join others of which `any` has the runs held times 2^-56.
+__device__ __forceinline__ float to_common(uint32_t mine, uint32_t any, int run) {
+  return ((any & ~mine) >> run) & 1 ? kDownBy : 1.f;
+}
+__device__ __forceinline__ float back(uint32_t large, int run) { return (large >> run) & 1 ? kUpBy : 1.f; }
+
 // Eight values of a query as one bf16 operand, or, of fp16, as the sum of two.
 template <typename T>
 __device__ __forceinline__ void query_parts(u32x4 raw, bf16x8& head, bf16x8& rest) {
@@ -296,15 +321,15 @@ __device__ __forceinline__ uint32_t rests_of(float a0, float a1, uint32_t h) {
               __builtin_amdgcn_fdot2_f32_bf16(x, __builtin_bit_cast(bf16x2, high), a1, false));
 }
 
-// A row's results from its sums: maximum m in units of log 2, sum l, `N` values from dim d0.
+// A row's results from its sums: maximum m in units of log 2, sum l, `N` values from dim d0, times `up`.
 template <typename T, int N, bool RANGE>
 __device__ __forceinline__ void store_row(const AttendArgs& A, long long at, int dim, int d0, float m, float l, float low,
-                                          const float* o) {
+                                          const float* o, float up) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
   typedef T vec __attribute__((ext_vector_type(N)));
   vec x;
 #pragma unroll
-  for (int c = 0; c < N; ++c) x[c] = (T)(o[c] * inv);
+  for (int c = 0; c < N; ++c) x[c] = (T)(o[c] * inv * up);
   *reinterpret_cast<vec*>((T*)A.out + at * dim + d0) = x;
   if (d0 == 0) {
     const bool bad = l != l;

@@ -59,9 +59,10 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// Writes the thread's share; whether it holds a run of NaN among the values, which are taken as zeros.
+// Writes the thread's share, values of the runs `large` times 2^-56; whether it holds a run of NaN among the values, which
+// are taken as zeros.
 template <int D, int W>
-__device__ __forceinline__ bool store(Operands<D>& o, const Share<D, W>& x, int wave, int lane) {
+__device__ __forceinline__ bool store(Operands<D>& o, const Share<D, W>& x, int wave, int lane, uint32_t large) {
   constexpr int kWords = Share<D, W>::kWords;
   const int m = lane & 15, g = lane >> 4, quarter = wave & 3, part = (wave >> 2) * kWords;
   const float sc = x.ks == kNanByte ? __uint_as_float(0x7fc00000u) : __uint_as_float(x.ks << 23);
@@ -76,6 +77,7 @@ __device__ __forceinline__ bool store(Operands<D>& o, const Share<D, W>& x, int 
     for (int j = 0; j < 4; ++j)
       if (((vs >> (8 * j)) & 0xffu) == kNanByte) vs &= ~(0xffu << (8 * j));
   }
+  if ((large >> (m * Kv4<D>::kDpl / kRun)) & 1) vs = down(vs);
   float f[4];
   uint32_t v[D / 32];
 #pragma unroll
@@ -103,6 +105,19 @@ __device__ __forceinline__ bool store(Operands<D>& o, const Share<D, W>& x, int 
   return odd;
 }
 
+// The bit of the thread's run, if one of its tokens before `most` has a unit of kLargeByte or more.
+template <int D, int W>
+__device__ __forceinline__ uint32_t large_run(const Share<D, W>& x, int wave, int lane, int unit, int most) {
+  const int first = unit * kUnit + ((wave & 3) >> 1) * 32 + (wave & 1) * 16 + (lane >> 4) * 4;
+  bool is = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t byte = (x.vs >> (8 * j)) & 0xffu;
+    is = is || (byte >= kLargeByte && byte != kNanByte && first + j < most);
+  }
+  return is ? 1u << ((lane & 15) * Kv4<D>::kDpl / kRun) : 0;
+}
+
 template <typename T, int D, bool RANGE, int W>
 __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs A) {
   using L = Kv4<D>;
@@ -111,6 +126,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   constexpr int kStep = W / 4;  // units between two barriers: a page where the LDS is one workgroup's
   __shared__ Operands<D> s_x[2][kStep];
   __shared__ int s_odd[2][kStep];  // 1 + the unit whose values hold a run of NaN
+  __shared__ uint32_t s_large[2];  // runs with units of kLargeByte or more, a bit each
 
   Item it;
   if (!locate(A, blockIdx.x, it)) return;
@@ -145,6 +161,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   float top = -INFINITY, sum = 0.f, low = INFINITY;
   const float scale2 = A.scale * kLog2e;
   float ref = -kLift, factor = scale2;
+  uint32_t large = 0;  // runs whose sums are held times 2^-56, the workgroup's
 
   const int* table = A.table + it.b * A.table_stride;
   const uint8_t* pool = A.pool + it.h * L::kBytes;
@@ -152,31 +169,48 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   auto page_of = [&](int pg) { return pool + (pg < 0 || pg >= A.pages ? 0 : pg) * each; };
   const typename Share<D, W>::Offsets offsets(wave, lane);
   Share<D, W> x[kStep];
-  auto load = [&](int pg, int first) {
-    const uint8_t* page = page_of(pg);
+  auto load = [&](Share<D, W>* x, const uint8_t* page, int first) {
 #pragma unroll
     for (int n = 0; n < kStep; ++n) x[n].load(page, kStep == 2 ? n : first & 1, offsets);
   };
   int pg = 0, next = 0, step = u0 / kStep * kStep;
   if (threadIdx.x < 2 * kStep) s_odd[threadIdx.x / kStep][threadIdx.x % kStep] = 0;
+  if (threadIdx.x < 2) s_large[threadIdx.x] = 0;
   if (step < u1) {
     pg = __builtin_amdgcn_readfirstlane(table[step >> 1]);
-    load(pg, step);
+    load(x, page_of(pg), step);
     if (step + kStep < u1) next = table[(step + kStep) >> 1];
   }
   __syncthreads();
   for (int turn = 0; step < u1; step += kStep, turn ^= 1) {
     Operands<D>(&os)[kStep] = s_x[turn];
-#pragma unroll
-    for (int n = 0; n < kStep; ++n)
-      if (store(os[n], x[n], wave, lane)) s_odd[turn][n] = step + n + 1;
     const bool there = pg >= 0 && pg < A.pages;
+#pragma unroll
+    for (int n = 0; n < kStep; ++n) {
+      if (store(os[n], x[n], wave, lane, large)) s_odd[turn][n] = step + n + 1;
+      if (there && has_large(x[n].vs)) atomicOr(&s_large[turn], large_run(x[n], wave, lane, step + n, most));
+    }
     const uint8_t* page = page_of(pg);
     pg = __builtin_amdgcn_readfirstlane(next);
-    if (step + kStep < u1) load(pg, step + kStep);
+    if (step + kStep < u1) load(x, page_of(pg), step + kStep);
     if (step + 2 * kStep < u1) next = table[(step + 2 * kStep) >> 1];
     __syncthreads();
     if (!there) continue;
+    if (const uint32_t fresh = __builtin_amdgcn_readfirstlane(s_large[turn]) & ~large) {
+      // the first such units of their runs: the same for all waves, which make this step's operands again
+      large |= fresh;
+      Share<D, W> again[kStep];
+      load(again, page, step);
+#pragma unroll
+      for (int n = 0; n < kStep; ++n) store(os[n], again[n], wave, lane, large);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if ((fresh >> ((i >> 2) * (D / 4) / kRun)) & 1) {  // registers 4 q .. 4 q + 3 have dims D / 4 q ..
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d) acc[d][i] *= kDownBy;
+        }
+    }
 #pragma unroll 1
     for (int n = 0; n < kStep; ++n) {
       const int u = step + n;
@@ -293,7 +327,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
   const int qr = row / A.group, qc = row % A.group;
   const long long out = (S.q0 + qr) * (long long)(A.heads * A.group) + it.h * A.group + qc;
   const long long at = (long long)it.slot * A.rows + (row - first);
-  if (it.slots > 1 && h == 0) *reinterpret_cast<f32x4*>(A.stat + at * 4) = f32x4{top, sum, low, 0.f};
+  if (it.slots > 1 && h == 0) *reinterpret_cast<f32x4*>(A.stat + at * 4) = f32x4{top, sum, low, __uint_as_float(large)};
   // registers 4 q + 2 p + b of tile d: dim (2 h + 4 q + p) kDpl + 2 d + b of the lane's row
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -305,7 +339,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
 #pragma unroll
       for (int d = 0; d < kDpl; d += 4) *reinterpret_cast<f32x4*>(A.sums + at * D + d0 + d) = f32x4{v[d], v[d + 1], v[d + 2], v[d + 3]};
     } else {
-      store_row<T, kDpl, RANGE>(A, out, D, d0, top, sum, low, v);
+      store_row<T, kDpl, RANGE>(A, out, D, d0, top, sum, low, v, back(large, d0 / kRun));
     }
   }
 }
