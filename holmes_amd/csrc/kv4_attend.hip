@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
         t[i][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][k], factor, -ref));
         sum += t[i][k];
       }
-      hi[i] = u32x2{heads_of(t[i][0], t[i][1]), heads_of(t[i][2], t[i][3])};
+      hi[i] = u32x2{pack(t[i][0], t[i][1]), pack(t[i][2], t[i][3])};
       lo[i] = u32x2{rests_of(t[i][0], t[i][1], hi[i][0]), rests_of(t[i][2], t[i][3], hi[i][1])};
     }
 

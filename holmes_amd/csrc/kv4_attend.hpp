@@ -306,11 +306,7 @@ __device__ __forceinline__ float log2_sum(float m, float l) {
   return fabsf(m) == INFINITY ? m + l : above(m) + (__builtin_amdgcn_logf(l) - kLift);
 }
 
-// Packs the upper halves of two numbers.
-__device__ __forceinline__ uint32_t heads_of(float a, float b) {
-  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-}
-// What they leave: a0 - h0 and a1 - h1 for h of two such halves, each in one instruction (times 1 and 0: exact).
+// What two numbers' nearest bf16 leave: a0 - h0 and a1 - h1, each in one instruction (times 1 and 0: exact).
 // The factors (-1, 0) and (0, -1) come out of registers: as constants the compiler makes them one inline -1.0.
 __device__ __forceinline__ uint32_t rests_of(float a0, float a1, uint32_t h) {
   uint32_t low, high;

@@ -302,7 +302,7 @@ __global__ __launch_bounds__(64 * W, waves_of_many(D)) void k_prompt(AttendArgs 
         for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[j >> 1][8 * (j & 1) + e], factor, -ref));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          hi[e] = heads_of(p[2 * e], p[2 * e + 1]);
+          hi[e] = pack(p[2 * e], p[2 * e + 1]);
           lo[e] = rests_of(p[2 * e], p[2 * e + 1], hi[e]);
           part[e & 1] += p[2 * e] + p[2 * e + 1];
         }
