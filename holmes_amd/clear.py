@@ -142,7 +142,7 @@ class ClearKVPages:
         ``causal`` off, all.  ``most`` bounds the queries of one sequence (default: 1 without ``starts``, else
         all rows) and only saves work; a sequence with more has the rest left unwritten, as has any row that no
         sequence covers.  A page outside the pool counts as tokens that are not there.  ``scale`` multiplies
-        the scores (default head_dim^-1/2); ``ranges`` asks for their least and largest."""
+        the scores (default head_dim^-1/2; at most 2^126); ``ranges`` asks for their least and largest."""
 
         got = self._native.attend(*self._pool, queries, table, lengths, starts, most, causal, scale, ranges)
         if type(got) is int:

@@ -155,7 +155,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     scale = PyFloat_AsDouble(a[11]);
     if (scale == -1.0 && PyErr_Occurred()) throw python_error();
   }
-  need(scale > 0.0 && std::isfinite(scale), "scale must be positive and finite");
+  need((float)scale > 0.f && scale <= 0x1p126, "scale must be positive, and 2^126 at most");
   const int64_t group = heads / p.heads;
   // what the C entry point's arguments do not hold, it could not refuse itself
   need(seqs <= INT32_MAX && group <= INT32_MAX && most <= INT32_MAX && cols <= INT32_MAX, "too many sequences, heads or columns");

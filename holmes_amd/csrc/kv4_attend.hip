@@ -530,7 +530,8 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
                               size_t workspace_bytes, void* stream) {
   if (hck::kv4_bytes(head_dim) == 0 || (type != HCK_BF16 && type != HCK_F16)) return HCK_ERR_UNSUPPORTED;
   if (!pool || pages < 1 || !hck::shape_ok(tokens, seqs, kv_heads, group, most, table_columns)) return HCK_ERR_ARG;
-  if (!(scale > 0.f) || scale > 3.0e38f || (low == nullptr) != (high == nullptr)) return HCK_ERR_ARG;
+  // (times log2 e it is at most 2^127, and so is the power of 2 that stands for it beyond kFar)
+  if (!(scale > 0.f) || scale > 0x1p126f || (low == nullptr) != (high == nullptr)) return HCK_ERR_ARG;
   if (tokens == 0 || seqs == 0 || most == 0) return HCK_OK;
   if (!queries || !lengths || (!table && table_columns > 0) || !out || !lse) return HCK_ERR_ARG;
   if (!starts && tokens < seqs) return HCK_ERR_ARG;
