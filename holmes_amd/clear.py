@@ -17,7 +17,7 @@ b for each run of 32 values along the head dimension: b is the exponent of the r
 rounded to one mantissa bit, less 2 (kept in 2..252), so the largest becomes 4 or 6 units and no value is
 off by more than half a step.  A run that holds an infinity or a NaN is held, and read, as NaN.
 
-Everything runs in libholmes_ckks on the current stream without synchronising; there is no CPU path.
+Everything runs in libholmes_ckks on the current stream of its tensors' device without synchronising; there is no CPU path.
 """
 
 from __future__ import annotations

@@ -7,6 +7,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -48,6 +49,7 @@ long long whole(PyObject* o) {
 PyObject* wrap(Tensor t) { return THPVariable_Wrap(std::move(t)); }
 PyObject* none() { return Py_NewRef(Py_None); }
 
+// (A launch goes to the current device, whatever the stream: each call makes its tensors' device that first.)
 void* stream_of(at::DeviceIndex index) { return (void*)c10::hip::getCurrentHIPStream(index).stream(); }
 
 Tensor make(at::IntArrayRef size, ScalarType type, at::Device device) {
@@ -91,6 +93,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         x->scalar_type() != k.scalar_type() || x->device() != p.device)
       refuse("keys and values must be [" + std::to_string(tokens) + ", " + std::to_string(p.heads) + ", " +
              std::to_string(p.dim) + "], contiguous along the last axis, in one type on the pool's device");
+  const c10::DeviceGuard guard(p.device);
   return PyLong_FromLong(hck_kv4_append(p.at, p.pages, p.heads, p.dim, type, k.data_ptr(), k.stride(0), k.stride(1),
                                         v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr<int64_t>(), tokens,
                                         stream_of(p.device.index())));
@@ -108,6 +111,7 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int type = type_of(out);
   need(type >= 0, "dtype must be bfloat16, float16 or float32");
   const int64_t tokens = slots.numel();
+  const c10::DeviceGuard guard(p.device);
   Tensor k = make({tokens, p.heads, p.dim}, out, p.device), v = make({tokens, p.heads, p.dim}, out, p.device);
   const int err = hck_kv4_read(p.at, p.pages, p.heads, p.dim, type, slots.data_ptr<int64_t>(), tokens, k.data_ptr(),
                                v.data_ptr(), stream_of(p.device.index()));
@@ -159,6 +163,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t group = heads / p.heads;
   // what the C entry point's arguments do not hold, it could not refuse itself
   need(seqs <= INT32_MAX && group <= INT32_MAX && most <= INT32_MAX && cols <= INT32_MAX, "too many sequences, heads or columns");
+  const c10::DeviceGuard guard(p.device);
   Tensor out = make({tokens, heads, p.dim}, q.scalar_type(), p.device), lse = make({tokens, heads}, at::kFloat, p.device);
   Tensor low, high, work;
   if (ranges) {
@@ -204,6 +209,7 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return nullptr;
   }
   const at::Device dev = x.device();
+  const c10::DeviceGuard guard(dev);
   Tensor entropy = make({rows}, at::kFloat, dev), given, ids, logs, work;
   if (tokens.defined()) given = make({rows}, at::kFloat, dev);
   if (top) {
