@@ -102,7 +102,7 @@ class ClearKVPages:
         self.buf = torch.zeros((self.pages, self.kv_heads, self._lib.hck_kv4_page_bytes(self.head_dim)),
                                dtype=torch.uint8, device=device)
         self._native = _bound()
-        self._pool = (self.buf.data_ptr(), self.pages, self.kv_heads, self.head_dim, self.buf.device.index)
+        self._shape = (self.pages, self.kv_heads, self.head_dim, self.buf.device.index)
 
     @property
     def device(self) -> torch.device:
@@ -117,7 +117,7 @@ class ClearKVPages:
         the last axis contiguous) into ``slots`` [tokens].  A slot outside the pool, as -1 for padding, leaves
         its token out; the slots of one call must differ."""
 
-        err = self._native.append(*self._pool, keys, values, slots)
+        err = self._native.append(self.buf, *self._shape, keys, values, slots)
         if err:
             nat.check(err, "hck_kv4_append")
 
@@ -125,7 +125,7 @@ class ClearKVPages:
         """What ``slots`` hold, as ``(keys, values)`` [tokens][kv_heads][head_dim] in ``dtype``: exact in bf16
         and fp32; in fp16 rounded, with its largest value for any above.  Zeros for a slot outside the pool."""
 
-        got = self._native.read(*self._pool, slots, dtype)
+        got = self._native.read(self.buf, *self._shape, slots, dtype)
         if type(got) is int:
             nat.check(got, "hck_kv4_read")
         return got
@@ -144,7 +144,7 @@ class ClearKVPages:
         sequence covers.  A page outside the pool counts as tokens that are not there.  ``scale`` multiplies
         the scores (default head_dim^-1/2; at most 2^126); ``ranges`` asks for their least and largest."""
 
-        got = self._native.attend(*self._pool, queries, table, lengths, starts, most, causal, scale, ranges)
+        got = self._native.attend(self.buf, *self._shape, queries, table, lengths, starts, most, causal, scale, ranges)
         if type(got) is int:
             nat.check(got, "hck_kv4_attend")
         return Attended._make(got)

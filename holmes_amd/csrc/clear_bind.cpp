@@ -56,15 +56,24 @@ Tensor make(at::IntArrayRef size, ScalarType type, at::Device device) {
   return at::detail::empty_cuda(size, type, device, std::nullopt);
 }
 
-// A pool: its address, pages, key heads, head dimension and device, as the first five arguments.
+// A pool: its bytes, pages, key heads, head dimension and device, as the first five arguments.
 struct Pool {
-  void* at;
+  PyObject* buf;
   int64_t pages;
   int heads, dim;
   at::Device device;
   explicit Pool(PyObject* const* a)
-      : at((void*)whole(a[0])), pages(whole(a[1])), heads((int)whole(a[2])), dim((int)whole(a[3])),
+      : buf(a[0]), pages(whole(a[1])), heads((int)whole(a[2])), dim((int)whole(a[3])),
         device(at::kCUDA, (at::DeviceIndex)whole(a[4])) {}
+  // The address of its bytes.  They are a tensor that a program can replace or resize: asked for at each call.
+  void* at() const {
+    const Tensor& t = tensor(buf, "the pool's buf");
+    const int64_t bytes = pages * heads * (int64_t)hck_kv4_page_bytes(dim);
+    need(t.scalar_type() == at::kByte && t.device() == device && t.numel() == bytes && t.is_contiguous() &&
+             t.storage_offset() + bytes <= (int64_t)t.storage().nbytes(),
+         "the pool's buf must be its pages' bytes, contiguous uint8 on the pool's device");
+    return t.data_ptr();
+  }
 };
 
 Tensor slots_of(PyObject* o, const Pool& p) {
@@ -93,8 +102,9 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         x->scalar_type() != k.scalar_type() || x->device() != p.device)
       refuse("keys and values must be [" + std::to_string(tokens) + ", " + std::to_string(p.heads) + ", " +
              std::to_string(p.dim) + "], contiguous along the last axis, in one type on the pool's device");
+  void* at = p.at();
   const c10::DeviceGuard guard(p.device);
-  return PyLong_FromLong(hck_kv4_append(p.at, p.pages, p.heads, p.dim, type, k.data_ptr(), k.stride(0), k.stride(1),
+  return PyLong_FromLong(hck_kv4_append(at, p.pages, p.heads, p.dim, type, k.data_ptr(), k.stride(0), k.stride(1),
                                         v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr<int64_t>(), tokens,
                                         stream_of(p.device.index())));
   END_HANDLE_TH_ERRORS
@@ -111,9 +121,10 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int type = type_of(out);
   need(type >= 0, "dtype must be bfloat16, float16 or float32");
   const int64_t tokens = slots.numel();
+  const void* at = p.at();
   const c10::DeviceGuard guard(p.device);
   Tensor k = make({tokens, p.heads, p.dim}, out, p.device), v = make({tokens, p.heads, p.dim}, out, p.device);
-  const int err = hck_kv4_read(p.at, p.pages, p.heads, p.dim, type, slots.data_ptr<int64_t>(), tokens, k.data_ptr(),
+  const int err = hck_kv4_read(at, p.pages, p.heads, p.dim, type, slots.data_ptr<int64_t>(), tokens, k.data_ptr(),
                                v.data_ptr(), stream_of(p.device.index()));
   if (err) return PyLong_FromLong(err);
   return Py_BuildValue("(NN)", wrap(std::move(k)), wrap(std::move(v)));
@@ -163,6 +174,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t group = heads / p.heads;
   // what the C entry point's arguments do not hold, it could not refuse itself
   need(seqs <= INT32_MAX && group <= INT32_MAX && most <= INT32_MAX && cols <= INT32_MAX, "too many sequences, heads or columns");
+  const void* at = p.at();
   const c10::DeviceGuard guard(p.device);
   Tensor out = make({tokens, heads, p.dim}, q.scalar_type(), p.device), lse = make({tokens, heads}, at::kFloat, p.device);
   Tensor low, high, work;
@@ -174,7 +186,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       hck_kv4_attend_workspace_bytes(tokens, (int)seqs, p.heads, (int)group, p.dim, (int)most, (int)cols);
   if (bytes) work = make({(int64_t)bytes}, at::kByte, p.device);
   const int err = hck_kv4_attend(
-      p.at, p.pages, p.heads, p.dim, type, q.data_ptr(), tokens, (int)group, q.stride(0), q.stride(1),
+      at, p.pages, p.heads, p.dim, type, q.data_ptr(), tokens, (int)group, q.stride(0), q.stride(1),
       table.data_ptr<int32_t>(), table.stride(0), (int)cols, lengths.data_ptr<int32_t>(), starts, (int)seqs, (int)most, causal,
       (float)scale, out.data_ptr(), lse.data_ptr<float>(), ranges ? low.data_ptr<float>() : nullptr,
       ranges ? high.data_ptr<float>() : nullptr, bytes ? work.data_ptr() : nullptr, bytes, stream_of(p.device.index()));

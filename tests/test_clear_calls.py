@@ -113,7 +113,7 @@ def inputs(stub, device):
     def on(size, dtype):
         return stub[0].on(size, torch.zeros(0, dtype=dtype), device)
 
-    pool = (on([4, 2, 128 * 136], torch.uint8).data_ptr(), 4, 2, 128, device)
+    pool = (on([4, 2, 128 * 136], torch.uint8), 4, 2, 128, device)
     return dict(pool=pool, kv=on([3, 2, 128], torch.bfloat16), slots=on([3], torch.int64), table=on([3, 1], torch.int32),
                 lengths=on([3], torch.int32), starts=on([4], torch.int32), logits=on([3, 10], torch.float32),
                 tokens=on([3], torch.int64))
@@ -135,3 +135,19 @@ def test_each_call_launches_on_its_tensors_device(stub, device):
         assert stub[0].current() == 0      # the caller's device is as it was
         for t in got if isinstance(got, tuple) else ():
             assert t.device == torch.device("cuda", device)
+
+
+def test_the_pools_bytes_are_asked_for_at_each_call(stub):
+    """An address kept from the pool's making would outlive its tensor."""
+    x = inputs(stub, 1)
+    like = torch.zeros(0, dtype=torch.uint8)
+    buf = x["pool"][0]
+    for bad in (stub[0].on([4, 2, 128 * 136 - 1], like, 1), stub[0].on([4, 2, 128 * 136], like, 0), buf.transpose(0, 1),
+                buf[:3], stub[0].on([4, 2, 128 * 136], torch.zeros(0), 1), torch.zeros((4, 2, 128 * 136), dtype=torch.uint8)):
+        for call in calls(stub, {**x, "pool": (bad, *x["pool"][1:])})[:3]:
+            with pytest.raises(ValueError, match="buf"):
+                call()
+    for call in calls(stub, {**x, "pool": (buf.data_ptr(), *x["pool"][1:])})[:3]:
+        with pytest.raises(TypeError, match="buf"):
+            call()
+    assert stub[0].launches() == []
