@@ -18,6 +18,7 @@ rounded to one mantissa bit, less 2 (kept in 2..252), so the largest becomes 4 o
 off by more than half a step.  A run that holds an infinity or a NaN is held, and read, as NaN.
 
 Everything runs in libholmes_ckks on the current stream of its tensors' device without synchronising; there is no CPU path.
+Nothing has a backward pass: an input that requires a gradient is refused, but under ``torch.no_grad()``.
 """
 
 from __future__ import annotations

@@ -8,6 +8,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -38,6 +39,12 @@ void need(bool condition, const char* message) {
 const Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) throw torch::TypeError(std::string(name) + " must be a tensor");
   return THPVariable_Unpack(o);
+}
+
+// Nothing here has a backward pass, and a result without one would pass for a constant.
+void no_gradient(const Tensor& t, const char* name) {
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    refuse(std::string(name) + " require a gradient, which this call does not have: detach them, or call it under torch.no_grad()");
 }
 
 long long whole(PyObject* o) {
@@ -102,6 +109,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         x->scalar_type() != k.scalar_type() || x->device() != p.device)
       refuse("keys and values must be [" + std::to_string(tokens) + ", " + std::to_string(p.heads) + ", " +
              std::to_string(p.dim) + "], contiguous along the last axis, in one type on the pool's device");
+  no_gradient(k, "keys");
+  no_gradient(v, "values");
   void* at = p.at();
   const c10::DeviceGuard guard(p.device);
   return PyLong_FromLong(hck_kv4_append(at, p.pages, p.heads, p.dim, type, k.data_ptr(), k.stride(0), k.stride(1),
@@ -174,6 +183,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t group = heads / p.heads;
   // what the C entry point's arguments do not hold, it could not refuse itself
   need(seqs <= INT32_MAX && group <= INT32_MAX && most <= INT32_MAX && cols <= INT32_MAX, "too many sequences, heads or columns");
+  no_gradient(q, "queries");
   const void* at = p.at();
   const c10::DeviceGuard guard(p.device);
   Tensor out = make({tokens, heads, p.dim}, q.scalar_type(), p.device), lse = make({tokens, heads}, at::kFloat, p.device);
@@ -220,6 +230,7 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyErr_SetString(PyExc_RuntimeError, "token scores run on a GPU: there is no CPU path");
     return nullptr;
   }
+  no_gradient(x, "logits");
   const at::Device dev = x.device();
   const c10::DeviceGuard guard(dev);
   Tensor entropy = make({rows}, at::kFloat, dev), given, ids, logs, work;

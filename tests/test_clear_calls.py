@@ -151,3 +151,19 @@ def test_the_pools_bytes_are_asked_for_at_each_call(stub):
         with pytest.raises(TypeError, match="buf"):
             call()
     assert stub[0].launches() == []
+
+
+def test_inputs_that_require_a_gradient(stub):
+    """Results without a graph would pass for constants: refused, but where gradients are off."""
+    x = inputs(stub, 1)
+    x["kv"].requires_grad_()
+    x["logits"].requires_grad_()
+    append, read, attend, scores = calls(stub, x)
+    for call, name in ((append, "keys"), (attend, "queries"), (scores, "logits")):
+        with pytest.raises(ValueError, match=f"{name} require a gradient"):
+            call()
+    assert stub[0].launches() == []
+    with torch.no_grad():
+        for call in (append, read, attend, scores):
+            call()
+    assert stub[0].launches() == [1] * 4
