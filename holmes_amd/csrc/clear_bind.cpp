@@ -90,6 +90,9 @@ Tensor slots_of(PyObject* o, const Pool& p) {
   return s.contiguous();
 }
 
+// Contiguous along axis i; of one element or none the stride says nothing.
+bool dense(const Tensor& t, int i) { return t.size(i) <= 1 || t.stride(i) == 1; }
+
 void count(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) throw torch::TypeError(std::to_string(n) + " arguments instead of " + std::to_string(want));
 }
@@ -157,14 +160,13 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
        "table must be [sequences][columns] and lengths [sequences]");
   const int64_t seqs = table.size(0), cols = table.size(1);
   need(table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt && table.device() == p.device &&
-           lengths.device() == p.device && (table.numel() == 0 || table.stride(1) == 1) &&
-           (seqs == 0 || lengths.stride(0) == 1),
+           lengths.device() == p.device && dense(table, 1) && dense(lengths, 0),
        "table and lengths must be int32 on the pool's device, contiguous along the last axis");
   const int32_t* starts = nullptr;
   if (a[8] != Py_None) {
     const Tensor& s = tensor(a[8], "starts");
     need(s.dim() == 1 && s.size(0) == seqs + 1, "starts must be [sequences + 1], or there is one query for each sequence");
-    need(s.scalar_type() == at::kInt && s.device() == p.device && s.stride(0) == 1,
+    need(s.scalar_type() == at::kInt && s.device() == p.device && dense(s, 0),
          "starts must be int32 on the pool's device, contiguous along the last axis");
     starts = s.data_ptr<int32_t>();
   } else {
@@ -213,7 +215,7 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor& x = tensor(a[0], "logits");
   const int type = type_of(x.scalar_type());
   need(type >= 0, "logits must be bfloat16, float16 or float32");
-  need(x.dim() == 2 && x.size(1) >= 1 && (x.stride(1) == 1 || x.size(1) == 1),
+  need(x.dim() == 2 && x.size(1) >= 1 && dense(x, 1),
        "logits must be [rows][vocabulary], contiguous along the last axis");
   const int64_t rows = x.size(0), vocab = x.size(1);
   const long long top = whole(a[2]), limit = std::min<int64_t>(HCK_TOP_MAX, vocab);

@@ -167,3 +167,17 @@ def test_inputs_that_require_a_gradient(stub):
         for call in (append, read, attend, scores):
             call()
     assert stub[0].launches() == [1] * 4
+
+
+def test_strides_of_single_elements(stub):
+    """One sequence's length out of a table of several numbers, one column out of wider tables."""
+    x = inputs(stub, 0)
+    one = torch.zeros(0, dtype=torch.int32)
+    wide = stub[0].on([3, 4], one, 0)
+    x["kv"], x["starts"] = x["kv"][:1], stub[0].on([2], one, 0)
+    for lengths, table in ((wide[:1, 1], wide[:1]), (wide[:1, 0], wide[:1, ::4]), (wide[:1, 0], wide[:1].t()[:1].t())):
+        assert lengths.stride(0) == 4
+        stub[1].attend(*x["pool"], x["kv"], table, lengths, x["starts"], 1, True, None, False)
+    assert stub[0].launches() == [0] * 3
+    with pytest.raises(ValueError, match="contiguous"):
+        stub[1].attend(*x["pool"], x["kv"], wide[:1, ::2], wide[:1, 0], x["starts"], 1, True, None, False)
