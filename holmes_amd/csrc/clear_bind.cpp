@@ -91,7 +91,7 @@ Tensor slots_of(PyObject* o, const Pool& p) {
 }
 
 // Contiguous along axis i; of one element or none the stride says nothing.
-bool dense(const Tensor& t, int i) { return t.size(i) <= 1 || t.stride(i) == 1; }
+bool dense(const Tensor& t, int i) { return t.size(i) <= 1 || t.stride(i) == 1 || t.numel() == 0; }
 
 void count(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) throw torch::TypeError(std::to_string(n) + " arguments instead of " + std::to_string(want));

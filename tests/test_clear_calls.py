@@ -178,6 +178,8 @@ def test_strides_of_single_elements(stub):
     for lengths, table in ((wide[:1, 1], wide[:1]), (wide[:1, 0], wide[:1, ::4]), (wide[:1, 0], wide[:1].t()[:1].t())):
         assert lengths.stride(0) == 4
         stub[1].attend(*x["pool"], x["kv"], table, lengths, x["starts"], 1, True, None, False)
-    assert stub[0].launches() == [0] * 3
+    none = stub[0].on([1], one, 0)
+    stub[1].attend(*x["pool"], x["kv"][:0], wide[:0, ::2], wide[:0, 0], none, 0, True, None, False)
+    assert stub[0].launches() == [0] * 4
     with pytest.raises(ValueError, match="contiguous"):
         stub[1].attend(*x["pool"], x["kv"], wide[:1, ::2], wide[:1, 0], x["starts"], 1, True, None, False)
