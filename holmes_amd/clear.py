@@ -17,7 +17,8 @@ b for each run of 32 values along the head dimension: b is the exponent of the r
 rounded to one mantissa bit, less 2 (kept in 2..252), so the largest becomes 4 or 6 units and no value is
 off by more than half a step.  A run that holds an infinity or a NaN is held, and read, as NaN.
 
-Everything runs in libholmes_ckks on the current stream of its tensors' device without synchronising; there is no CPU path.
+Everything but ``softmax_ranges`` runs in libholmes_ckks on the current stream of its tensors' device without
+synchronising; there is no CPU path.
 Nothing has a backward pass: an input that requires a gradient is refused, but under ``torch.no_grad()``.
 """
 
@@ -25,6 +26,7 @@ from __future__ import annotations
 
 import importlib.util
 import math
+import sys
 from typing import NamedTuple
 
 import torch
@@ -155,16 +157,29 @@ def softmax_ranges(low: torch.Tensor, high: torch.Tensor, lse: torch.Tensor, mar
     """The encrypted softmax's shift U and intervals for the rows that ``attend(..., ranges=True)`` saw:
     mapped = (s - U) / 2 runs over ``exp_interval``, made even about 0, and sum exp(2 mapped) over
     ``rsqrt_interval``, both widened by ``margin`` of their width (of their logarithm's, for the sum).  Rows
-    that see no token do not count."""
+    that see no token do not count; a row with a NaN or an infinity, and sums beyond float64, are refused.
+    Waits for the device, and so cannot be captured."""
 
-    seen = torch.isfinite(lse)
-    if not bool(seen.any()):
+    empty = torch.isneginf(lse) & torch.isposinf(low)
+    odd = ~empty & ~(torch.isfinite(low) & torch.isfinite(high) & torch.isfinite(lse))
+    if lse.numel() == 0:
         raise ValueError("no row saw a token")
-    lo, hi = float(low[seen].min()), float(high[seen].max())
+    inf = torch.full((), math.inf, dtype=torch.float64, device=lse.device)
+    sums = lse.double()
+    empties, odds, lo, hi, a, b = torch.stack([
+        empty.sum().double(), odd.sum().double(), torch.where(empty, inf, low.double()).min(),
+        torch.where(empty, -inf, high.double()).max(), torch.where(empty, inf, sums).min(),
+        torch.where(empty, -inf, sums).max()]).tolist()
+    if empties == lse.numel():
+        raise ValueError("no row saw a token")
+    if odds:
+        raise ValueError(f"{int(odds)} rows have a score or a sum that is NaN or infinite")
     shift = 0.5 * (lo + hi)
     half = max(0.25 * (hi - lo) * (1.0 + 2.0 * margin), 1e-3)
-    a, b = float(lse[seen].min()) - shift, float(lse[seen].max()) - shift
+    a, b = a - shift, b - shift
     pad = max(margin * (b - a), 1e-3)
+    if a - pad < math.log(sys.float_info.min) or b + pad > math.log(sys.float_info.max):
+        raise ValueError(f"scores from {lo:.6g} to {hi:.6g}: the sums of their exponentials are beyond float64")
     return SoftmaxRanges(shift, (-half, half), (math.exp(a - pad), math.exp(b + pad)))
 
 
