@@ -5,7 +5,7 @@
 One attention layer of the decode step's shape (32 query heads over 8 key heads of 128) with random
 weights runs in the clear: the prompt's keys and values go into 4-bit pages, its attention gives the
 outputs and the range of every row's scores, and ``DecodeSpec`` takes the softmax's shift and intervals
-from them.  Then single tokens follow, as they would be served, and the answers are scored: log
+from them, widened by what the keys' 4 bits can have moved them by.  Then single tokens follow, as they would be served, and the answers are scored: log
 probabilities of the tokens that came, entropies, the most likely alternatives.  Random weights say
 nothing about language; what the example shows is which call follows which.
 """
@@ -44,15 +44,16 @@ def run(tokens: int = 2048, steps: int = 4, vocab: int = 32000, seed: int = 0) -
     def write(first, x):
         place = torch.arange(first, first + x.shape[0], device="cuda")
         slots = table[0].long()[place // clear.PAGE_TOKENS] * clear.PAGE_TOKENS + place % clear.PAGE_TOKENS
-        pool.append((x @ wk).view(-1, kv_heads, dim), (x @ wv).view(-1, kv_heads, dim), slots)
-        return slots
+        keys = (x @ wk).view(-1, kv_heads, dim)
+        pool.append(keys, (x @ wv).view(-1, kv_heads, dim), slots)
+        return keys, slots
 
     def logits(x, attended):
         return (x + attended.out.flatten(1) @ wo) @ (embed.T / math.sqrt(hidden))
 
     # the prompt
     x = embed[text[:tokens]]
-    slots = write(0, x)
+    keys, slots = write(0, x)
     queries = (x @ wq).view(-1, heads, dim)
     lengths = torch.tensor([tokens], dtype=torch.int32, device="cuda")
     starts = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
@@ -61,13 +62,13 @@ def run(tokens: int = 2048, steps: int = 4, vocab: int = 32000, seed: int = 0) -
 
     # the encrypted softmax's shift and intervals, from the rows that see at least a page as its steps do
     rows = slice(clear.PAGE_TOKENS - 1, None)
-    ranges = clear.softmax_ranges(prompt.low[rows], prompt.high[rows], prompt.lse[rows])
+    rounding = clear.score_rounding(queries[rows], keys, pool.read(slots, torch.float32)[0])
+    ranges = clear.softmax_ranges(prompt.low[rows], prompt.high[rows], prompt.lse[rows], rounding=rounding)
     spec = DecodeSpec(score_shift=ranges.score_shift, exp_interval=ranges.exp_interval, rsqrt_interval=ranges.rsqrt_interval)
     exp_series = DecodePolynomials.fit(spec).exp
 
-    # how well the series does on the last token's scores: its first query head, against the held keys
-    keys, _ = pool.read(slots, torch.float32)
-    s = (keys[:, 0] @ queries[-1, 0].float()).double().cpu().numpy() / math.sqrt(dim)
+    # how well the series does on the last token's scores: its first query head, against the keys as they came
+    s = (keys[:, 0].float() @ queries[-1, 0].float()).double().cpu().numpy() / math.sqrt(dim)
     mapped = (s - ranges.score_shift) / 2
     lo, hi = ranges.exp_interval
     e = np.polynomial.chebyshev.chebval((2 * mapped - lo - hi) / (hi - lo), exp_series) ** 2
@@ -82,8 +83,8 @@ def run(tokens: int = 2048, steps: int = 4, vocab: int = 32000, seed: int = 0) -
         lengths += 1
         step = pool.attend((x @ wq).view(-1, heads, dim), table, lengths)
         answers.append(clear.token_logprobs(logits(x, step), text[tokens + i + 1:tokens + i + 2], top=4))
-    return {"ranges": ranges, "softmax_error": error, "prompt": scores, "answers": answers, "cache_bytes": pool.nbytes,
-            "mapped": mapped, "total": exact.sum()}
+    return {"ranges": ranges, "rounding": rounding, "softmax_error": error, "prompt": scores, "answers": answers,
+            "cache_bytes": pool.nbytes, "mapped": mapped, "total": exact.sum(), "queries": queries, "keys": keys}
 
 
 def main() -> None:
@@ -95,6 +96,7 @@ def main() -> None:
     r = got["ranges"]
     print(f"{args.tokens} tokens in {got['cache_bytes'] / 2**20:.1f} MiB of 4-bit pages")
     print(f"score_shift {r.score_shift:.4f}, exp_interval {r.exp_interval}, rsqrt_interval {r.rsqrt_interval}")
+    print(f"of which up to {got['rounding']:.3f} either way for the scores' rounding by 4-bit keys")
     print(f"degree-15 exponential on those: {got['softmax_error']:.1e} of the largest probability")
     print(f"prompt: mean log probability {got['prompt'].logprobs.mean():.3f}, entropy {got['prompt'].entropy.mean():.3f}")
     for a in got["answers"]:

@@ -9,16 +9,17 @@ operators here run that model's attention over real prompts at their full length
   cache's; ``append`` quantises keys and values as they are written, ``read`` gives back what is held,
   ``attend`` is the attention of queries over it, with the log of every row's sum of exponentials and
   the least and largest of its scores;
-* ``softmax_ranges``: the encrypted softmax's shift and intervals from those;
+* ``softmax_ranges``: the encrypted softmax's shift and intervals from those, and ``score_rounding`` what the keys'
+  4 bits can have moved them by;
 * ``token_logprobs``: log probabilities of given tokens, entropy and top alternatives of logits.
 
 Values are held as a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6 units.  A unit is 2^(b - 127) with one byte
 b for each run of 32 values along the head dimension: b is the exponent of the run's largest magnitude
 rounded to one mantissa bit, less 2 (kept in 2..252), so the largest becomes 4 or 6 units and no value is
-off by more than half a step.  A run that holds an infinity or a NaN is held, and read, as NaN.
+off by more than half a step (a step of 2 above 4; magnitudes beyond 7 2^125 become 6 2^125).  A run that holds an infinity or a NaN is held, and read, as NaN.
 
-Everything but ``softmax_ranges`` runs in libholmes_ckks on the current stream of its tensors' device without
-synchronising; there is no CPU path.
+Everything but ``softmax_ranges`` and ``score_rounding`` runs in libholmes_ckks on the current stream of its
+tensors' device without synchronising; there is no CPU path.
 Nothing has a backward pass: an input that requires a gradient is refused, but under ``torch.no_grad()``.
 """
 
@@ -33,7 +34,7 @@ import torch
 
 from . import _native as nat
 
-__all__ = ["PAGE_TOKENS", "Attended", "ClearKVPages", "SoftmaxRanges", "TokenScores", "softmax_ranges",
+__all__ = ["PAGE_TOKENS", "Attended", "ClearKVPages", "SoftmaxRanges", "TokenScores", "score_rounding", "softmax_ranges",
            "token_logprobs"]
 
 PAGE_TOKENS = 128
@@ -153,13 +154,39 @@ class ClearKVPages:
         return Attended._make(got)
 
 
-def softmax_ranges(low: torch.Tensor, high: torch.Tensor, lse: torch.Tensor, margin: float = 0.05) -> SoftmaxRanges:
+def score_rounding(queries: torch.Tensor, keys: torch.Tensor, held: torch.Tensor, scale: float | None = None) -> float:
+    """How far scores over the pages are from those of ``keys`` [tokens][kv_heads][head_dim] where nothing rounds
+    them to 4 bits, as in the encrypted layer: the largest |scale q.(k - held)| of all ``queries`` [rows][query
+    heads][head_dim] and tokens, with ``held`` what ``read`` gives for the keys, and the products' own rounding in
+    32 bits on top.  Plain products of rows by tokens, some 64 M of them at a time.  Waits for the device."""
+
+    heads = keys.shape[1]
+    if keys.shape != held.shape or queries.shape[2] != keys.shape[2] or queries.shape[1] % max(heads, 1):
+        raise ValueError("queries must be [rows][query heads][head_dim], and keys and held [tokens][kv_heads][head_dim]")
+    if keys.numel() == 0 or queries.numel() == 0:
+        return 0.0
+    most = torch.zeros((), device=keys.device)
+    for q, off in zip(queries.float().chunk(heads, 1), (keys.float() - held.float()).unbind(1)):
+        q, size = q.flatten(0, 1), torch.linalg.vector_norm(off, dim=1).max()
+        for rows in q.split(max(1, (1 << 26) // len(off))):
+            slack = keys.shape[2] * 2.0**-24 * torch.linalg.vector_norm(rows, dim=1).max() * size
+            most = torch.maximum(most, torch.matmul(rows, off.T.contiguous()).abs().max() + slack)
+    return float(most) * (1.0 / math.sqrt(keys.shape[2]) if scale is None else scale)
+
+
+def softmax_ranges(low: torch.Tensor, high: torch.Tensor, lse: torch.Tensor, margin: float = 0.05,
+                   rounding: float = 0.0) -> SoftmaxRanges:
     """The encrypted softmax's shift U and intervals for the rows that ``attend(..., ranges=True)`` saw:
     mapped = (s - U) / 2 runs over ``exp_interval``, made even about 0, and sum exp(2 mapped) over
-    ``rsqrt_interval``, both widened by ``margin`` of their width (of their logarithm's, for the sum).  Rows
-    that see no token do not count; a row with a NaN or an infinity, and sums beyond float64, are refused.
+    ``rsqrt_interval``, both widened by ``margin`` of their width (of their logarithm's, for the sum).  Scores
+    and the sums' logarithms are moreover taken up to ``rounding`` further out: ``attend`` measures the keys as
+    the pages hold them, the encrypted layer has them unrounded, and ``score_rounding`` gives the difference.
+    These are ``DecodeSpec``'s fields; ``PrefillSpec``'s are of scores less their row's mean, which the ranges
+    do not tell.  Rows that see no token do not count; a row with a NaN or an infinity, and sums beyond float64, are refused.
     Waits for the device, and so cannot be captured."""
 
+    if not 0.0 <= rounding < math.inf:
+        raise ValueError("rounding must be finite and not negative")
     empty = torch.isneginf(lse) & torch.isposinf(low)
     odd = ~empty & ~(torch.isfinite(low) & torch.isfinite(high) & torch.isfinite(lse))
     if lse.numel() == 0:
@@ -175,6 +202,7 @@ def softmax_ranges(low: torch.Tensor, high: torch.Tensor, lse: torch.Tensor, mar
     if odds:
         raise ValueError(f"{int(odds)} rows have a score or a sum that is NaN or infinite")
     shift = 0.5 * (lo + hi)
+    lo, hi, a, b = lo - rounding, hi + rounding, a - rounding, b + rounding
     half = max(0.25 * (hi - lo) * (1.0 + 2.0 * margin), 1e-3)
     a, b = a - shift, b - shift
     pad = max(margin * (b - a), 1e-3)
