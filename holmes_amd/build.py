@@ -3,7 +3,9 @@
 Run ``python -m holmes_amd.build`` (or ``__graft_entry__.build()``).  Each ``.hip`` file is
 compiled to an object in parallel, then linked into one shared library exporting the C ABI of
 ``include/holmes_ckks.h``.  ``csrc/clear_bind.cpp``, the Python side of the cleartext operators, becomes the
-extension module holmes_amd/_lib/_clear.so (host code only, against the installed PyTorch).
+extension module holmes_amd/_lib/_clear.so (host code only, against the installed PyTorch).  It takes g++ and
+PyTorch's and Python's headers; where they are missing the library is there all the same, and only
+``holmes_amd.clear`` is not.
 """
 
 from __future__ import annotations
@@ -54,13 +56,14 @@ def _compile(src: str, build_dir: Path) -> Path:
 
 
 def _compile_binding(build_dir: Path) -> Path:
+    import torch
     from torch.utils import cpp_extension
 
     obj = build_dir / "clear_bind.o"
     paths = [*cpp_extension.include_paths(), str(Path(HIPCC).resolve().parent.parent / "include"), "/opt/rocm/include",
              sysconfig.get_paths()["include"]]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1", *(f"-isystem{p}" for p in paths),
-           "-c", str(CSRC / "clear_bind.cpp"), "-o", str(obj)]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-isystem{p}" for p in paths), "-c", str(CSRC / "clear_bind.cpp"), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for clear_bind.cpp:\n{res.stderr}")
@@ -86,14 +89,17 @@ def build(verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, 8)) as pool:
         binding = pool.submit(_compile_binding, build_dir)
         objs = list(pool.map(lambda s: _compile(s, build_dir), SOURCES))
-        binding = binding.result()
     tmp = LIB.with_suffix(f".so.tmp{os.getpid()}")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
-    _link_binding(binding)
+    try:
+        _link_binding(binding.result())
+    except (ImportError, OSError, RuntimeError) as e:  # no PyTorch, no g++, or one of them failed
+        CLEAR.unlink(missing_ok=True)   # none rather than an old one
+        print(f"holmes_amd.clear is not available: {CLEAR.name} was not built: {e}", file=sys.stderr)
     if verbose:
         print(f"built {LIB}")
     return LIB
