@@ -47,7 +47,7 @@ struct Kv4 {
   }
 };
 
-constexpr int64_t kLastCache = 256 << 20, kL2s = 32 << 20;  // bytes of the card's last cache, of the XCDs' L2s together
+constexpr int64_t kL2s = 32 << 20;  // bytes of the XCDs' L2 caches together
 
 // Bytes of one head's part of a page (host side; 0: no such head dimension).
 inline int kv4_bytes(int head_dim) {

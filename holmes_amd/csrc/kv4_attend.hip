@@ -21,7 +21,7 @@
 namespace hck {
 namespace {
 
-// A load that passes the caches by where nothing is read twice and they could not hold it.
+// A load that passes the caches by where nothing is read twice.
 template <bool ONCE, typename V>
 __device__ __forceinline__ V fetch(const uint8_t* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
@@ -100,7 +100,7 @@ __device__ __forceinline__ float over_row(float x, F f) {
 // share of the 64 tokens, so that no exponential is taken for an empty column, and goes into the second
 // product with zeros for the other copies' tokens; the copies' sums are added at the end.
 //
-// ONCE: with loads past the caches (48 sequences of 12000 to 24576 tokens, 917 MB: 187 us through them, 167 us past, then).
+// ONCE: with loads past the caches (Way::once).
 //
 // Keys of the next unit are loaded as soon as the first product is done with this one's, its values after the
 // second, so that loads are in flight throughout without registers of their own.
@@ -571,7 +571,7 @@ extern "C" int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int
   A.slots = (int)W.slots;
   A.least = W.least;
   A.join = W.join;
-  A.once = W.tiles == 1 && (int64_t)seqs * table_columns * kv_heads * hck::kv4_bytes(head_dim) > hck::kLastCache;
+  A.once = W.once(seqs, table_columns, pages, kv_heads, head_dim);
   A.scale = scale;
   hipStream_t s = (hipStream_t)stream;
   const bool range = low != nullptr;

@@ -49,7 +49,7 @@ struct AttendArgs {
   int seqs, tiles;     // tiles of rows that the longest sequence can have
   int size, rows;      // rows of a tile, and of a slot
   int slots, least;    // workgroups to share the work out to, units that are not worth sharing
-  int join, once;      // once: keys and values are read once, and are more than the caches hold
+  int join, once;      // once: no key or value is read twice, and there is room for more than the L2s hold (Way::once)
   float scale;
 };
 
@@ -364,6 +364,15 @@ struct Way {
     join = pairs <= 64 * kPairs && units > (few ? 4 * kWaves : 8) && !even;
     most_slots = std::min((units + least - 1) / least, slots / heads + 1);
     items = !join ? pairs * heads : std::min(pairs * ((units + least - 1) / least), pairs + (slots + heads - 1) / heads) * heads;
+  }
+  // Whether loads go past the caches: one tile of rows for each sequence, so that nothing is read twice, and room for more
+  // than the L2s hold.  Lengths are not known here; no more is held than the tables have room for, nor than the pool.
+  // Single tokens, 8 key heads of 128, through the caches and past them, with what was read before in the last cache or
+  // not: 4 sequences, 4 MB, 9.9 and 10.5 us (there or not); one of 36 MB 16.8 and 16.9 there, 18.0 and 16.7 not there; 32,
+  // 63 MB, 20.4 and 20.5, 22.1 and 21.1; one of 143 MB 33.7 and 33.6, 38.9 and 34.9; 32, 209 MB, 41.6 and 43.5, 50.5 and
+  // 50.2; 48, 418 MB, 89.0 and 79.8.
+  bool once(int64_t seqs, int64_t cols, int64_t pages, int heads, int dim) const {
+    return tiles == 1 && std::min(seqs * cols, pages) > kL2s / ((int64_t)heads * kv4_bytes(dim));
   }
   size_t bytes(int heads, int dim) const {
     return join ? (size_t)items * rows * (4 + dim) * sizeof(float) + (size_t)pairs * heads * 2 * sizeof(int) : 0;
