@@ -116,3 +116,25 @@ def test_fp16_outputs(value):
     assert math.isinf(float(got[0, 0, 40])) == (float(want[40]) > 65520)
     ok = want < 65520
     assert ((got[0][:, ok] - want[ok]).abs() <= 2.0**-10 * want[ok]).all()
+
+
+@pytest.mark.parametrize("seqs,counts", [([12000, 300, 9000, 40], [70, 33, 66, 5])])
+def test_split_tiles_of_256_rows(seqs, counts):
+    """Large tokens in some shares of a history and not in others, on either side of a border inside a page."""
+    from .test_gpu_clear_split_256 import DIM, GROUP, HEADS, MOST as BOUND, check as compare, share_of
+
+    print("large values, split 256 rows", flush=True)
+    g = torch.Generator().manual_seed(6)
+    pool, table, keys, values = build(seqs, HEADS, DIM, g)
+    border = 64 * share_of(seqs, counts)
+    assert border % PAGE == 64
+    for t, r, value in ((border - 1, 0, 2.0**112), (3 * border, 1, MOST), (3 * border + 70, 0, 2.0**90), (0, 3, 2.0**74)):
+        for b in (0, 2):
+            put(pool, table, keys, values, b, t, r, value)
+    put(pool, table, keys, values, 1, 299, 2, MOST)     # the last token: seen by the last query alone
+    q = torch.randn((sum(counts), HEADS * GROUP, DIM), generator=g).to(torch.bfloat16).cuda()
+    got = pool.attend(q, widen(table, 400), torch.tensor(seqs, dtype=torch.int32).cuda(), starts=starts_of(counts), most=BOUND,
+                      ranges=True)
+    there = [torch.ones(n, dtype=torch.bool) for n in seqs]
+    assert torch.isfinite(got.out).all()
+    compare(got, q, keys, values, counts, there, True)
