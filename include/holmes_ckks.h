@@ -437,7 +437,8 @@ int hck_lincomb_rescale(const hck_context* ctx, int level_limbs, int groups, int
 size_t hck_kv4_page_bytes(int head_dim);
 
 /* Quantises `tokens` keys and values into the slots slots[i] (device; page * 128 + place; outside the
- * pool: the token is left out; a slot named twice holds either token's values).  Token i, head h is at
+ * pool: the token is left out).  The slots of one call must differ: what one named twice holds is undefined (its
+ * codes and scale bytes are stored apart, and may be of different tokens).  Token i, head h is at
  * i * token_stride + h * head_stride elements, its head_dim values contiguous. */
 int hck_kv4_append(void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* keys,
                    int64_t key_token_stride, int64_t key_head_stride, const void* values, int64_t value_token_stride,
