@@ -10,12 +10,13 @@
 //
 // Roundings: codes times scales are exact in bf16 (two significant bits), and so is a bf16 query; an
 // fp16 query goes in as two bf16 parts (16 bits).  Scores, maxima, sums and outputs are held in 32
-// bits.  The probabilities go in as two bf16 parts as well, which leaves 2^-17 of each, far below the
+// bits.  The probabilities go in as two bf16 parts as well, the nearest and the rest's, which leaves 2^-17 of each, far below the
 // rounding of the output; the sum l takes the unrounded ones.
 //
 // What bounds it (8 key heads of 128, 4 query heads each): over 48 sequences of 12000 to 24576 tokens the bytes,
-// 917 MB in 161 us or 5.7 TB/s (the same loads without arithmetic: 5.9); over 131072 tokens 29 us for 142 MB, of
-// which 5 go by before the first product; over 257 tokens the chain of loads (length, page number, codes), 5 to 7 us.
+// 917 MB in 163 us or 5.6 TB/s (the same loads without arithmetic: 5.9); over 131072 tokens 34 us with the join for
+// 142 MB, of which 5 go by before the first product; over 257 tokens the chain of loads (length, page number, codes),
+// 5 to 7 us.
 #include "kv4_attend.hpp"
 
 namespace hck {

@@ -5,12 +5,14 @@
 // both are busy.  Making operands of the codes takes some 190 vector instructions per 64 tokens, as many as the
 // softmax of 32 rows; so it is done once for a workgroup: each of its 4 or 8 waves makes its share of them, in the
 // lanes' order, in LDS (keys and values 32 KB per 64 tokens, twice, so that one barrier is enough; with 8 waves two
-// units to a barrier), and takes all of them for its own 32 rows.  The next codes are in flight meanwhile.
+// units to a barrier), and takes all of them for its own 32 rows.  The next codes are in flight meanwhile.  Which runs are
+// summed times 2^-56 (kLargeByte) is the workgroup's, known after the barrier; where a step brings a new one, its
+// operands are made again.
 //
-// What bounds it: per 64 tokens and 32 rows 48 matrix and some 370 vector instructions (D = 128), which two waves of
-// a SIMD issue through one port.  4096 tokens, 32 query heads over 8 key heads of 128: 139 GFLOP in 194 us, or
-// 716 TFLOP/s, and 1.07 PFLOP/s of the products that are done (three for two, by the probabilities' two parts);
-// a bf16 8192^3 product runs at 1.20 PFLOP/s.
+// What bounds it: per 64 tokens and 32 rows 48 matrix and some 350 vector instructions (D = 128), which two waves of
+// a SIMD issue through one port.  4096 tokens, 32 query heads over 8 key heads of 128: 139 GFLOP in 195 to 205 us on
+// different cards, at 198 us 702 TFLOP/s, and 1.05 PFLOP/s of the products that are done (three for two, by the
+// probabilities' two parts); a bf16 8192^3 product runs at 1.20 PFLOP/s.
 #include "kv4_attend.hpp"
 
 namespace hck {
