@@ -504,9 +504,10 @@ int launch(const AttendArgs& A, const Way& W, hipStream_t s) {
   return HCK_OK;
 }
 
+// (Columns below 2^24: a token's number, and the first one behind its unit, are within 31 bits.)
 bool shape_ok(int64_t tokens, int seqs, int kv_heads, int group, int most, int cols) {
   return tokens >= 0 && seqs >= 0 && seqs <= 65535 && kv_heads >= 1 && kv_heads <= 65535 && group >= 1 &&
-         group <= 1024 && most >= 0 && cols >= 0 && cols <= (1 << 24) && (int64_t)most * group <= (1 << 30) &&
+         group <= 1024 && most >= 0 && cols >= 0 && cols < (1 << 24) && (int64_t)most * group <= (1 << 30) &&
          tokens * kv_heads * group <= ((int64_t)1 << 32);
 }
 

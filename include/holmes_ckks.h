@@ -457,7 +457,7 @@ int hck_kv4_read(const void* pool, int64_t pages, int kv_heads, int head_dim, in
  * are device arrays: a page outside the pool counts as tokens that are not there.  out is dense, of the
  * queries' type; lse, low and high (both NULL or both given) are [tokens][kv_heads * group] float: log sum
  * exp and the least and largest of a row's scaled scores.  A row that sees nothing gives 0, -inf, inf, -inf.
- * A token that no sequence covers is left unwritten.  scale is positive, and 2^126 at most. */
+ * A token that no sequence covers is left unwritten.  table_columns is below 2^24; scale is positive, and 2^126 at most. */
 size_t hck_kv4_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim, int most,
                                       int table_columns);
 int hck_kv4_attend(const void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* queries,
