@@ -305,10 +305,11 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
   // values before the first 16-byte border, whole pieces, and the rest
   const int head = min(A.vocab, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
   const int pieces = (A.vocab - head) / kPer, tail = head + pieces * kPer;
+  const int left = A.vocab - tail;  // (tail + lane may pass 31 bits)
   const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   const int blocks = (pieces + 64 * kVecs - 1) / (64 * kVecs);
   const int first = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + wave), stride = A.splits * kWaves;
-  const bool heads = first == 0 && head > 0, tails = first == stride - 1 && tail < A.vocab;
+  const bool heads = first == 0 && head > 0, tails = first == stride - 1 && left > 0;
   Sums a;
   Most most;
   if (heads) take<1>(a, most, -1, [&](int) { return lane < head ? (float)x[lane] : -INFINITY; });
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
     }
     take<kVecs * kPer>(a, most, bl, [&](int n) { return element<T>(v[n / kPer], n % kPer); });
   }
-  if (tails) take<1>(a, most, -1, [&](int) { return tail + lane < A.vocab ? (float)x[tail + lane] : -INFINITY; });
+  if (tails) take<1>(a, most, -1, [&](int) { return lane < left ? (float)x[tail + lane] : -INFINITY; });
 
   bool listed = true;
   // A thread a value and all of them listed: where fewer threads than `top` have a piece, which leaves no key to reach
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
           if (k == least - 1) C.offer(k, (uint32_t)i, k);
         }
       }
-      if (tails && tail + lane < A.vocab) C.offer(key_of((float)x[tail + lane]), (uint32_t)(tail + lane), least);
+      if (tails && lane < left) C.offer(key_of((float)x[tail + lane]), (uint32_t)(tail + lane), least);
       listed = C.sort(A.top);
     }
   }
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArgs A) {
 #pragma unroll
         for (int e = 0; e < kPer; ++e) offer(p < pieces, element<T>(v, e), head + p * kPer + e);
       }
-    if (tails) offer(tail + lane < A.vocab, tail + lane < A.vocab ? (float)x[tail + lane] : 0.f, tail + lane);
+    if (tails) offer(lane < left, lane < left ? (float)x[tail + lane] : 0.f, tail + lane);
     static_assert(kWaves * kMaxTop <= kList, "the waves' lists");
     if (lane < A.top) C.list[wave * kMaxTop + lane] = Candidates::order(best.key, best.index);
     __syncthreads();
