@@ -239,6 +239,54 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
       lo[i] = u32x2{rests_of(t[i][0], t[i][1], hi[i][0]), rests_of(t[i][2], t[i][3], hi[i][1])};
     }
 
+    if (__builtin_expect(large || __any(has_large(x.vs[0][0]) || has_large(x.vs[0][1]) || has_large(x.vs[1][0]) || has_large(x.vs[1][1])), false)) {
+      bool beyond = false;
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  It is taken as zeros
+        // in the product, and counted for the rows that see it by a product of truth values.
+        uint32_t vs[2] = {i ? x.vs[1][0] : x.vs[0][0], i ? x.vs[1][1] : x.vs[0][1]};
+        bf16x8 bad, see;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t byte = (vs[k >> 2] >> (8 * (k & 3))) & 0xffu;
+          const int token = base + 32 * i + 16 * (k >> 2) + (k & 3);
+          const bool is = byte == kNanByte;
+          bad[k] = (__bf16)(is ? 1.f : 0.f);
+          see[k] = (__bf16)(token < seen ? 1.f : 0.f);
+          if (is) vs[k >> 2] &= ~(0xffu << (8 * (k & 3)));
+          else beyond = beyond || (byte >= kLargeByte && token < most);
+        }
+        x.vs[0][0] = i ? x.vs[0][0] : vs[0], x.vs[0][1] = i ? x.vs[0][1] : vs[1];
+        x.vs[1][0] = i ? vs[0] : x.vs[1][0], x.vs[1][1] = i ? vs[1] : x.vs[1][1];
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        const f32x4 n = mfma(bad, see, zero);
+#pragma unroll
+        for (int d = 0; d < kDpl; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n[k] > 0.f) acc[d][k] = __uint_as_float(0x7fc00000u);
+      }
+      const unsigned long long all4 = __ballot(beyond);
+      uint32_t lanes = (uint32_t)all4 | (uint32_t)(all4 >> 32), runs = 0;
+      lanes |= lanes >> 16;  // of every g
+#pragma unroll
+      for (int r = 0; r < L::kRuns; ++r)  // a run's lanes: kRun / kDpl neighbours
+        runs |= (lanes >> (r * (kRun / kDpl))) & ((1u << (kRun / kDpl)) - 1) ? 1u << r : 0u;
+      int here = lane;  // (worked out here and not kept from before the loop)
+      asm volatile("" : "+v"(here));
+      if (const uint32_t fresh = runs & ~large) {
+        large |= fresh;
+        const float by = (fresh >> ((here >> 4) * (D / 4) / kRun)) & 1 ? kDownBy : 1.f;
+#pragma unroll
+        for (int d = 0; d < kDpl; ++d) acc[d] *= by;
+      }
+      if ((large >> ((here & 15) * kDpl / kRun)) & 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x.vs[i][0] = down(x.vs[i][0]), x.vs[i][1] = down(x.vs[i][1]);
+      }
+    }
+
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       auto part = [&](const u32x2* p) {
@@ -251,49 +299,9 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_few(D, __is_same(T, _Float16)
         return operand(w[0][0], w[0][1], w[1][0], w[1][1]);
       };
       const bf16x8 ph = part(hi), pl = part(lo);
-      uint32_t vs[2] = {x.vs[i][0], x.vs[i][1]};
       float sc[8];
-      // A run of NaN must reach the rows that see its token, and no other: 0 * NaN is NaN.  It is taken
-      // as zeros here, and counted for the rows that see it by a product of truth values.
-      if (__builtin_expect(large || __any(has_large(vs[0]) || has_large(vs[1])), false)) {
-        bf16x8 bad, see;
-        bool beyond = false;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t byte = (vs[k >> 2] >> (8 * (k & 3))) & 0xffu;
-          const int token = base + 32 * i + 16 * (k >> 2) + (k & 3);
-          const bool is = byte == kNanByte;
-          bad[k] = (__bf16)(is ? 1.f : 0.f);
-          see[k] = (__bf16)(token < seen ? 1.f : 0.f);
-          if (is) vs[k >> 2] &= ~(0xffu << (8 * (k & 3)));
-          else beyond = beyond || (byte >= kLargeByte && token < most);
-        }
-        const unsigned long long all4 = __ballot(beyond);
-        uint32_t lanes = (uint32_t)all4 | (uint32_t)(all4 >> 32), runs = 0;
-        lanes |= lanes >> 16;  // of every g
-#pragma unroll
-        for (int r = 0; r < L::kRuns; ++r)  // a run's lanes: kRun / kDpl neighbours
-          runs |= (lanes >> (r * (kRun / kDpl))) & ((1u << (kRun / kDpl)) - 1) ? 1u << r : 0u;
-        int here = lane;  // (worked out here and not kept from before the loop)
-        asm volatile("" : "+v"(here));
-        if (const uint32_t fresh = runs & ~large) {
-          large |= fresh;
-          if ((fresh >> ((here >> 4) * (D / 4) / kRun)) & 1) {
-#pragma unroll
-            for (int d = 0; d < kDpl; ++d) acc[d] *= kDownBy;
-          }
-        }
-        if ((large >> ((here & 15) * kDpl / kRun)) & 1) vs[0] = down(vs[0]), vs[1] = down(vs[1]);
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const f32x4 n = mfma(bad, see, zero);
-#pragma unroll
-        for (int d = 0; d < kDpl; ++d)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n[k] > 0.f) acc[d][k] = __uint_as_float(0x7fc00000u);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sc[k] = scale_of(vs[k >> 2], k & 3);
+      for (int k = 0; k < 8; ++k) sc[k] = scale_of(x.vs[i][k >> 2], k & 3);
       bf16x8 e, o;
       auto step = [&](auto B) {
         constexpr int kB = decltype(B)::value;
