@@ -30,6 +30,7 @@ HCK_BF16 = 0
 HCK_F16 = 1
 HCK_F32 = 2
 HCK_TOP_MAX = 32   # include/holmes_ckks.h: alternatives of hck_token_scores
+HCK_ROTARY_MAX = 512   # include/holmes_ckks.h: head_dim of hck_rotary
 
 # Every symbol include/holmes_ckks.h declares, with (restype, argtypes).
 _vp = ctypes.c_void_p
@@ -119,6 +120,14 @@ SIGNATURES = {
                             ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "hck_token_scores_workspace_bytes": (_sz, [_i64, _i, _i, _i]),
     "hck_token_scores": (_i, [_vp, _i, _i64, _i, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "hck_rotary": (_i, [_vp, _i, _i64, _vp, _i, _i, _i, ctypes.c_float, _i, _i, _vp, _i64, _i64, _i, _vp, _vp, _i64, _i64,
+                        _i, _vp, _vp]),
+    "hck_prompt_attend": (_i, [_vp, _vp, _vp, _i, _i64, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i, _i, _i,
+                               ctypes.c_double, _vp, _vp, _vp, _vp, _vp]),
+    "hck_kv4_weigh": (_i, [_vp, _i64, _i, _i, _i, _vp, _i64, _i, _i64, _i64, _vp, _i64, _i, _vp, _vp, _i, _i, _i,
+                           ctypes.c_double, _vp, _vp, _i64, _i64, _i, _vp, _vp]),
+    "hck_kv4_evict": (_i, [_vp, _i64, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _i64, _i64, _i, _vp, _i64, _i, _i, _i, _vp, _vp,
+                           _vp, _vp]),
 }
 
 _lib = None

@@ -2,10 +2,10 @@
 
 Run ``python -m holmes_amd.build`` (or ``__graft_entry__.build()``).  Each ``.hip`` file is
 compiled to an object in parallel, then linked into one shared library exporting the C ABI of
-``include/holmes_ckks.h``.  ``csrc/clear_bind.cpp``, the Python side of the cleartext operators, becomes the
-extension module holmes_amd/_lib/_clear.so (host code only, against the installed PyTorch).  It takes g++ and
-PyTorch's and Python's headers; where they are missing the library is there all the same, and only
-``holmes_amd.clear`` is not.
+``include/holmes_ckks.h``.  ``csrc/clear_bind.cpp`` and ``csrc/window_bind.cpp``, the Python sides of the cleartext
+operators, become the extension modules holmes_amd/_lib/_clear.so and _window.so (host code only, against the installed
+PyTorch).  They take g++ and PyTorch's and Python's headers; where these are missing the library is there all the same, and
+only ``holmes_amd.clear`` is not.
 """
 
 from __future__ import annotations
@@ -23,11 +23,12 @@ CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libholmes_ckks.so"
 CLEAR = OUT_DIR / "_clear.so"
+BINDINGS = {"clear_bind.cpp": "_clear.so", "window_bind.cpp": "_window.so"}   # beside the library
 ARCH = os.environ.get("HOLMES_AMD_ARCH", "gfx950")
 
 SOURCES = ["context.hip", "ntt.hip", "poly.hip", "keyswitch.hip", "ksfused.hip", "bsgs.hip", "encode.hip",
            "mul.hip", "noalloc.hip", "wide.hip", "wide_fused.hip", "kv4.hip", "kv4_attend.hip", "kv4_prompt.hip",
-           "scores.hip"]
+           "scores.hip", "rotary.hip", "prompt.hip", "kv4_weigh.hip", "kv4_evict.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
@@ -55,32 +56,40 @@ def _compile(src: str, build_dir: Path) -> Path:
     return obj
 
 
-def _compile_binding(build_dir: Path) -> Path:
+def _compile_binding(build_dir: Path) -> dict:
     import torch
     from torch.utils import cpp_extension
 
-    obj = build_dir / "clear_bind.o"
     paths = [*cpp_extension.include_paths(), str(Path(HIPCC).resolve().parent.parent / "include"), "/opt/rocm/include",
              sysconfig.get_paths()["include"]]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-isystem{p}" for p in paths), "-c", str(CSRC / "clear_bind.cpp"), "-o", str(obj)]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for clear_bind.cpp:\n{res.stderr}")
-    return obj
+
+    def one(src: str) -> Path:
+        obj = build_dir / (Path(src).stem + ".o")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-isystem{p}" for p in paths), "-c", str(CSRC / src), "-o", str(obj)]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed for {src}:\n{res.stderr}")
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(BINDINGS)) as pool:
+        return dict(zip(BINDINGS.values(), pool.map(one, BINDINGS)))
 
 
-def _link_binding(obj: Path) -> None:
+def _link_binding(objs: dict) -> None:
     import torch
 
-    tmp = CLEAR.with_suffix(f".so.tmp{os.getpid()}")
-    cmd = ["g++", "-shared", "-o", str(tmp), str(obj), f"-L{OUT_DIR}", f"-l:{LIB.name}",
-           f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
-           "-Wl,-rpath,$ORIGIN"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"link failed:\n{res.stderr}")
-    os.replace(tmp, CLEAR)
+    made = {}
+    for name, obj in objs.items():
+        made[name] = tmp = (OUT_DIR / name).with_suffix(f".so.tmp{os.getpid()}")
+        cmd = ["g++", "-shared", "-o", str(tmp), str(obj), f"-L{OUT_DIR}", f"-l:{LIB.name}",
+               f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
+               "-Wl,-rpath,$ORIGIN"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"link failed:\n{res.stderr}")
+    for name, tmp in made.items():   # all or none
+        os.replace(tmp, OUT_DIR / name)
 
 
 def build(verbose: bool = False) -> Path:
@@ -98,8 +107,9 @@ def build(verbose: bool = False) -> Path:
     try:
         _link_binding(binding.result())
     except (ImportError, OSError, RuntimeError) as e:  # no PyTorch, no g++, or one of them failed
-        CLEAR.unlink(missing_ok=True)   # none rather than an old one
-        print(f"holmes_amd.clear is not available: {CLEAR.name} was not built: {e}", file=sys.stderr)
+        for name in BINDINGS.values():
+            (OUT_DIR / name).unlink(missing_ok=True)   # none rather than an old one
+        print(f"holmes_amd.clear is not available: its extension modules were not built: {e}", file=sys.stderr)
     if verbose:
         print(f"built {LIB}")
     return LIB

@@ -5,10 +5,14 @@ the interval of the softmax's scores and the interval of their exponentials' sum
 ranges, and the decrypted answers are judged by the probabilities that they give to known tokens.  The
 operators here run that model's attention over real prompts at their full length:
 
+* ``RotaryPositions``: rotary positions on queries and keys;
+* ``prompt_attention``: attention over whole prompts whose keys and values are as they came, as the encrypted layer has
+  them, with the log of every row's sum of exponentials and the least and largest of its scores;
 * ``ClearKVPages``: a key/value cache in 4 bits on the GPU, in pages of 128 tokens like the encrypted
   cache's; ``append`` quantises keys and values as they are written, ``read`` gives back what is held,
-  ``attend`` is the attention of queries over it, with the log of every row's sum of exponentials and
-  the least and largest of its scores;
+  ``attend`` is the attention of queries over it, with the same numbers of every row; ``weigh`` sums what attention has
+  given each cached token, and ``evict`` brings a sequence down to its heaviest ones, as the few pages of the encrypted
+  layer's cache want it;
 * ``softmax_ranges``: the encrypted softmax's shift and intervals from those, and ``score_rounding`` what the keys'
   4 bits can have moved them by;
 * ``token_logprobs``: log probabilities of given tokens, entropy and top alternatives of logits.
@@ -28,14 +32,15 @@ from __future__ import annotations
 import importlib.util
 import math
 import sys
+from fractions import Fraction
 from typing import NamedTuple
 
 import torch
 
 from . import _native as nat
 
-__all__ = ["PAGE_TOKENS", "Attended", "ClearKVPages", "SoftmaxRanges", "TokenScores", "score_rounding", "softmax_ranges",
-           "token_logprobs"]
+__all__ = ["PAGE_TOKENS", "Attended", "ClearKVPages", "Evicted", "RotaryPositions", "RotaryScaling", "SoftmaxRanges",
+           "TokenScores", "prompt_attention", "score_rounding", "softmax_ranges", "token_logprobs"]
 
 PAGE_TOKENS = 128
 
@@ -61,6 +66,35 @@ class TokenScores(NamedTuple):
     top_logprobs: torch.Tensor | None
 
 
+class Evicted(NamedTuple):
+    """Of every sequence and key head the places that the kept tokens had, in order (int32, -1 behind the last);
+    of every sequence their number (int32); and their weights (float32, 0 behind the last), which ``weigh`` takes as
+    ``prior`` from there on."""
+
+    kept: torch.Tensor
+    lengths: torch.Tensor
+    weights: torch.Tensor
+
+
+class RotaryScaling(NamedTuple):
+    """Rotary frequencies for more tokens than the ``original`` they were made for, ``factor`` times as many:
+
+    * "linear": all divided by ``factor``;
+    * "base": the base times factor^(d / (d - 2)) for d rotated dims, so that the last pair is divided and the first
+      is as it was;
+    * "wavelength": a pair that makes fewer than ``low`` turns in the original length is divided, one that makes more
+      than ``high`` is as it was, and between them the two are blended evenly over the turns;
+    * "ramp": the same ends, but blended evenly over the pairs' numbers, whose first is the whole number below the
+      (fractional) pair of ``high`` turns and whose last the one above that of ``low``; and the rotated values are
+      multiplied by 0.1 log(factor) + 1."""
+
+    kind: str
+    factor: float
+    original: int = 8192
+    low: float = 1.0
+    high: float = 4.0
+
+
 class SoftmaxRanges(NamedTuple):
     """``DecodeSpec``'s ``score_shift``, ``exp_interval`` and ``rsqrt_interval``."""
 
@@ -69,24 +103,31 @@ class SoftmaxRanges(NamedTuple):
     rsqrt_interval: tuple
 
 
-_binding = None
+_modules: dict = {}
+
+
+def _load(name: str):
+    nat.lib()  # the library it calls; raises if it has not been built
+    path = nat.LIB_PATH.with_name(f"{name}.so")
+    if not path.exists():
+        raise RuntimeError(f"{path} is missing: build the HIP extension first (python -m holmes_amd.build)")
+    spec = importlib.util.spec_from_file_location(name, path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return _modules.setdefault(name, module)
 
 
 def _bound():
     """The extension module of csrc/clear_bind.cpp: a call on a few tokens costs what the host does for it, so
     the checks of tensors, the outputs' allocation and the launch are one native call."""
 
-    global _binding
-    if _binding is None:
-        nat.lib()  # the library it calls; raises if it has not been built
-        path = nat.LIB_PATH.with_name("_clear.so")
-        if not path.exists():
-            raise RuntimeError(f"{path} is missing: build the HIP extension first (python -m holmes_amd.build)")
-        spec = importlib.util.spec_from_file_location("_clear", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
-        _binding = module
-    return _binding
+    return _modules.get("_clear") or _load("_clear")
+
+
+def _window():
+    """The extension module of csrc/window_bind.cpp, likewise."""
+
+    return _modules.get("_window") or _load("_window")
 
 
 class ClearKVPages:
@@ -105,7 +146,7 @@ class ClearKVPages:
         self._lib = nat.lib()
         self.buf = torch.zeros((self.pages, self.kv_heads, self._lib.hck_kv4_page_bytes(self.head_dim)),
                                dtype=torch.uint8, device=device)
-        self._native = _bound()
+        self._native, self._more = _bound(), _window()
         self._shape = (self.pages, self.kv_heads, self.head_dim, self.buf.device.index)
 
     @property
@@ -153,6 +194,140 @@ class ClearKVPages:
         if type(got) is int:
             nat.check(got, "hck_kv4_attend")
         return Attended._make(got)
+
+
+    def weigh(self, queries: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, lse: torch.Tensor, *,
+              starts: torch.Tensor | None = None, most: int | None = None, causal: bool = True,
+              scale: float | None = None, prior: torch.Tensor | None = None) -> torch.Tensor:
+        """What the attention of ``queries`` has given each cached token: the sum of exp(score - lse) over the rows that
+        see it, of the queries of one key head, [sequences][kv_heads][columns * 128] float32.  The arguments are
+        ``attend``'s, and ``lse`` is what it returned for them (a row of -inf gives nothing).  ``prior`` [sequences][kv_heads][places], what
+        earlier calls gave, is added, as 0 where it has no place; places behind a sequence's end are 0.  Without
+        ``causal`` and ``most`` as for ``attend``."""
+
+        got = self._more.weigh(self.buf, *self._shape, queries, table, lengths, lse, starts, most, causal, scale, prior)
+        if type(got) is int:
+            nat.check(got, "hck_kv4_weigh")
+        return got
+
+    def evict(self, table: torch.Tensor, lengths: torch.Tensor, weights: torch.Tensor, into: torch.Tensor, keep: int, *,
+              recent: int = 0) -> Evicted:
+        """Brings every sequence down to ``keep`` tokens for each key head: its last ``recent`` ones, and of the others
+        those of the largest ``weights`` [sequences][kv_heads][places] (float32; 0 behind the last place, NaN above
+        all, the earlier one where they tie).  They are copied, in their order, to the pages ``into`` (int32
+        [sequences][at least keep / 128]), of which each head then holds tokens of its own choice; the pages of ``table`` stay as they are.
+        A sequence of fewer tokens keeps all.  A token whose page is outside the pool is not kept, and a page of ``into``
+        outside it takes nothing.  The pages of ``into`` must be none of the tables' and differ (else what they hold is undefined);
+        places in them behind the kept tokens stay as they were."""
+
+        got = self._more.evict(self.buf, *self._shape, table, lengths, weights, into, keep, recent)
+        if type(got) is int:
+            nat.check(got, "hck_kv4_evict")
+        return Evicted._make(got)
+
+
+# pi to 180 bits
+_PI = Fraction(0x3243F6A8885A308D313198A2E03707344A4093822299F3, 1 << 180)
+
+
+def _rotary_frequencies(rotated: int, base: float, scaling: RotaryScaling | None) -> tuple:
+    """Radians per token of every pair, and what the rotated values are multiplied by."""
+
+    def plain(base):
+        return [base ** (-2 * i / rotated) for i in range(rotated // 2)]
+
+    if scaling is None:
+        return plain(base), 1.0
+    kind, factor, original, low, high = scaling
+    if not (factor >= 1.0 and math.isfinite(factor)):
+        raise ValueError("the factor of a scaling must be finite, and 1 at least")
+    if kind == "linear":
+        return [f / factor for f in plain(base)], 1.0
+    if kind == "base":
+        if rotated < 4:
+            raise ValueError("a scaled base needs two pairs")
+        return plain(base * factor ** (rotated / (rotated - 2))), 1.0
+    if kind not in ("wavelength", "ramp"):
+        raise ValueError('the kind of a scaling must be "linear", "base", "wavelength" or "ramp"')
+    if not (original >= 1 and 0.0 < low < high and math.isfinite(high)):
+        raise ValueError("a blended scaling needs original >= 1 and 0 < low < high")
+
+    if kind == "wavelength":
+        def whole(i, f):
+            return (original * f / (2.0 * math.pi) - low) / (high - low)
+        amount = 1.0
+    else:
+        if base <= 1.0:
+            raise ValueError("a ramp needs a base above 1")
+
+        def pair(turns):
+            return rotated * math.log(original / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
+        first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), rotated - 1)
+
+        def whole(i, f):
+            return 1.0 - (i - first) / max(last - first, 0.001)
+        amount = 0.1 * math.log(factor) + 1.0
+    got = []
+    for i, f in enumerate(plain(base)):
+        w = min(max(whole(i, f), 0.0), 1.0)
+        got.append(w * f + (1.0 - w) * (f / factor))
+    return got, amount
+
+
+class RotaryPositions:
+    """Rotary positions: of the first ``rotated`` dims of a head (default: all), pairs (i, i + rotated / 2), or, with
+    ``interleaved``, (2 i, 2 i + 1), are turned by position * base^(-2 i / rotated) radians; the dims behind stay.  The
+    default is what ``DecodeSpec`` and ``PrefillSpec`` take (pairs of halves, rope_theta 500000).  ``scaling``: for long
+    contexts.  The angle of any position below 2^31 is exact to 2^-34 turns."""
+
+    def __init__(self, head_dim: int = 128, *, base: float = 500000.0, rotated: int | None = None,
+                 interleaved: bool = False, scaling: RotaryScaling | None = None, device="cuda"):
+        rotated = head_dim if rotated is None else rotated
+        if not 2 <= head_dim <= nat.HCK_ROTARY_MAX or head_dim % 2:
+            raise ValueError(f"head_dim must be even, in 2..{nat.HCK_ROTARY_MAX}")
+        if not 2 <= rotated <= head_dim or rotated % 2:
+            raise ValueError("rotated must be even, in 2..head_dim")
+        if not (0.0 < base < math.inf):
+            raise ValueError("base must be positive")
+        self.frequencies, self.amount = _rotary_frequencies(rotated, float(base), scaling)
+        if torch.device(device).type != "cuda" or not torch.cuda.is_available():
+            raise RuntimeError("positions are rotated on a GPU: there is no CPU path")
+        self.head_dim, self.rotated, self.interleaved = int(head_dim), int(rotated), bool(interleaved)
+        # turns per token in units of 2^-64: position times that, modulo 2^64, is the angle's part of a turn
+        turns = [round(Fraction(f) * (1 << 63) / _PI) % (1 << 64) for f in self.frequencies]
+        self._turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
+        self._native = _window()
+
+    def rotate(self, positions: torch.Tensor, queries: torch.Tensor, keys: torch.Tensor | None = None, *,
+               inverse: bool = False):
+        """``queries`` [tokens][heads][head_dim] (bf16, fp16 or fp32, any strides but the last axis contiguous), and
+        ``keys`` [tokens][kv_heads][head_dim] of the same type in the same launch, turned by ``positions`` [tokens] (int64 or
+        int32, any, also negative): new dense tensors, one or both.  ``inverse`` turns back (times the same amount, if ``scaling`` has one)."""
+
+        got = self._native.rotate(self._turns, self.head_dim, self.rotated, self.interleaved, self.amount, positions,
+                                  queries, keys, inverse)
+        if type(got) is int:
+            nat.check(got, "hck_rotary")
+        return got
+
+
+def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                     starts: torch.Tensor | None = None, *, most: int | None = None, causal: bool = True,
+                     scale: float | None = None, ranges: bool = False) -> Attended:
+    """Attention over whole prompts: ``queries`` [tokens][query heads][head_dim] and ``keys`` and ``values``
+    [tokens][kv_heads][head_dim] of 64 or 128 dims, all bf16 or all fp16 (any strides but the last axis contiguous; tensors that
+    16 bytes cannot be loaded from at a time are copied first; query heads a multiple of kv_heads, neighbours sharing a key head).
+
+    Sequence b is the tokens ``starts[b] .. starts[b + 1]`` (int32 [sequences + 1], not decreasing; without ``starts`` there
+    is one of all tokens), and query i of it sees its tokens up to i, or, with ``causal`` off, all.  ``most`` bounds the tokens
+    of one sequence (default: all) and only saves work; a longer one has the rest left unwritten, as has any row that no sequence
+    covers.  ``scale`` and ``ranges`` as for ``ClearKVPages.attend``: the ranges here are those of keys that nothing has
+    rounded, so ``softmax_ranges`` needs no ``rounding`` for them."""
+
+    got = _window().prompt(queries, keys, values, starts, most, causal, scale, ranges)
+    if type(got) is int:
+        nat.check(got, "hck_prompt_attend")
+    return Attended._make(got)
 
 
 def score_rounding(queries: torch.Tensor, keys: torch.Tensor, held: torch.Tensor, scale: float | None = None) -> float:
@@ -218,7 +393,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     NaN), the entropies, and the ``top`` (up to 32) most likely tokens, int64 and log probabilities.  A logit
     of -inf is a token that cannot be; a row of nothing else gives -inf, and 0 for the entropy."""
 
-    got = (_binding or _bound()).scores(logits, tokens, top)
+    got = _bound().scores(logits, tokens, top)
     if type(got) is int:
         nat.check(got, "hck_token_scores")
     return TokenScores._make(got)

@@ -1,0 +1,391 @@
+// Attention over whole prompts whose keys and values are as the projections left them, packed one behind the other.
+//
+//   s = scale q.k over the tokens of the query's sequence up to its own (or all of them), m = max s, l = sum exp(s - m),
+//   out = sum exp(s - m) v / l, lse = m + log l
+//
+// One pass over the keys with a running m and l.  A workgroup of four waves has 128 rows (row = query * group + head, so the
+// heads that share a key head are side by side, whatever their number), 32 to a wave, and takes 64 tokens at a time.  Both
+// products are transposed, S^T = K Q^T and O^T = V^T P^T: the scores that a lane holds after the first are exactly the ones
+// that the second wants of it, and a lane's scores are all of one row.
+//
+// Keys and values go from memory straight into LDS (two units, so that the next one is in flight), 16 bytes a lane, with the
+// 16-byte pieces of a token put where the reads meet no bank twice: keys, read as they lie, at piece ^ token; values, read
+// four tokens by 16 dims at a time through the transposing LDS read, at piece ^ 4 (token % 4).  What lies behind a
+// sequence's end is out of the loads' bounds and becomes zeros.
+//
+// Probabilities are rounded to the values' type for the second product (half a step each; an output's error is that of a sum of
+// rounded terms, of the size of its own rounding); l, and with it lse, is the sum of the unrounded ones.  References of the
+// exponentials are multiples of 8 in units of log 2, so that going over to another is an exact power of two and seldom done.
+#include "kv4_attend.hpp"
+
+namespace hck {
+namespace {
+
+constexpr int kRowsOfWave = 32, kPromptWaves = 4, kTileRows = kRowsOfWave * kPromptWaves;
+
+struct PromptArgs {
+  const void *q, *k, *v;
+  const int* starts;  // null: one sequence of all tokens
+  void* out;
+  float *lse, *low, *high;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, tokens;
+  int seqs, heads, group, causal, most, tiles;  // tiles that the longest sequence can have
+  float scale2;                                 // scale log2 e
+};
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct Eight;
+template <>
+struct Eight<__bf16> {
+  typedef bf16x8 type;
+};
+template <>
+struct Eight<_Float16> {
+  typedef f16x8 type;
+};
+
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_as(float a, float b) {
+  typedef T two __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, two{(T)a, (T)b});
+}
+
+// An infinity or a NaN among eight values: an exponent of ones carries into the sign's bit.
+template <typename T>
+__device__ __forceinline__ uint32_t odd_values(u32x4 x) {
+  constexpr uint32_t kExponent = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t kOne = __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= (x[i] & kExponent) + kOne;
+  return any & 0x80008000u;
+}
+
+// A sequence's tokens, and a tile of its rows.
+struct Tile {
+  int64_t first;
+  int n, rows, tile;
+};
+
+__device__ __forceinline__ void sequence(const PromptArgs& A, int b, int64_t& first, int& n) {
+  first = 0;
+  int64_t last = A.tokens;
+  if (A.starts) {
+    first = max((int64_t)A.starts[b], (int64_t)0);
+    last = min((int64_t)A.starts[b + 1], A.tokens);
+  }
+  n = (int)max(last - first, (int64_t)0);
+}
+__device__ __forceinline__ int rows_of(const PromptArgs& A, int n) { return min(n, A.most) * A.group; }
+
+// Tile r of all sequences' tiles, a sequence's last ones (which see most) first.
+__device__ __forceinline__ bool locate_tile(const PromptArgs& A, int r, Tile& t) {
+  int b = 0;
+  const int lane = threadIdx.x & 63;
+  if (A.seqs > 1) {
+    for (b = 0;; b += 64) {
+      if (b >= A.seqs) return false;
+      int64_t first;
+      int n = 0;
+      if (b + lane < A.seqs) sequence(A, b + lane, first, n);
+      const int mine = (rows_of(A, n) + kTileRows - 1) / kTileRows;
+      const int upto = upto_lane(mine), all = __builtin_amdgcn_readlane(upto, 63);
+      if (r < all) {
+        const int owner = __popcll(__ballot(upto <= r));
+        b += owner;
+        r -= __builtin_amdgcn_readlane(upto - mine, owner);
+        break;
+      }
+      r -= all;
+    }
+  }
+  sequence(A, b, t.first, t.n);
+  t.rows = rows_of(A, t.n);
+  const int tiles = (t.rows + kTileRows - 1) / kTileRows;
+  if (r >= tiles) return false;
+  t.tile = tiles - 1 - r;
+  return true;
+}
+
+template <int D>
+struct Staged {
+  static constexpr int kPieces = D / 8;  // of 16 bytes a token
+  static constexpr int kEach = kUnit * kPieces / (64 * kPromptWaves);  // pieces of a thread
+  static constexpr int kStep = 64 * kPromptWaves / kPieces;            // tokens between a thread's pieces
+  static constexpr int kBytes = kUnit * D * 2;
+  __device__ static int key_at(int token, int piece) {
+    return token * kPieces + (piece ^ (D == 128 ? token & 15 : (token >> 1) & 7));
+  }
+  __device__ static int value_at(int token, int piece) {
+    return token * kPieces + (piece ^ (D == 128 ? (token & 3) << 2 : ((token >> 1) & 1) << 2));
+  }
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+template <typename T, int D, bool RANGE>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
+  using S = Staged<D>;
+  using vec = typename Eight<T>::type;
+  constexpr int kSteps = D / 16, kTiles = D / 32;
+  __shared__ u32x4 s_k[2][kUnit * S::kPieces], s_v[2][kUnit * S::kPieces];
+
+  Tile t;
+  const int h = blockIdx.x % A.heads;
+  if (!locate_tile(A, blockIdx.x / A.heads, t)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int n = __builtin_amdgcn_readfirstlane(t.n), rows = __builtin_amdgcn_readfirstlane(t.rows);
+  const int tile = __builtin_amdgcn_readfirstlane(t.tile);
+  const int64_t first = t.first;
+  auto sees = [&](int row) { return A.causal ? row / A.group + 1 : n; };
+  const int most = sees(min(tile * kTileRows + kTileRows, rows) - 1);
+  const int units = (most + kUnit - 1) / kUnit;
+  const int mine = tile * kTileRows + wave * kRowsOfWave;
+  const int least = mine < rows ? sees(mine) : 0, last = mine < rows ? sees(min(mine + kRowsOfWave, rows) - 1) : 0;
+  const int row = mine + (lane & 31);
+  const bool live = row < rows;
+  const int qi = live ? row / A.group : 0, qo = live ? row % A.group : 0;
+  const int seen = live ? sees(row) : 0;
+
+  // what a thread brings of each unit: pieces of tokens kStep apart
+  const int token0 = threadIdx.x / S::kPieces, piece0 = threadIdx.x % S::kPieces;
+  const uint32_t k_off = (uint32_t)(token0 * A.k_ts * 2) + (S::key_at(token0, piece0) - token0 * S::kPieces) * 16;
+  const uint32_t v_off = (uint32_t)(token0 * A.v_ts * 2) + (S::value_at(token0, piece0) - token0 * S::kPieces) * 16;
+  const char* kp = (const char*)A.k + (first * A.k_ts + h * A.k_hs) * 2;
+  const char* vp = (const char*)A.v + (first * A.v_ts + h * A.v_hs) * 2;
+  auto bring = [&](int u, u32x4* ks, u32x4* vs) {
+    const int left = min(n - u * kUnit, kUnit);
+    const auto kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)u * kUnit * A.k_ts * 2), 0,
+                                                      (int)((left - 1) * A.k_ts * 2 + D * 2), 0x00020000);
+    const auto vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + (int64_t)u * kUnit * A.v_ts * 2), 0,
+                                                      (int)((left - 1) * A.v_ts * 2 + D * 2), 0x00020000);
+#pragma unroll
+    for (int j = 0; j < S::kEach; ++j) {
+      const int at = j * (64 * kPromptWaves) + wave * 64;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr)(ks + at), 16, k_off + (uint32_t)(j * S::kStep * A.k_ts * 2), 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr)(vs + at), 16, v_off + (uint32_t)(j * S::kStep * A.v_ts * 2), 0, 0, 0);
+    }
+  };
+  if (units > 0) bring(0, s_k[0], s_v[0]);
+
+  vec q[kSteps];
+  const T* qp = (const T*)A.q + (first + qi) * A.q_ts + (int64_t)(h * A.group + qo) * A.q_hs + half * 8;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    u32x4 raw = {0, 0, 0, 0};
+    if (live) raw = *reinterpret_cast<const u32x4*>(qp + s * 16);
+    q[s] = __builtin_bit_cast(vec, raw);
+  }
+
+  // Where the lane reads: keys of token lane % 32 (and 32 on); values of the tokens 4 half + lane % 16 / 4 (and 8 on), of
+  // which lane i of 16 gets dim i.
+  const int vt = 4 * half + ((lane & 15) >> 2), vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+  // Exponentials times 2^lift.  fp16: the largest up to 2^15, so that those down to 2^-29 of it keep all bits.  bf16: such
+  // that their sum is at most 1, and no sum of values overflows.
+  const float lift = __is_same(T, _Float16) ? 15.f : (float)(__builtin_clz(n) - 32);
+
+  f32x16 acc[kTiles];
+#pragma unroll
+  for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  float top = -INFINITY, sum = 0.f, low = INFINITY;
+  float ref = -lift, factor = A.scale2;
+
+  auto unit = [&](int u, const u32x4* ks, const u32x4* vs) {
+    const int here = u * kUnit;
+    if (here >= last) return;
+    f32x16 c[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c[0][i] = c[1][i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const vec k = __builtin_bit_cast(vec, ks[S::key_at(32 * x + (lane & 31), 2 * s + half)]);
+        c[x] = mfma32(k, q[s], c[x]);
+      }
+    const int base = here + 4 * half;  // of the lane's tokens base + 32 x + 8 (i / 4) + i % 4
+    const bool partly = here + kUnit > least;
+    if (partly) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool see = base + 32 * x + 8 * (i >> 2) + (i & 3) < seen;
+          if constexpr (RANGE) low = see ? fminf(low, c[x][i]) : low;
+          c[x][i] = see ? c[x][i] : -INFINITY;
+        }
+    } else if constexpr (RANGE) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) low = smaller(low, c[x][i]);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = larger(mx, c[x][i]);
+    const float raw = over_half(mx, fmax2);
+    mx = fmaxf(top, raw * A.scale2);
+    const float f = rebase(top, mx);
+    top = mx;
+    if (__any(f != 1.f)) {
+      if (f != 1.f) {
+        refer(mx, raw, A.scale2, ref, factor);
+        ref += kLift - lift;
+      }
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) acc[d] *= f;
+    }
+
+    // (the transposing reads of 16 tokens and 32 dims)
+    auto values = [&](int j, int d) {
+      s16x4 x[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const u32x4* at = vs + S::value_at(16 * j + 8 * p + vt, 4 * d + vc);
+        x[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)((const char*)at + (lane & 1) * 8));
+      }
+      const u32x2 a = __builtin_bit_cast(u32x2, x[0]), b = __builtin_bit_cast(u32x2, x[1]);
+      return u32x4{a[0], a[1], b[0], b[1]};
+    };
+    float part[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float e[8];
+      u32x4 p, v[kTiles];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[j >> 1][8 * (j & 1) + i], factor, -ref));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = pack_as<T>(e[2 * i], e[2 * i + 1]);
+        part[i & 1] += e[2 * i] + e[2 * i + 1];
+      }
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) v[d] = values(j, d);
+      if (partly) {
+        // Tokens that a row does not see have a probability of 0, and 0 times an infinity or a NaN is NaN.  Where there
+        // is one, the tokens go one by one, each for the rows that see it.
+        uint32_t odd = 0;
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) odd |= odd_values<T>(v[d]);
+        if (__any(odd != 0)) {
+#pragma unroll 1
+          for (int k = 0; k < 16; ++k) {
+            const int at = k & 7;  // of the eight of half k / 8
+            u32x4 only;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) only[i] = half == k >> 3 && at >> 1 == i ? (at & 1 ? 0xffff0000u : 0xffffu) : 0u;
+            const bool see = here + 16 * j + 8 * (at >> 2) + 4 * (k >> 3) + (at & 3) < seen;
+#pragma unroll
+            for (int d = 0; d < kTiles; ++d) {
+              f32x16 one;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) one[i] = 0.f;
+              one = mfma32(__builtin_bit_cast(vec, v[d] & only), __builtin_bit_cast(vec, p & only), one);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[d][i] += see ? one[i] : 0.f;
+            }
+          }
+          continue;
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(__builtin_bit_cast(vec, v[d]), __builtin_bit_cast(vec, p), acc[d]);
+    }
+    sum += part[0] + part[1];
+  };
+
+  for (int u = 0; u < units; u += 2) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // this thread's loads have come (vmcnt 0)
+    __syncthreads();
+    if (u + 1 < units) bring(u + 1, s_k[1], s_v[1]);
+    unit(u, s_k[0], s_v[0]);
+    if (u + 1 >= units) break;
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (u + 2 < units) bring(u + 2, s_k[0], s_v[0]);
+    unit(u + 1, s_k[1], s_v[1]);
+  }
+
+  sum = over_half(sum, [](float a, float c) { return a + c; });
+  if constexpr (RANGE) low = over_half(low, fmin2) * A.scale2;
+  if (!live) return;
+  const int64_t at = (first + qi) * (int64_t)(A.heads * A.group) + h * A.group + qo;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* out = (T*)A.out + at * D + 4 * half;
+#pragma unroll
+  for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = pack_as<T>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv);
+      const uint32_t b = pack_as<T>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv);
+      *reinterpret_cast<u32x2*>(out + 32 * d + 8 * i) = u32x2{a, b};
+    }
+  if (half) return;
+  const bool bad = sum != sum;
+  A.lse[at] = fabsf(top) == INFINITY ? top + sum : (above(top) + (__builtin_amdgcn_logf(sum) - lift)) * kLn2;
+  if constexpr (RANGE) A.low[at] = bad ? sum : low * kLn2, A.high[at] = bad ? sum : top * kLn2;
+}
+
+template <typename T, int D>
+int launch(const PromptArgs& A, int64_t items, hipStream_t s) {
+  const unsigned groups = (unsigned)(items * A.heads);
+  if (A.low) k_whole<T, D, true><<<groups, 64 * kPromptWaves, 0, s>>>(A);
+  else k_whole<T, D, false><<<groups, 64 * kPromptWaves, 0, s>>>(A);
+  HCK_CHECK_LAUNCH();
+  return HCK_OK;
+}
+
+}  // namespace
+}  // namespace hck
+
+extern "C" int hck_prompt_attend(const void* queries, const void* keys, const void* values, int type, int64_t tokens,
+                                 int kv_heads, int group, int head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                                 int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                 const int32_t* starts, int seqs, int most, int causal, double scale, void* out, float* lse,
+                                 float* low, float* high, void* stream) {
+  if ((head_dim != 64 && head_dim != 128) || (type != HCK_BF16 && type != HCK_F16)) return HCK_ERR_UNSUPPORTED;
+  if (tokens < 0 || tokens > INT32_MAX || kv_heads < 1 || group < 1 || (int64_t)kv_heads * group > INT32_MAX || seqs < 0 ||
+      most < 0 || !((float)scale > 0.f && scale <= 0x1p126) || (low == nullptr) != (high == nullptr))
+    return HCK_ERR_ARG;
+  if (!starts && seqs != 1) return HCK_ERR_ARG;
+  most = (int)std::min<int64_t>(most, tokens);
+  if (seqs == 0 || most == 0) return HCK_OK;
+  if (!queries || !keys || !values || !out || !lse || (int64_t)most * group > INT32_MAX - 256) return HCK_ERR_ARG;
+  if (((uintptr_t)queries | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out) % 16) return HCK_ERR_ARG;
+  for (int64_t stride : {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride})
+    if (stride % 8) return HCK_ERR_ARG;
+  // a unit's loads count its bytes in 31 bits, and tell a sequence's end by them
+  for (int64_t stride : {k_token_stride, v_token_stride})
+    if (tokens > 1 && (stride < head_dim || stride > 1 << 23)) return HCK_ERR_ARG;
+  hck::PromptArgs A = {};
+  A.q = queries, A.k = keys, A.v = values, A.starts = starts, A.out = out, A.lse = lse, A.low = low, A.high = high;
+  A.q_ts = q_token_stride, A.q_hs = q_head_stride, A.tokens = tokens;
+  A.k_ts = tokens > 1 ? k_token_stride : head_dim, A.k_hs = k_head_stride;
+  A.v_ts = tokens > 1 ? v_token_stride : head_dim, A.v_hs = v_head_stride;
+  A.seqs = seqs, A.heads = kv_heads, A.group = group, A.causal = causal != 0, A.most = most;
+  A.scale2 = (float)(scale * 1.4426950408889634);
+  // every sequence has a tile that may not be full, beside the full ones
+  const int64_t tiles = ((int64_t)most * group + hck::kTileRows - 1) / hck::kTileRows;
+  const int64_t items = std::min(tiles * seqs, tokens * group / hck::kTileRows + seqs);
+  if (items * kv_heads > INT32_MAX) return HCK_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (head_dim == 128) return type == HCK_BF16 ? hck::launch<__bf16, 128>(A, items, s) : hck::launch<_Float16, 128>(A, items, s);
+  return type == HCK_BF16 ? hck::launch<__bf16, 64>(A, items, s) : hck::launch<_Float16, 64>(A, items, s);
+}

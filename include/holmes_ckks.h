@@ -475,6 +475,53 @@ int hck_token_scores(const void* logits, int type, int64_t rows, int vocab, int6
                      int top, float* given, float* entropy, int64_t* top_ids, float* top_logs, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* Rotary positions: pairs (i, i + rotated / 2), or with `interleaved` (2 i, 2 i + 1), of the first `rotated` dims of every
+ * head turned by position * frequency and multiplied by `amount`, the dims behind copied; backwards with `inverse`.
+ * positions[tokens] are device integers of position_bytes (4 or 8); turns[rotated / 2] (device) are the frequencies in
+ * turns per token, in units of 2^-64.  Queries and keys are [tokens][heads][head_dim] with element strides, the last axis
+ * contiguous, of one type (HCK_BF16, HCK_F16, HCK_F32); either may have no heads.  Outputs are dense, and must not
+ * overlap the inputs.  head_dim is even and at most HCK_ROTARY_MAX; heads + kv_heads at most 65535, and times head_dim at
+ * most HCK_ROTARY_TOKEN. */
+#define HCK_ROTARY_MAX 512
+#define HCK_ROTARY_TOKEN (1 << 20)
+int hck_rotary(const void* positions, int position_bytes, int64_t tokens, const uint64_t* turns, int rotated, int interleaved,
+               int inverse, float amount, int type, int head_dim, const void* queries, int64_t q_token_stride,
+               int64_t q_head_stride, int heads, void* out_queries, const void* keys, int64_t k_token_stride,
+               int64_t k_head_stride, int kv_heads, void* out_keys, void* stream);
+
+/* Attention of whole prompts: sequence b is the tokens starts[b] .. starts[b + 1] (device, not decreasing; starts NULL: one
+ * sequence of all tokens) of queries [tokens][kv_heads * group][head_dim] and keys and values [tokens][kv_heads][head_dim],
+ * all bf16 or all fp16, and its queries see its tokens up to their own (with `causal` 0: all of them).  Element strides,
+ * multiples of 8, from 16-byte aligned addresses; tokens of keys and values lie head_dim to 2^23 elements apart.  `most` is at
+ * least the largest number of tokens of a sequence.  out, lse, low, high and scale are as for hck_kv4_attend; a token that no
+ * sequence covers is left unwritten. */
+int hck_prompt_attend(const void* queries, const void* keys, const void* values, int type, int64_t tokens, int kv_heads,
+                      int group, int head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                      int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const int32_t* starts, int seqs,
+                      int most, int causal, double scale, void* out, float* lse, float* low, float* high, void* stream);
+
+/* What attention has given each cached token: weights[b][h][j] = prior + the sum over the rows of key head h that see token j
+ * of exp(scale q.k_j - lse), for the queries, pages and masks of hck_kv4_attend and the lse that it gave (a row of -inf
+ * gives nothing).  weights is dense, [seqs][kv_heads][table_columns * 128]; places behind a sequence's length become 0, and a
+ * page outside the pool adds nothing.  prior (NULL with prior_places 0: none) has prior_places places a row, and counts as
+ * 0 behind them.  table_columns is below 2^23. */
+int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* queries, int64_t tokens,
+                  int group, int64_t q_token_stride, int64_t q_head_stride, const int32_t* table, int64_t table_stride,
+                  int table_columns, const int32_t* lengths, const int32_t* starts, int seqs, int most, int causal,
+                  double scale, const float* lse, const float* prior, int64_t prior_seq_stride, int64_t prior_head_stride,
+                  int prior_places, float* weights, void* stream);
+
+/* Of every sequence and key head `keep` tokens go to the pages into[b * into_stride ..] (at least keep / 128, rounded up):
+ * the last `recent` (at most keep) and the heaviest others, ties to the lowest place, NaN above all, in their order.  Weights
+ * have weight_places places a row and count as 0 behind them.  kept [seqs][kv_heads][keep] are the places that they had (-1
+ * where there are fewer), new_weights their weights (0 there), new_lengths [seqs] their number.  A token whose page is
+ * outside the pool is not kept; a target page outside it takes nothing.  Target pages must not be pages of the tables, nor
+ * twice in `into`: what those hold is undefined.  Places of a target page behind the kept tokens stay as they were. */
+int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_dim, const int32_t* table, int64_t table_stride,
+                  int table_columns, const int32_t* lengths, int seqs, const float* weights, int64_t weight_seq_stride,
+                  int64_t weight_head_stride, int weight_places, const int32_t* into, int64_t into_stride, int into_columns,
+                  int keep, int recent, int32_t* kept, int32_t* new_lengths, float* new_weights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
