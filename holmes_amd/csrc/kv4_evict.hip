@@ -10,7 +10,7 @@
 // written whole.
 #include "../../include/holmes_ckks.h"
 #include "internal.hpp"
-#include "kv4.hpp"
+#include "kv4_attend.hpp"
 
 namespace hck {
 namespace {
@@ -41,123 +41,169 @@ __device__ __forceinline__ int lanes_below(unsigned long long mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// One row: a sequence and a key head.
+// Sums over the threads up to each, and over all; `part` has a place for every wave.
+__device__ __forceinline__ int upto_thread(int x, int* part, int& all) {
+  const int upto = upto_lane(x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();  // what was read of `part` before
+  if (lane == 63) part[wave] = upto;
+  __syncthreads();
+  const int sums = upto_lane(lane < kSelectWaves ? part[lane] : 0);
+  all = __builtin_amdgcn_readlane(sums, kSelectWaves - 1);
+  return upto + (wave ? __builtin_amdgcn_readlane(sums, __builtin_amdgcn_readfirstlane(wave) - 1) : 0);
+}
+
+// One row: a sequence and a key head.  Thread t has the keys of places t, 1024 + t, .. in registers, R of them, read at once
+// and looked at four times; a row of more goes through them in pieces, read anew each time.  A key of 0 is no choice.
+//
+// Counts of the first digit, which is mostly the exponents', would meet in few places, so every eighth lane has counts of
+// its own.
+template <int R>
 __global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
-  __shared__ int s_bins[kBins];
-  __shared__ int s_above[kSelectWaves], s_at[kSelectWaves], s_last[kSelectWaves];
-  __shared__ int s_found[2];
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kCopies = R >= 4 ? 8 : 1, kPiece = R * kSelect;
+  __shared__ int s_bins[kBins * kCopies];
+  __shared__ int s_stay[R * kSelectWaves], s_tie[R * kSelectWaves], s_part[kSelectWaves], s_found[2];
+  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = (int)min((int64_t)max(A.lengths[b], 0), (int64_t)A.cols * kPageTokens);
   const int last = max(n - A.recent, 0);  // from here on all stay
   const int* table = A.table + b * A.table_stride;
   const float* weights = A.weights + b * A.w_seq + h * A.w_head;
   int* kept = A.kept + ((int64_t)b * A.heads + h) * A.keep;
   float* out = A.new_weights + ((int64_t)b * A.heads + h) * A.keep;
-  auto there = [&](int j) {  // whether place j's page is in the pool
+
+  // Places whose page is not in the pool: as a rule there are none, and no place asks again.
+  int gone = 0;
+  for (int i = threadIdx.x; i * kPageTokens < n; i += kSelect) {
+    const int pg = table[i];
+    gone |= pg < 0 || pg >= A.pages;
+  }
+  const bool whole = !__syncthreads_or(gone);
+  auto there = [&](int j) {
+    if (whole) return true;
     const int pg = table[j / kPageTokens];
     return pg >= 0 && pg < A.pages;
   };
-  auto weight = [&](int j) { return j < A.width ? weights[j] : 0.f; };
+
+  uint32_t key[R];
+  const int pieces = (n + kPiece - 1) / kPiece;
+  auto load = [&](int piece) {
+    float w[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int j = piece * kPiece + r * kSelect + threadIdx.x;
+      w[r] = j < last && j < A.width ? weights[j] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int j = piece * kPiece + r * kSelect + threadIdx.x;
+      key[r] = j < last && there(j) ? key_of(w[r]) : 0;
+    }
+  };
+  if (pieces) load(0);
 
   // how many there are to choose from, and how many of the last
-  if (threadIdx.x < 2) s_found[threadIdx.x] = 0;
-  __syncthreads();
-  int mine = 0, lasts = 0;
-  for (int j = threadIdx.x; j < n; j += kSelect)
-    if (there(j)) (j < last ? mine : lasts) += 1;
-  atomicAdd(&s_found[0], mine), atomicAdd(&s_found[1], lasts);
-  __syncthreads();
-  const int choice = s_found[0], must = s_found[1];
+  int choice = last, must = n - last;
+  if (!whole) {
+    int mine = 0, lasts = 0, all;
+    for (int j = threadIdx.x; j < n; j += kSelect)
+      if (there(j)) (j < last ? mine : lasts) += 1;
+    upto_thread(mine, s_part, all);
+    choice = all;
+    upto_thread(lasts, s_part, all);
+    must = all;
+  }
   const int want = min(choice, A.keep - must);  // of those to choose from (recent is at most keep)
-  __syncthreads();
 
   // T, and how many tokens at T stay
   uint32_t prefix = 0;
   int left = want;
-  if (want > 0 && want < choice) {
+  const bool all = want == choice, none = want <= 0;
+  if (!all && !none) {
     for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-      for (int i = threadIdx.x; i < kBins; i += kSelect) s_bins[i] = 0;
+      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11, bins = 1 << bits;
+      for (int i = threadIdx.x; i < kBins * kCopies; i += kSelect) s_bins[i] = 0;
       __syncthreads();
-      const int bins = 1 << bits;
-      for (int j = threadIdx.x; j < last; j += kSelect) {
-        if (!there(j)) continue;
-        const uint32_t key = key_of(weight(j));
-        if (digit && (key >> (shift + bits)) != prefix) continue;
-        atomicAdd(&s_bins[(key >> shift) & (bins - 1)], 1);
+      for (int piece = 0; piece < pieces; ++piece) {
+        if (pieces > 1) load(piece);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (key[r] && (digit == 0 || (key[r] >> (shift + bits)) == prefix))
+            atomicAdd(&s_bins[((key[r] >> shift) & (bins - 1)) * kCopies + lane % kCopies], 1);
       }
       __syncthreads();
-      // the largest bin with `left` tokens or more in it and above it: one wave, 32 bins a lane
-      if (wave == 0) {
-        int sum = 0;
-        const int per = bins / 64, top = bins - 1 - lane * per;
-        for (int i = 0; i < per; ++i) sum += s_bins[top - i];
-        int upto = sum;
-        for (int d = 1; d < 64; d *= 2) {
-          const int o = __shfl_up(upto, d);
-          if (lane >= d) upto += o;
-        }
-        int before = upto - sum;
-        if (before < left && upto >= left) {  // one lane
-          int i = 0;
-          for (; before + s_bins[top - i] < left; ++i) before += s_bins[top - i];
-          s_found[0] = top - i, s_found[1] = left - before;
-        }
+      // the largest bin with `left` tokens or more in it and above it: two bins a thread, from the top
+      const int top = bins - 1 - 2 * (int)threadIdx.x;
+      int count[2] = {0, 0}, total;
+      if (top > 0) {
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) count[0] += s_bins[top * kCopies + c], count[1] += s_bins[(top - 1) * kCopies + c];
+      }
+      const int upto = upto_thread(count[0] + count[1], s_part, total), before = upto - count[0] - count[1];
+      if (before < left && upto >= left) {  // one thread
+        const bool second = before + count[0] < left;
+        s_found[0] = second ? top - 1 : top, s_found[1] = left - before - (second ? count[0] : 0);
       }
       __syncthreads();
       prefix = prefix << bits | (uint32_t)s_found[0];
       left = s_found[1];
-      __syncthreads();
     }
   }
-  const bool all = want == choice, none = want <= 0;
-  // Tokens above T, at T and among the last, by waves: each has a run of the places.
-  const int run = ((n + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
-  const int from = min(wave * run, n), to = from + min(run, n - from);
-  int above = 0, at = 0, tail = 0;
-  for (int j0 = from; j0 < to; j0 += 64) {
-    const int j = j0 + lane;
-    if (j >= to || !there(j)) continue;
-    if (j >= last) ++tail;
-    else if (all) ++above;
-    else if (!none) {
-      const uint32_t key = key_of(weight(j));
-      above += key > prefix, at += key == prefix;
-    }
-  }
-  for (int d = 32; d; d /= 2) above += __shfl_xor(above, d), at += __shfl_xor(at, d), tail += __shfl_xor(tail, d);
-  if (lane == 0) s_above[wave] = above, s_at[wave] = at, s_last[wave] = tail;
-  __syncthreads();
+
+  // What stays, 64 places at a time: how many for certain and how many at T; where each 64 begin; and then each place.
   int place = 0, ties = 0;
-  for (int w = 0; w < wave; ++w) {
-    const int t = min(s_at[w], left - ties);
-    place += s_above[w] + s_last[w] + (all || none ? 0 : t), ties += all || none ? 0 : t;
-  }
-  for (int j0 = from; j0 < to; j0 += 64) {
-    const int j = j0 + lane;
-    bool stay = false, tie = false;
-    float w = 0.f;
-    if (j < to && there(j)) {
-      w = weight(j);
-      if (j >= last || all) stay = true;
-      else if (!none) {
-        const uint32_t key = key_of(w);
-        stay = key > prefix, tie = key == prefix;
+  for (int piece = 0; piece < pieces; ++piece) {
+    if (pieces > 1) load(piece);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int j = piece * kPiece + r * kSelect + threadIdx.x;
+      const bool sure = j >= last ? j < n && there(j) : key[r] && (all || (!none && key[r] > prefix));
+      const bool tie = key[r] && !all && !none && key[r] == prefix;
+      const unsigned long long sures = __ballot(sure), tied = __ballot(tie);
+      if (lane == 0) s_stay[r * kSelectWaves + wave] = (int)__popcll(sures), s_tie[r * kSelectWaves + wave] = (int)__popcll(tied);
+    }
+    __syncthreads();
+    constexpr int kMine = (R * kSelectWaves + kSelect - 1) / kSelect;
+    int sum = 0, at[kMine], stay[kMine], got;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int e = threadIdx.x * kMine + i;
+      at[i] = e < R * kSelectWaves ? s_tie[e] : 0, stay[i] = e < R * kSelectWaves ? s_stay[e] : 0, sum += at[i];
+    }
+    int rank = ties + upto_thread(sum, s_part, got) - sum;  // ties before the thread's first 64
+    ties += got;
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int e = threadIdx.x * kMine + i;
+      if (e < R * kSelectWaves) s_tie[e] = rank;
+      const int taken = max(0, min(at[i], left - rank));
+      rank += at[i], stay[i] += taken, sum += stay[i];
+    }
+    int begin = place + upto_thread(sum, s_part, got) - sum;
+    place += got;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int e = threadIdx.x * kMine + i;
+      if (e < R * kSelectWaves) s_stay[e] = begin;
+      begin += stay[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int j = piece * kPiece + r * kSelect + threadIdx.x;
+      bool stays = j >= last ? j < n && there(j) : key[r] && (all || (!none && key[r] > prefix));
+      const bool tie = key[r] && !all && !none && key[r] == prefix;
+      const unsigned long long tied = __ballot(tie);
+      if (tie && s_tie[r * kSelectWaves + wave] + lanes_below(tied) < left) stays = true;
+      const unsigned long long staying = __ballot(stays);
+      if (stays) {
+        const int p = s_stay[r * kSelectWaves + wave] + lanes_below(staying);
+        kept[p] = j, out[p] = j < A.width ? weights[j] : 0.f;
       }
     }
-    const unsigned long long tied = __ballot(tie);
-    if (tie && ties + lanes_below(tied) < left) stay = true;
-    ties = min(left, ties + (int)__popcll(tied));
-    const unsigned long long staying = __ballot(stay);
-    if (stay) {
-      const int p = place + lanes_below(staying);
-      kept[p] = j, out[p] = w;
-    }
-    place += (int)__popcll(staying);
   }
-  const int total = max(want, 0) + must;
-  for (int p = total + threadIdx.x; p < A.keep; p += kSelect) kept[p] = -1, out[p] = 0.f;
-  if (h == 0 && threadIdx.x == 0) A.new_lengths[b] = total;
+  for (int p = place + threadIdx.x; p < A.keep; p += kSelect) kept[p] = -1, out[p] = 0.f;
+  if (h == 0 && threadIdx.x == 0) A.new_lengths[b] = place;
 }
 
 // One head's part of a target page.  A place that takes no token has itself for its source: its bytes stay.
@@ -247,7 +293,13 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
   A.w_head = weight_head_stride, A.cols = table_columns, A.heads = kv_heads, A.width = weight_places,
   A.into_cols = into_columns, A.keep = keep, A.recent = recent;
   hipStream_t s = (hipStream_t)stream;
-  hck::k_select<<<dim3(kv_heads, seqs), hck::kSelect, 0, s>>>(A);
+  // the least keys a thread for which a row goes through the registers once, as far as a table tells
+  const int64_t room = (int64_t)table_columns * hck::kPageTokens;
+  auto* select = room <= 1 * hck::kSelect   ? hck::k_select<1>
+                 : room <= 4 * hck::kSelect ? hck::k_select<4>
+                 : room <= 16 * hck::kSelect ? hck::k_select<16>
+                                             : hck::k_select<64>;
+  select<<<dim3(kv_heads, seqs), hck::kSelect, 0, s>>>(A);
   HCK_CHECK_LAUNCH();
   if (need) {
     const dim3 grid((unsigned)need, kv_heads, seqs);

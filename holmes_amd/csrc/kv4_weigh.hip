@@ -13,8 +13,9 @@ struct WeighArgs {
   AttendArgs a;  // of which: pool, q, table, lengths, starts, strides, shapes
   const float *row_lse, *prior;
   float* weights;
+  float* parts;  // with more than one: [part][seq][head][place]
   int64_t prior_seq, prior_head;
-  int prior_places;
+  int prior_places, split;  // split: parts that the rows of 256 tokens are cut into
   float scale2, rest;  // scale log2 e in 32 bits, and what its rounding left over, divided by scale
 };
 
@@ -120,14 +121,253 @@ __global__ __launch_bounds__(64 * kWaves) void k_weigh(WeighArgs W) {
   *to = sum;
 }
 
+
+// Many rows: the keys of 64 tokens stay in a wave's registers as the right operand, 32 tokens to a product, and the rows pass
+// by, 64 at a time through LDS for the four waves of 256 tokens.  A lane has one token (two in all) and 16 of 32 rows, so its
+// sums need no other lane until the end; what comes off a row's scores is read from LDS, four rows at a time.  Rows that come
+// in parts (few tokens, many rows) leave sums of their own, which k_weigh_join adds in order.
+//
+// A sum over many rows is taken over 64 of them and then over those, with what each addition of the latter loses carried on.
+constexpr int kStage = 64, kBlock = kUnit * kWaves;  // rows at a time, tokens of a workgroup
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
+  using L = Kv4<D>;
+  constexpr int kSteps = D / 16, kPieces = D / 8, kEach = kStage * kPieces / (64 * kWaves), kApart = 64 * kWaves / kPieces;
+  constexpr bool kHalf = __is_same(T, _Float16);
+  constexpr int kParts = kHalf ? 2 : 1;
+  __shared__ u32x4 s_q[2][kParts][kStage * kPieces];
+  __shared__ float s_off[2][kStage], s_factor[2][kStage];
+  __shared__ int s_seen[2][kStage], s_least[2][2];
+  const AttendArgs& A = W.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, half = lane >> 5;
+  // (the tokens that most rows see first)
+  const int h = blockIdx.x % A.heads, part = blockIdx.x / A.heads % W.split, block = blockIdx.x / A.heads / W.split, b = blockIdx.y;
+  const Rows R(A, b);
+  const int first = block * kBlock, here = first + wave * kUnit;
+  const int64_t width = (int64_t)A.cols * kPageTokens, line = (int64_t)b * A.heads + h;
+  if (first >= R.length) {
+    const int j = first + threadIdx.x;
+    if (W.split == 1 && j < width) W.weights[line * width + j] = 0.f;
+    return;
+  }
+  int pg = -1;
+  if (here < R.length) pg = A.table[b * A.table_stride + here / kPageTokens];
+  const bool there = pg >= 0 && pg < A.pages;
+
+  bf16x8 k[2][kSteps];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int t = (here & (kPageTokens - 1)) + 32 * x + n;  // within the page
+    const uint8_t* page = A.pool + ((int64_t)(there ? pg : 0) * A.heads + h) * L::kBytes;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {  // dims (2 p + half) D / 4 ..
+      typedef uint32_t words __attribute__((ext_vector_type(D / 32)));
+      const words c = *reinterpret_cast<const words*>(page + L::key_code(t, (2 * p + half) * (D / 4)));
+      const int byte = page[L::key_scale(t, (2 * p + half) * (D / 4) / kRun)];
+      const float sc = __uint_as_float(byte == kNanByte ? 0x7fc00000u : (uint32_t)byte << 23);
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s)
+        k[x][p * (D / 32) + s] = operand(cvt<0>(c[s], sc), cvt<1>(c[s], sc), cvt<2>(c[s], sc), cvt<3>(c[s], sc));
+    }
+  }
+
+  // the part's rows, from the first query that sees one of the workgroup's tokens
+  const int skip = A.causal ? (int)min((int64_t)R.rows, (int64_t)max(0, first - (R.length - R.nq)) * A.group) / kStage * kStage : 0;
+  const int stages = (R.rows - skip + kStage - 1) / kStage, each = (stages + W.split - 1) / W.split;
+  const int from = skip + min(part * each, stages) * kStage, to = min(R.rows, skip + min((part + 1) * each, stages) * kStage);
+
+  // A thread brings pieces of rows kApart apart; row = query * group + head goes on by additions.
+  const int piece = threadIdx.x % kPieces, row0 = threadIdx.x / kPieces;
+  int qi = (from + row0) / A.group, qo = (from + row0) % A.group;
+  const int step_i = kApart / A.group, step_o = kApart % A.group;
+  u32x4 raw[kEach];
+  auto bring = [&](int at) {  // rows at .. at + kStage - 1
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      raw[j] = u32x4{0, 0, 0, 0};
+      if (at + row0 + j * kApart < to)
+        raw[j] = reinterpret_cast<const Loose16*>((const T*)A.q + (R.q0 + qi) * A.q_ts + (int64_t)(h * A.group + qo) * A.q_hs +
+                                                  piece * 8)->v;
+      qi += step_i, qo += step_o;
+      if (qo >= A.group) qo -= A.group, ++qi;
+    }
+  };
+  auto place = [](int row, int p) { return row * kPieces + (p ^ (D == 128 ? row & 15 : (row >> 1) & 7)); };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int at = place(row0 + j * kApart, piece);
+      if constexpr (kHalf) {
+        bf16x8 head, rest;
+        query_parts<T>(raw[j], head, rest);
+        s_q[buf][0][at] = __builtin_bit_cast(u32x4, head);
+        s_q[buf][kParts - 1][at] = __builtin_bit_cast(u32x4, rest);
+      } else {
+        s_q[buf][0][at] = raw[j];
+      }
+    }
+  };
+  auto terms = [&](int buf, int at) {  // one wave
+    const RowTerm t = row_term(W, R, h, at + lane);
+    const int seen = at + lane < to ? t.seen : 0;
+    s_off[buf][lane] = t.off, s_factor[buf][lane] = t.factor, s_seen[buf][lane] = seen;
+    int least = seen;
+    for (int d = 1; d < 32; d *= 2) least = min(least, __shfl_xor(least, d));
+    if (n == 0) s_least[buf][half] = least;
+  };
+
+  float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};
+  if (from < to) {
+    bring(from);
+    put(0);
+    if (wave == 0) terms(0, from);
+  }
+  __syncthreads();
+  for (int at = from, buf = 0; at < to; at += kStage, buf ^= 1) {
+    const bool more = at + kStage < to;
+    if (more) bring(at + kStage);
+    if (there) {
+      float now[2] = {0.f, 0.f};
+#pragma unroll 1
+      for (int y = 0; y < 2; ++y) {
+        f32x16 c[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c[0][i] = c[1][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const int at = place(32 * y + n, (2 * (s / (D / 32)) + half) * (D / 32) + s % (D / 32));
+          const bf16x8 q = __builtin_bit_cast(bf16x8, s_q[buf][0][at]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) c[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, k[x][s], c[x], 0, 0, 0);
+          if constexpr (kHalf) {
+            const bf16x8 r = __builtin_bit_cast(bf16x8, s_q[buf][kParts - 1][at]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) c[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(r, k[x][s], c[x], 0, 0, 0);
+          }
+        }
+        const bool partly = here + kUnit > __builtin_amdgcn_readfirstlane(s_least[buf][y]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // rows 8 i + 4 half ..
+          const int r = 32 * y + 8 * i + 4 * half;
+          const f32x4 off = *reinterpret_cast<const f32x4*>(&s_off[buf][r]);
+          const f32x4 factor = *reinterpret_cast<const f32x4*>(&s_factor[buf][r]);
+          float p[2][4];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              p[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][4 * i + e], W.scale2, -off[e]));
+          if (partly) {
+            typedef int i32x4 __attribute__((ext_vector_type(4)));
+            const i32x4 seen = *reinterpret_cast<const i32x4*>(&s_seen[buf][r]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[x][e] = here + 32 * x + n < seen[e] ? p[x][e] : 0.f;
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) now[x] = __builtin_fmaf(p[x][e], factor[e], now[x]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float add = now[x] - lost[x], all = sum[x] + add;
+        lost[x] = fabsf(all) < INFINITY ? (all - sum[x]) - add : 0.f;
+        sum[x] = all;
+      }
+    }
+    if (more) {
+      put(buf ^ 1);
+      if (wave == ((at / kStage) & 3)) terms(buf ^ 1, at + kStage);
+    }
+    __syncthreads();
+  }
+  const float s0 = over_half(sum[0], [](float a, float c) { return a + c; });
+  const float s1 = over_half(sum[1], [](float a, float c) { return a + c; });
+  float total = half ? s1 : s0;
+  const int mine = here + lane;
+  if (mine >= width) return;
+  if (W.split > 1) {
+    W.parts[((int64_t)part * A.seqs * A.heads + line) * width + mine] = total;
+    return;
+  }
+  if (mine >= R.length) total = 0.f;
+  else if (W.prior && mine < W.prior_places) total += W.prior[b * W.prior_seq + h * W.prior_head + mine];
+  W.weights[line * width + mine] = total;
+}
+
+// The parts' sums, what was there before, and zeros behind the end.
+__global__ __launch_bounds__(256) void k_weigh_join(WeighArgs W) {
+  const AttendArgs& A = W.a;
+  const int h = blockIdx.y, b = blockIdx.z, j = blockIdx.x * 256 + threadIdx.x;
+  const int64_t width = (int64_t)A.cols * kPageTokens, line = (int64_t)b * A.heads + h;
+  if (j >= width) return;
+  float total = 0.f;
+  if (j < min((int64_t)max(A.lengths[b], 0), width)) {
+    for (int p = 0; p < W.split; ++p) total += W.parts[((int64_t)p * A.seqs * A.heads + line) * width + j];
+    if (W.prior && j < W.prior_places) total += W.prior[b * W.prior_seq + h * W.prior_head + j];
+  }
+  W.weights[line * width + j] = total;
+}
+
+// How a call is run, from what the host knows of it.
+struct WeighWay {
+  bool many;
+  int split;
+  int64_t blocks;
+  WeighWay(int64_t seqs, int heads, int group, int most, int cols) {
+    const int64_t rows = (int64_t)most * group;
+    many = rows > 64;
+    blocks = ((int64_t)cols * kPageTokens + kBlock - 1) / kBlock;
+    // some workgroups for every compute unit, of four stages at the least
+    split = many ? (int)std::min<int64_t>((rows + 4 * kStage - 1) / (4 * kStage), (4 * kComputeUnits) / std::max<int64_t>(1, blocks * heads * seqs) + 1) : 1;
+  }
+  size_t bytes(int64_t seqs, int heads, int cols) const {
+    return split > 1 ? (size_t)split * seqs * heads * cols * kPageTokens * sizeof(float) : 0;
+  }
+};
+
+template <typename T, int D>
+int launch(const WeighArgs& W, const WeighWay& way, hipStream_t s) {
+  const AttendArgs& A = W.a;
+  if (!way.many) {
+    const int64_t groups = ((int64_t)A.cols * 2 + kWaves - 1) / kWaves * A.heads;
+    if (groups > INT32_MAX) return HCK_ERR_ARG;
+    k_weigh<T, D><<<dim3((unsigned)groups, A.seqs), 256, 0, s>>>(W);
+  } else {
+    const int64_t groups = way.blocks * way.split * A.heads;
+    if (groups > INT32_MAX) return HCK_ERR_ARG;
+    k_weigh_many<T, D><<<dim3((unsigned)groups, A.seqs), 64 * kWaves, 0, s>>>(W);
+  }
+  HCK_CHECK_LAUNCH();
+  if (way.split > 1) {
+    k_weigh_join<<<dim3((unsigned)(A.cols * (kPageTokens / 128) + 1) / 2, A.heads, A.seqs), 256, 0, s>>>(W);
+    HCK_CHECK_LAUNCH();
+  }
+  return HCK_OK;
+}
+
 }  // namespace
 }  // namespace hck
+
+extern "C" size_t hck_kv4_weigh_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int most,
+                                                int table_columns) {
+  if (tokens <= 0 || seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 65535 || group < 1 || most < 0 ||
+      table_columns < 1 || table_columns >= 1 << 23 || (int64_t)most * group > INT32_MAX)
+    return 0;
+  return hck::WeighWay(seqs, kv_heads, group, (int)std::min<int64_t>(most, tokens), table_columns).bytes(seqs, kv_heads, table_columns);
+}
 
 extern "C" int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* queries,
                              int64_t tokens, int group, int64_t q_token_stride, int64_t q_head_stride, const int32_t* table,
                              int64_t table_stride, int table_columns, const int32_t* lengths, const int32_t* starts, int seqs,
                              int most, int causal, double scale, const float* lse, const float* prior, int64_t prior_seq_stride,
-                             int64_t prior_head_stride, int prior_places, float* weights, void* stream) {
+                             int64_t prior_head_stride, int prior_places, float* weights, void* workspace, size_t workspace_bytes, void* stream) {
   if (hck::kv4_bytes(head_dim) == 0 || (type != HCK_BF16 && type != HCK_F16)) return HCK_ERR_UNSUPPORTED;
   if (!pool || pages < 1 || kv_heads < 1 || kv_heads > 65535 || tokens < 0 || tokens > INT32_MAX || group < 1 || seqs < 0 ||
       seqs > 65535 || most < 0 || table_columns < 0 || table_columns >= 1 << 23 || prior_places < 0 ||
@@ -141,22 +381,16 @@ extern "C" int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int 
   A.pool = (const uint8_t*)pool, A.q = queries, A.table = table, A.lengths = lengths, A.starts = starts;
   A.q_ts = q_token_stride, A.q_hs = q_head_stride, A.tokens = tokens, A.pages = pages, A.table_stride = table_stride;
   A.cols = table_columns, A.heads = kv_heads, A.group = group, A.causal = causal != 0, A.seqs = seqs;
-  A.tiles = most, A.size = group;
+  A.tiles = (int)std::min<int64_t>(most, tokens), A.size = group;
   W.row_lse = lse, W.prior = prior, W.weights = weights, W.prior_seq = prior_seq_stride, W.prior_head = prior_head_stride;
   W.prior_places = prior ? prior_places : 0;
   const double scale2 = scale * 1.4426950408889634;
   W.scale2 = (float)scale2, W.rest = (float)((scale2 - W.scale2) / scale);
-  const int64_t groups = ((int64_t)table_columns * 2 + hck::kWaves - 1) / hck::kWaves * kv_heads;
-  if (groups > INT32_MAX) return HCK_ERR_ARG;
-  const dim3 grid((unsigned)groups, seqs);
+  const hck::WeighWay way(seqs, kv_heads, group, (int)std::min<int64_t>(most, tokens), table_columns);
+  const size_t need = tokens ? way.bytes(seqs, kv_heads, table_columns) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return HCK_ERR_WORKSPACE;
+  W.parts = (float*)workspace, W.split = way.split;
   hipStream_t s = (hipStream_t)stream;
-  if (head_dim == 128) {
-    if (type == HCK_BF16) hck::k_weigh<__bf16, 128><<<grid, 256, 0, s>>>(W);
-    else hck::k_weigh<_Float16, 128><<<grid, 256, 0, s>>>(W);
-  } else {
-    if (type == HCK_BF16) hck::k_weigh<__bf16, 64><<<grid, 256, 0, s>>>(W);
-    else hck::k_weigh<_Float16, 64><<<grid, 256, 0, s>>>(W);
-  }
-  HCK_CHECK_LAUNCH();
-  return HCK_OK;
+  if (head_dim == 128) return type == HCK_BF16 ? hck::launch<__bf16, 128>(W, way, s) : hck::launch<_Float16, 128>(W, way, s);
+  return type == HCK_BF16 ? hck::launch<__bf16, 64>(W, way, s) : hck::launch<_Float16, 64>(W, way, s);
 }

@@ -197,11 +197,14 @@ PyObject* weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
   lse = lse.contiguous();
   Tensor out = make({seqs, p.heads, cols * 128}, at::kFloat, p.device);
   const bool has = prior.defined() && prior.numel();
+  const size_t bytes = hck_kv4_weigh_workspace_bytes(tokens, (int)seqs, p.heads, (int)group, (int)most, (int)cols);
+  Tensor work;
+  if (bytes) work = make({(int64_t)bytes}, at::kByte, p.device);
   const int err = hck_kv4_weigh(at, p.pages, p.heads, p.dim, type, q.data_ptr(), tokens, (int)group, q.stride(0), q.stride(1),
                                 ints(table), table.stride(0), (int)cols, ints(lengths), ints(starts), (int)seqs, (int)most,
                                 causal, scale, lse.data_ptr<float>(), has ? prior.data_ptr<float>() : nullptr,
                                 has ? prior.stride(0) : 0, has ? prior.stride(1) : 0, has ? (int)prior.size(2) : 0,
-                                out.data_ptr<float>(), stream_of(p.device.index()));
+                                out.data_ptr<float>(), bytes ? work.data_ptr() : nullptr, bytes, stream_of(p.device.index()));
   if (err) return PyLong_FromLong(err);
   return wrap(std::move(out));
   END_HANDLE_TH_ERRORS

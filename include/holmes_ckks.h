@@ -504,12 +504,13 @@ int hck_prompt_attend(const void* queries, const void* keys, const void* values,
  * of exp(scale q.k_j - lse), for the queries, pages and masks of hck_kv4_attend and the lse that it gave (a row of -inf
  * gives nothing).  weights is dense, [seqs][kv_heads][table_columns * 128]; places behind a sequence's length become 0, and a
  * page outside the pool adds nothing.  prior (NULL with prior_places 0: none) has prior_places places a row, and counts as
- * 0 behind them.  table_columns is below 2^23. */
+ * 0 behind them.  table_columns is below 2^23, seqs below 2^16. */
+size_t hck_kv4_weigh_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int most, int table_columns);
 int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* queries, int64_t tokens,
                   int group, int64_t q_token_stride, int64_t q_head_stride, const int32_t* table, int64_t table_stride,
                   int table_columns, const int32_t* lengths, const int32_t* starts, int seqs, int most, int causal,
                   double scale, const float* lse, const float* prior, int64_t prior_seq_stride, int64_t prior_head_stride,
-                  int prior_places, float* weights, void* stream);
+                  int prior_places, float* weights, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Of every sequence and key head `keep` tokens go to the pages into[b * into_stride ..] (at least keep / 128, rounded up):
  * the last `recent` (at most keep) and the heaviest others, ties to the lowest place, NaN above all, in their order.  Weights

@@ -109,9 +109,9 @@ def test_prompt_refuses():
 
 
 def weigh(pool=P, pages=1, heads=1, dim=128, kind=0, q=P, tokens=1, group=1, table=P, cols=1, lengths=P, starts=None, seqs=1,
-          most=1, scale=1.0, lse=P, prior=None, places=0, out=P):
+          most=1, scale=1.0, lse=P, prior=None, places=0, out=P, work=None, size=0):
     return nat.lib().hck_kv4_weigh(pool, pages, heads, dim, kind, q, tokens, group, 0, 0, table, 0, cols, lengths, starts, seqs,
-                                   most, 1, scale, lse, prior, 0, 0, places, out, None)
+                                   most, 1, scale, lse, prior, 0, 0, places, out, work, size, None)
 
 
 def test_weigh_refuses():
@@ -122,6 +122,10 @@ def test_weigh_refuses():
                 dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(places=-1), dict(places=3),
                 dict(cols=(1 << 23) - 1, heads=60000)):
         assert weigh(**bad) == nat.HCK_ERR_ARG, bad
+    need = nat.lib().hck_kv4_weigh_workspace_bytes(1000, 1, 1, 4, 1000, 8)
+    assert need > 0
+    many = dict(tokens=1000, group=4, most=1000, cols=8, starts=P)
+    assert weigh(**many) == weigh(**many, work=P, size=need - 1) == nat.HCK_ERR_WORKSPACE
     assert weigh(seqs=0, tokens=0, q=None, lse=None) == weigh(cols=0, out=None) == 0
 
 
