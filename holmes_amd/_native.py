@@ -128,7 +128,8 @@ SIGNATURES = {
                            ctypes.c_double, _vp, _vp, _i64, _i64, _i, _vp, _vp, _sz, _vp]),
     "hck_kv4_weigh_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i]),
     "hck_kv4_evict": (_i, [_vp, _i64, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _i64, _i64, _i, _vp, _i64, _i, _i, _i, _vp, _vp,
-                           _vp, _vp]),
+                           _vp, _vp, _sz, _vp]),
+    "hck_kv4_evict_workspace_bytes": (_sz, [_i, _i, _i]),
 }
 
 _lib = None

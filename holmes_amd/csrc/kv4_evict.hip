@@ -23,6 +23,7 @@ struct EvictArgs {
   float* new_weights;
   int64_t pages, table_stride, into_stride, w_seq, w_head;
   int cols, heads, width, into_cols, keep, recent;
+  int *counts, segs;  // of long rows: Counts of each row, and its segments
 };
 
 constexpr int kSelect = 1024;  // threads that choose
@@ -52,158 +53,255 @@ __device__ __forceinline__ int upto_thread(int x, int* part, int& all) {
   return upto + (wave ? __builtin_amdgcn_readlane(sums, __builtin_amdgcn_readfirstlane(wave) - 1) : 0);
 }
 
-// One row: a sequence and a key head.  Thread t has the keys of places t, 1024 + t, .. in registers, R of them, read at once
-// and looked at four times; a row of more goes through them in pieces, read anew each time.  A key of 0 is no choice.
-//
-// Counts of the first digit, which is mostly the exponents', would meet in few places, so every eighth lane has counts of
-// its own.
-template <int R>
-__global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
-  constexpr int kCopies = R >= 4 ? 8 : 1, kPiece = R * kSelect;
-  __shared__ int s_bins[kBins * kCopies];
-  __shared__ int s_stay[R * kSelectWaves], s_tie[R * kSelectWaves], s_part[kSelectWaves], s_found[2];
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = (int)min((int64_t)max(A.lengths[b], 0), (int64_t)A.cols * kPageTokens);
-  const int last = max(n - A.recent, 0);  // from here on all stay
-  const int* table = A.table + b * A.table_stride;
-  const float* weights = A.weights + b * A.w_seq + h * A.w_head;
-  int* kept = A.kept + ((int64_t)b * A.heads + h) * A.keep;
-  float* out = A.new_weights + ((int64_t)b * A.heads + h) * A.keep;
-
-  // Places whose page is not in the pool: as a rule there are none, and no place asks again.
-  int gone = 0;
-  for (int i = threadIdx.x; i * kPageTokens < n; i += kSelect) {
-    const int pg = table[i];
-    gone |= pg < 0 || pg >= A.pages;
+// A row: a sequence and a key head.
+struct Row {
+  int n, last, seq, line;  // last: from here on all stay
+  const int* table;
+  const float* weights;
+  int* kept;
+  float* out;
+  __device__ __forceinline__ Row(const EvictArgs& A, int b, int h) {
+    n = (int)min((int64_t)max(A.lengths[b], 0), (int64_t)A.cols * kPageTokens);
+    last = max(n - A.recent, 0), seq = b, line = b * A.heads + h;
+    table = A.table + b * A.table_stride;
+    weights = A.weights + b * A.w_seq + h * A.w_head;
+    kept = A.kept + (int64_t)line * A.keep, out = A.new_weights + (int64_t)line * A.keep;
   }
-  const bool whole = !__syncthreads_or(gone);
-  auto there = [&](int j) {
-    if (whole) return true;
-    const int pg = table[j / kPageTokens];
+  __device__ __forceinline__ bool in_pool(const EvictArgs& A, int page) const {
+    const int pg = table[page];
     return pg >= 0 && pg < A.pages;
-  };
+  }
+};
 
+// Thread t has the keys of places first + t, first + 1024 + t, .. in registers, R of them, read at once.  A key of 0 is no
+// choice.
+template <int R>
+struct Keys {
   uint32_t key[R];
-  const int pieces = (n + kPiece - 1) / kPiece;
-  auto load = [&](int piece) {
+  int first;
+  bool whole;  // no place's page is outside the pool, as a rule: then no place asks again
+  __device__ __forceinline__ bool there(const EvictArgs& A, const Row& row, int j) const {
+    return whole || row.in_pool(A, j / kPageTokens);
+  }
+  __device__ __forceinline__ int place(int r) const { return first + r * kSelect + (int)threadIdx.x; }
+  __device__ __forceinline__ void load(const EvictArgs& A, const Row& row, int from) {
+    first = from;
     float w[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int j = piece * kPiece + r * kSelect + threadIdx.x;
-      w[r] = j < last && j < A.width ? weights[j] : 0.f;
-    }
+    for (int r = 0; r < R; ++r) w[r] = place(r) < row.last && place(r) < A.width ? row.weights[place(r)] : 0.f;
+    const int page = first / kPageTokens + threadIdx.x;
+    const bool gone = threadIdx.x < R * kSelect / kPageTokens && page * kPageTokens < row.n && !row.in_pool(A, page);
+    whole = !__syncthreads_or(gone);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int j = piece * kPiece + r * kSelect + threadIdx.x;
-      key[r] = j < last && there(j) ? key_of(w[r]) : 0;
-    }
-  };
-  if (pieces) load(0);
-
-  // how many there are to choose from, and how many of the last
-  int choice = last, must = n - last;
-  if (!whole) {
-    int mine = 0, lasts = 0, all;
-    for (int j = threadIdx.x; j < n; j += kSelect)
-      if (there(j)) (j < last ? mine : lasts) += 1;
-    upto_thread(mine, s_part, all);
-    choice = all;
-    upto_thread(lasts, s_part, all);
-    must = all;
+    for (int r = 0; r < R; ++r) key[r] = place(r) < row.last && there(A, row, place(r)) ? key_of(w[r]) : 0;
   }
-  const int want = min(choice, A.keep - must);  // of those to choose from (recent is at most keep)
-
-  // T, and how many tokens at T stay
-  uint32_t prefix = 0;
-  int left = want;
-  const bool all = want == choice, none = want <= 0;
-  if (!all && !none) {
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11, bins = 1 << bits;
-      for (int i = threadIdx.x; i < kBins * kCopies; i += kSelect) s_bins[i] = 0;
-      __syncthreads();
-      for (int piece = 0; piece < pieces; ++piece) {
-        if (pieces > 1) load(piece);
+  // the tokens to choose from, and those of the last
+  __device__ __forceinline__ void number(const EvictArgs& A, const Row& row, int* part, int& choice, int& must) const {
+    const int to = min(first + R * kSelect, row.n);
+    choice = max(0, min(to, row.last) - first), must = max(0, to - max(first, row.last));
+    if (whole) return;
+    int mine = 0, lasts = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (key[r] && (digit == 0 || (key[r] >> (shift + bits)) == prefix))
-            atomicAdd(&s_bins[((key[r] >> shift) & (bins - 1)) * kCopies + lane % kCopies], 1);
-      }
-      __syncthreads();
-      // the largest bin with `left` tokens or more in it and above it: two bins a thread, from the top
-      const int top = bins - 1 - 2 * (int)threadIdx.x;
-      int count[2] = {0, 0}, total;
+    for (int r = 0; r < R; ++r) mine += key[r] != 0, lasts += place(r) >= row.last && place(r) < row.n && there(A, row, place(r));
+    upto_thread(mine, part, choice);
+    upto_thread(lasts, part, must);
+  }
+};
+
+__device__ __forceinline__ int shift_of(int digit) { return digit == 0 ? 21 : digit == 1 ? 10 : 0; }
+__device__ __forceinline__ int bits_of(int digit) { return digit == 2 ? 10 : 11; }
+
+// Counts of a digit among the keys that agree with the digits before it.  The first digit is mostly the exponents', of which
+// there are few, so every eighth lane counts by itself.
+template <int R, int kCopies>
+__device__ __forceinline__ void count_digit(const Keys<R>& K, int digit, uint32_t prefix, int* bins) {
+  const int shift = shift_of(digit), bits = bits_of(digit);
+  for (int i = threadIdx.x; i < kBins * kCopies; i += kSelect) bins[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (K.key[r] && (digit == 0 || (K.key[r] >> (shift + bits)) == prefix))
+      atomicAdd(&bins[((K.key[r] >> shift) & ((1 << bits) - 1)) * kCopies + threadIdx.x % kCopies], 1);
+  __syncthreads();
+}
+
+// The bins that a thread looks at, from the top: top_bin and the one below it (none: -1).
+__device__ __forceinline__ int top_bin(int digit) { return (1 << bits_of(digit)) - 1 - 2 * (int)threadIdx.x; }
+
+// The largest digit with `left` keys or more at it and above it, from a thread's two counts; `left` becomes how many of those
+// at it.  found: two places.
+__device__ __forceinline__ void find_digit(int digit, int high, int low, int* part, int* found, uint32_t& prefix, int& left) {
+  int total;
+  const int upto = upto_thread(high + low, part, total), before = upto - high - low;
+  if (before < left && upto >= left) {  // one thread
+    const bool second = before + high < left;
+    found[0] = top_bin(digit) - second, found[1] = left - before - (second ? high : 0);
+  }
+  __syncthreads();
+  prefix = prefix << bits_of(digit) | (uint32_t)found[0];
+  left = found[1];
+  __syncthreads();
+}
+
+// What stays of the keys, above T or among the first `left` at T (of which `ties` come before these keys): 64 places at a time,
+// how many for certain and how many at T; where each 64 begin; and then each place, from `place` on.
+template <int R>
+__device__ __forceinline__ void write_kept(const EvictArgs& A, const Row& row, const Keys<R>& K, uint32_t T, int left, int ties,
+                                           int place, int* s_stay, int* s_tie, int* part) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto sure = [&](int r) {
+    const int j = K.place(r);
+    return j >= row.last ? j < row.n && K.there(A, row, j) : K.key[r] > T;
+  };
+  auto tie = [&](int r) { return K.key[r] != 0 && K.key[r] == T; };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const unsigned long long sures = __ballot(sure(r)), tied = __ballot(tie(r));
+    if (lane == 0) s_stay[r * kSelectWaves + wave] = (int)__popcll(sures), s_tie[r * kSelectWaves + wave] = (int)__popcll(tied);
+  }
+  __syncthreads();
+  static_assert(R * kSelectWaves <= kSelect, "a thread sums up 64 places");
+  const int e = threadIdx.x, mine = e < R * kSelectWaves ? s_tie[e] : 0;
+  int stay = e < R * kSelectWaves ? s_stay[e] : 0, all;
+  const int rank = ties + upto_thread(mine, part, all) - mine;
+  stay += max(0, min(mine, left - rank));
+  const int begin = place + upto_thread(stay, part, all) - stay;
+  if (e < R * kSelectWaves) s_tie[e] = rank, s_stay[e] = begin;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    bool stays = sure(r);
+    const bool t = tie(r);
+    const unsigned long long tied = __ballot(t);
+    if (t && s_tie[r * kSelectWaves + wave] + lanes_below(tied) < left) stays = true;
+    const unsigned long long staying = __ballot(stays);
+    if (stays) {
+      const int p = s_stay[r * kSelectWaves + wave] + lanes_below(staying), j = K.place(r);
+      row.kept[p] = j, row.out[p] = j < A.width ? row.weights[j] : 0.f;
+    }
+  }
+}
+
+__device__ __forceinline__ void write_rest(const EvictArgs& A, const Row& row, int total) {
+  for (int p = total + threadIdx.x; p < A.keep; p += kSelect) row.kept[p] = -1, row.out[p] = 0.f;
+  if (row.line % A.heads == 0 && threadIdx.x == 0) A.new_lengths[row.seq] = total;
+}
+
+// A row of up to R * 1024 places by one workgroup.
+template <int R>
+__global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
+  constexpr int kCopies = R >= 4 ? 8 : 1;
+  __shared__ int s_bins[kBins * kCopies], s_stay[R * kSelectWaves], s_tie[R * kSelectWaves], s_part[kSelectWaves], s_found[2];
+  const Row row(A, blockIdx.y, blockIdx.x);
+  Keys<R> K;
+  K.load(A, row, 0);
+  int choice, must;
+  K.number(A, row, s_part, choice, must);
+  const int want = min(choice, A.keep - must);  // of those to choose from (recent is at most keep)
+  uint32_t T = want < choice ? 0xffffffffu : 0;  // none, or all
+  int left = 0;
+  if (want > 0 && want < choice) {
+    T = 0, left = want;
+    for (int digit = 0; digit < 3; ++digit) {
+      count_digit<R, kCopies>(K, digit, T, s_bins);
+      const int top = top_bin(digit);
+      int high = 0, low = 0;
       if (top > 0) {
 #pragma unroll
-        for (int c = 0; c < kCopies; ++c) count[0] += s_bins[top * kCopies + c], count[1] += s_bins[(top - 1) * kCopies + c];
+        for (int c = 0; c < kCopies; ++c) high += s_bins[top * kCopies + c], low += s_bins[(top - 1) * kCopies + c];
       }
-      const int upto = upto_thread(count[0] + count[1], s_part, total), before = upto - count[0] - count[1];
-      if (before < left && upto >= left) {  // one thread
-        const bool second = before + count[0] < left;
-        s_found[0] = second ? top - 1 : top, s_found[1] = left - before - (second ? count[0] : 0);
-      }
-      __syncthreads();
-      prefix = prefix << bits | (uint32_t)s_found[0];
-      left = s_found[1];
+      find_digit(digit, high, low, s_part, s_found, T, left);
     }
   }
+  write_kept<R>(A, row, K, T, left, 0, 0, s_stay, s_tie, s_part);
+  write_rest(A, row, want + must);
+}
 
-  // What stays, 64 places at a time: how many for certain and how many at T; where each 64 begin; and then each place.
-  int place = 0, ties = 0;
-  for (int piece = 0; piece < pieces; ++piece) {
-    if (pieces > 1) load(piece);
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int j = piece * kPiece + r * kSelect + threadIdx.x;
-      const bool sure = j >= last ? j < n && there(j) : key[r] && (all || (!none && key[r] > prefix));
-      const bool tie = key[r] && !all && !none && key[r] == prefix;
-      const unsigned long long sures = __ballot(sure), tied = __ballot(tie);
-      if (lane == 0) s_stay[r * kSelectWaves + wave] = (int)__popcll(sures), s_tie[r * kSelectWaves + wave] = (int)__popcll(tied);
-    }
-    __syncthreads();
-    constexpr int kMine = (R * kSelectWaves + kSelect - 1) / kSelect;
-    int sum = 0, at[kMine], stay[kMine], got;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int e = threadIdx.x * kMine + i;
-      at[i] = e < R * kSelectWaves ? s_tie[e] : 0, stay[i] = e < R * kSelectWaves ? s_stay[e] : 0, sum += at[i];
-    }
-    int rank = ties + upto_thread(sum, s_part, got) - sum;  // ties before the thread's first 64
-    ties += got;
-    sum = 0;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int e = threadIdx.x * kMine + i;
-      if (e < R * kSelectWaves) s_tie[e] = rank;
-      const int taken = max(0, min(at[i], left - rank));
-      rank += at[i], stay[i] += taken, sum += stay[i];
-    }
-    int begin = place + upto_thread(sum, s_part, got) - sum;
-    place += got;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int e = threadIdx.x * kMine + i;
-      if (e < R * kSelectWaves) s_stay[e] = begin;
-      begin += stay[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int j = piece * kPiece + r * kSelect + threadIdx.x;
-      bool stays = j >= last ? j < n && there(j) : key[r] && (all || (!none && key[r] > prefix));
-      const bool tie = key[r] && !all && !none && key[r] == prefix;
-      const unsigned long long tied = __ballot(tie);
-      if (tie && s_tie[r * kSelectWaves + wave] + lanes_below(tied) < left) stays = true;
-      const unsigned long long staying = __ballot(stays);
-      if (stays) {
-        const int p = s_stay[r * kSelectWaves + wave] + lanes_below(staying);
-        kept[p] = j, out[p] = j < A.width ? weights[j] : 0.f;
-      }
+// Longer rows, by a workgroup for every segment of 16384 places and a launch for every digit: each looks at its keys again, adds up
+// the segments' counts of the digit before, and counts the next among its own.  The last launch writes what stays, from where
+// the segments before end.
+constexpr int kSegment = 16, kSegmentPlaces = kSegment * kSelect;
+struct Counts {  // of one row
+  int *bins, *choice, *must, *above, *state;  // [digit][segment][bin], [segment], [segment], [digit < 2][segment], [digit < 2][2]
+  static __host__ __device__ int64_t ints(int segs) { return (int64_t)segs * (3 * kBins + 4) + 4; }
+  __device__ __forceinline__ Counts(const EvictArgs& A, int line) {
+    bins = A.counts + line * ints(A.segs), choice = bins + (int64_t)A.segs * 3 * kBins, must = choice + A.segs;
+    above = must + A.segs, state = above + 2 * A.segs;
+  }
+};
+
+template <int PHASE>
+__global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
+  constexpr int R = kSegment, kCopies = PHASE == 0 ? 8 : 1;
+  __shared__ int s_bins[PHASE < 3 ? kBins * kCopies : 1], s_stay[R * kSelectWaves], s_tie[R * kSelectWaves];
+  __shared__ int s_part[kSelectWaves], s_found[2];
+  const int seg = blockIdx.z;
+  const Row row(A, blockIdx.y, blockIdx.x);
+  const Counts C(A, row.line);
+  const int segs = (row.n + kSegmentPlaces - 1) / kSegmentPlaces;
+  if (seg >= max(segs, 1)) return;
+  Keys<R> K;
+  K.load(A, row, seg * kSegmentPlaces);
+  if constexpr (PHASE == 0) {
+    int choice, must;
+    K.number(A, row, s_part, choice, must);
+    if (threadIdx.x == 0) C.choice[seg] = choice, C.must[seg] = must;
+  }
+  // the numbers of the whole row, and of the segments before
+  int choice = 0, must = 0, choice_before = 0, must_before = 0;
+  uint32_t T = 0;
+  int left = 0;
+  if constexpr (PHASE > 0) {
+    for (int s = 0; s < segs; ++s) {
+      if (s == seg) choice_before = choice, must_before = must;
+      choice += C.choice[s], must += C.must[s];
     }
   }
-  for (int p = place + threadIdx.x; p < A.keep; p += kSelect) kept[p] = -1, out[p] = 0.f;
-  if (h == 0 && threadIdx.x == 0) A.new_lengths[b] = place;
+  const int want = min(choice, A.keep - must);
+  const bool some = PHASE == 0 || (want > 0 && want < choice);
+  int before = 0, ties_before = 0;  // of the last digit
+  if (PHASE > 0 && some) {
+    // the digit before this one, from all segments' counts
+    constexpr int digit = PHASE - 1;
+    if (digit == 0) left = want;
+    else T = (uint32_t)C.state[2 * (digit - 1)], left = C.state[2 * (digit - 1) + 1];
+    const int top = top_bin(digit);
+    int high = 0, low = 0, own_high = 0, own_low = 0;  // own: of this segment; in the last launch, of those before
+    if (top > 0)
+      for (int s = 0; s < segs; ++s) {
+        const int2 two = *reinterpret_cast<const int2*>(C.bins + ((int64_t)digit * A.segs + s) * kBins + top - 1);
+        high += two.y, low += two.x;
+        if (PHASE == 3 ? s < seg : s == seg) own_high += two.y, own_low += two.x;
+      }
+    find_digit(digit, high, low, s_part, s_found, T, left);
+    const int at = (int)(T & ((1u << bits_of(digit)) - 1));
+    int all;
+    upto_thread((top > at ? own_high : 0) + (top - 1 > at ? own_low : 0), s_part, all);
+    if constexpr (PHASE < 3) {
+      if (threadIdx.x == 0) C.above[digit * A.segs + seg] = all;
+      if (threadIdx.x == 0 && seg == 0) C.state[2 * digit] = (int)T, C.state[2 * digit + 1] = left;
+    } else {
+      before = all;
+      upto_thread(top == at ? own_high : top - 1 == at ? own_low : 0, s_part, all);
+      ties_before = all;
+      for (int s = 0; s < seg; ++s) before += C.above[s] + C.above[A.segs + s];
+    }
+  }
+  if constexpr (PHASE < 3) {
+    if (!some) return;
+    count_digit<R, kCopies>(K, PHASE, T, s_bins);
+    int* bins = C.bins + ((int64_t)PHASE * A.segs + seg) * kBins;
+    for (int i = threadIdx.x; i < kBins; i += kSelect) {
+      int sum = 0;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) sum += s_bins[i * kCopies + c];
+      bins[i] = sum;
+    }
+  } else {
+    if (!some) T = want < choice ? 0xffffffffu : 0, left = 0, before = want < choice ? 0 : choice_before;
+    write_kept<R>(A, row, K, T, left, ties_before, before + min(left, ties_before) + must_before, s_stay, s_tie, s_part);
+    if (seg == 0) write_rest(A, row, want + must);
+  }
 }
 
 // One head's part of a target page.  A place that takes no token has itself for its source: its bytes stay.
@@ -267,14 +365,27 @@ __global__ __launch_bounds__(256) void k_move(EvictArgs A) {
   }
 }
 
+// Segments of a row with room for so many pages; 0: one workgroup takes it.
+int segments(int cols) {
+  const int64_t room = (int64_t)cols * kPageTokens;
+  return room <= kSegmentPlaces ? 0 : (int)((room + kSegmentPlaces - 1) / kSegmentPlaces);
+}
+
 }  // namespace
 }  // namespace hck
+
+extern "C" size_t hck_kv4_evict_workspace_bytes(int seqs, int kv_heads, int table_columns) {
+  if (seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 65535 || table_columns < 0 || table_columns >= 1 << 23) return 0;
+  const int segs = hck::segments(table_columns);
+  return segs ? (size_t)seqs * kv_heads * hck::Counts::ints(segs) * sizeof(int) : 0;
+}
 
 extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_dim, const int32_t* table,
                              int64_t table_stride, int table_columns, const int32_t* lengths, int seqs,
                              const float* weights, int64_t weight_seq_stride, int64_t weight_head_stride, int weight_places,
                              const int32_t* into, int64_t into_stride, int into_columns, int keep, int recent,
-                             int32_t* kept, int32_t* new_lengths, float* new_weights, void* stream) {
+                             int32_t* kept, int32_t* new_lengths, float* new_weights, void* workspace, size_t workspace_bytes,
+                             void* stream) {
   if (hck::kv4_bytes(head_dim) == 0) return HCK_ERR_UNSUPPORTED;
   if (!pool || pages < 1 || kv_heads < 1 || kv_heads > 65535 || seqs < 0 || seqs > 65535 || table_columns < 0 ||
       table_columns >= 1 << 23 || weight_places < 0 || keep < 0 || recent < 0 || recent > keep || into_columns < 0 ||
@@ -292,14 +403,23 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
   A.pages = pages, A.table_stride = table_stride, A.into_stride = into_stride, A.w_seq = weight_seq_stride,
   A.w_head = weight_head_stride, A.cols = table_columns, A.heads = kv_heads, A.width = weight_places,
   A.into_cols = into_columns, A.keep = keep, A.recent = recent;
+  A.segs = hck::segments(table_columns), A.counts = (int*)workspace;
+  if (A.segs > 65535) return HCK_ERR_ARG;
+  const size_t bytes = hck_kv4_evict_workspace_bytes(seqs, kv_heads, table_columns);
+  if (bytes && (!workspace || workspace_bytes < bytes)) return HCK_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   // the least keys a thread for which a row goes through the registers once, as far as a table tells
   const int64_t room = (int64_t)table_columns * hck::kPageTokens;
-  auto* select = room <= 1 * hck::kSelect   ? hck::k_select<1>
-                 : room <= 4 * hck::kSelect ? hck::k_select<4>
-                 : room <= 16 * hck::kSelect ? hck::k_select<16>
-                                             : hck::k_select<64>;
-  select<<<dim3(kv_heads, seqs), hck::kSelect, 0, s>>>(A);
+  if (A.segs == 0) {
+    auto* select = room <= 1 * hck::kSelect ? hck::k_select<1> : room <= 4 * hck::kSelect ? hck::k_select<4> : hck::k_select<16>;
+    select<<<dim3(kv_heads, seqs), hck::kSelect, 0, s>>>(A);
+  } else {
+    const dim3 grid(kv_heads, seqs, A.segs);
+    hck::k_select_long<0><<<grid, hck::kSelect, 0, s>>>(A);
+    hck::k_select_long<1><<<grid, hck::kSelect, 0, s>>>(A);
+    hck::k_select_long<2><<<grid, hck::kSelect, 0, s>>>(A);
+    hck::k_select_long<3><<<grid, hck::kSelect, 0, s>>>(A);
+  }
   HCK_CHECK_LAUNCH();
   if (need) {
     const dim3 grid((unsigned)need, kv_heads, seqs);

@@ -233,10 +233,14 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::DeviceGuard guard(p.device);
   Tensor kept = make({seqs, p.heads, keep}, at::kInt, p.device), now = make({seqs}, at::kInt, p.device),
          left = make({seqs, p.heads, keep}, at::kFloat, p.device);
+  const size_t bytes = hck_kv4_evict_workspace_bytes((int)seqs, p.heads, (int)table.size(1));
+  Tensor work;
+  if (bytes) work = make({(int64_t)bytes}, at::kByte, p.device);
   const int err = hck_kv4_evict(at, p.pages, p.heads, p.dim, ints(table), table.stride(0), (int)table.size(1), ints(lengths),
                                 (int)seqs, weights.data_ptr<float>(), weights.stride(0), weights.stride(1),
                                 (int)weights.size(2), ints(into), into.stride(0), (int)into.size(1), (int)keep, (int)recent,
-                                ints(kept), ints(now), left.data_ptr<float>(), stream_of(p.device.index()));
+                                ints(kept), ints(now), left.data_ptr<float>(), bytes ? work.data_ptr() : nullptr, bytes,
+                                stream_of(p.device.index()));
   if (err) return PyLong_FromLong(err);
   return Py_BuildValue("(NNN)", wrap(std::move(kept)), wrap(std::move(now)), wrap(std::move(left)));
   END_HANDLE_TH_ERRORS

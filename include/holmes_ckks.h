@@ -517,11 +517,14 @@ int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int head_dim, i
  * have weight_places places a row and count as 0 behind them.  kept [seqs][kv_heads][keep] are the places that they had (-1
  * where there are fewer), new_weights their weights (0 there), new_lengths [seqs] their number.  A token whose page is
  * outside the pool is not kept; a target page outside it takes nothing.  Target pages must not be pages of the tables, nor
- * twice in `into`: what those hold is undefined.  Places of a target page behind the kept tokens stay as they were. */
+ * twice in `into`: what those hold is undefined.  Places of a target page behind the kept tokens stay as they were.
+ * table_columns is below 2^23, seqs below 2^16. */
+size_t hck_kv4_evict_workspace_bytes(int seqs, int kv_heads, int table_columns);
 int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_dim, const int32_t* table, int64_t table_stride,
                   int table_columns, const int32_t* lengths, int seqs, const float* weights, int64_t weight_seq_stride,
                   int64_t weight_head_stride, int weight_places, const int32_t* into, int64_t into_stride, int into_columns,
-                  int keep, int recent, int32_t* kept, int32_t* new_lengths, float* new_weights, void* stream);
+                  int keep, int recent, int32_t* kept, int32_t* new_lengths, float* new_weights, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -130,9 +130,9 @@ def test_weigh_refuses():
 
 
 def evict(pool=P, pages=1, heads=1, dim=128, table=P, cols=1, lengths=P, seqs=1, weights=P, places=128, into=P, into_cols=1,
-          keep=10, recent=2, kept=P, now=P, left=P):
+          keep=10, recent=2, kept=P, now=P, left=P, work=None, size=0):
     return nat.lib().hck_kv4_evict(pool, pages, heads, dim, table, 0, cols, lengths, seqs, weights, 0, 0, places, into, 0,
-                                   into_cols, keep, recent, kept, now, left, None)
+                                   into_cols, keep, recent, kept, now, left, work, size, None)
 
 
 def test_evict_refuses():
@@ -142,6 +142,9 @@ def test_evict_refuses():
                 dict(cols=1 << 23), dict(seqs=-1), dict(seqs=65536), dict(places=-1), dict(into_cols=-1), dict(keep=-1),
                 dict(keep=129), dict(recent=-1), dict(recent=11), dict(into_cols=1 << 23)):
         assert evict(**bad) == nat.HCK_ERR_ARG, bad
+    need = nat.lib().hck_kv4_evict_workspace_bytes(1, 1, 129)
+    assert need > 0 and nat.lib().hck_kv4_evict_workspace_bytes(1, 1, 128) == 0
+    assert evict(cols=129) == evict(cols=129, work=P, size=need - 1) == nat.HCK_ERR_WORKSPACE
     assert evict(seqs=0, lengths=None, now=None) == 0
 
 

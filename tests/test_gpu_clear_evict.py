@@ -106,18 +106,24 @@ def test_weights_of_all_kinds(what):
     check(pool, before, table.cpu(), seqs, w, into, keep, recent, pool.evict(table, lengths, w, into, keep, recent=recent))
 
 
-def test_long_rows():
-    print("long", flush=True)
+@pytest.mark.parametrize("keep,recent", [(5000, 100), (5000, 5000), (20000, 17000), (1, 0), (16500, 0)])
+def test_long_rows(keep, recent):
+    """Rows of one segment and of several, whole ones and ones with pages outside the pool."""
+    print("long", keep, recent, flush=True)
     g = torch.Generator().manual_seed(6)
-    seqs, heads, keep = [40000, 9000], 1, 5000
-    pool, table, _, _ = build(seqs, heads, 64, g, spare=82)
+    seqs, heads = [40000, 9000, 0, 16384, 32769], 1
+    pool, table, _, _ = build(seqs, heads, 64, g, spare=5 * -(-keep // PAGE))
     lengths = torch.tensor(seqs, dtype=torch.int32).cuda()
     into = pages_for(pool, table, seqs, keep, g)
-    for w in (torch.rand((2, heads, table.shape[1] * PAGE), generator=g),
-              torch.randint(0, 3, (2, heads, table.shape[1] * PAGE), generator=g).float()):
-        w = w.cuda()
+    shape = (5, heads, table.shape[1] * PAGE)
+    there = [torch.ones(n, dtype=torch.bool) for n in seqs]
+    for i, w in enumerate((torch.rand(shape, generator=g), torch.randint(0, 3, shape, generator=g).float(), torch.zeros(shape))):
+        if i == 1:
+            table[0, 5], table[0, 250], table[4, 255:] = -1, pool.pages, 2**31 - 1
+            there[0][5 * PAGE:6 * PAGE] = there[0][250 * PAGE:251 * PAGE] = there[4][255 * PAGE:] = False
         before = everything(pool)
-        check(pool, before, table.cpu(), seqs, w, into, keep, 100, pool.evict(table, lengths, w, into, keep, recent=100))
+        got = pool.evict(table, lengths, w.cuda(), into, keep, recent=recent)
+        check(pool, before, table.cpu(), seqs, w, into, keep, recent, got, there=there)
 
 
 def test_pages_outside_the_pool_and_nan_tokens():
