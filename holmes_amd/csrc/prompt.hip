@@ -132,14 +132,31 @@ struct Staged {
   }
 };
 
-typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef uint32_t rsrc_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+// 16 bytes for each lane from base + off into LDS, lane after lane from `to` on; zeros for what is out of the bounds.
+// Written out, because the compiler waits for such loads before any transposing read; whoever issues them waits with
+// all_loaded().  (m0 holds the address, a wait state ahead of its use.)
+__device__ __forceinline__ void load_lds(uint32_t to, uint32_t off, rsrc_t from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void all_loaded() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ rsrc_t bounds(const char* base, int bytes) {
+  const uint64_t at = (uint64_t)base;
+  return rsrc_t{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)),
+                (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
 
 template <typename T, int D, bool RANGE>
 __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   using S = Staged<D>;
   using vec = typename Eight<T>::type;
   constexpr int kSteps = D / 16, kTiles = D / 32;
-  __shared__ u32x4 s_k[2][kUnit * S::kPieces], s_v[2][kUnit * S::kPieces];
+  __shared__ u32x4 s_x[2][2][kUnit * S::kPieces];  // [turn][keys, values]
 
   Tile t;
   const int h = blockIdx.x % A.heads;
@@ -152,7 +169,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   const int most = sees(min(tile * kTileRows + kTileRows, rows) - 1);
   const int units = (most + kUnit - 1) / kUnit;
   const int mine = tile * kTileRows + wave * kRowsOfWave;
-  const int least = mine < rows ? sees(mine) : 0, last = mine < rows ? sees(min(mine + kRowsOfWave, rows) - 1) : 0;
+  const int last = mine < rows ? sees(min(mine + kRowsOfWave, rows) - 1) : 0;
   const int row = mine + (lane & 31);
   const bool live = row < rows;
   const int qi = live ? row / A.group : 0, qo = live ? row % A.group : 0;
@@ -162,22 +179,22 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   const int token0 = threadIdx.x / S::kPieces, piece0 = threadIdx.x % S::kPieces;
   const uint32_t k_off = (uint32_t)(token0 * A.k_ts * 2) + (S::key_at(token0, piece0) - token0 * S::kPieces) * 16;
   const uint32_t v_off = (uint32_t)(token0 * A.v_ts * 2) + (S::value_at(token0, piece0) - token0 * S::kPieces) * 16;
+  const uint32_t k_step = (uint32_t)(S::kStep * A.k_ts * 2), v_step = (uint32_t)(S::kStep * A.v_ts * 2);
   const char* kp = (const char*)A.k + (first * A.k_ts + h * A.k_hs) * 2;
   const char* vp = (const char*)A.v + (first * A.v_ts + h * A.v_hs) * 2;
-  auto bring = [&](int u, u32x4* ks, u32x4* vs) {
+  const uint32_t lds = lds_address(s_x) + wave * 1024;
+  auto bring = [&](int u) {
     const int left = min(n - u * kUnit, kUnit);
-    const auto kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)u * kUnit * A.k_ts * 2), 0,
-                                                      (int)((left - 1) * A.k_ts * 2 + D * 2), 0x00020000);
-    const auto vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + (int64_t)u * kUnit * A.v_ts * 2), 0,
-                                                      (int)((left - 1) * A.v_ts * 2 + D * 2), 0x00020000);
+    const uint32_t to = lds + (u & 1) * (2 * S::kBytes);
+    const rsrc_t kr = bounds(kp + (int64_t)u * kUnit * A.k_ts * 2, (int)((left - 1) * A.k_ts * 2 + D * 2));
+    const rsrc_t vr = bounds(vp + (int64_t)u * kUnit * A.v_ts * 2, (int)((left - 1) * A.v_ts * 2 + D * 2));
 #pragma unroll
     for (int j = 0; j < S::kEach; ++j) {
-      const int at = j * (64 * kPromptWaves) + wave * 64;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr)(ks + at), 16, k_off + (uint32_t)(j * S::kStep * A.k_ts * 2), 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr)(vs + at), 16, v_off + (uint32_t)(j * S::kStep * A.v_ts * 2), 0, 0, 0);
+      load_lds(to + j * (1024 * kPromptWaves), k_off + j * k_step, kr);
+      load_lds(to + j * (1024 * kPromptWaves) + S::kBytes, v_off + j * v_step, vr);
     }
   };
-  if (units > 0) bring(0, s_k[0], s_v[0]);
+  if (units > 0) bring(0);
 
   vec q[kSteps];
   const T* qp = (const T*)A.q + (first + qi) * A.q_ts + (int64_t)(h * A.group + qo) * A.q_hs + half * 8;
@@ -203,9 +220,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   float top = -INFINITY, sum = 0.f, low = INFINITY;
   float ref = -lift, factor = A.scale2;
 
-  auto unit = [&](int u, const u32x4* ks, const u32x4* vs) {
+  // PARTLY: some of the wave's rows do not see some of the unit's tokens.
+  auto unit = [&](int u, auto PARTLY) {
+    constexpr bool kPartly = decltype(PARTLY)::value;
+    const u32x4 *ks = s_x[u & 1][0], *vs = s_x[u & 1][1];
     const int here = u * kUnit;
-    if (here >= last) return;
     f32x16 c[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) c[0][i] = c[1][i] = 0.f;
@@ -216,9 +235,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
         const vec k = __builtin_bit_cast(vec, ks[S::key_at(32 * x + (lane & 31), 2 * s + half)]);
         c[x] = mfma32(k, q[s], c[x]);
       }
-    const int base = here + 4 * half;  // of the lane's tokens base + 32 x + 8 (i / 4) + i % 4
-    const bool partly = here + kUnit > least;
-    if (partly) {
+    if constexpr (kPartly) {
+      const int base = here + 4 * half;  // of the lane's tokens base + 32 x + 8 (i / 4) + i % 4
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -252,7 +270,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       for (int d = 0; d < kTiles; ++d) acc[d] *= f;
     }
 
-    // (the transposing reads of 16 tokens and 32 dims)
+    // the left operand of 16 tokens and 32 dims
     auto values = [&](int j, int d) {
       s16x4 x[2];
 #pragma unroll
@@ -265,10 +283,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       return u32x4{a[0], a[1], b[0], b[1]};
     };
     float part[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    auto probabilities = [&](int j) {
       float e[8];
-      u32x4 p, v[kTiles];
+      u32x4 p;
 #pragma unroll
       for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[j >> 1][8 * (j & 1) + i], factor, -ref));
 #pragma unroll
@@ -276,15 +293,18 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
         p[i] = pack_as<T>(e[2 * i], e[2 * i + 1]);
         part[i & 1] += e[2 * i] + e[2 * i + 1];
       }
+      return p;
+    };
+    if constexpr (kPartly) {
+      // Tokens that a row does not see have a probability of 0, and 0 times an infinity or a NaN is NaN.  Where there
+      // is one, the tokens go one by one, each for the rows that see it.
+      uint32_t odd = 0;
+#pragma unroll 4
+      for (int i = 0; i < kUnit * S::kPieces / 64; ++i) odd |= odd_values<T>(vs[i * 64 + lane]);
+      if (__any(odd != 0)) {
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) v[d] = values(j, d);
-      if (partly) {
-        // Tokens that a row does not see have a probability of 0, and 0 times an infinity or a NaN is NaN.  Where there
-        // is one, the tokens go one by one, each for the rows that see it.
-        uint32_t odd = 0;
-#pragma unroll
-        for (int d = 0; d < kTiles; ++d) odd |= odd_values<T>(v[d]);
-        if (__any(odd != 0)) {
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 p = probabilities(j);
 #pragma unroll 1
           for (int k = 0; k < 16; ++k) {
             const int at = k & 7;  // of the eight of half k / 8
@@ -297,30 +317,40 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
               f32x16 one;
 #pragma unroll
               for (int i = 0; i < 16; ++i) one[i] = 0.f;
-              one = mfma32(__builtin_bit_cast(vec, v[d] & only), __builtin_bit_cast(vec, p & only), one);
+              one = mfma32(__builtin_bit_cast(vec, values(j, d) & only), __builtin_bit_cast(vec, p & only), one);
 #pragma unroll
               for (int i = 0; i < 16; ++i) acc[d][i] += see ? one[i] : 0.f;
             }
           }
-          continue;
         }
+        sum += part[0] + part[1];
+        return;
       }
+    }
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) acc[d] = mfma32(__builtin_bit_cast(vec, v[d]), __builtin_bit_cast(vec, p), acc[d]);
+    for (int j = 0; j < 4; ++j) {
+      const u32x4 p = probabilities(j);
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d)
+        acc[d] = mfma32(__builtin_bit_cast(vec, values(j, d)), __builtin_bit_cast(vec, p), acc[d]);
     }
     sum += part[0] + part[1];
   };
 
-  for (int u = 0; u < units; u += 2) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // this thread's loads have come (vmcnt 0)
+  auto next = [&](int u) {
+    all_loaded();  // this wave's, and after the barrier all waves'; which are also done with the unit before
     __syncthreads();
-    if (u + 1 < units) bring(u + 1, s_k[1], s_v[1]);
-    unit(u, s_k[0], s_v[0]);
-    if (u + 1 >= units) break;
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
-    if (u + 2 < units) bring(u + 2, s_k[0], s_v[0]);
-    unit(u + 1, s_k[1], s_v[1]);
+    if (u + 1 < units) bring(u + 1);
+  };
+  const int full = sees(tile * kTileRows) / kUnit;  // units that all of the tile's rows see
+  int u = 0;
+  for (; u < full; ++u) {
+    next(u);
+    unit(u, std::false_type());
+  }
+  for (; u < units; ++u) {
+    next(u);
+    if (u * kUnit < last) unit(u, std::true_type());
   }
 
   sum = over_half(sum, [](float a, float c) { return a + c; });
