@@ -235,6 +235,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
         const vec k = __builtin_bit_cast(vec, ks[S::key_at(32 * x + (lane & 31), 2 * s + half)]);
         c[x] = mfma32(k, q[s], c[x]);
       }
+    if constexpr (!kPartly && D == 128) {
+      // Six reads ahead of the products, which alone the compiler would not have (8192 tokens: 576 -> 566 us; at 64 dims,
+      // with half the products for as many exponentials, it costs 4 %).
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int s = 0; s < 2 * kSteps - 6; ++s) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+    }
     if constexpr (kPartly) {
       const int base = here + 4 * half;  // of the lane's tokens base + 32 x + 8 (i / 4) + i % 4
 #pragma unroll
@@ -249,13 +260,13 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) low = smaller(low, c[x][i]);
+        for (int i = 0; i < 16; i += 2) low = __builtin_elementwise_minimum(__builtin_elementwise_minimum(low, c[x][i]), c[x][i + 1]);
     }
     float mx = -INFINITY;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = larger(mx, c[x][i]);
+      for (int i = 0; i < 16; i += 2) mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, c[x][i]), c[x][i + 1]);
     const float raw = over_half(mx, fmax2);
     mx = fmaxf(top, raw * A.scale2);
     const float f = rebase(top, mx);
@@ -282,6 +293,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       const u32x2 a = __builtin_bit_cast(u32x2, x[0]), b = __builtin_bit_cast(u32x2, x[1]);
       return u32x4{a[0], a[1], b[0], b[1]};
     };
+    // (a wave in its softmax and second product goes before one in its first, which only waits for the matrix unit: 582 -> 576 us)
+    if constexpr (D == 128) __builtin_amdgcn_s_setprio(1);
     float part[2] = {0.f, 0.f};
     auto probabilities = [&](int j) {
       float e[8];
@@ -324,6 +337,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
           }
         }
         sum += part[0] + part[1];
+        if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
         return;
       }
     }
@@ -335,6 +349,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
         acc[d] = mfma32(__builtin_bit_cast(vec, values(j, d)), __builtin_bit_cast(vec, p), acc[d]);
     }
     sum += part[0] + part[1];
+    if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
   };
 
   auto next = [&](int u) {
