@@ -15,7 +15,7 @@ struct WeighArgs {
   float* weights;
   float* parts;  // with more than one: [part][seq][head][place]
   int64_t prior_seq, prior_head;
-  int prior_places, split;  // split: parts that the rows of 256 tokens are cut into
+  int prior_places, split, units;  // split: parts that the rows of 256 tokens are cut into; units: of a wave, with few rows
   float scale2, rest;  // scale log2 e in 32 bits, and what its rounding left over, divided by scale
 };
 
@@ -25,13 +25,12 @@ struct RowTerm {
   float off, factor;
   int seen;
 };
-__device__ __forceinline__ RowTerm row_term(const WeighArgs& W, const Rows& R, int h, int row) {
-  RowTerm r = {0.f, 1.f, 0};
-  if (row >= R.rows) return r;
-  const int64_t at = (int64_t)(R.q0 + row / W.a.group) * ((int64_t)W.a.heads * W.a.group) + h * W.a.group + row % W.a.group;
-  const float lse = W.row_lse[at];
-  r.off = lse * kLog2e;
-  r.seen = lse == -INFINITY ? 0 : R.seen(W.a, row);  // such a row gave nothing
+__device__ __forceinline__ float row_lse(const WeighArgs& W, const Rows& R, int h, int row) {
+  if (row >= R.rows) return -INFINITY;
+  return W.row_lse[(int64_t)(R.q0 + row / W.a.group) * ((int64_t)W.a.heads * W.a.group) + h * W.a.group + row % W.a.group];
+}
+__device__ __forceinline__ RowTerm row_term(const WeighArgs& W, const Rows& R, int row, float lse) {
+  RowTerm r = {lse * kLog2e, 1.f, lse == -INFINITY ? 0 : R.seen(W.a, row)};  // a row of -inf gave nothing
   if (fabsf(lse) < INFINITY) {
     const float low = __builtin_fmaf(lse, kLog2e, -r.off) + lse * 1.9259629911266174e-8f;  // (log2 e in two parts)
     r.factor = 1.f + kLn2 * (lse * W.rest - low);
@@ -39,88 +38,103 @@ __device__ __forceinline__ RowTerm row_term(const WeighArgs& W, const Rows& R, i
   return r;
 }
 
-// 64 tokens of a key head to a wave; 16 rows at a time.
+// Up to 16 rows: a wave takes units of 64 tokens in turn, the next one's keys in flight, with the rows' operands and terms in its
+// registers throughout.  The product's 16 rows are the left operand, so a lane has one token of each 16 and four of its rows.
+// Bound by the keys' bytes; a unit a wave, with nothing in flight behind the lookup of its page, took 82 us for 32 histories
+// of 2000 to 24576 tokens.
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves) void k_weigh(WeighArgs W) {
+__global__ __launch_bounds__(64 * kWaves) void k_weigh_few(WeighArgs W) {
   using L = Kv4<D>;
   constexpr int kSteps = D / 32;
   constexpr bool kHalf = __is_same(T, _Float16);
   const AttendArgs& A = W.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % A.heads, u = blockIdx.x / A.heads * kWaves + wave, b = blockIdx.y;
-  if (u >= 2 * A.cols) return;
-  const int here = u * kUnit, mine = here + g * 16 + m;  // the token that the lane writes
-  float* to = W.weights + ((int64_t)b * A.heads + h) * ((int64_t)A.cols * kPageTokens) + mine;
+  const int h = blockIdx.x % A.heads, b = blockIdx.y;
+  int u = blockIdx.x / A.heads * (kWaves * W.units) + wave;
+  const int u1 = min(u + kWaves * W.units, 2 * A.cols);
+  if (u >= u1) return;
+  const int* table = A.table + b * A.table_stride;
+  int pg = table[u >> 1];  // (a column of the table, whatever the length)
   const Rows R(A, b);
-  if (here >= R.length) {
-    *to = 0.f;
+  const int line = b * A.heads + h;
+  float* to = W.weights + (int64_t)line * A.cols * kPageTokens + lane;
+  const float* prior = W.prior + b * W.prior_seq + h * W.prior_head + lane;
+
+  typedef uint32_t words __attribute__((ext_vector_type(kSteps)));
+  words codes[4];
+  uint32_t scales = 0;
+  float old = 0.f;
+  auto there = [&](int pg) { return pg >= 0 && pg < A.pages; };
+  auto load = [&](int u, int pg) {  // unit u, of a page that is page 0 where it is none
+    const uint8_t* page = A.pool + ((int64_t)(there(pg) ? pg : 0) * A.heads + h) * L::kBytes;
+    const uint8_t* at = page + (u & 1) * (32 * D) + lane * (D / 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) codes[i] = __builtin_nontemporal_load(reinterpret_cast<const words*>(at + i * (8 * D)));
+    scales = *reinterpret_cast<const uint32_t*>(page + L::kKScales + (u & 1) * (64 * L::kRuns) + g * (D / 4) / kRun * 64 + m * 4);
+    const int j = u * kUnit + lane;
+    old = W.prior && j < W.prior_places ? prior[u * kUnit] : 0.f;
+  };
+  if (u * kUnit >= R.length) {
+    for (; u < u1; u += kWaves) to[u * kUnit] = 0.f;
     return;
   }
-  const int pg = A.table[b * A.table_stride + (u >> 1)];
-  const bool there = pg >= 0 && pg < A.pages;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  if (there) {
-    const uint8_t* page = A.pool + ((int64_t)pg * A.heads + h) * L::kBytes;
-    const uint8_t* codes = page + (u & 1) * (32 * D);
-    typedef uint32_t words __attribute__((ext_vector_type(kSteps)));
-    words c[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = *reinterpret_cast<const words*>(codes + i * (8 * D) + lane * (D / 8));
-    const uint32_t scales =
-        *reinterpret_cast<const uint32_t*>(page + L::kKScales + (u & 1) * (64 * L::kRuns) + g * (D / 4) / kRun * 64 + m * 4);
-    bf16x8 k[4][kSteps];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t byte = (scales >> (8 * i)) & 0xffu;
-      const float sc = byte == kNanByte ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        k[i][s] = operand(cvt<0>(c[i][s], sc), cvt<1>(c[i][s], sc), cvt<2>(c[i][s], sc), cvt<3>(c[i][s], sc));
-    }
-    // rows that see a token of these: from the first query that does
-    const int skip = A.causal ? (int)((int64_t)max(0, here - (R.length - R.nq)) * A.group / 16) : 0;
-    for (int tile = skip; tile * 16 < R.rows; ++tile) {
-      const int row = tile * 16 + m;
-      const bool live = row < R.rows;
-      const T* qp = (const T*)A.q + (R.q0 + (live ? row / A.group : 0)) * A.q_ts +
-                    (int64_t)(h * A.group + (live ? row % A.group : 0)) * A.q_hs + g * (D / 4);
-      f32x4 s[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int d = 0; d < kSteps; ++d) {
-        u32x4 raw = {0, 0, 0, 0};
-        if (live) raw = reinterpret_cast<const Loose16*>(qp + 8 * d)->v;
-        bf16x8 head, rest;
-        query_parts<T>(raw, head, rest);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[i] = mfma(head, k[i][d], s[i]);
-          if constexpr (kHalf) s[i] = mfma(rest, k[i][d], s[i]);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const RowTerm t = row_term(W, R, h, tile * 16 + 4 * g + r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], W.scale2, -t.off));
-          acc[i] = __builtin_fmaf(here + 16 * i + m < t.seen ? p : 0.f, t.factor, acc[i]);
-        }
-      }
-    }
-  }
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float all = over_g(acc[i], [](float a, float c) { return a + c; });
-    sum = g == i ? all : sum;
-  }
-  if (mine >= R.length) sum = 0.f;
-  else if (W.prior && mine < W.prior_places) sum += W.prior[b * W.prior_seq + h * W.prior_head + mine];
-  *to = sum;
-}
+  pg = __builtin_amdgcn_readfirstlane(pg);
+  int next = u + kWaves < u1 ? table[(u + kWaves) >> 1] : 0;
+  load(u, pg);
 
+  bf16x8 q[kSteps], rest[kSteps];
+  const bool live = m < R.rows;
+  const T* qp = (const T*)A.q + (R.q0 + (live ? m / A.group : 0)) * A.q_ts + (int64_t)(h * A.group + (live ? m % A.group : 0)) * A.q_hs + g * (D / 4);
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    u32x4 raw = {0, 0, 0, 0};
+    if (live) raw = reinterpret_cast<const Loose16*>(qp + 8 * s)->v;
+    query_parts<T>(raw, q[s], rest[s]);
+  }
+  RowTerm t[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) t[r] = row_term(W, R, 4 * g + r, row_lse(W, R, h, 4 * g + r));
+
+  for (; u < u1; u += kWaves) {
+    const int here = u * kUnit;
+    if (here >= R.length) {
+      to[here] = 0.f;
+      continue;
+    }
+    const bool seen = there(pg);
+    words now[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) now[i] = codes[i];
+    const uint32_t bytes = scales;
+    float total = old;
+    pg = __builtin_amdgcn_readfirstlane(next);
+    if (u + 2 * kWaves < u1) next = table[(u + 2 * kWaves) >> 1];
+    if (u + kWaves < u1 && here + kWaves * kUnit < R.length) load(u + kWaves, pg);
+    if (seen) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t byte = (bytes >> (8 * i)) & 0xffu;
+        const float sc = byte == kNanByte ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          const bf16x8 k = operand(cvt<0>(now[i][d], sc), cvt<1>(now[i][d], sc), cvt<2>(now[i][d], sc), cvt<3>(now[i][d], sc));
+          s = mfma(q[d], k, s);
+          if constexpr (kHalf) s = mfma(rest[d], k, s);
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], W.scale2, -t[r].off));
+          sum = __builtin_fmaf(here + 16 * i + m < t[r].seen ? p : 0.f, t[r].factor, sum);
+        }
+        sum = over_g(sum, [](float a, float c) { return a + c; });
+        if (g == i) total += sum;
+      }
+    }
+    to[here] = here + lane < R.length ? total : 0.f;
+  }
+}
 
 // Many rows: the keys of 64 tokens stay in a wave's registers as the right operand, 32 tokens to a product, and the rows pass
 // by, 64 at a time through LDS for the four waves of 256 tokens.  A lane has one token (two in all) and 16 of 32 rows, so its
@@ -210,8 +224,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
       }
     }
   };
-  auto terms = [&](int buf, int at) {  // one wave
-    const RowTerm t = row_term(W, R, h, at + lane);
+  float lse = 0.f;
+  auto terms = [&](int buf, int at) {  // one wave, whose lanes have the rows' lse
+    const RowTerm t = row_term(W, R, at + lane, lse);
     const int seen = at + lane < to ? t.seen : 0;
     s_off[buf][lane] = t.off, s_factor[buf][lane] = t.factor, s_seen[buf][lane] = seen;
     int least = seen;
@@ -222,13 +237,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
   float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};
   if (from < to) {
     bring(from);
+    if (wave == 0) lse = row_lse(W, R, h, from + lane);
     put(0);
     if (wave == 0) terms(0, from);
   }
   __syncthreads();
   for (int at = from, buf = 0; at < to; at += kStage, buf ^= 1) {
-    const bool more = at + kStage < to;
-    if (more) bring(at + kStage);
+    const bool more = at + kStage < to, mine = wave == ((at / kStage) & (kWaves - 1));
+    if (more) {
+      bring(at + kStage);
+      if (mine) lse = row_lse(W, R, h, at + kStage + lane);
+    }
     if (there) {
       float now[2] = {0.f, 0.f};
 #pragma unroll 1
@@ -283,7 +302,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
     }
     if (more) {
       put(buf ^ 1);
-      if (wave == ((at / kStage) & 3)) terms(buf ^ 1, at + kStage);
+      if (mine) terms(buf ^ 1, at + kStage);
     }
     __syncthreads();
   }
@@ -318,11 +337,14 @@ __global__ __launch_bounds__(256) void k_weigh_join(WeighArgs W) {
 // How a call is run, from what the host knows of it.
 struct WeighWay {
   bool many;
-  int split;
+  int split, units;
   int64_t blocks;
   WeighWay(int64_t seqs, int heads, int group, int most, int cols) {
     const int64_t rows = (int64_t)most * group;
-    many = rows > 64;
+    many = rows > kFew;
+    // More units a wave share the rows' loading, fewer even the work out (32 histories of 2000 to 24576 tokens: 2 58 us, 3 52,
+    // 4 51, 8 53); no more than leave 8 waves for every SIMD.
+    units = (int)std::min<int64_t>(4, std::max<int64_t>(1, (int64_t)cols * 2 * heads * seqs / (32 * kComputeUnits)));
     blocks = ((int64_t)cols * kPageTokens + kBlock - 1) / kBlock;
     // some workgroups for every compute unit, of four stages at the least
     split = many ? (int)std::min<int64_t>((rows + 4 * kStage - 1) / (4 * kStage), (4 * kComputeUnits) / std::max<int64_t>(1, blocks * heads * seqs) + 1) : 1;
@@ -336,9 +358,9 @@ template <typename T, int D>
 int launch(const WeighArgs& W, const WeighWay& way, hipStream_t s) {
   const AttendArgs& A = W.a;
   if (!way.many) {
-    const int64_t groups = ((int64_t)A.cols * 2 + kWaves - 1) / kWaves * A.heads;
+    const int64_t groups = ((int64_t)A.cols * 2 + kWaves * W.units - 1) / (kWaves * W.units) * A.heads;
     if (groups > INT32_MAX) return HCK_ERR_ARG;
-    k_weigh<T, D><<<dim3((unsigned)groups, A.seqs), 256, 0, s>>>(W);
+    k_weigh_few<T, D><<<dim3((unsigned)groups, A.seqs), 64 * kWaves, 0, s>>>(W);
   } else {
     const int64_t groups = way.blocks * way.split * A.heads;
     if (groups > INT32_MAX) return HCK_ERR_ARG;
@@ -389,7 +411,7 @@ extern "C" int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int 
   const hck::WeighWay way(seqs, kv_heads, group, (int)std::min<int64_t>(most, tokens), table_columns);
   const size_t need = tokens ? way.bytes(seqs, kv_heads, table_columns) : 0;
   if (need && (!workspace || workspace_bytes < need)) return HCK_ERR_WORKSPACE;
-  W.parts = (float*)workspace, W.split = way.split;
+  W.parts = (float*)workspace, W.split = way.split, W.units = way.units;
   hipStream_t s = (hipStream_t)stream;
   if (head_dim == 128) return type == HCK_BF16 ? hck::launch<__bf16, 128>(W, way, s) : hck::launch<_Float16, 128>(W, way, s);
   return type == HCK_BF16 ? hck::launch<__bf16, 64>(W, way, s) : hck::launch<_Float16, 64>(W, way, s);
