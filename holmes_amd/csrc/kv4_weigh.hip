@@ -195,18 +195,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
 
   // A thread brings pieces of rows kApart apart; row = query * group + head goes on by additions.
   const int piece = threadIdx.x % kPieces, row0 = threadIdx.x / kPieces;
-  int qi = (from + row0) / A.group, qo = (from + row0) % A.group;
-  const int step_i = kApart / A.group, step_o = kApart % A.group;
+  int qo = (from + row0) % A.group;
+  const T* next = (const T*)A.q + (R.q0 + (int64_t)((from + row0) / A.group)) * A.q_ts + (int64_t)(h * A.group + qo) * A.q_hs + piece * 8;
+  const int step_o = kApart % A.group;
+  const int64_t step = (kApart / A.group) * A.q_ts + step_o * A.q_hs, wrap = A.q_ts - A.group * A.q_hs;
   u32x4 raw[kEach];
   auto bring = [&](int at) {  // rows at .. at + kStage - 1
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       raw[j] = u32x4{0, 0, 0, 0};
-      if (at + row0 + j * kApart < to)
-        raw[j] = reinterpret_cast<const Loose16*>((const T*)A.q + (R.q0 + qi) * A.q_ts + (int64_t)(h * A.group + qo) * A.q_hs +
-                                                  piece * 8)->v;
-      qi += step_i, qo += step_o;
-      if (qo >= A.group) qo -= A.group, ++qi;
+      if (at + row0 + j * kApart < to) raw[j] = reinterpret_cast<const Loose16*>(next)->v;
+      next += step, qo += step_o;
+      if (qo >= A.group) qo -= A.group, next += wrap;
     }
   };
   auto place = [](int row, int p) { return row * kPieces + (p ^ (D == 128 ? row & 15 : (row >> 1) & 7)); };
@@ -234,6 +234,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
     if (n == 0) s_least[buf][half] = least;
   };
 
+  // The sums over 64 rows.  PARTLY: some of them do not see some of the wave's tokens.
+  float now[2];
+  auto stage = [&](int buf, auto PARTLY) {
+    now[0] = now[1] = 0.f;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      f32x16 c[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[0][i] = c[1][i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int at = place(32 * y + n, (2 * (s / (D / 32)) + half) * (D / 32) + s % (D / 32));
+        const bf16x8 q = __builtin_bit_cast(bf16x8, s_q[buf][0][at]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) c[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, k[x][s], c[x], 0, 0, 0);
+        if constexpr (kHalf) {
+          const bf16x8 r = __builtin_bit_cast(bf16x8, s_q[buf][kParts - 1][at]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) c[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(r, k[x][s], c[x], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // rows 8 i + 4 half ..
+        const int r = 32 * y + 8 * i + 4 * half;
+        const f32x4 off = *reinterpret_cast<const f32x4*>(&s_off[buf][r]);
+        const f32x4 factor = *reinterpret_cast<const f32x4*>(&s_factor[buf][r]);
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        i32x4 seen;
+        if constexpr (decltype(PARTLY)::value) seen = *reinterpret_cast<const i32x4*>(&s_seen[buf][r]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][4 * i + e], W.scale2, -off[e]));
+            if constexpr (decltype(PARTLY)::value) p = here + 32 * x + n < seen[e] ? p : 0.f;
+            now[x] = __builtin_fmaf(p, factor[e], now[x]);
+          }
+      }
+    }
+  };
+
   float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};
   if (from < to) {
     bring(from);
@@ -249,50 +290,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
       if (mine) lse = row_lse(W, R, h, at + kStage + lane);
     }
     if (there) {
-      float now[2] = {0.f, 0.f};
-#pragma unroll 1
-      for (int y = 0; y < 2; ++y) {
-        f32x16 c[2];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) c[0][i] = c[1][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const int at = place(32 * y + n, (2 * (s / (D / 32)) + half) * (D / 32) + s % (D / 32));
-          const bf16x8 q = __builtin_bit_cast(bf16x8, s_q[buf][0][at]);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) c[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, k[x][s], c[x], 0, 0, 0);
-          if constexpr (kHalf) {
-            const bf16x8 r = __builtin_bit_cast(bf16x8, s_q[buf][kParts - 1][at]);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) c[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(r, k[x][s], c[x], 0, 0, 0);
-          }
-        }
-        const bool partly = here + kUnit > __builtin_amdgcn_readfirstlane(s_least[buf][y]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // rows 8 i + 4 half ..
-          const int r = 32 * y + 8 * i + 4 * half;
-          const f32x4 off = *reinterpret_cast<const f32x4*>(&s_off[buf][r]);
-          const f32x4 factor = *reinterpret_cast<const f32x4*>(&s_factor[buf][r]);
-          float p[2][4];
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              p[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[x][4 * i + e], W.scale2, -off[e]));
-          if (partly) {
-            typedef int i32x4 __attribute__((ext_vector_type(4)));
-            const i32x4 seen = *reinterpret_cast<const i32x4*>(&s_seen[buf][r]);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) p[x][e] = here + 32 * x + n < seen[e] ? p[x][e] : 0.f;
-          }
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) now[x] = __builtin_fmaf(p[x][e], factor[e], now[x]);
-        }
-      }
+      if (here + kUnit <= __builtin_amdgcn_readfirstlane(min(s_least[buf][0], s_least[buf][1]))) stage(buf, std::false_type());
+      else stage(buf, std::true_type());
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float add = now[x] - lost[x], all = sum[x] + add;
@@ -347,7 +346,7 @@ struct WeighWay {
     units = (int)std::min<int64_t>(4, std::max<int64_t>(1, (int64_t)cols * 2 * heads * seqs / (32 * kComputeUnits)));
     blocks = ((int64_t)cols * kPageTokens + kBlock - 1) / kBlock;
     // some workgroups for every compute unit, of four stages at the least
-    split = many ? (int)std::min<int64_t>((rows + 4 * kStage - 1) / (4 * kStage), (4 * kComputeUnits) / std::max<int64_t>(1, blocks * heads * seqs) + 1) : 1;
+    split = many ? (int)std::min<int64_t>((rows + 4 * kStage - 1) / (4 * kStage), (8 * kComputeUnits) / std::max<int64_t>(1, blocks * heads * seqs) + 1) : 1;
   }
   size_t bytes(int64_t seqs, int heads, int cols) const {
     return split > 1 ? (size_t)split * seqs * heads * cols * kPageTokens * sizeof(float) : 0;
