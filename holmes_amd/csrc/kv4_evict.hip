@@ -129,18 +129,18 @@ __device__ __forceinline__ void count_digit(const Keys<R>& K, int digit, uint32_
 __device__ __forceinline__ int top_bin(int digit) { return (1 << bits_of(digit)) - 1 - 2 * (int)threadIdx.x; }
 
 // The largest digit with `left` keys or more at it and above it, from a thread's two counts; `left` becomes how many of those
-// at it.  found: two places.
-__device__ __forceinline__ void find_digit(int digit, int high, int low, int* part, int* found, uint32_t& prefix, int& left) {
+// at it; returns how many there are.  found: three places, not written again before a barrier.
+__device__ __forceinline__ int find_digit(int digit, int high, int low, int* part, int* found, uint32_t& prefix, int& left) {
   int total;
   const int upto = upto_thread(high + low, part, total), before = upto - high - low;
   if (before < left && upto >= left) {  // one thread
     const bool second = before + high < left;
-    found[0] = top_bin(digit) - second, found[1] = left - before - (second ? high : 0);
+    found[0] = top_bin(digit) - second, found[1] = left - before - (second ? high : 0), found[2] = second ? low : high;
   }
   __syncthreads();
   prefix = prefix << bits_of(digit) | (uint32_t)found[0];
   left = found[1];
-  __syncthreads();
+  return found[2];
 }
 
 // What stays of the keys, above T or among the first `left` at T (of which `ties` come before these keys): 64 places at a time,
@@ -191,7 +191,7 @@ __device__ __forceinline__ void write_rest(const EvictArgs& A, const Row& row, i
 template <int R>
 __global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
   constexpr int kCopies = R >= 4 ? 8 : 1;
-  __shared__ int s_bins[kBins * kCopies], s_stay[R * kSelectWaves], s_tie[R * kSelectWaves], s_part[kSelectWaves], s_found[2];
+  __shared__ int s_bins[kBins * kCopies], s_stay[R * kSelectWaves], s_tie[R * kSelectWaves], s_part[kSelectWaves], s_found[3];
   const Row row(A, blockIdx.y, blockIdx.x);
   Keys<R> K;
   K.load(A, row, 0);
@@ -203,14 +203,22 @@ __global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
   if (want > 0 && want < choice) {
     T = 0, left = want;
     for (int digit = 0; digit < 3; ++digit) {
-      count_digit<R, kCopies>(K, digit, T, s_bins);
       const int top = top_bin(digit);
       int high = 0, low = 0;
-      if (top > 0) {
+      if (digit == 0) {
+        count_digit<R, kCopies>(K, digit, T, s_bins);
+        if (top > 0) {
 #pragma unroll
-        for (int c = 0; c < kCopies; ++c) high += s_bins[top * kCopies + c], low += s_bins[(top - 1) * kCopies + c];
+          for (int c = 0; c < kCopies; ++c) high += s_bins[top * kCopies + c], low += s_bins[(top - 1) * kCopies + c];
+        }
+      } else {
+        count_digit<R, 1>(K, digit, T, s_bins);
+        if (top > 0) high = s_bins[top], low = s_bins[top - 1];
       }
-      find_digit(digit, high, low, s_part, s_found, T, left);
+      if (find_digit(digit, high, low, s_part, s_found, T, left) == left) {  // all that agree so far stay
+        T = (T << shift_of(digit)) - 1, left = 0;
+        break;
+      }
     }
   }
   write_kept<R>(A, row, K, T, left, 0, 0, s_stay, s_tie, s_part);
@@ -234,7 +242,7 @@ template <int PHASE>
 __global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
   constexpr int R = kSegment, kCopies = PHASE == 0 ? 8 : 1;
   __shared__ int s_bins[PHASE < 3 ? kBins * kCopies : 1], s_stay[R * kSelectWaves], s_tie[R * kSelectWaves];
-  __shared__ int s_part[kSelectWaves], s_found[2];
+  __shared__ int s_part[kSelectWaves], s_found[3];
   const int seg = blockIdx.z;
   const Row row(A, blockIdx.y, blockIdx.x);
   const Counts C(A, row.line);
@@ -252,9 +260,11 @@ __global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
   uint32_t T = 0;
   int left = 0;
   if constexpr (PHASE > 0) {
-    for (int s = 0; s < segs; ++s) {
-      if (s == seg) choice_before = choice, must_before = must;
-      choice += C.choice[s], must += C.must[s];
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < segs; s0 += 64) {
+      const int s = s0 + lane, c = s < segs ? C.choice[s] : 0, m = s < segs ? C.must[s] : 0;
+      choice += over_wave(c), must += over_wave(m);
+      choice_before += over_wave(s < seg ? c : 0), must_before += over_wave(s < seg ? m : 0);
     }
   }
   const int want = min(choice, A.keep - must);
@@ -267,12 +277,14 @@ __global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
     else T = (uint32_t)C.state[2 * (digit - 1)], left = C.state[2 * (digit - 1) + 1];
     const int top = top_bin(digit);
     int high = 0, low = 0, own_high = 0, own_low = 0;  // own: of this segment; in the last launch, of those before
-    if (top > 0)
+    if (top > 0) {
+#pragma unroll 8
       for (int s = 0; s < segs; ++s) {
         const int2 two = *reinterpret_cast<const int2*>(C.bins + ((int64_t)digit * A.segs + s) * kBins + top - 1);
         high += two.y, low += two.x;
         if (PHASE == 3 ? s < seg : s == seg) own_high += two.y, own_low += two.x;
       }
+    }
     find_digit(digit, high, low, s_part, s_found, T, left);
     const int at = (int)(T & ((1u << bits_of(digit)) - 1));
     int all;
@@ -284,7 +296,10 @@ __global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
       before = all;
       upto_thread(top == at ? own_high : top - 1 == at ? own_low : 0, s_part, all);
       ties_before = all;
-      for (int s = 0; s < seg; ++s) before += C.above[s] + C.above[A.segs + s];
+      for (int s0 = 0; s0 < seg; s0 += 64) {
+        const int s = s0 + (threadIdx.x & 63);
+        before += over_wave(s < seg ? C.above[s] + C.above[A.segs + s] : 0);
+      }
     }
   }
   if constexpr (PHASE < 3) {

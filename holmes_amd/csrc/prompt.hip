@@ -61,15 +61,12 @@ __device__ __forceinline__ uint32_t pack_as(float a, float b) {
   return __builtin_bit_cast(uint32_t, two{(T)a, (T)b});
 }
 
-// An infinity or a NaN among eight values: an exponent of ones carries into the sign's bit.
+// The sign bits of those of two values that are an infinity or a NaN: an exponent of ones carries into the sign's bit.
 template <typename T>
-__device__ __forceinline__ uint32_t odd_values(u32x4 x) {
+__device__ __forceinline__ uint32_t odd_values(uint32_t x) {
   constexpr uint32_t kExponent = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
   constexpr uint32_t kOne = __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
-  uint32_t any = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) any |= (x[i] & kExponent) + kOne;
-  return any & 0x80008000u;
+  return ((x & kExponent) + kOne) & 0x80008000u;
 }
 
 // A sequence's tokens, and a tile of its rows.
@@ -89,18 +86,22 @@ __device__ __forceinline__ void sequence(const PromptArgs& A, int b, int64_t& fi
 }
 __device__ __forceinline__ int rows_of(const PromptArgs& A, int n) { return min(n, A.most) * A.group; }
 
-// Tile r of all sequences' tiles, a sequence's last ones (which see most) first.
+// Tile r of all sequences' tiles.  Of up to 64 sequences (a lane has one) the tiles with the highest numbers, which see most, come
+// first: those of number t and above are sum max(0, tiles - t), and t is found by halving.  Of more, a sequence's last come first.
 __device__ __forceinline__ bool locate_tile(const PromptArgs& A, int r, Tile& t) {
   int b = 0;
   const int lane = threadIdx.x & 63;
-  if (A.seqs > 1) {
+  auto count = [&](int b) {
+    int64_t first;
+    int n = 0;
+    if (b < A.seqs) sequence(A, b, first, n);
+    return (rows_of(A, n) + kTileRows - 1) / kTileRows;
+  };
+  int last = -1;
+  if (A.seqs > 64) {
     for (b = 0;; b += 64) {
       if (b >= A.seqs) return false;
-      int64_t first;
-      int n = 0;
-      if (b + lane < A.seqs) sequence(A, b + lane, first, n);
-      const int mine = (rows_of(A, n) + kTileRows - 1) / kTileRows;
-      const int upto = upto_lane(mine), all = __builtin_amdgcn_readlane(upto, 63);
+      const int mine = count(b + lane), upto = upto_lane(mine), all = __builtin_amdgcn_readlane(upto, 63);
       if (r < all) {
         const int owner = __popcll(__ballot(upto <= r));
         b += owner;
@@ -109,12 +110,26 @@ __device__ __forceinline__ bool locate_tile(const PromptArgs& A, int r, Tile& t)
       }
       r -= all;
     }
+  } else if (A.seqs > 1) {
+    const int mine = count(lane);
+    if (r >= over_wave(mine)) return false;
+    int at = 0, none = A.tiles;  // more than r tiles of number `at` and above; no more than r of `none`
+    while (none - at > 1) {
+      const int middle = (at + none) / 2;
+      if (over_wave(max(0, mine - middle)) > r) at = middle;
+      else none = middle;
+    }
+    r -= over_wave(max(0, mine - at - 1));
+    const unsigned long long has = __ballot(mine > at);
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+    b = __builtin_ctzll(__ballot(mine > at && before == r));
+    last = at;
   }
   sequence(A, b, t.first, t.n);
   t.rows = rows_of(A, t.n);
   const int tiles = (t.rows + kTileRows - 1) / kTileRows;
-  if (r >= tiles) return false;
-  t.tile = tiles - 1 - r;
+  if (last < 0 && r >= tiles) return false;
+  t.tile = last < 0 ? tiles - 1 - r : last;
   return true;
 }
 
@@ -310,34 +325,40 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
     };
     if constexpr (kPartly) {
       // Tokens that a row does not see have a probability of 0, and 0 times an infinity or a NaN is NaN.  Where there
-      // is one, the tokens go one by one, each for the rows that see it.
+      // is one it goes into the product as 0, and is then added to the rows that see it.
       uint32_t odd = 0;
 #pragma unroll 4
-      for (int i = 0; i < kUnit * S::kPieces / 64; ++i) odd |= odd_values<T>(vs[i * 64 + lane]);
+      for (int i = 0; i < kUnit * S::kPieces / 64; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= odd_values<T>(vs[i * 64 + lane][e]);
       if (__any(odd != 0)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const u32x4 p = probabilities(j);
-#pragma unroll 1
-          for (int k = 0; k < 16; ++k) {
-            const int at = k & 7;  // of the eight of half k / 8
-            u32x4 only;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) only[i] = half == k >> 3 && at >> 1 == i ? (at & 1 ? 0xffff0000u : 0xffffu) : 0u;
-            const bool see = here + 16 * j + 8 * (at >> 2) + 4 * (k >> 3) + (at & 3) < seen;
+          for (int d = 0; d < kTiles; ++d) {
+            u32x4 v = values(j, d);
 #pragma unroll
-            for (int d = 0; d < kTiles; ++d) {
-              f32x16 one;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) one[i] = 0.f;
-              one = mfma32(__builtin_bit_cast(vec, values(j, d) & only), __builtin_bit_cast(vec, p & only), one);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[d][i] += see ? one[i] : 0.f;
-            }
+            for (int e = 0; e < 4; ++e) v[e] &= ~((odd_values<T>(v[e]) >> 15) * 0xffffu);
+            acc[d] = mfma32(__builtin_bit_cast(vec, v), __builtin_bit_cast(vec, p), acc[d]);
           }
         }
         sum += part[0] + part[1];
         if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
+#pragma unroll 1
+        for (int t = 0; t < kUnit; ++t)
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // dims 32 d + 8 i + 4 half ..
+              typedef T four __attribute__((ext_vector_type(4)));
+              const u32x2 w = *reinterpret_cast<const u32x2*>((const char*)(vs + S::value_at(t, 4 * d + i)) + half * 8);
+              const four v = __builtin_bit_cast(four, w);
+              const uint32_t o[2] = {odd_values<T>(w[0]), odd_values<T>(w[1])};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[d][4 * i + e] += here + t < seen && (o[e >> 1] >> (e & 1 ? 31 : 15) & 1) ? (float)v[e] : 0.f;
+            }
         return;
       }
     }
@@ -425,10 +446,10 @@ extern "C" int hck_prompt_attend(const void* queries, const void* keys, const vo
   A.k_ts = tokens > 1 ? k_token_stride : head_dim, A.k_hs = k_head_stride;
   A.v_ts = tokens > 1 ? v_token_stride : head_dim, A.v_hs = v_head_stride;
   A.seqs = seqs, A.heads = kv_heads, A.group = group, A.causal = causal != 0, A.most = most;
+  A.tiles = (int)(((int64_t)most * group + hck::kTileRows - 1) / hck::kTileRows);
   A.scale2 = (float)(scale * 1.4426950408889634);
   // every sequence has a tile that may not be full, beside the full ones
-  const int64_t tiles = ((int64_t)most * group + hck::kTileRows - 1) / hck::kTileRows;
-  const int64_t items = std::min(tiles * seqs, tokens * group / hck::kTileRows + seqs);
+  const int64_t items = std::min((int64_t)A.tiles * seqs, tokens * group / hck::kTileRows + seqs);
   if (items * kv_heads > INT32_MAX) return HCK_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (head_dim == 128) return type == HCK_BF16 ? hck::launch<__bf16, 128>(A, items, s) : hck::launch<_Float16, 128>(A, items, s);
