@@ -123,7 +123,8 @@ SIGNATURES = {
     "hck_rotary": (_i, [_vp, _i, _i64, _vp, _i, _i, _i, ctypes.c_float, _i, _i, _vp, _i64, _i64, _i, _vp, _vp, _i64, _i64,
                         _i, _vp, _vp]),
     "hck_prompt_attend": (_i, [_vp, _vp, _vp, _i, _i64, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i, _i, _i,
-                               ctypes.c_double, _vp, _vp, _vp, _vp, _vp]),
+                               ctypes.c_double, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "hck_prompt_attend_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i, _i]),
     "hck_kv4_weigh": (_i, [_vp, _i64, _i, _i, _i, _vp, _i64, _i, _i64, _i64, _vp, _i64, _i, _vp, _vp, _i, _i, _i,
                            ctypes.c_double, _vp, _vp, _i64, _i64, _i, _vp, _vp, _sz, _vp]),
     "hck_kv4_weigh_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i]),

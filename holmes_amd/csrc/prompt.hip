@@ -30,6 +30,10 @@ struct PromptArgs {
   float *lse, *low, *high;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, tokens;
   int seqs, heads, group, causal, most, tiles;  // tiles that the longest sequence can have
+  // where tiles' units are shared out: units of a part, parts that a tile can have, and [slot][wave][piece][lane] of four floats,
+  // of which the first piece is (m, l, least score, -) of the lane's row and the others are its sums
+  int part, parts, items;
+  f32x4* slots;
   float scale2;                                 // scale log2 e
 };
 
@@ -166,7 +170,38 @@ __device__ __forceinline__ rsrc_t bounds(const char* base, int bytes) {
                 (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
 }
 
-template <typename T, int D, bool RANGE>
+// A row's results from its sums: maximum m in units of log 2, sum l, dims 32 d + 8 i + 4 half .. from sums(d, i).
+template <typename T, int D, bool RANGE, typename F>
+__device__ __forceinline__ void write_row(const PromptArgs& A, int64_t at, int half, float m, float l, float low, float lift, F sums) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = (T*)A.out + at * D + 4 * half;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 x = sums(d, i) * inv;
+      *reinterpret_cast<u32x2*>(out + 32 * d + 8 * i) = u32x2{pack_as<T>(x[0], x[1]), pack_as<T>(x[2], x[3])};
+    }
+  if (half) return;
+  A.lse[at] = fabsf(m) == INFINITY ? m + l : (above(m) + (__builtin_amdgcn_logf(l) - lift)) * kLn2;
+  if constexpr (RANGE) A.low[at] = l != l ? l : low * kLn2, A.high[at] = l != l ? l : m * kLn2;
+}
+
+// Exponentials are taken times 2^lift.  fp16: the largest up to 2^15, so that those down to 2^-29 of it keep all bits.  bf16:
+// such that their sum over n tokens is at most 1, and no sum of values overflows.
+template <typename T>
+__device__ __forceinline__ float lift_of(int n) {
+  return __is_same(T, _Float16) ? 15.f : (float)(__builtin_clz(n) - 32);
+}
+
+constexpr int kPieces(int dim) { return 1 + dim / 8; }  // of a lane in a slot
+__device__ __forceinline__ f32x4* slot_of(const PromptArgs& A, int item, int part, int h, int wave, int dim) {
+  return A.slots + (((int64_t)item * A.parts + part) * A.heads + h) * (kPromptWaves * 64 * kPieces(dim)) + wave * 64 * kPieces(dim) +
+         (threadIdx.x & 63);
+}
+
+// SPLIT: a workgroup takes a part of a tile's units; parts of a tile that has several are joined by k_whole_join.
+template <typename T, int D, bool RANGE, bool SPLIT>
 __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   using S = Staged<D>;
   using vec = typename Eight<T>::type;
@@ -175,14 +210,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
 
   Tile t;
   const int h = blockIdx.x % A.heads;
-  if (!locate_tile(A, blockIdx.x / A.heads, t)) return;
+  // (neighbours are on different XCDs: parts next to each other would leave the first ones, of which there are most, to some)
+  const int part = SPLIT ? blockIdx.x / A.heads / A.items : 0, item = blockIdx.x / A.heads % (SPLIT ? A.items : 0x7fffffff);
+  if (!locate_tile(A, item, t)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int n = __builtin_amdgcn_readfirstlane(t.n), rows = __builtin_amdgcn_readfirstlane(t.rows);
   const int tile = __builtin_amdgcn_readfirstlane(t.tile);
   const int64_t first = t.first;
   auto sees = [&](int row) { return A.causal ? row / A.group + 1 : n; };
   const int most = sees(min(tile * kTileRows + kTileRows, rows) - 1);
-  const int units = (most + kUnit - 1) / kUnit;
+  const int all = (most + kUnit - 1) / kUnit, begin = SPLIT ? part * A.part : 0, units = SPLIT ? min(all, begin + A.part) : all;
+  if (SPLIT && part && begin >= all) return;
   const int mine = tile * kTileRows + wave * kRowsOfWave;
   const int last = mine < rows ? sees(min(mine + kRowsOfWave, rows) - 1) : 0;
   const int row = mine + (lane & 31);
@@ -209,7 +247,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       load_lds(to + j * (1024 * kPromptWaves) + S::kBytes, v_off + j * v_step, vr);
     }
   };
-  if (units > 0) bring(0);
+  if (begin < units) bring(begin);
 
   vec q[kSteps];
   const T* qp = (const T*)A.q + (first + qi) * A.q_ts + (int64_t)(h * A.group + qo) * A.q_hs + half * 8;
@@ -223,9 +261,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   // Where the lane reads: keys of token lane % 32 (and 32 on); values of the tokens 4 half + lane % 16 / 4 (and 8 on), of
   // which lane i of 16 gets dim i.
   const int vt = 4 * half + ((lane & 15) >> 2), vc = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-  // Exponentials times 2^lift.  fp16: the largest up to 2^15, so that those down to 2^-29 of it keep all bits.  bf16: such
-  // that their sum is at most 1, and no sum of values overflows.
-  const float lift = __is_same(T, _Float16) ? 15.f : (float)(__builtin_clz(n) - 32);
+  const float lift = lift_of<T>(n);
 
   f32x16 acc[kTiles];
 #pragma unroll
@@ -379,8 +415,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
     if (u + 1 < units) bring(u + 1);
   };
   const int full = sees(tile * kTileRows) / kUnit;  // units that all of the tile's rows see
-  int u = 0;
-  for (; u < full; ++u) {
+  int u = begin;
+  for (; u < min(full, units); ++u) {
     next(u);
     unit(u, std::false_type());
   }
@@ -391,29 +427,93 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
 
   sum = over_half(sum, [](float a, float c) { return a + c; });
   if constexpr (RANGE) low = over_half(low, fmin2) * A.scale2;
+  auto sums = [&](int d, int i) { return f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]}; };
+  if (SPLIT && all > A.part) {
+    f32x4* to = slot_of(A, item, part, h, wave, D);
+    to[0] = f32x4{top, sum, low, 0.f};
+#pragma unroll
+    for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[64 * (1 + 4 * d + i)] = sums(d, i);
+    return;
+  }
   if (!live) return;
-  const int64_t at = (first + qi) * (int64_t)(A.heads * A.group) + h * A.group + qo;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* out = (T*)A.out + at * D + 4 * half;
-#pragma unroll
-  for (int d = 0; d < kTiles; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a = pack_as<T>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv);
-      const uint32_t b = pack_as<T>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv);
-      *reinterpret_cast<u32x2*>(out + 32 * d + 8 * i) = u32x2{a, b};
-    }
-  if (half) return;
-  const bool bad = sum != sum;
-  A.lse[at] = fabsf(top) == INFINITY ? top + sum : (above(top) + (__builtin_amdgcn_logf(sum) - lift)) * kLn2;
-  if constexpr (RANGE) A.low[at] = bad ? sum : low * kLn2, A.high[at] = bad ? sum : top * kLn2;
+  write_row<T, D, RANGE>(A, (first + qi) * (int64_t)(A.heads * A.group) + h * A.group + qo, half, top, sum, low, lift, sums);
 }
 
+// The parts of a tile's rows, lane by lane as they were left.
+template <typename T, int D, bool RANGE>
+__global__ __launch_bounds__(64 * kPromptWaves) void k_whole_join(PromptArgs A) {
+  constexpr int kTiles = D / 32;
+  Tile t;
+  const int h = blockIdx.x % A.heads, item = blockIdx.x / A.heads;
+  if (!locate_tile(A, item, t)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int end = min(t.tile * kTileRows + kTileRows, t.rows) - 1;
+  const int all = ((A.causal ? end / A.group + 1 : t.n) + kUnit - 1) / kUnit, parts = (all + A.part - 1) / A.part;
+  const int row = t.tile * kTileRows + wave * kRowsOfWave + (lane & 31);
+  if (parts <= 1 || row >= t.rows) return;
+  const int64_t apart = (int64_t)A.heads * (kPromptWaves * 64 * kPieces(D));
+  const f32x4* from = slot_of(A, item, 0, h, wave, D);
+  float top = -INFINITY, sum = 0.f, low = INFINITY;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, from[p * apart][0]);
+  f32x4 acc[kTiles * 4];
+#pragma unroll
+  for (int i = 0; i < kTiles * 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int p = 0; p < parts; ++p) {
+    const f32x4 s = from[p * apart];
+    const float f = rebase(s[0], top);
+    sum += s[1] * f, low = fminf(low, s[2]);
+#pragma unroll
+    for (int i = 0; i < kTiles * 4; ++i) acc[i] += from[p * apart + 64 * (1 + i)] * f;
+  }
+  write_row<T, D, RANGE>(A, (t.first + row / A.group) * (int64_t)(A.heads * A.group) + h * A.group + row % A.group, half, top, sum, low,
+                         lift_of<T>(t.n), [&](int d, int i) { return acc[4 * d + i]; });
+}
+
+// How a call is run, from what the host knows of it.
+struct WholeWay {
+  int64_t items;
+  int tiles, part, parts;
+  WholeWay(int64_t tokens, int64_t seqs, int heads, int group, int most, bool causal) {
+    tiles = (int)(((int64_t)most * group + kTileRows - 1) / kTileRows);
+    // every sequence has a tile that may not be full, beside the full ones
+    items = std::min((int64_t)tiles * seqs, tokens * group / kTileRows + seqs);
+    // Few tiles of long sequences are cut into parts, as many as run at once and no more: of the tiles of one sequence with
+    // `causal` that is longest / 2 / part + 1 / 2 for each; of several, whose lengths the host does not know, half as many parts
+    // are reckoned with.  A part costs its sums' way through memory and the join some 5 us, which
+    // is what 8 units take (one sequence, 128 dims, whole and in parts: 4000 tokens, 6 heads over 2, 85 and 53 us; 6000, 8 over
+    // 4, 144 and 105; 2000, 32 over 8, in more parts than run at once, 53 and 72).
+    const int64_t longest = ((int64_t)most + kUnit - 1) / kUnit, each = items * heads;
+    int64_t units = longest;
+    if (causal && 2 * kSlots > each) units = (longest / (seqs > 1 ? 2 : 1) * each + 2 * kSlots - each - 1) / (2 * kSlots - each);
+    if (!causal && kSlots > each) units = (longest + kSlots / each - 1) / (kSlots / each);
+    part = (int)std::min(longest, std::max<int64_t>(kLeast, units));
+    parts = longest > part + kJoin ? (int)((longest + part - 1) / part) : 1;
+  }
+  size_t bytes(int heads, int dim) const {
+    return parts > 1 ? (size_t)items * parts * heads * (kPromptWaves * 64 * kPieces(dim)) * sizeof(f32x4) : 0;
+  }
+  static constexpr int kSlots = 2 * kComputeUnits, kLeast = 8, kJoin = 8;
+};
+
 template <typename T, int D>
-int launch(const PromptArgs& A, int64_t items, hipStream_t s) {
-  const unsigned groups = (unsigned)(items * A.heads);
-  if (A.low) k_whole<T, D, true><<<groups, 64 * kPromptWaves, 0, s>>>(A);
-  else k_whole<T, D, false><<<groups, 64 * kPromptWaves, 0, s>>>(A);
+int launch(const PromptArgs& A, const WholeWay& way, hipStream_t s) {
+  const unsigned tiles = (unsigned)(way.items * A.heads);
+  constexpr int kThreads = 64 * kPromptWaves;
+  if (way.parts == 1) {
+    if (A.low) k_whole<T, D, true, false><<<tiles, kThreads, 0, s>>>(A);
+    else k_whole<T, D, false, false><<<tiles, kThreads, 0, s>>>(A);
+    HCK_CHECK_LAUNCH();
+    return HCK_OK;
+  }
+  if (A.low) k_whole<T, D, true, true><<<tiles * way.parts, kThreads, 0, s>>>(A);
+  else k_whole<T, D, false, true><<<tiles * way.parts, kThreads, 0, s>>>(A);
+  HCK_CHECK_LAUNCH();
+  if (A.low) k_whole_join<T, D, true><<<tiles, kThreads, 0, s>>>(A);
+  else k_whole_join<T, D, false><<<tiles, kThreads, 0, s>>>(A);
   HCK_CHECK_LAUNCH();
   return HCK_OK;
 }
@@ -421,11 +521,19 @@ int launch(const PromptArgs& A, int64_t items, hipStream_t s) {
 }  // namespace
 }  // namespace hck
 
+extern "C" size_t hck_prompt_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim, int most,
+                                                    int causal) {
+  if (tokens < 1 || tokens > INT32_MAX || seqs < 1 || kv_heads < 1 || group < 1 || most < 1 ||
+      (head_dim != 64 && head_dim != 128) || std::min<int64_t>(most, tokens) * group > INT32_MAX - 256)
+    return 0;
+  return hck::WholeWay(tokens, seqs, kv_heads, group, (int)std::min<int64_t>(most, tokens), causal != 0).bytes(kv_heads, head_dim);
+}
+
 extern "C" int hck_prompt_attend(const void* queries, const void* keys, const void* values, int type, int64_t tokens,
                                  int kv_heads, int group, int head_dim, int64_t q_token_stride, int64_t q_head_stride,
                                  int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
                                  const int32_t* starts, int seqs, int most, int causal, double scale, void* out, float* lse,
-                                 float* low, float* high, void* stream) {
+                                 float* low, float* high, void* workspace, size_t workspace_bytes, void* stream) {
   if ((head_dim != 64 && head_dim != 128) || (type != HCK_BF16 && type != HCK_F16)) return HCK_ERR_UNSUPPORTED;
   if (tokens < 0 || tokens > INT32_MAX || kv_heads < 1 || group < 1 || (int64_t)kv_heads * group > INT32_MAX || seqs < 0 ||
       most < 0 || !((float)scale > 0.f && scale <= 0x1p126) || (low == nullptr) != (high == nullptr))
@@ -446,12 +554,13 @@ extern "C" int hck_prompt_attend(const void* queries, const void* keys, const vo
   A.k_ts = tokens > 1 ? k_token_stride : head_dim, A.k_hs = k_head_stride;
   A.v_ts = tokens > 1 ? v_token_stride : head_dim, A.v_hs = v_head_stride;
   A.seqs = seqs, A.heads = kv_heads, A.group = group, A.causal = causal != 0, A.most = most;
-  A.tiles = (int)(((int64_t)most * group + hck::kTileRows - 1) / hck::kTileRows);
+  const hck::WholeWay way(tokens, seqs, kv_heads, group, most, causal != 0);
+  if (way.items * way.parts * kv_heads > INT32_MAX) return HCK_ERR_ARG;
+  const size_t need = way.bytes(kv_heads, head_dim);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return HCK_ERR_WORKSPACE;
+  A.tiles = way.tiles, A.part = way.part, A.parts = way.parts, A.items = (int)way.items, A.slots = (hck::f32x4*)workspace;
   A.scale2 = (float)(scale * 1.4426950408889634);
-  // every sequence has a tile that may not be full, beside the full ones
-  const int64_t items = std::min((int64_t)A.tiles * seqs, tokens * group / hck::kTileRows + seqs);
-  if (items * kv_heads > INT32_MAX) return HCK_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
-  if (head_dim == 128) return type == HCK_BF16 ? hck::launch<__bf16, 128>(A, items, s) : hck::launch<_Float16, 128>(A, items, s);
-  return type == HCK_BF16 ? hck::launch<__bf16, 64>(A, items, s) : hck::launch<_Float16, 64>(A, items, s);
+  if (head_dim == 128) return type == HCK_BF16 ? hck::launch<__bf16, 128>(A, way, s) : hck::launch<_Float16, 128>(A, way, s);
+  return type == HCK_BF16 ? hck::launch<__bf16, 64>(A, way, s) : hck::launch<_Float16, 64>(A, way, s);
 }

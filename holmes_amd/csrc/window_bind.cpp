@@ -135,11 +135,15 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
     low = make({tokens, heads}, at::kFloat, dev);
     high = make({tokens, heads}, at::kFloat, dev);
   }
+  const size_t bytes =
+      hck_prompt_attend_workspace_bytes(tokens, (int)seqs, (int)kv_heads, (int)(heads / kv_heads), (int)dim, (int)most, causal);
+  Tensor work;
+  if (bytes) work = make({(int64_t)bytes}, at::kByte, dev);
   const int err = hck_prompt_attend(
       ql.data_ptr(), kl.data_ptr(), vl.data_ptr(), type, tokens, (int)kv_heads, (int)(heads / kv_heads), (int)dim,
       stride_of(ql, 0), stride_of(ql, 1), stride_of(kl, 0), stride_of(kl, 1), stride_of(vl, 0), stride_of(vl, 1), ints(starts),
       (int)seqs, (int)most, causal, scale, out.data_ptr(), lse.data_ptr<float>(), ranges ? low.data_ptr<float>() : nullptr,
-      ranges ? high.data_ptr<float>() : nullptr, stream_of(dev.index()));
+      ranges ? high.data_ptr<float>() : nullptr, bytes ? work.data_ptr() : nullptr, bytes, stream_of(dev.index()));
   if (err) return PyLong_FromLong(err);
   return Py_BuildValue("(NNNN)", wrap(std::move(out)), wrap(std::move(lse)), ranges ? wrap(std::move(low)) : none(),
                        ranges ? wrap(std::move(high)) : none());

@@ -495,10 +495,12 @@ int hck_rotary(const void* positions, int position_bytes, int64_t tokens, const 
  * multiples of 8, from 16-byte aligned addresses; tokens of keys and values lie head_dim to 2^23 elements apart.  `most` is at
  * least the largest number of tokens of a sequence.  out, lse, low, high and scale are as for hck_kv4_attend; a token that no
  * sequence covers is left unwritten. */
+size_t hck_prompt_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim, int most, int causal);
 int hck_prompt_attend(const void* queries, const void* keys, const void* values, int type, int64_t tokens, int kv_heads,
                       int group, int head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
                       int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const int32_t* starts, int seqs,
-                      int most, int causal, double scale, void* out, float* lse, float* low, float* high, void* stream);
+                      int most, int causal, double scale, void* out, float* lse, float* low, float* high, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* What attention has given each cached token: weights[b][h][j] = prior + the sum over the rows of key head h that see token j
  * of exp(scale q.k_j - lse), for the queries, pages and masks of hck_kv4_attend and the lse that it gave (a row of -inf

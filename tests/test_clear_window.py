@@ -88,9 +88,9 @@ def test_rotary_refuses():
 
 
 def prompt(q=P, k=P, v=P, kind=0, tokens=10, heads=2, group=2, dim=128, strides=(512, 128, 256, 128, 256, 128), starts=None,
-           seqs=1, most=10, scale=1.0, out=P, lse=P, low=None, high=None):
+           seqs=1, most=10, scale=1.0, out=P, lse=P, low=None, high=None, work=None, size=0):
     return nat.lib().hck_prompt_attend(q, k, v, kind, tokens, heads, group, dim, *strides, starts, seqs, most, 1, scale, out,
-                                       lse, low, high, None)
+                                       lse, low, high, work, size, None)
 
 
 def test_prompt_refuses():
@@ -105,6 +105,10 @@ def test_prompt_refuses():
                 dict(strides=(512, 128, 256, 128, 1 << 24, 128)), dict(tokens=1 << 30, most=1 << 30),
                 dict(tokens=1 << 24, most=1 << 24, group=200)):
         assert prompt(**bad) == nat.HCK_ERR_ARG, bad
+    need = nat.lib().hck_prompt_attend_workspace_bytes(4000, 1, 2, 2, 128, 4000, 1)
+    assert need > 0
+    long = dict(tokens=4000, most=4000)
+    assert prompt(**long) == prompt(**long, work=P, size=need - 1) == prompt(**long, work=odd, size=need) == nat.HCK_ERR_WORKSPACE
     assert prompt(seqs=0, starts=P, q=None) == prompt(tokens=0, q=None) == prompt(most=0, q=None) == 0
 
 

@@ -91,6 +91,34 @@ def test_one_sequence(kind, heads, group, dim, tokens):
     check(clear_call(q, k, v, scale=0.01), q, k, v, [tokens], scale=0.01)
 
 
+@pytest.mark.parametrize("kind,heads,group,dim", [("bf16", 1, 2, 128), ("fp16", 2, 1, 64)])
+@pytest.mark.parametrize("causal,ranges", [(True, True), (False, False), (True, False), (False, True)])
+def test_rows_in_parts(kind, heads, group, dim, causal, ranges):
+    """Few rows of many tokens: parts of a tile's tokens join; some tiles have one part, some rows see nothing of a part."""
+    print("parts", kind, heads, group, dim, causal, ranges, flush=True)
+    from holmes_amd import _native as nat
+
+    g = torch.Generator().manual_seed(20)
+    for counts in ([1500], [700, 3, 1300, 513]):
+        n = sum(counts)
+        assert nat.lib().hck_prompt_attend_workspace_bytes(n, len(counts), heads, group, dim, max(counts), causal) > 0
+        q, k, v = inputs(g, n, heads, group, dim, kind, spread=1.5)
+        got = clear_call(q, k, v, starts_of(counts), most=max(counts), causal=causal, ranges=ranges)
+        check(got, q, k, v, counts, causal=causal)
+        again = clear_call(q, k, v, starts_of(counts), most=max(counts), causal=causal, ranges=ranges)
+        assert torch.equal(got.out, again.out) and torch.equal(got.lse, again.lse)
+    k[1200, 0, 2], v[900, 0, 1] = math.nan, math.inf   # of the third sequence, 703 .. 2002, and the same parts of others
+    bad = clear_call(q, k, v, starts_of(counts), most=max(counts), causal=causal)
+    lost = torch.isnan(bad.lse).any(1).cpu()
+    want = torch.zeros(n, dtype=torch.bool)
+    want[(1200 if causal else 703):2003] = True
+    assert torch.equal(lost, want) and torch.isnan(bad.out[want.cuda()][:, :group]).all()
+    rows = torch.zeros(n, dtype=torch.bool)
+    rows[(900 if causal else 703):2003] = True
+    rows &= ~want
+    assert torch.isposinf(bad.out[rows.cuda()][:, :group, 1]).all() and torch.isfinite(bad.out[~(rows | want).cuda()]).all()
+
+
 def test_many_sequences():
     """More than a wave's lanes, of very different lengths, with `most` and without."""
     print("many", flush=True)
@@ -115,7 +143,7 @@ def test_rows_that_no_sequence_covers_are_left_alone():
     out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 9.0).cuda()
     nat.check(nat.lib().hck_prompt_attend(q.data_ptr(), k.data_ptr(), v.data_ptr(), nat.HCK_BF16, n, 2, 2, 128, 512, 128, 256,
                                           128, 256, 128, starts.data_ptr(), 2, 60, 1, 0.1, out.data_ptr(), lse.data_ptr(), None,
-                                          None, torch.cuda.current_stream().cuda_stream), "hck_prompt_attend")
+                                          None, None, 0, torch.cuda.current_stream().cuda_stream), "hck_prompt_attend")
     torch.cuda.synchronize()
     rows = torch.zeros(n, dtype=torch.bool)
     rows[:first] = rows[-tail:] = rows[first + 40 + 60:first + 110] = True     # 60: the second sequence's rest
