@@ -3,7 +3,7 @@
 Tolerance, for a row with scores s = scale q.k over n tokens and probabilities p: the scores' 32-bit sums of D products
 (e below: 2^-24 (D + 8) of the sum of magnitudes, twice, for the score and the reference's; the exponential's and its
 argument's roundings, 2^-22 (2 + max s - min s); the sum over a lane's n / 2 tokens, 2^-24 (n / 2 + 64)); a probability in
-the type of the values (half a step, 2^-9 or 2^-12 of it at the worst, twice as relative error of a sum and its divisor); half a
+the type of the values (half a step, 2^-8 or 2^-11 of it at the worst, taken twice); half a
 step of the output's type (below its least normal number, one step)."""
 
 import math
