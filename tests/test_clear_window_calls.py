@@ -39,7 +39,12 @@ struct Devices final : c10::impl::DeviceGuardImplInterface {
   c10::Stream exchangeStream(c10::Stream s) const override { return s; }
   c10::DeviceIndex deviceCount() const noexcept override { return 4; }
 };
-C10_REGISTER_GUARD_IMPL(CUDA, Devices)
+// (Another test of this process may have put its own in place; its devices do as well.)
+const bool registered = [] {
+  if (!c10::impl::hasDeviceGuardImpl(at::kCUDA)) c10::impl::DeviceGuardImplRegistrar(at::kCUDA, new Devices());
+  return true;
+}();
+int met() { return c10::impl::getDeviceGuardImpl(at::kCUDA)->getDevice().index(); }
 
 Tensor on(at::IntArrayRef size, ScalarType type, int device) {
   int64_t n = 1;
@@ -65,35 +70,35 @@ extern "C" {
 size_t hck_kv4_page_bytes(int dim) { return (size_t)dim * 136; }
 int hck_rotary(const void*, int size, int64_t tokens, const uint64_t*, int rotated, int, int, float, int, int dim, const void*,
                int64_t, int64_t, int heads, void*, const void*, int64_t, int64_t, int kv, void*, void*) {
-  launches.push_back({current, size, tokens, rotated, dim, heads, kv});
+  launches.push_back({met(), size, tokens, rotated, dim, heads, kv});
   return 0;
 }
 size_t hck_prompt_attend_workspace_bytes(int64_t, int, int, int, int, int, int) { return 64; }
 int hck_prompt_attend(const void*, const void*, const void*, int, int64_t tokens, int heads, int group, int dim, int64_t, int64_t,
                       int64_t, int64_t, int64_t, int64_t, const int32_t* starts, int seqs, int most, int, double, void*, float*, float*,
                       float*, void* work, size_t bytes, void*) {
-  launches.push_back({current, tokens, heads, group, dim, starts != nullptr, seqs, most, work != nullptr, (int64_t)bytes});
+  launches.push_back({met(), tokens, heads, group, dim, starts != nullptr, seqs, most, work != nullptr, (int64_t)bytes});
   return 0;
 }
 size_t hck_kv4_weigh_workspace_bytes(int64_t, int, int, int, int, int) { return 64; }
 int hck_kv4_weigh(const void*, int64_t, int, int, int, const void*, int64_t, int group, int64_t, int64_t, const int32_t*, int64_t,
                   int cols, const int32_t*, const int32_t* starts, int seqs, int most, int, double, const float*, const float* prior,
                   int64_t, int64_t, int places, float*, void* work, size_t bytes, void*) {
-  launches.push_back({current, group, cols, starts != nullptr, seqs, most, prior != nullptr, places, work != nullptr, (int64_t)bytes});
+  launches.push_back({met(), group, cols, starts != nullptr, seqs, most, prior != nullptr, places, work != nullptr, (int64_t)bytes});
   return 0;
 }
 size_t hck_kv4_evict_workspace_bytes(int, int, int) { return 64; }
 int hck_kv4_evict(void*, int64_t, int, int, const int32_t*, int64_t, int cols, const int32_t*, int seqs, const float*, int64_t, int64_t,
                   int places, const int32_t*, int64_t, int into, int keep, int recent, int32_t*, int32_t*, float*, void* work, size_t bytes,
                   void*) {
-  launches.push_back({current, cols, seqs, places, into, keep, recent, work != nullptr, (int64_t)bytes});
+  launches.push_back({met(), cols, seqs, places, into, keep, recent, work != nullptr, (int64_t)bytes});
   return 0;
 }
 }
 
 PYBIND11_MODULE(_stub, m) {
   m.def("on", [](std::vector<int64_t> size, at::Tensor like, int device) { return on(size, like.scalar_type(), device); });
-  m.def("current", [] { return current; });
+  m.def("current", [] { return met(); });
   m.def("launches", [] { auto got = launches; launches.clear(); return got; });
 }
 """
