@@ -41,7 +41,11 @@ struct Devices final : c10::impl::DeviceGuardImplInterface {
 };
 // (Another test of this process may have put its own in place; its devices do as well.)
 const bool registered = [] {
-  if (!c10::impl::hasDeviceGuardImpl(at::kCUDA)) c10::impl::DeviceGuardImplRegistrar(at::kCUDA, new Devices());
+  try {
+    c10::impl::getDeviceGuardImpl(at::kCUDA)->getDevice();
+  } catch (...) {  // the real one, which finds no device here
+    c10::impl::DeviceGuardImplRegistrar(at::kCUDA, new Devices());
+  }
   return true;
 }();
 int met() { return c10::impl::getDeviceGuardImpl(at::kCUDA)->getDevice().index(); }
