@@ -100,7 +100,7 @@ int hck_kv4_evict(void*, int64_t, int, int, const int32_t*, int64_t, int cols, c
 }
 }
 
-PYBIND11_MODULE(_stub, m) {
+PYBIND11_MODULE(_window_stub, m) {
   m.def("on", [](std::vector<int64_t> size, at::Tensor like, int device) { return on(size, like.scalar_type(), device); });
   m.def("current", [] { return met(); });
   m.def("launches", [] { auto got = launches; launches.clear(); return got; });
@@ -125,7 +125,7 @@ def stub(tmp_path_factory):
                            "-ltorch_python"], capture_output=True, text=True)
     assert done.returncode == 0, done.stderr[-3000:]
     modules = []
-    for name in ("_stub", "_window"):
+    for name in ("_window_stub", "_window"):
         spec = importlib.util.spec_from_file_location(name, so)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
