@@ -22,7 +22,7 @@ struct EvictArgs {
   int *kept, *new_lengths;
   float* new_weights;
   int64_t pages, table_stride, into_stride, w_seq, w_head;
-  int cols, heads, width, into_cols, keep, recent;
+  int cols, heads, seqs, width, into_cols, keep, recent;
   int *counts, segs;  // of long rows: Counts of each row, and its segments
 };
 
@@ -78,14 +78,14 @@ struct Row {
 template <int R>
 struct Keys {
   uint32_t key[R];
-  int first;
+  int first, rounds;  // rounds: of R, those that have places
   bool whole;  // no place's page is outside the pool, as a rule: then no place asks again
   __device__ __forceinline__ bool there(const EvictArgs& A, const Row& row, int j) const {
     return whole || row.in_pool(A, j / kPageTokens);
   }
   __device__ __forceinline__ int place(int r) const { return first + r * kSelect + (int)threadIdx.x; }
   __device__ __forceinline__ void load(const EvictArgs& A, const Row& row, int from) {
-    first = from;
+    first = from, rounds = min(R, (max(row.n - first, 0) + kSelect - 1) / kSelect);
     float w[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) w[r] = place(r) < row.last && place(r) < A.width ? row.weights[place(r)] : 0.f;
@@ -120,7 +120,7 @@ __device__ __forceinline__ void count_digit(const Keys<R>& K, int digit, uint32_
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (K.key[r] && (digit == 0 || (K.key[r] >> (shift + bits)) == prefix))
+    if (r < K.rounds && K.key[r] && (digit == 0 || (K.key[r] >> (shift + bits)) == prefix))
       atomicAdd(&bins[((K.key[r] >> shift) & ((1 << bits) - 1)) * kCopies + threadIdx.x % kCopies], 1);
   __syncthreads();
 }
@@ -156,20 +156,22 @@ __device__ __forceinline__ void write_kept(const EvictArgs& A, const Row& row, c
   auto tie = [&](int r) { return K.key[r] != 0 && K.key[r] == T; };
 #pragma unroll
   for (int r = 0; r < R; ++r) {
+    if (r >= K.rounds) break;
     const unsigned long long sures = __ballot(sure(r)), tied = __ballot(tie(r));
     if (lane == 0) s_stay[r * kSelectWaves + wave] = (int)__popcll(sures), s_tie[r * kSelectWaves + wave] = (int)__popcll(tied);
   }
   __syncthreads();
   static_assert(R * kSelectWaves <= kSelect, "a thread sums up 64 places");
-  const int e = threadIdx.x, mine = e < R * kSelectWaves ? s_tie[e] : 0;
-  int stay = e < R * kSelectWaves ? s_stay[e] : 0, all;
+  const int e = threadIdx.x, entries = K.rounds * kSelectWaves, mine = e < entries ? s_tie[e] : 0;
+  int stay = e < entries ? s_stay[e] : 0, all;
   const int rank = ties + upto_thread(mine, part, all) - mine;
   stay += max(0, min(mine, left - rank));
   const int begin = place + upto_thread(stay, part, all) - stay;
-  if (e < R * kSelectWaves) s_tie[e] = rank, s_stay[e] = begin;
+  if (e < entries) s_tie[e] = rank, s_stay[e] = begin;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
+    if (r >= K.rounds) break;
     bool stays = sure(r);
     const bool t = tie(r);
     const unsigned long long tied = __ballot(t);
@@ -187,8 +189,79 @@ __device__ __forceinline__ void write_rest(const EvictArgs& A, const Row& row, i
   if (row.line % A.heads == 0 && threadIdx.x == 0) A.new_lengths[row.seq] = total;
 }
 
-// A row of up to R * 1024 places by one workgroup.
-template <int R>
+// One head's part of target page p, by a workgroup's threads.  A place that takes no token has itself for its source: its bytes
+// stay.
+struct Sources {
+  const uint8_t* from[kPageTokens];  // one head's part of the source page
+  int place[kPageTokens];
+};
+template <int D>
+__device__ __forceinline__ void move_page(const EvictArgs& A, int b, int h, int p, Sources& S) {
+  using L = Kv4<D>;
+  const int threads = blockDim.x;
+  const int pg = A.into[b * A.into_stride + p];
+  if (pg < 0 || pg >= A.pages) return;
+  const int64_t each = (int64_t)A.heads * L::kBytes;
+  uint8_t* to = A.pool + pg * each + h * L::kBytes;
+  if (threadIdx.x < kPageTokens) {
+    const int t = threadIdx.x, i = p * kPageTokens + t;
+    const int j = i < A.keep ? A.kept[((int64_t)b * A.heads + h) * A.keep + i] : -1;
+    S.from[t] = j < 0 ? to : A.pool + A.table[b * A.table_stride + j / kPageTokens] * each + h * L::kBytes;
+    S.place[t] = j < 0 ? t : j % kPageTokens;
+  }
+  __syncthreads();
+  constexpr int kKey = D / 8;         // bytes of a token's keys that lie together
+  constexpr int kValue = L::kDpl / 2; // and of its values
+  typedef uint32_t piece __attribute__((ext_vector_type(kKey / 4)));
+  for (int w = threadIdx.x; w < kPageTokens * 4; w += threads) {  // keys: [tile][g][token]
+    const int t = (w >> 6) * 16 + (w & 15), g = (w >> 4) & 3;
+    *reinterpret_cast<piece*>(to + L::key_code(t, g * (D / 4))) =
+        *reinterpret_cast<const piece*>(S.from[t] + L::key_code(S.place[t], g * (D / 4)));
+  }
+  for (int w = threadIdx.x; w < kPageTokens * 16 * kValue / 16; w += threads) {  // values: 16 / kValue tokens of a lane (g, c)
+    const int c = w & 15, g = (w >> 4) & 3, half = w >> 6;                   // half: a block of 32 tokens, or half of one
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (kValue == 4) {
+        const int t = half * 16 + 4 * g + k;
+        x[k] = *reinterpret_cast<const uint32_t*>(S.from[t] + L::value_code(S.place[t], c));
+      } else {
+        x[k] = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = 2 * k + e, t = half * 32 + (j >> 2) * 16 + 4 * g + (j & 3);
+          x[k] |= (uint32_t)*reinterpret_cast<const uint16_t*>(S.from[t] + L::value_code(S.place[t], c)) << (16 * e);
+        }
+      }
+    }
+    const int first = kValue == 4 ? half * 16 + 4 * g : half * 32 + 4 * g;
+    *reinterpret_cast<uint4*>(to + L::value_code(first, c)) = uint4{x[0], x[1], x[2], x[3]};
+  }
+  for (int w = threadIdx.x; w < kPageTokens / 4 * L::kRuns; w += threads) {  // scales, four tokens at a time
+    const int run = w % L::kRuns, q = w / L::kRuns;
+    uint32_t ks = 0, vs = 0;
+    const int k0 = (q >> 4) * 64 + (q & 15), v0 = (q >> 3) * 32 + ((q >> 2) & 1) * 16 + (q & 3) * 4;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = k0 + 16 * k, v = v0 + k;
+      ks |= (uint32_t)S.from[t][L::key_scale(S.place[t], run)] << (8 * k);
+      vs |= (uint32_t)S.from[v][L::value_scale(S.place[v], run)] << (8 * k);
+    }
+    *reinterpret_cast<uint32_t*>(to + L::key_scale(k0, run)) = ks;
+    *reinterpret_cast<uint32_t*>(to + L::value_scale(v0, run)) = vs;
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void k_move(EvictArgs A) {
+  __shared__ Sources s_sources;
+  move_page<D>(A, blockIdx.z, blockIdx.y, blockIdx.x, s_sources);
+}
+
+// A row of up to R * 1024 places by one workgroup, which with D moves the kept tokens as well: where they are one page or two, a
+// second launch costs more than it brings (384 tokens, 256 kept and read back: 15.0 us with it, 12.9 without).
+template <int R, int D>
 __global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
   constexpr int kCopies = R >= 4 ? 8 : 1;
   __shared__ int s_bins[kBins * kCopies], s_stay[R * kSelectWaves], s_tie[R * kSelectWaves], s_part[kSelectWaves], s_found[3];
@@ -223,6 +296,20 @@ __global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
   }
   write_kept<R>(A, row, K, T, left, 0, 0, s_stay, s_tie, s_part);
   write_rest(A, row, want + must);
+  if constexpr (D != 0) {
+    __shared__ Sources s_sources;
+    for (int p = 0; p * kPageTokens < A.keep; ++p) {
+      __syncthreads();  // what was kept has been written, and the sources of the page before read
+      move_page<D>(A, blockIdx.y, blockIdx.x, p, s_sources);
+    }
+  }
+}
+
+constexpr int kMovedPages = 2;
+template <int D>
+void launch_select(const EvictArgs& A, int64_t room, hipStream_t s) {
+  auto* select = room <= 1 * kSelect ? k_select<1, D> : room <= 4 * kSelect ? k_select<4, D> : k_select<16, D>;
+  select<<<dim3(A.heads, A.seqs), kSelect, 0, s>>>(A);
 }
 
 // Longer rows, by a workgroup for every segment of 16384 places and a launch for every digit: each looks at its keys again, adds up
@@ -319,67 +406,6 @@ __global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
   }
 }
 
-// One head's part of a target page.  A place that takes no token has itself for its source: its bytes stay.
-template <int D>
-__global__ __launch_bounds__(256) void k_move(EvictArgs A) {
-  using L = Kv4<D>;
-  __shared__ const uint8_t* s_from[kPageTokens];  // one head's part of the source page
-  __shared__ int s_place[kPageTokens];
-  const int p = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int pg = A.into[b * A.into_stride + p];
-  if (pg < 0 || pg >= A.pages) return;
-  const int64_t each = (int64_t)A.heads * L::kBytes;
-  uint8_t* to = A.pool + pg * each + h * L::kBytes;
-  if (threadIdx.x < kPageTokens) {
-    const int t = threadIdx.x, i = p * kPageTokens + t;
-    const int j = i < A.keep ? A.kept[((int64_t)b * A.heads + h) * A.keep + i] : -1;
-    s_from[t] = j < 0 ? to : A.pool + A.table[b * A.table_stride + j / kPageTokens] * each + h * L::kBytes;
-    s_place[t] = j < 0 ? t : j % kPageTokens;
-  }
-  __syncthreads();
-  constexpr int kKey = D / 8;         // bytes of a token's keys that lie together
-  constexpr int kValue = L::kDpl / 2; // and of its values
-  typedef uint32_t piece __attribute__((ext_vector_type(kKey / 4)));
-  for (int w = threadIdx.x; w < kPageTokens * 4; w += 256) {  // keys: [tile][g][token]
-    const int t = (w >> 6) * 16 + (w & 15), g = (w >> 4) & 3;
-    *reinterpret_cast<piece*>(to + L::key_code(t, g * (D / 4))) =
-        *reinterpret_cast<const piece*>(s_from[t] + L::key_code(s_place[t], g * (D / 4)));
-  }
-  for (int w = threadIdx.x; w < kPageTokens * 16 * kValue / 16; w += 256) {  // values: 16 / kValue tokens of a lane (g, c)
-    const int c = w & 15, g = (w >> 4) & 3, half = w >> 6;                   // half: a block of 32 tokens, or half of one
-    uint32_t x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (kValue == 4) {
-        const int t = half * 16 + 4 * g + k;
-        x[k] = *reinterpret_cast<const uint32_t*>(s_from[t] + L::value_code(s_place[t], c));
-      } else {
-        x[k] = 0;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 2 * k + e, t = half * 32 + (j >> 2) * 16 + 4 * g + (j & 3);
-          x[k] |= (uint32_t)*reinterpret_cast<const uint16_t*>(s_from[t] + L::value_code(s_place[t], c)) << (16 * e);
-        }
-      }
-    }
-    const int first = kValue == 4 ? half * 16 + 4 * g : half * 32 + 4 * g;
-    *reinterpret_cast<uint4*>(to + L::value_code(first, c)) = uint4{x[0], x[1], x[2], x[3]};
-  }
-  for (int w = threadIdx.x; w < kPageTokens / 4 * L::kRuns; w += 256) {  // scales, four tokens at a time
-    const int run = w % L::kRuns, q = w / L::kRuns;
-    uint32_t ks = 0, vs = 0;
-    const int k0 = (q >> 4) * 64 + (q & 15), v0 = (q >> 3) * 32 + ((q >> 2) & 1) * 16 + (q & 3) * 4;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int t = k0 + 16 * k, v = v0 + k;
-      ks |= (uint32_t)s_from[t][L::key_scale(s_place[t], run)] << (8 * k);
-      vs |= (uint32_t)s_from[v][L::value_scale(s_place[v], run)] << (8 * k);
-    }
-    *reinterpret_cast<uint32_t*>(to + L::key_scale(k0, run)) = ks;
-    *reinterpret_cast<uint32_t*>(to + L::value_scale(v0, run)) = vs;
-  }
-}
-
 // Segments of a row with room for so many pages; 0: one workgroup takes it.
 int segments(int cols) {
   const int64_t room = (int64_t)cols * kPageTokens;
@@ -416,7 +442,7 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
   A.pool = (uint8_t*)pool, A.table = table, A.lengths = lengths, A.into = into, A.weights = weights;
   A.kept = kept, A.new_lengths = new_lengths, A.new_weights = new_weights;
   A.pages = pages, A.table_stride = table_stride, A.into_stride = into_stride, A.w_seq = weight_seq_stride,
-  A.w_head = weight_head_stride, A.cols = table_columns, A.heads = kv_heads, A.width = weight_places,
+  A.w_head = weight_head_stride, A.cols = table_columns, A.heads = kv_heads, A.seqs = seqs, A.width = weight_places,
   A.into_cols = into_columns, A.keep = keep, A.recent = recent;
   A.segs = hck::segments(table_columns), A.counts = (int*)workspace;
   if (A.segs > 65535) return HCK_ERR_ARG;
@@ -425,9 +451,11 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
   hipStream_t s = (hipStream_t)stream;
   // the least keys a thread for which a row goes through the registers once, as far as a table tells
   const int64_t room = (int64_t)table_columns * hck::kPageTokens;
+  const bool moved = A.segs == 0 && need <= hck::kMovedPages;
   if (A.segs == 0) {
-    auto* select = room <= 1 * hck::kSelect ? hck::k_select<1> : room <= 4 * hck::kSelect ? hck::k_select<4> : hck::k_select<16>;
-    select<<<dim3(kv_heads, seqs), hck::kSelect, 0, s>>>(A);
+    if (!moved || need == 0) hck::launch_select<0>(A, room, s);
+    else if (head_dim == 128) hck::launch_select<128>(A, room, s);
+    else hck::launch_select<64>(A, room, s);
   } else {
     const dim3 grid(kv_heads, seqs, A.segs);
     hck::k_select_long<0><<<grid, hck::kSelect, 0, s>>>(A);
@@ -436,7 +464,7 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
     hck::k_select_long<3><<<grid, hck::kSelect, 0, s>>>(A);
   }
   HCK_CHECK_LAUNCH();
-  if (need) {
+  if (need && !moved) {
     const dim3 grid((unsigned)need, kv_heads, seqs);
     if (head_dim == 128) hck::k_move<128><<<grid, 256, 0, s>>>(A);
     else hck::k_move<64><<<grid, 256, 0, s>>>(A);
