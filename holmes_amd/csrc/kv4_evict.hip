@@ -156,7 +156,7 @@ __device__ __forceinline__ void write_kept(const EvictArgs& A, const Row& row, c
   auto tie = [&](int r) { return K.key[r] != 0 && K.key[r] == T; };
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    if (r >= K.rounds) break;
+    if (r >= K.rounds) continue;
     const unsigned long long sures = __ballot(sure(r)), tied = __ballot(tie(r));
     if (lane == 0) s_stay[r * kSelectWaves + wave] = (int)__popcll(sures), s_tie[r * kSelectWaves + wave] = (int)__popcll(tied);
   }
@@ -171,7 +171,7 @@ __device__ __forceinline__ void write_kept(const EvictArgs& A, const Row& row, c
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    if (r >= K.rounds) break;
+    if (r >= K.rounds) continue;
     bool stays = sure(r);
     const bool t = tie(r);
     const unsigned long long tied = __ballot(t);
