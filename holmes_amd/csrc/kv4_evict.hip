@@ -308,14 +308,16 @@ __global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
 constexpr int kMovedPages = 2;
 template <int D>
 void launch_select(const EvictArgs& A, int64_t room, hipStream_t s) {
-  auto* select = room <= 1 * kSelect ? k_select<1, D> : room <= 4 * kSelect ? k_select<4, D> : k_select<16, D>;
+  auto* select = room <= 1 * kSelect ? k_select<1, D> : room <= 4 * kSelect ? k_select<4, D> : k_select<kWhole, D>;
   select<<<dim3(A.heads, A.seqs), kSelect, 0, s>>>(A);
 }
 
-// Longer rows, by a workgroup for every segment of 16384 places and a launch for every digit: each looks at its keys again, adds up
-// the segments' counts of the digit before, and counts the next among its own.  The last launch writes what stays, from where
-// the segments before end.
-constexpr int kSegment = 16, kSegmentPlaces = kSegment * kSelect;
+// Longer rows, by a workgroup for every segment of 8192 places and a launch for every digit: each looks at its keys again, adds
+// up the segments' counts of the digit before, and counts the next among its own.  The last launch writes what stays, from where
+// the segments before end.  8 heads of 131072 places, 8192 kept: 42 us with the move (16384 places a segment 47, 4096 43; by one
+// workgroup a row 306); of 20000 31, where one of 8000 takes 12.
+constexpr int kWhole = 16;  // thousands of places that one workgroup takes
+constexpr int kSegment = 8, kSegmentPlaces = kSegment * kSelect;
 struct Counts {  // of one row
   int *bins, *choice, *must, *above, *state;  // [digit][segment][bin], [segment], [segment], [digit < 2][segment], [digit < 2][2]
   static __host__ __device__ int64_t ints(int segs) { return (int64_t)segs * (3 * kBins + 4) + 4; }
@@ -330,8 +332,8 @@ __global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
   constexpr int R = kSegment, kCopies = PHASE == 0 ? 8 : 1;
   __shared__ int s_bins[PHASE < 3 ? kBins * kCopies : 1], s_stay[R * kSelectWaves], s_tie[R * kSelectWaves];
   __shared__ int s_part[kSelectWaves], s_found[3];
-  const int seg = blockIdx.z;
-  const Row row(A, blockIdx.y, blockIdx.x);
+  const int seg = blockIdx.x;
+  const Row row(A, blockIdx.z, blockIdx.y);
   const Counts C(A, row.line);
   const int segs = (row.n + kSegmentPlaces - 1) / kSegmentPlaces;
   if (seg >= max(segs, 1)) return;
@@ -409,7 +411,7 @@ __global__ __launch_bounds__(kSelect) void k_select_long(EvictArgs A) {
 // Segments of a row with room for so many pages; 0: one workgroup takes it.
 int segments(int cols) {
   const int64_t room = (int64_t)cols * kPageTokens;
-  return room <= kSegmentPlaces ? 0 : (int)((room + kSegmentPlaces - 1) / kSegmentPlaces);
+  return room <= kWhole * kSelect ? 0 : (int)((room + kSegmentPlaces - 1) / kSegmentPlaces);
 }
 
 }  // namespace
@@ -445,7 +447,6 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
   A.w_head = weight_head_stride, A.cols = table_columns, A.heads = kv_heads, A.seqs = seqs, A.width = weight_places,
   A.into_cols = into_columns, A.keep = keep, A.recent = recent;
   A.segs = hck::segments(table_columns), A.counts = (int*)workspace;
-  if (A.segs > 65535) return HCK_ERR_ARG;
   const size_t bytes = hck_kv4_evict_workspace_bytes(seqs, kv_heads, table_columns);
   if (bytes && (!workspace || workspace_bytes < bytes)) return HCK_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
@@ -457,7 +458,7 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
     else if (head_dim == 128) hck::launch_select<128>(A, room, s);
     else hck::launch_select<64>(A, room, s);
   } else {
-    const dim3 grid(kv_heads, seqs, A.segs);
+    const dim3 grid(A.segs, kv_heads, seqs);
     hck::k_select_long<0><<<grid, hck::kSelect, 0, s>>>(A);
     hck::k_select_long<1><<<grid, hck::kSelect, 0, s>>>(A);
     hck::k_select_long<2><<<grid, hck::kSelect, 0, s>>>(A);
