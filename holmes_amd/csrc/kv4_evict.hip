@@ -306,6 +306,7 @@ __global__ __launch_bounds__(kSelect) void k_select(EvictArgs A) {
 }
 
 constexpr int kMovedPages = 2;
+constexpr int kWhole = 16;  // places in thousands that one workgroup takes
 template <int D>
 void launch_select(const EvictArgs& A, int64_t room, hipStream_t s) {
   auto* select = room <= 1 * kSelect ? k_select<1, D> : room <= 4 * kSelect ? k_select<4, D> : k_select<kWhole, D>;
@@ -316,7 +317,6 @@ void launch_select(const EvictArgs& A, int64_t room, hipStream_t s) {
 // up the segments' counts of the digit before, and counts the next among its own.  The last launch writes what stays, from where
 // the segments before end.  8 heads of 131072 places, 8192 kept: 42 us with the move (16384 places a segment 47, 4096 43; by one
 // workgroup a row 306); of 20000 31, where one of 8000 takes 12.
-constexpr int kWhole = 16;  // thousands of places that one workgroup takes
 constexpr int kSegment = 8, kSegmentPlaces = kSegment * kSelect;
 struct Counts {  // of one row
   int *bins, *choice, *must, *above, *state;  // [digit][segment][bin], [segment], [segment], [digit < 2][segment], [digit < 2][2]
