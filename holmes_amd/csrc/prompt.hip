@@ -271,18 +271,21 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   float top = -INFINITY, sum = 0.f, low = INFINITY;
   float ref = -lift, factor = A.scale2;
 
-  // PARTLY: some of the wave's rows do not see some of the unit's tokens.
-  auto unit = [&](int u, auto PARTLY) {
+  // The unit's tokens from `skip` on: all 64 (skip 0), or, PARTLY, 32 of which some of the wave's rows do not see some.
+  auto unit = [&](int u, int skip, auto PARTLY) {
     constexpr bool kPartly = decltype(PARTLY)::value;
-    const u32x4 *ks = s_x[u & 1][0], *vs = s_x[u & 1][1];
-    const int here = u * kUnit;
-    f32x16 c[2];
+    constexpr int kX = kPartly ? 1 : 2;  // 32 tokens each
+    const u32x4 *ks = s_x[u & 1][0] + skip * S::kPieces, *vs = s_x[u & 1][1] + skip * S::kPieces;
+    const int here = u * kUnit + skip;
+    f32x16 c[kX];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) c[0][i] = c[1][i] = 0.f;
+    for (int x = 0; x < kX; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[x][i] = 0.f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < kX; ++x) {
         const vec k = __builtin_bit_cast(vec, ks[S::key_at(32 * x + (lane & 31), 2 * s + half)]);
         c[x] = mfma32(k, q[s], c[x]);
       }
@@ -298,24 +301,23 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
     }
     if constexpr (kPartly) {
-      const int base = here + 4 * half;  // of the lane's tokens base + 32 x + 8 (i / 4) + i % 4
+      const int base = here + 4 * half;  // of the lane's tokens base + 8 (i / 4) + i % 4
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool see = base + 32 * x + 8 * (i >> 2) + (i & 3) < seen;
-          if constexpr (RANGE) low = see ? fminf(low, c[x][i]) : low;
-          c[x][i] = see ? c[x][i] : -INFINITY;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const bool see = base + 8 * (i >> 2) + (i & 3) < seen;
+        if constexpr (RANGE) low = see ? fminf(low, c[0][i]) : low;
+        c[0][i] = see ? c[0][i] : -INFINITY;
+      }
     } else if constexpr (RANGE) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < kX; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) low = __builtin_elementwise_minimum(__builtin_elementwise_minimum(low, c[x][i]), c[x][i + 1]);
+        for (int i = 0; i < 16; i += 2)
+          low = __builtin_elementwise_minimum(__builtin_elementwise_minimum(low, c[x][i]), c[x][i + 1]);
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < kX; ++x)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, c[x][i]), c[x][i + 1]);
     const float raw = over_half(mx, fmax2);
@@ -364,12 +366,12 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       // is one it goes into the product as 0, and is then added to the rows that see it.
       uint32_t odd = 0;
 #pragma unroll 4
-      for (int i = 0; i < kUnit * S::kPieces / 64; ++i)
+      for (int i = 0; i < 32 * S::kPieces / 64; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd |= odd_values<T>(vs[i * 64 + lane][e]);
       if (__any(odd != 0)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2 * kX; ++j) {
           const u32x4 p = probabilities(j);
 #pragma unroll
           for (int d = 0; d < kTiles; ++d) {
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
         sum += part[0] + part[1];
         if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
 #pragma unroll 1
-        for (int t = 0; t < kUnit; ++t)
+        for (int t = 0; t < 32; ++t)
 #pragma unroll
           for (int d = 0; d < kTiles; ++d)
 #pragma unroll
@@ -399,7 +401,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2 * kX; ++j) {
       const u32x4 p = probabilities(j);
 #pragma unroll
       for (int d = 0; d < kTiles; ++d)
@@ -418,11 +420,13 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   int u = begin;
   for (; u < min(full, units); ++u) {
     next(u);
-    unit(u, std::false_type());
+    unit(u, 0, std::false_type());
   }
   for (; u < units; ++u) {
     next(u);
-    if (u * kUnit < last) unit(u, std::true_type());
+#pragma unroll 1
+    for (int skip = 0; skip < kUnit; skip += 32)
+      if (u * kUnit + skip < last) unit(u, skip, std::true_type());
   }
 
   sum = over_half(sum, [](float a, float c) { return a + c; });
