@@ -83,14 +83,15 @@ __global__ __launch_bounds__(64 * kWaves) void k_weigh_few(WeighArgs W) {
   load(u, pg);
 
   bf16x8 q[kSteps], rest[kSteps];
-  const bool live = m < R.rows;
-  const T* qp = (const T*)A.q + (R.q0 + (live ? m / A.group : 0)) * A.q_ts + (int64_t)(h * A.group + (live ? m % A.group : 0)) * A.q_hs + g * (D / 4);
+  u32x4 raw[kSteps] = {};
+  if (R.rows > 0) {  // (a lane without a row has the first one's values, which see nothing)
+    const int row = m < R.rows ? m : 0;
+    const T* qp = (const T*)A.q + (R.q0 + row / A.group) * A.q_ts + (int64_t)(h * A.group + row % A.group) * A.q_hs + g * (D / 4);
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    u32x4 raw = {0, 0, 0, 0};
-    if (live) raw = reinterpret_cast<const Loose16*>(qp + 8 * s)->v;
-    query_parts<T>(raw, q[s], rest[s]);
+    for (int s = 0; s < kSteps; ++s) raw[s] = reinterpret_cast<const Loose16*>(qp + 8 * s)->v;
   }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) query_parts<T>(raw[s], q[s], rest[s]);
   RowTerm t[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) t[r] = row_term(W, R, 4 * g + r, row_lse(W, R, h, 4 * g + r));

@@ -251,11 +251,14 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
 
   vec q[kSteps];
   const T* qp = (const T*)A.q + (first + qi) * A.q_ts + (int64_t)(h * A.group + qo) * A.q_hs + half * 8;
+  u32x4 raw[kSteps];  // (a lane without a row has the sequence's first, whose results it does not write)
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) raw[s] = *reinterpret_cast<const u32x4*>(qp + s * 16);
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    u32x4 raw = {0, 0, 0, 0};
-    if (live) raw = *reinterpret_cast<const u32x4*>(qp + s * 16);
-    q[s] = __builtin_bit_cast(vec, raw);
+    // (used here, or every unit's first product would wait for these loads, and with them for the next unit's)
+    asm volatile("" : "+v"(raw[s]));
+    q[s] = __builtin_bit_cast(vec, raw[s]);
   }
 
   // Where the lane reads: keys of token lane % 32 (and 32 on); values of the tokens 4 half + lane % 16 / 4 (and 8 on), of
