@@ -26,7 +26,6 @@ struct RowTerm {
   int seen;
 };
 __device__ __forceinline__ float row_lse(const WeighArgs& W, const Rows& R, int h, int row) {
-  if (row >= R.rows) return -INFINITY;
   return W.row_lse[(int64_t)(R.q0 + row / W.a.group) * ((int64_t)W.a.heads * W.a.group) + h * W.a.group + row % W.a.group];
 }
 __device__ __forceinline__ RowTerm row_term(const WeighArgs& W, const Rows& R, int row, float lse) {
@@ -84,17 +83,20 @@ __global__ __launch_bounds__(64 * kWaves) void k_weigh_few(WeighArgs W) {
 
   bf16x8 q[kSteps], rest[kSteps];
   u32x4 raw[kSteps] = {};
-  if (R.rows > 0) {  // (a lane without a row has the first one's values, which see nothing)
+  float lse[4] = {};
+  if (R.rows > 0) {  // (a lane without a row has the first one's values, which see nothing; loads under a condition each would wait each)
     const int row = m < R.rows ? m : 0;
     const T* qp = (const T*)A.q + (R.q0 + row / A.group) * A.q_ts + (int64_t)(h * A.group + row % A.group) * A.q_hs + g * (D / 4);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) raw[s] = reinterpret_cast<const Loose16*>(qp + 8 * s)->v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lse[r] = row_lse(W, R, h, min(4 * g + r, R.rows - 1));
   }
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) query_parts<T>(raw[s], q[s], rest[s]);
   RowTerm t[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) t[r] = row_term(W, R, 4 * g + r, row_lse(W, R, h, 4 * g + r));
+  for (int r = 0; r < 4; ++r) t[r] = row_term(W, R, 4 * g + r, 4 * g + r < R.rows ? lse[r] : -INFINITY);
 
   for (; u < u1; u += kWaves) {
     const int here = u * kUnit;
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
   };
   float lse = 0.f;
   auto terms = [&](int buf, int at) {  // one wave, whose lanes have the rows' lse
-    const RowTerm t = row_term(W, R, at + lane, lse);
+    const RowTerm t = row_term(W, R, at + lane, at + lane < to ? lse : -INFINITY);
     const int seen = at + lane < to ? t.seen : 0;
     s_off[buf][lane] = t.off, s_factor[buf][lane] = t.factor, s_seen[buf][lane] = seen;
     int least = seen;
@@ -279,7 +281,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
   float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};
   if (from < to) {
     bring(from);
-    if (wave == 0) lse = row_lse(W, R, h, from + lane);
+    if (wave == 0) lse = row_lse(W, R, h, min(from + lane, R.rows - 1));
     put(0);
     if (wave == 0) terms(0, from);
   }
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
     const bool more = at + kStage < to, mine = wave == ((at / kStage) & (kWaves - 1));
     if (more) {
       bring(at + kStage);
-      if (mine) lse = row_lse(W, R, h, at + kStage + lane);
+      if (mine) lse = row_lse(W, R, h, min(at + kStage + lane, R.rows - 1));
     }
     if (there) {
       if (here + kUnit <= __builtin_amdgcn_readfirstlane(min(s_least[buf][0], s_least[buf][1]))) stage(buf, std::false_type());
