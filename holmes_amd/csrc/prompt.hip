@@ -13,8 +13,10 @@
 // four tokens by 16 dims at a time through the transposing LDS read, at piece ^ 4 (token % 4).  What lies behind a
 // sequence's end is out of the loads' bounds and becomes zeros.
 //
-// Probabilities are rounded to the values' type for the second product (half a step each; an output's error is that of a sum of
-// rounded terms, of the size of its own rounding); l, and with it lse, is the sum of the unrounded ones.  References of the
+// Probabilities are rounded to the values' type for the second product: half a step each, so that an output's error is that of a
+// sum of rounded terms, of the size of its own rounding where there are many.  Rows of few tokens, where it would be half as
+// much again, see them in units that others of their tile see in part: there the rounding's rest goes in as well, by a second
+// product.  l, and with it lse, is the sum of the unrounded ones.  References of the
 // exponentials are multiples of 8 in units of log 2, so that going over to another is an exact power of two and seldom done.
 #include "kv4_attend.hpp"
 
@@ -188,10 +190,11 @@ __device__ __forceinline__ void write_row(const PromptArgs& A, int64_t at, int h
 }
 
 // Exponentials are taken times 2^lift.  fp16: the largest up to 2^15, so that those down to 2^-29 of it keep all bits.  bf16:
-// such that their sum over n tokens is at most 1, and no sum of values overflows.
+// such that their sum over n tokens is at most 1, and no sum of values overflows (by eights: references, which are multiples of
+// 8, stay exact to 2^27).
 template <typename T>
 __device__ __forceinline__ float lift_of(int n) {
-  return __is_same(T, _Float16) ? 15.f : (float)(__builtin_clz(n) - 32);
+  return __is_same(T, _Float16) ? 15.f : -(float)((39 - __builtin_clz(n)) / 8 * 8);
 }
 
 constexpr int kPieces(int dim) { return 1 + dim / 8; }  // of a lane in a slot
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
     // (a wave in its softmax and second product goes before one in its first, which only waits for the matrix unit: 582 -> 576 us)
     if constexpr (D == 128) __builtin_amdgcn_s_setprio(1);
     float part[2] = {0.f, 0.f};
-    auto probabilities = [&](int j) {
+    auto probabilities = [&](int j, u32x4& rest) {  // PARTLY: and what their rounding left over
       float e[8];
       u32x4 p;
 #pragma unroll
@@ -361,6 +364,12 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       for (int i = 0; i < 4; ++i) {
         p[i] = pack_as<T>(e[2 * i], e[2 * i + 1]);
         part[i & 1] += e[2 * i] + e[2 * i + 1];
+        if constexpr (kPartly) {
+          typedef T two __attribute__((ext_vector_type(2)));
+          const uint32_t w = p[i];  // (a cast of the vector's element itself would be one of its first)
+          const two near = __builtin_bit_cast(two, w);
+          rest[i] = pack_as<T>(e[2 * i] - (float)near[0], e[2 * i + 1] - (float)near[1]);
+        }
       }
       return p;
     };
@@ -375,13 +384,15 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
       if (__any(odd != 0)) {
 #pragma unroll
         for (int j = 0; j < 2 * kX; ++j) {
-          const u32x4 p = probabilities(j);
+          u32x4 rest;
+          const u32x4 p = probabilities(j, rest);
 #pragma unroll
           for (int d = 0; d < kTiles; ++d) {
             u32x4 v = values(j, d);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] &= ~((odd_values<T>(v[e]) >> 15) * 0xffffu);
             acc[d] = mfma32(__builtin_bit_cast(vec, v), __builtin_bit_cast(vec, p), acc[d]);
+            acc[d] = mfma32(__builtin_bit_cast(vec, v), __builtin_bit_cast(vec, rest), acc[d]);
           }
         }
         sum += part[0] + part[1];
@@ -405,10 +416,14 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
     }
 #pragma unroll
     for (int j = 0; j < 2 * kX; ++j) {
-      const u32x4 p = probabilities(j);
+      u32x4 rest;
+      const u32x4 p = probabilities(j, rest);
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d)
-        acc[d] = mfma32(__builtin_bit_cast(vec, values(j, d)), __builtin_bit_cast(vec, p), acc[d]);
+      for (int d = 0; d < kTiles; ++d) {
+        const vec v = __builtin_bit_cast(vec, values(j, d));
+        acc[d] = mfma32(v, __builtin_bit_cast(vec, p), acc[d]);
+        if constexpr (kPartly) acc[d] = mfma32(v, __builtin_bit_cast(vec, rest), acc[d]);
+      }
     }
     sum += part[0] + part[1];
     if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
