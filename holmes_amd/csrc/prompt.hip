@@ -164,9 +164,10 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 }
 // 16 bytes for each lane from base + off into LDS, lane after lane from `to` on; zeros for what is out of the bounds.
 // Written out, because the compiler waits for such loads before any transposing read; whoever issues them waits with
-// all_loaded().  (m0 holds the address, a wait state ahead of its use.)
+// all_loaded().  (m0 holds the address, a wait state ahead of its use; the bounds' registers may have been written by a vector
+// instruction, five ahead.)
 __device__ __forceinline__ void load_lds(uint32_t to, uint32_t off, rsrc_t from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(from) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(from) : "memory", "m0");
 }
 __device__ __forceinline__ void all_loaded() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ rsrc_t bounds(const char* base, int bytes) {

@@ -10,10 +10,13 @@
 // sine and cosine are their Taylor polynomials there (terms up to x^9 and x^10: off by less than 2^-26).
 //
 // Bound by the bytes.  A workgroup takes all heads of a few tokens, so that each angle is made once, into LDS, for queries
-// and keys together.  32768 tokens, 32 query heads and 8 key heads of 128 in bf16, 671 MB: 126 us, 5.3 TB/s (a large copy
-// reaches 5.1); one token 2.7 us, of a call's 5.
+// and keys together.  32768 tokens, 32 query heads and 8 key heads of 128 in bf16, 671 MB: 108 us, 6.2 TB/s (a large copy
+// through the caches reaches 5.1); one token 2.7 us, of a call's 5.
 #include "../../include/holmes_ckks.h"
 #include "internal.hpp"
+#include "kv4.hpp"
+
+#include <algorithm>
 
 namespace hck {
 namespace {
@@ -53,20 +56,25 @@ __device__ __forceinline__ float2 turned_by(uint64_t t) {
 template <typename T, int V>
 struct Some {
   T v[V];
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  template <bool PAST>
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (V * sizeof(T) == 16) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      const u32x4* at = reinterpret_cast<const u32x4*>(p);
+      const u32x4 w = PAST ? __builtin_nontemporal_load(at) : *at;
       __builtin_memcpy(v, &w, 16);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = p[i];
     }
   }
+  template <bool PAST>
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (V * sizeof(T) == 16) {
-      uint4 w;
+      u32x4 w;
       __builtin_memcpy(&w, v, 16);
-      *reinterpret_cast<uint4*>(p) = w;
+      if constexpr (PAST) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+      else *reinterpret_cast<u32x4*>(p) = w;
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) p[i] = v[i];
@@ -74,7 +82,9 @@ struct Some {
   }
 };
 
-template <typename T, int V, bool INTERLEAVED>
+// PAST: more is written than the L2 caches hold; loads and stores go past them (32768 tokens: 108 us; the stores alone 110, through
+// the caches 114).
+template <typename T, int V, bool INTERLEAVED, bool PAST>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs A) {
   __shared__ float2 s_turn[kAngles];
   const int64_t first = (int64_t)blockIdx.x * A.per;
@@ -102,14 +112,14 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs A) {
     Some<T, V> a, b;
     if ((int)u >= A.turned) {  // behind the pairs
       const int d = 2 * A.pairs + ((int)u - A.turned) * V;
-      a.load(x + d);
-      a.store(y + d);
+      a.template load<PAST>(x + d);
+      a.template store<PAST>(y + d);
       continue;
     }
     const float2* turn = s_turn + i * A.pairs;
     if constexpr (INTERLEAVED) {
       const int d = (int)u * V;
-      a.load(x + d);
+      a.template load<PAST>(x + d);
 #pragma unroll
       for (int k = 0; k < V; k += 2) {
         const float2 cs = turn[(d + k) / 2];
@@ -117,11 +127,11 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs A) {
         a.v[k] = (T)(p * cs.x - q * cs.y);
         a.v[k + 1] = (T)(q * cs.x + p * cs.y);
       }
-      a.store(y + d);
+      a.template store<PAST>(y + d);
     } else {
       const int d = (int)u * V;
-      a.load(x + d);
-      b.load(x + A.pairs + d);
+      a.template load<PAST>(x + d);
+      b.template load<PAST>(x + A.pairs + d);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const float2 cs = turn[d + k];
@@ -129,8 +139,8 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs A) {
         a.v[k] = (T)(p * cs.x - q * cs.y);
         b.v[k] = (T)(q * cs.x + p * cs.y);
       }
-      a.store(y + d);
-      b.store(y + A.pairs + d);
+      a.template store<PAST>(y + d);
+      b.template store<PAST>(y + A.pairs + d);
     }
   }
 }
@@ -152,19 +162,23 @@ int launch(RotaryArgs A, int rotated, bool interleaved, hipStream_t s) {
   A.units = A.turned + (A.dim - rotated) / v;
   const int heads = A.heads[0] + A.heads[1];
   A.by_units = inverse_of(A.units), A.by_heads = inverse_of(heads);
-  // tokens of a workgroup: some 1024 units, what the angles have room for, and no more than leave 1024 workgroups
-  const int64_t many = 1024 / ((int64_t)heads * A.units) + 1;
+  // tokens of a workgroup: up to 600 units (32768 tokens of 320 units: one 113 us, two 120, four 126; 6001 of 144: two 8.8, four
+  // 8.0, five 8.1), what the angles have room for, and no more than leave 1024 workgroups
+  const int64_t many = 600 / ((int64_t)heads * A.units);
   A.per = (int)std::max<int64_t>(1, std::min({many, (int64_t)kAngles / A.pairs, A.tokens / 1024}));
   if ((int64_t)A.per * heads * A.units >= 1 << 16 && A.per > 1) A.per = 1;
   const int64_t groups = (A.tokens + A.per - 1) / A.per;
   if (groups > 0x7fffffff) return HCK_ERR_ARG;
   const dim3 grid((unsigned)groups);
+  const bool past = wide && A.tokens * heads * A.dim * (int64_t)sizeof(T) > kL2s;
   if (interleaved) {
-    if (wide) k_rotary<T, kWide, true><<<grid, kThreads, 0, s>>>(A);
-    else k_rotary<T, 2, true><<<grid, kThreads, 0, s>>>(A);
+    if (past) k_rotary<T, kWide, true, true><<<grid, kThreads, 0, s>>>(A);
+    else if (wide) k_rotary<T, kWide, true, false><<<grid, kThreads, 0, s>>>(A);
+    else k_rotary<T, 2, true, false><<<grid, kThreads, 0, s>>>(A);
   } else {
-    if (wide) k_rotary<T, kWide, false><<<grid, kThreads, 0, s>>>(A);
-    else k_rotary<T, 1, false><<<grid, kThreads, 0, s>>>(A);
+    if (past) k_rotary<T, kWide, false, true><<<grid, kThreads, 0, s>>>(A);
+    else if (wide) k_rotary<T, kWide, false, false><<<grid, kThreads, 0, s>>>(A);
+    else k_rotary<T, 1, false, false><<<grid, kThreads, 0, s>>>(A);
   }
   HCK_CHECK_LAUNCH();
   return HCK_OK;

@@ -109,6 +109,25 @@ def test_strides_and_odd_values():
     assert b.shape == (3, 0, 64)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_more_than_the_caches_hold(interleaved, kind):
+    """Large calls, which go past the caches, give what their tokens do in small ones."""
+    from holmes_amd import clear
+
+    print("large", interleaved, kind, flush=True)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    plan = clear.RotaryPositions(128, rotated=96, interleaved=interleaved)
+    positions = torch.arange(3500, device="cuda") * 7
+    q = torch.randn((3500, 32, 128), generator=g, device="cuda").to(TYPES[kind])
+    k = torch.randn((3500, 8, 128), generator=g, device="cuda").to(TYPES[kind])
+    a, b = plan.rotate(positions, q, k)
+    check(plan, positions[::500], q[::500], a[::500].contiguous())
+    for i in range(0, 3500, 500):
+        c, d = plan.rotate(positions[i:i + 500], q[i:i + 500], k[i:i + 500])
+        assert torch.equal(a[i:i + 500], c) and torch.equal(b[i:i + 500], d)
+
+
 def test_back_and_forth_and_the_encrypted_layers_phases():
     """The default plan is DecodeSpec's embedding: its phases in 32 bits are off by the angle's rounding there."""
     from holmes_amd import clear
