@@ -159,8 +159,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_weigh_many(WeighArgs W) {
   constexpr bool kHalf = __is_same(T, _Float16);
   constexpr int kParts = kHalf ? 2 : 1;
   __shared__ u32x4 s_q[2][kParts][kStage * kPieces];
-  __shared__ float s_off[2][kStage], s_factor[2][kStage];
-  __shared__ int s_seen[2][kStage], s_least[2][2];
+  __shared__ alignas(16) float s_off[2][kStage], s_factor[2][kStage];
+  __shared__ alignas(16) int s_seen[2][kStage];
+  __shared__ int s_least[2][2];
   const AttendArgs& A = W.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, half = lane >> 5;
   // (the tokens that most rows see first)

@@ -20,7 +20,7 @@
 //
 // What bounds it: per 64 tokens and 32 rows 32 matrix instructions (1024 of the SIMD's cycles at D = 128) and some 150 vector ones, 32 of
 // them exponentials (730), of two waves that share a SIMD.  8192 tokens, 32 query heads over 8 key heads of 128, bf16: 555 GFLOP in
-// 540 to 562 us on different cards, 0.99 to 1.03 PFLOP/s at the 1.95 GHz that the clock falls to; a bf16 8192^3 product runs at 1.23.  References of the
+// 541 to 567 us on different cards, 0.98 to 1.03 PFLOP/s at the 1.95 GHz that the clock falls to; a bf16 8192^3 product runs at 1.23.  References of the
 // exponentials are multiples of 8 in units of log 2, so that going over to another is an exact power of two and seldom done.
 #include "kv4_attend.hpp"
 
