@@ -37,6 +37,19 @@ __device__ __forceinline__ RowTerm row_term(const WeighArgs& W, const Rows& R, i
   return r;
 }
 
+// Sums over pairs of lanes LANES apart, of a in the first of each two groups of so many lanes, of b in the second.
+template <int LANES>
+__device__ __forceinline__ float beside(float a, float b) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  if constexpr (LANES == 32) {
+    const auto p = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  } else {
+    const auto p = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+}
+
 // Up to 16 rows: a wave takes units of 64 tokens in turn, the next one's keys in flight, with the rows' operands and terms in its
 // registers throughout.  The product's 16 rows are the left operand, so a lane has one token of each 16 and four of its rows.
 // Bound by the keys' bytes: 32 histories of 2000 to 24576 tokens, 8 key heads of 128, 178 MB with the weights, 40 us, 4.4 TB/s; with
@@ -114,6 +127,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_weigh_few(WeighArgs W) {
     if (u + 2 * kWaves < u1) next = table[(u + 2 * kWaves) >> 1];
     if (u + kWaves < u1 && here + kWaves * kUnit < R.length) load(u + kWaves, pg);
     if (seen) {
+      float part[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t byte = (bytes >> (8 * i)) & 0xffu;
@@ -131,9 +145,10 @@ __global__ __launch_bounds__(64 * kWaves) void k_weigh_few(WeighArgs W) {
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], W.scale2, -t[r].off));
           sum = __builtin_fmaf(here + 16 * i + m < t[r].seen ? p : 0.f, t[r].factor, sum);
         }
-        sum = over_g(sum, [](float a, float c) { return a + c; });
-        if (g == i) total += sum;
+        part[i] = sum;
       }
+      // over the four lanes of a token, and lane (m, g) gets token 16 g + m: the halves' sums of two 16s side by side, then the 16s'
+      total += beside<16>(beside<32>(part[0], part[2]), beside<32>(part[1], part[3]));
     }
     to[here] = here + lane < R.length ? total : 0.f;
   }
