@@ -202,8 +202,8 @@ class ClearKVPages:
         """What the attention of ``queries`` has given each cached token: the sum of exp(score - lse) over the rows that
         see it, of the queries of one key head, [sequences][kv_heads][columns * 128] float32.  The arguments are
         ``attend``'s, and ``lse`` is what it returned for them (a row of -inf gives nothing).  ``prior`` [sequences][kv_heads][places], what
-        earlier calls gave, is added, as 0 where it has no place; places behind a sequence's end are 0.  Without
-        ``causal`` and ``most`` as for ``attend``."""
+        earlier calls gave, is added, as 0 where it has no place; places behind a sequence's end are 0.  (``most`` saves
+        more here than there: sequences of few queries each are taken another way than prompts.)"""
 
         got = self._more.weigh(self.buf, *self._shape, queries, table, lengths, lse, starts, most, causal, scale, prior)
         if type(got) is int:
@@ -239,8 +239,8 @@ def _rotary_frequencies(rotated: int, base: float, scaling: RotaryScaling | None
     if scaling is None:
         return plain(base), 1.0
     kind, factor, original, low, high = scaling
-    if not (factor >= 1.0 and math.isfinite(factor)):
-        raise ValueError("the factor of a scaling must be finite, and 1 at least")
+    if not 1.0 <= factor <= 1 << 20:
+        raise ValueError("the factor of a scaling must be in 1..2^20")
     if kind == "linear":
         return [f / factor for f in plain(base)], 1.0
     if kind == "base":
@@ -249,8 +249,8 @@ def _rotary_frequencies(rotated: int, base: float, scaling: RotaryScaling | None
         return plain(base * factor ** (rotated / (rotated - 2))), 1.0
     if kind not in ("wavelength", "ramp"):
         raise ValueError('the kind of a scaling must be "linear", "base", "wavelength" or "ramp"')
-    if not (original >= 1 and 0.0 < low < high and math.isfinite(high)):
-        raise ValueError("a blended scaling needs original >= 1 and 0 < low < high")
+    if not (1 <= original < math.inf and 0.0 < low < high < math.inf):
+        raise ValueError("a blended scaling needs original >= 1 and 0 < low < high, all finite")
 
     if kind == "wavelength":
         def whole(i, f):
@@ -287,8 +287,8 @@ class RotaryPositions:
             raise ValueError(f"head_dim must be even, in 2..{nat.HCK_ROTARY_MAX}")
         if not 2 <= rotated <= head_dim or rotated % 2:
             raise ValueError("rotated must be even, in 2..head_dim")
-        if not (0.0 < base < math.inf):
-            raise ValueError("base must be positive")
+        if not 1.0 <= base <= 1e30:
+            raise ValueError("base must be in 1..1e30")
         self.frequencies, self.amount = _rotary_frequencies(rotated, float(base), scaling)
         if torch.device(device).type != "cuda" or not torch.cuda.is_available():
             raise RuntimeError("positions are rotated on a GPU: there is no CPU path")

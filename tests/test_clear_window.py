@@ -49,7 +49,8 @@ def test_blended_frequencies():
 @pytest.mark.parametrize("change,match", [
     (dict(head_dim=0), "head_dim"), (dict(head_dim=63), "head_dim"), (dict(head_dim=514), "head_dim"),
     (dict(rotated=130), "rotated"), (dict(rotated=0), "rotated"), (dict(rotated=3), "rotated"),
-    (dict(base=0.0), "base"), (dict(base=-1.0), "base"), (dict(base=math.nan), "base"), (dict(base=math.inf), "base"),
+    (dict(base=0.0), "base"), (dict(base=5e-324), "base"), (dict(base=1e300), "base"), (dict(base=-1.0), "base"),
+    (dict(scaling=clear.RotaryScaling("base", 1e300), rotated=4), "factor"), (dict(scaling=clear.RotaryScaling("ramp", 2.0, math.inf)), "blended"), (dict(base=math.nan), "base"), (dict(base=math.inf), "base"),
     (dict(scaling=clear.RotaryScaling("none", 2.0)), "kind"), (dict(scaling=clear.RotaryScaling("linear", 0.5)), "factor"),
     (dict(scaling=clear.RotaryScaling("linear", math.nan)), "factor"), (dict(rotated=2, scaling=clear.RotaryScaling("base", 2.0)), "pairs"),
     (dict(scaling=clear.RotaryScaling("wavelength", 2.0, 0)), "blended"),
