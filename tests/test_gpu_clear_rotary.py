@@ -50,7 +50,7 @@ def check(plan, positions, x, got, sign=1.0):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dim,rotated,heads,kv_heads,tokens", [
     (128, 128, 32, 8, 1), (128, 64, 5, 1, 7), (64, 32, 3, 3, 33), (64, 6, 1, 2, 5), (10, 6, 2, 1, 9), (512, 512, 2, 1, 3),
-    (2, 2, 1, 1, 1), (96, 48, 3, 1, 1030)])
+    (2, 2, 1, 1, 1), (96, 48, 3, 1, 1030), (64, 16, 2, 1, 4101)])
 def test_rotate(dim, rotated, heads, kv_heads, tokens, interleaved, kind):
     from holmes_amd import clear
 

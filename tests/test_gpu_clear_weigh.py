@@ -70,6 +70,39 @@ def test_single_tokens(heads, group, dim, kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads,group,dim,causal", [(2, 4, 128, True), (1, 5, 64, True), (2, 1, 128, False), (1, 3, 64, False)])
+def test_few_queries_each(heads, group, dim, causal, kind):
+    """Up to 16 rows of several queries: some see a part of a unit, some sequences have fewer queries than others, or none."""
+    print("few", heads, group, dim, causal, kind, flush=True)
+    g = torch.Generator().manual_seed(heads * 7 + group)
+    seqs, counts = [3, 64, 130, 1, 65, 257, 0, 700], [3, 2, 3, 1, 0, 3, 2, 3]
+    pool, table, keys, _ = build(seqs, heads, dim, g)
+    q = torch.randn((sum(counts), heads * group, dim), generator=g).to(TYPES[kind]).cuda()
+    lengths = torch.tensor(seqs, dtype=torch.int32).cuda()
+    lse = pool.attend(q, table, lengths, starts=starts_of(counts), most=3, causal=causal).lse
+    got = pool.weigh(q, table, lengths, lse, starts=starts_of(counts), most=3, causal=causal)
+    check(got, q, keys, lse, counts, group, causal=causal)
+
+
+def test_units_in_turn():
+    """A table with room for so much that a wave takes several units of 64 tokens, and most of them are behind the end."""
+    print("turns", flush=True)
+    g = torch.Generator().manual_seed(17)
+    seqs, heads, group = [1, 2, 63, 64, 65, 127, 128, 129, 700, 0, 256, 1300], 2, 3
+    pool, table, keys, _ = build(seqs, heads, 128, g)
+    q = torch.randn((len(seqs), heads * group, 128), generator=g).to(torch.bfloat16).cuda()
+    lengths = torch.tensor(seqs, dtype=torch.int32).cuda()
+    lse = pool.attend(q, table, lengths).lse
+    prior = torch.rand((len(seqs), heads, 1100), generator=g).cuda()
+    there = [torch.ones(n, dtype=torch.bool) for n in seqs]
+    there[11][256:384] = False
+    table = widen(table, 700)
+    table[11, 2] = -1
+    got = pool.weigh(q, table, lengths, lse, prior=prior)
+    check(got, q, keys, lse, [1] * len(seqs), group, prior=prior, there=there)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
 @pytest.mark.parametrize("heads,group,dim,causal,most", [(2, 4, 128, True, 300), (1, 7, 64, False, 300), (3, 1, 128, True, None),
                                                          (2, 3, 64, True, 333)])
 def test_many_rows(heads, group, dim, causal, most, kind):
