@@ -32,7 +32,6 @@ from __future__ import annotations
 import importlib.util
 import math
 import sys
-from fractions import Fraction
 from typing import NamedTuple
 
 import torch
@@ -226,8 +225,14 @@ class ClearKVPages:
         return Evicted._make(got)
 
 
-# pi to 180 bits
-_PI = Fraction(0x3243F6A8885A308D313198A2E03707344A4093822299F3, 1 << 180)
+_PI = 0x3243F6A8885A308D313198A2E03707344A4093822299F3   # times 2^-180
+
+
+def _turns(frequency: float) -> int:
+    """Radians per token as turns per token in units of 2^-64, modulo a turn."""
+
+    n, d = frequency.as_integer_ratio()
+    return ((n << 244) // (d * _PI) + 1 >> 1) % (1 << 64)
 
 
 def _rotary_frequencies(rotated: int, base: float, scaling: RotaryScaling | None) -> tuple:
@@ -294,7 +299,7 @@ class RotaryPositions:
             raise RuntimeError("positions are rotated on a GPU: there is no CPU path")
         self.head_dim, self.rotated, self.interleaved = int(head_dim), int(rotated), bool(interleaved)
         # turns per token in units of 2^-64: position times that, modulo 2^64, is the angle's part of a turn
-        turns = [round(Fraction(f) * (1 << 63) / _PI) % (1 << 64) for f in self.frequencies]
+        turns = map(_turns, self.frequencies)
         self._turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
         self._native = _window()
 

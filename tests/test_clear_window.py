@@ -3,6 +3,7 @@ launched (no GPU needed: every call here is refused for an argument, at the late
 
 import ctypes
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -25,6 +26,14 @@ def test_frequencies():
     got, _ = clear._rotary_frequencies(8, 10000.0, clear.RotaryScaling("base", 4.0))
     assert got[0] == 1.0 and got[3] == pytest.approx(0.001 / 4, rel=1e-13)
     assert got[1] / got[0] == pytest.approx(got[3] / got[2], rel=1e-13)
+
+
+def test_turns():
+    """Nearest multiples of 2^-64 turns, against 80 digits of pi."""
+    turn = 2 * Fraction(31415926535897932384626433832795028841971693993751058209749445923078164062862089, 10**79)
+    for f in [1.0, 0.1, 500000.0**-0.75, 1e-30, 0.0, 6.283185307179586, 3.0, *clear._rotary_frequencies(128, 500000.0, None)[0]]:
+        want = Fraction(f) / turn * 2**64
+        assert abs((clear._turns(f) - want + 2**63) % 2**64 - 2**63) <= Fraction(1, 2) + Fraction(1, 10**9), f
 
 
 def test_blended_frequencies():
