@@ -324,7 +324,7 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     16 bytes cannot be loaded from at a time are copied first; query heads a multiple of kv_heads, neighbours sharing a key head).
 
     Sequence b is the tokens ``starts[b] .. starts[b + 1]`` (int32 [sequences + 1], not decreasing; without ``starts`` there
-    is one of all tokens), and query i of it sees its tokens up to i, or, with ``causal`` off, all.  ``most`` bounds the tokens
+    is one of all tokens), and query i of it sees its tokens up to i, or, with ``causal`` off, all.  ``most`` bounds the queries
     of one sequence (default: all) and only saves work; a longer one has the rest left unwritten, as has any row that no sequence
     covers.  ``scale`` and ``ranges`` as for ``ClearKVPages.attend``: the ranges here are those of keys that nothing has
     rounded, so ``softmax_ranges`` needs no ``rounding`` for them."""

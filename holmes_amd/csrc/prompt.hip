@@ -22,12 +22,10 @@
 // them exponentials (730), of two waves that share a SIMD.  8192 tokens, 32 query heads over 8 key heads of 128, bf16: 555 GFLOP in
 // 541 to 567 us on different cards, 0.98 to 1.03 PFLOP/s at the 1.95 GHz that the clock falls to; a bf16 8192^3 product runs at 1.23.  References of the
 // exponentials are multiples of 8 in units of log 2, so that going over to another is an exact power of two and seldom done.
-#include "kv4_attend.hpp"
+#include "prompt_way.hpp"
 
 namespace hck {
 namespace {
-
-constexpr int kRowsOfWave = 32, kPromptWaves = 4, kTileRows = kRowsOfWave * kPromptWaves;
 
 struct PromptArgs {
   const void *q, *k, *v;
@@ -202,7 +200,6 @@ __device__ __forceinline__ float lift_of(int n) {
   return __is_same(T, _Float16) ? 15.f : -(float)((39 - __builtin_clz(n)) / 8 * 8);
 }
 
-constexpr int kPieces(int dim) { return 1 + dim / 8; }  // of a lane in a slot
 __device__ __forceinline__ f32x4* slot_of(const PromptArgs& A, int item, int part, int h, int wave, int dim) {
   return A.slots + (((int64_t)item * A.parts + part) * A.heads + h) * (kPromptWaves * 64 * kPieces(dim)) + wave * 64 * kPieces(dim) +
          (threadIdx.x & 63);
@@ -227,7 +224,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_whole(PromptArgs A) {
   const int64_t first = t.first;
   auto sees = [&](int row) { return A.causal ? row / A.group + 1 : n; };
   const int most = sees(min(tile * kTileRows + kTileRows, rows) - 1);
-  const int all = (most + kUnit - 1) / kUnit, begin = SPLIT ? part * A.part : 0, units = SPLIT ? min(all, begin + A.part) : all;
+  const int all = (most + kUnit - 1) / kUnit, begin = SPLIT ? part * A.part : 0;
+  const int units = SPLIT ? part_end(all, A.part, A.parts, part) : all;
   if (SPLIT && part && begin >= all) return;
   const int mine = tile * kTileRows + wave * kRowsOfWave;
   const int last = mine < rows ? sees(min(mine + kRowsOfWave, rows) - 1) : 0;
@@ -477,7 +475,7 @@ __global__ __launch_bounds__(64 * kPromptWaves) void k_whole_join(PromptArgs A) 
   if (!locate_tile(A, item, t)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int end = min(t.tile * kTileRows + kTileRows, t.rows) - 1;
-  const int all = ((A.causal ? end / A.group + 1 : t.n) + kUnit - 1) / kUnit, parts = (all + A.part - 1) / A.part;
+  const int all = ((A.causal ? end / A.group + 1 : t.n) + kUnit - 1) / kUnit, parts = parts_of(all, A.part, A.parts);
   const int row = t.tile * kTileRows + wave * kRowsOfWave + (lane & 31);
   if (parts <= 1 || row >= t.rows) return;
   const int64_t apart = (int64_t)A.heads * (kPromptWaves * 64 * kPieces(D));
@@ -499,32 +497,6 @@ __global__ __launch_bounds__(64 * kPromptWaves) void k_whole_join(PromptArgs A) 
   write_row<T, D, RANGE>(A, (t.first + row / A.group) * (int64_t)(A.heads * A.group) + h * A.group + row % A.group, half, top, sum, low,
                          lift_of<T>(t.n), [&](int d, int i) { return acc[4 * d + i]; });
 }
-
-// How a call is run, from what the host knows of it.
-struct WholeWay {
-  int64_t items;
-  int tiles, part, parts;
-  WholeWay(int64_t tokens, int64_t seqs, int heads, int group, int most, bool causal) {
-    tiles = (int)(((int64_t)most * group + kTileRows - 1) / kTileRows);
-    // every sequence has a tile that may not be full, beside the full ones
-    items = std::min((int64_t)tiles * seqs, tokens * group / kTileRows + seqs);
-    // Few tiles of long sequences are cut into parts, as many as run at once and no more: of the tiles of one sequence with
-    // `causal` that is longest / 2 / part + 1 / 2 for each; of several, whose lengths the host does not know, half as many parts
-    // are reckoned with.  A part costs its sums' way through memory and the join some 5 us, which
-    // is what 8 units take (one sequence, 128 dims, whole and in parts: 4000 tokens, 6 heads over 2, 85 and 53 us; 6000, 8 over
-    // 4, 144 and 105; 2000, 32 over 8, in more parts than run at once, 53 and 72).
-    const int64_t longest = ((int64_t)most + kUnit - 1) / kUnit, each = items * heads;
-    int64_t units = longest;
-    if (causal && 2 * kSlots > each) units = (longest / (seqs > 1 ? 2 : 1) * each + 2 * kSlots - each - 1) / (2 * kSlots - each);
-    if (!causal && kSlots > each) units = (longest + kSlots / each - 1) / (kSlots / each);
-    part = (int)std::min(longest, std::max<int64_t>(kLeast, units));
-    parts = longest > part + kJoin ? (int)((longest + part - 1) / part) : 1;
-  }
-  size_t bytes(int heads, int dim) const {
-    return parts > 1 ? (size_t)items * parts * heads * (kPromptWaves * 64 * kPieces(dim)) * sizeof(f32x4) : 0;
-  }
-  static constexpr int kSlots = 2 * kComputeUnits, kLeast = 8, kJoin = 8;
-};
 
 template <typename T, int D>
 int launch(const PromptArgs& A, const WholeWay& way, hipStream_t s) {

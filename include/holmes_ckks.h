@@ -492,9 +492,9 @@ int hck_rotary(const void* positions, int position_bytes, int64_t tokens, const 
 /* Attention of whole prompts: sequence b is the tokens starts[b] .. starts[b + 1] (device, not decreasing; starts NULL: one
  * sequence of all tokens) of queries [tokens][kv_heads * group][head_dim] and keys and values [tokens][kv_heads][head_dim],
  * all bf16 or all fp16, and its queries see its tokens up to their own (with `causal` 0: all of them).  Element strides,
- * multiples of 8, from 16-byte aligned addresses; tokens of keys and values lie head_dim to 2^23 elements apart.  `most` is at
- * least the largest number of tokens of a sequence.  out, lse, low, high and scale are as for hck_kv4_attend; a token that no
- * sequence covers is left unwritten. */
+ * multiples of 8, from 16-byte aligned addresses; tokens of keys and values lie head_dim to 2^23 elements apart.  Of each sequence
+ * the first `most` queries are taken.  out, lse, low, high and scale are as for hck_kv4_attend; the other queries of a longer
+ * sequence, and tokens that no sequence covers, are left unwritten. */
 size_t hck_prompt_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim, int most, int causal);
 int hck_prompt_attend(const void* queries, const void* keys, const void* values, int type, int64_t tokens, int kv_heads,
                       int group, int head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
