@@ -200,7 +200,9 @@ class ClearKVPages:
               scale: float | None = None, prior: torch.Tensor | None = None) -> torch.Tensor:
         """What the attention of ``queries`` has given each cached token: the sum of exp(score - lse) over the rows that
         see it, of the queries of one key head, [sequences][kv_heads][columns * 128] float32.  The arguments are
-        ``attend``'s, and ``lse`` is what it returned for them (a row of -inf gives nothing).  ``prior`` [sequences][kv_heads][places], what
+        ``attend``'s, and ``lse`` is what it returned for them (a row of -inf gives nothing).  Half a step of its 32 bits is a factor of
+        exp(|lse| 2^-24) to all that a row gives: rows with scores beyond some 2^22 give their tokens an order rather than shares.
+        ``prior`` [sequences][kv_heads][places], what
         earlier calls gave, is added, as 0 where it has no place; places behind a sequence's end are 0.  (``most`` saves
         more here than there: sequences of few queries each are taken another way than prompts.)"""
 

@@ -19,8 +19,10 @@ struct WeighArgs {
   float scale2, rest;  // scale log2 e in 32 bits, and what its rounding left over, divided by scale
 };
 
-// A row's share of the exponents: what comes off, in units of log 2, and a factor near 1 for what rounding took from
-// that and from scale log2 e (counted where the score is the row's lse, near which weights are large).
+// A row's share of the exponents: what comes off, in units of log 2, and a factor, near 1 for scores of ordinary size, for what
+// rounding took from that and from scale log2 e (counted where the score is the row's lse, near which weights are large).  Its
+// exponent is within 38 up to |lse| = 2^28, and kept within 64 beyond, where half a step of lse itself is e^16 or more: so
+// that no row's share is negative, or 0 times an infinity.
 struct RowTerm {
   float off, factor;
   int seen;
@@ -32,7 +34,7 @@ __device__ __forceinline__ RowTerm row_term(const WeighArgs& W, const Rows& R, i
   RowTerm r = {lse * kLog2e, 1.f, lse == -INFINITY ? 0 : R.seen(W.a, row)};  // a row of -inf gave nothing
   if (fabsf(lse) < INFINITY) {
     const float low = __builtin_fmaf(lse, kLog2e, -r.off) + lse * 1.9259629911266174e-8f;  // (log2 e in two parts)
-    r.factor = 1.f + kLn2 * (lse * W.rest - low);
+    r.factor = __builtin_amdgcn_exp2f(fminf(fmaxf(lse * W.rest - low, -64.f), 64.f));
   }
   return r;
 }
