@@ -24,7 +24,8 @@ off by more than half a step (a step of 2 above 4; magnitudes beyond 7 2^125 bec
 
 Everything but ``softmax_ranges`` and ``score_rounding`` runs in libholmes_ckks on the current stream of its
 tensors' device without synchronising; there is no CPU path.
-Nothing has a backward pass: an input that requires a gradient is refused, but under ``torch.no_grad()``.
+Nothing has a backward pass: an input that requires a gradient is refused, but under ``torch.no_grad()``; nor has anything a
+forward-mode derivative: an input with a tangent is refused.
 """
 
 from __future__ import annotations

@@ -5,6 +5,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
@@ -39,10 +40,12 @@ const Tensor& tensor(PyObject* o, const char* name) {
   return THPVariable_Unpack(o);
 }
 
-// Nothing here has a backward pass, and a result without one would pass for a constant.
+// Nothing here has a backward pass, nor a forward one, and a result without one would pass for a constant.
 void no_gradient(const Tensor& t, const char* name) {
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse(std::string(name) + " require a gradient, which this call does not have: detach them, or call it under torch.no_grad()");
+  if (t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    refuse(std::string(name) + " have a tangent (forward-mode derivatives), which this call does not pass on: detach them");
 }
 
 long long whole(PyObject* o) {
