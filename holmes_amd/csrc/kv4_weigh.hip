@@ -166,6 +166,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_weigh_few(WeighArgs W) {
 // What bounds it: per 64 rows and 64 tokens 32 matrix instructions (1024 cycles) and 192 vector ones, 64 of them exponentials (1024), and a
 // barrier.  4096 tokens and queries, 32 query heads over 8 key heads of 128: 70 GFLOP in 88 us and 5 for the join, 750 TFLOP/s.
 constexpr int kStage = 64, kBlock = kUnit * kWaves;  // rows at a time, tokens of a workgroup
+constexpr int kMostRows = INT32_MAX - 256;            // of a sequence and key head: whole stages are counted in 31 bits
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -405,7 +406,7 @@ int launch(const WeighArgs& W, const WeighWay& way, hipStream_t s) {
 extern "C" size_t hck_kv4_weigh_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int most,
                                                 int table_columns) {
   if (tokens <= 0 || seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 65535 || group < 1 || most < 0 ||
-      table_columns < 1 || table_columns >= 1 << 23 || (int64_t)most * group > INT32_MAX)
+      table_columns < 1 || table_columns >= 1 << 23 || (int64_t)most * group > hck::kMostRows)
     return 0;
   return hck::WeighWay(seqs, kv_heads, group, (int)std::min<int64_t>(most, tokens), table_columns).bytes(seqs, kv_heads, table_columns);
 }
@@ -418,7 +419,7 @@ extern "C" int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int 
   if (hck::kv4_bytes(head_dim) == 0 || (type != HCK_BF16 && type != HCK_F16)) return HCK_ERR_UNSUPPORTED;
   if (!pool || pages < 1 || kv_heads < 1 || kv_heads > 65535 || tokens < 0 || tokens > INT32_MAX || group < 1 || seqs < 0 ||
       seqs > 65535 || most < 0 || table_columns < 0 || table_columns >= 1 << 23 || prior_places < 0 ||
-      !((float)scale > 0.f && scale <= 0x1p126) || (int64_t)most * group > INT32_MAX || (int64_t)kv_heads * group > INT32_MAX)
+      !((float)scale > 0.f && scale <= 0x1p126) || (int64_t)most * group > hck::kMostRows || (int64_t)kv_heads * group > INT32_MAX)
     return HCK_ERR_ARG;
   if (!starts && tokens != seqs) return HCK_ERR_ARG;
   if (seqs == 0 || table_columns == 0) return HCK_OK;

@@ -185,7 +185,7 @@ PyObject* weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
   need(most >= 0, "most must not be negative");
   const bool causal = truth(a[11]);
   const double scale = scale_of(a[12], p.dim);
-  need(tokens <= INT32_MAX && heads <= INT32_MAX && most * group <= INT32_MAX, "too many tokens or heads");
+  need(tokens <= INT32_MAX && heads <= INT32_MAX && most * group <= INT32_MAX - 256, "too many tokens or heads");
   Tensor prior;
   if (a[13] != Py_None) {
     prior = tensor(a[13], "prior");
