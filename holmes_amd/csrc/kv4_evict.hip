@@ -421,7 +421,9 @@ int segments(int cols) {
 }  // namespace hck
 
 extern "C" size_t hck_kv4_evict_workspace_bytes(int seqs, int kv_heads, int table_columns) {
-  if (seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 65535 || table_columns < 0 || table_columns >= 1 << 23) return 0;
+  if (seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 65535 || table_columns < 0 || table_columns >= 1 << 23 ||
+      (int64_t)seqs * kv_heads > INT32_MAX)
+    return 0;
   const int segs = hck::segments(table_columns);
   return segs ? (size_t)seqs * kv_heads * hck::Counts::ints(segs) * sizeof(int) : 0;
 }
@@ -435,7 +437,7 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
   if (hck::kv4_bytes(head_dim) == 0) return HCK_ERR_UNSUPPORTED;
   if (!pool || pages < 1 || kv_heads < 1 || kv_heads > 65535 || seqs < 0 || seqs > 65535 || table_columns < 0 ||
       table_columns >= 1 << 23 || weight_places < 0 || keep < 0 || recent < 0 || recent > keep || into_columns < 0 ||
-      into_columns >= 1 << 23)  // (places of a sequence are counted in 30 bits)
+      into_columns >= 1 << 23 || (int64_t)seqs * kv_heads > INT32_MAX)  // (places of a sequence are counted in 30 bits, rows in 31)
     return HCK_ERR_ARG;
   const int need = (int)(((int64_t)keep + hck::kPageTokens - 1) / hck::kPageTokens);
   if (need > into_columns) return HCK_ERR_ARG;

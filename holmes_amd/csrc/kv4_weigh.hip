@@ -406,7 +406,7 @@ int launch(const WeighArgs& W, const WeighWay& way, hipStream_t s) {
 extern "C" size_t hck_kv4_weigh_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int most,
                                                 int table_columns) {
   if (tokens <= 0 || seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 65535 || group < 1 || most < 0 ||
-      table_columns < 1 || table_columns >= 1 << 23 || (int64_t)most * group > hck::kMostRows)
+      table_columns < 1 || table_columns >= 1 << 23 || (int64_t)most * group > hck::kMostRows || (int64_t)seqs * kv_heads > INT32_MAX)
     return 0;
   return hck::WeighWay(seqs, kv_heads, group, (int)std::min<int64_t>(most, tokens), table_columns).bytes(seqs, kv_heads, table_columns);
 }
@@ -419,7 +419,8 @@ extern "C" int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int 
   if (hck::kv4_bytes(head_dim) == 0 || (type != HCK_BF16 && type != HCK_F16)) return HCK_ERR_UNSUPPORTED;
   if (!pool || pages < 1 || kv_heads < 1 || kv_heads > 65535 || tokens < 0 || tokens > INT32_MAX || group < 1 || seqs < 0 ||
       seqs > 65535 || most < 0 || table_columns < 0 || table_columns >= 1 << 23 || prior_places < 0 ||
-      !((float)scale > 0.f && scale <= 0x1p126) || (int64_t)most * group > hck::kMostRows || (int64_t)kv_heads * group > INT32_MAX)
+      !((float)scale > 0.f && scale <= 0x1p126) || (int64_t)most * group > hck::kMostRows || (int64_t)kv_heads * group > INT32_MAX ||
+      (int64_t)seqs * kv_heads > INT32_MAX)
     return HCK_ERR_ARG;
   if (!starts && tokens != seqs) return HCK_ERR_ARG;
   if (seqs == 0 || table_columns == 0) return HCK_OK;

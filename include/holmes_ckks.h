@@ -506,7 +506,7 @@ int hck_prompt_attend(const void* queries, const void* keys, const void* values,
  * of exp(scale q.k_j - lse), for the queries, pages and masks of hck_kv4_attend and the lse that it gave (a row of -inf
  * gives nothing).  weights is dense, [seqs][kv_heads][table_columns * 128]; places behind a sequence's length become 0, and a
  * page outside the pool adds nothing.  prior (NULL with prior_places 0: none) has prior_places places a row, and counts as
- * 0 behind them.  table_columns is below 2^23, seqs below 2^16. */
+ * 0 behind them.  table_columns is below 2^23, seqs below 2^16, and seqs * kv_heads below 2^31. */
 size_t hck_kv4_weigh_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int most, int table_columns);
 int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int head_dim, int type, const void* queries, int64_t tokens,
                   int group, int64_t q_token_stride, int64_t q_head_stride, const int32_t* table, int64_t table_stride,
@@ -520,7 +520,7 @@ int hck_kv4_weigh(const void* pool, int64_t pages, int kv_heads, int head_dim, i
  * where there are fewer), new_weights their weights (0 there), new_lengths [seqs] their number.  A token whose page is
  * outside the pool is not kept; a target page outside it takes nothing.  Target pages must not be pages of the tables, nor
  * twice in `into`: what those hold is undefined.  Places of a target page behind the kept tokens stay as they were.
- * table_columns is below 2^23, seqs below 2^16. */
+ * table_columns is below 2^23, seqs below 2^16, and seqs * kv_heads below 2^31. */
 size_t hck_kv4_evict_workspace_bytes(int seqs, int kv_heads, int table_columns);
 int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_dim, const int32_t* table, int64_t table_stride,
                   int table_columns, const int32_t* lengths, int seqs, const float* weights, int64_t weight_seq_stride,
