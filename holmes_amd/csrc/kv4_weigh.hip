@@ -385,11 +385,11 @@ int launch(const WeighArgs& W, const WeighWay& way, hipStream_t s) {
   const AttendArgs& A = W.a;
   if (!way.many) {
     const int64_t groups = ((int64_t)A.cols * 2 + kWaves * W.units - 1) / (kWaves * W.units) * A.heads;
-    if (groups > INT32_MAX) return HCK_ERR_ARG;
+    if (!fits_grid(groups, 64 * kWaves)) return HCK_ERR_ARG;
     k_weigh_few<T, D><<<dim3((unsigned)groups, A.seqs), 64 * kWaves, 0, s>>>(W);
   } else {
     const int64_t groups = way.blocks * way.split * A.heads;
-    if (groups > INT32_MAX) return HCK_ERR_ARG;
+    if (!fits_grid(groups, 64 * kWaves)) return HCK_ERR_ARG;
     k_weigh_many<T, D><<<dim3((unsigned)groups, A.seqs), 64 * kWaves, 0, s>>>(W);
   }
   HCK_CHECK_LAUNCH();

@@ -517,13 +517,19 @@ int launch(const PromptArgs& A, const WholeWay& way, hipStream_t s) {
   return HCK_OK;
 }
 
+// Whether the products that WholeWay makes stay within 63 bits.  (2^40 rows are 2^47 bytes of outputs and more.)
+bool countable(int64_t tokens, int64_t seqs, int64_t heads, int64_t group) {
+  return seqs * heads <= INT32_MAX && heads * group <= INT32_MAX && tokens * (heads * group) <= 1ll << 40;
+}
+
 }  // namespace
 }  // namespace hck
 
 extern "C" size_t hck_prompt_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim, int most,
                                                     int causal) {
   if (tokens < 1 || tokens > INT32_MAX || seqs < 1 || kv_heads < 1 || group < 1 || most < 1 ||
-      (head_dim != 64 && head_dim != 128) || std::min<int64_t>(most, tokens) * group > INT32_MAX - 256)
+      (head_dim != 64 && head_dim != 128) || std::min<int64_t>(most, tokens) * group > INT32_MAX - 256 ||
+      !hck::countable(tokens, seqs, kv_heads, group))
     return 0;
   return hck::WholeWay(tokens, seqs, kv_heads, group, (int)std::min<int64_t>(most, tokens), causal != 0).bytes(kv_heads, head_dim);
 }
@@ -535,7 +541,8 @@ extern "C" int hck_prompt_attend(const void* queries, const void* keys, const vo
                                  float* low, float* high, void* workspace, size_t workspace_bytes, void* stream) {
   if ((head_dim != 64 && head_dim != 128) || (type != HCK_BF16 && type != HCK_F16)) return HCK_ERR_UNSUPPORTED;
   if (tokens < 0 || tokens > INT32_MAX || kv_heads < 1 || group < 1 || (int64_t)kv_heads * group > INT32_MAX || seqs < 0 ||
-      most < 0 || !((float)scale > 0.f && scale <= 0x1p126) || (low == nullptr) != (high == nullptr))
+      most < 0 || !((float)scale > 0.f && scale <= 0x1p126) || (low == nullptr) != (high == nullptr) ||
+      !hck::countable(tokens, seqs, kv_heads, group))
     return HCK_ERR_ARG;
   if (!starts && seqs != 1) return HCK_ERR_ARG;
   most = (int)std::min<int64_t>(most, tokens);
@@ -554,7 +561,7 @@ extern "C" int hck_prompt_attend(const void* queries, const void* keys, const vo
   A.v_ts = tokens > 1 ? v_token_stride : head_dim, A.v_hs = v_head_stride;
   A.seqs = seqs, A.heads = kv_heads, A.group = group, A.causal = causal != 0, A.most = most;
   const hck::WholeWay way(tokens, seqs, kv_heads, group, most, causal != 0);
-  if (way.items * way.parts * kv_heads > INT32_MAX) return HCK_ERR_ARG;
+  if (!hck::fits_grid(way.items * way.parts * kv_heads, 64 * hck::kPromptWaves)) return HCK_ERR_ARG;
   const size_t need = way.bytes(kv_heads, head_dim);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return HCK_ERR_WORKSPACE;
   A.tiles = way.tiles, A.part = way.part, A.parts = way.parts, A.items = (int)way.items, A.slots = (hck::f32x4*)workspace;

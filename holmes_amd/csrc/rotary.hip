@@ -168,7 +168,7 @@ int launch(RotaryArgs A, int rotated, bool interleaved, hipStream_t s) {
   A.per = (int)std::max<int64_t>(1, std::min({many, (int64_t)kAngles / A.pairs, A.tokens / 1024}));
   if ((int64_t)A.per * heads * A.units >= 1 << 16 && A.per > 1) A.per = 1;
   const int64_t groups = (A.tokens + A.per - 1) / A.per;
-  if (groups > 0x7fffffff) return HCK_ERR_ARG;
+  if (!fits_grid(groups, kThreads)) return HCK_ERR_ARG;
   const dim3 grid((unsigned)groups);
   const bool past = wide && A.tokens * heads * A.dim * (int64_t)sizeof(T) > kL2s;
   if (interleaved) {

@@ -494,7 +494,8 @@ int hck_rotary(const void* positions, int position_bytes, int64_t tokens, const 
  * all bf16 or all fp16, and its queries see its tokens up to their own (with `causal` 0: all of them).  Element strides,
  * multiples of 8, from 16-byte aligned addresses; tokens of keys and values lie head_dim to 2^23 elements apart.  Of each sequence
  * the first `most` queries are taken.  out, lse, low, high and scale are as for hck_kv4_attend; the other queries of a longer
- * sequence, and tokens that no sequence covers, are left unwritten. */
+ * sequence, and tokens that no sequence covers, are left unwritten.  seqs * kv_heads is below 2^31; and these calls, as those of
+ * rotary positions and weights, are refused where they take 2^24 workgroups or more. */
 size_t hck_prompt_attend_workspace_bytes(int64_t tokens, int seqs, int kv_heads, int group, int head_dim, int most, int causal);
 int hck_prompt_attend(const void* queries, const void* keys, const void* values, int type, int64_t tokens, int kv_heads,
                       int group, int head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
