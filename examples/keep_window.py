@@ -38,9 +38,9 @@ def run(tokens: int = 4096, keep: int = 256, recent: int = 64, seed: int = 0) ->
                                   (x @ wk).view(-1, kv_heads, dim))
     values = (x @ wv).view(-1, kv_heads, dim)
 
-    # the prompt, over keys that nothing has rounded: the softmax's intervals, from rows that see a page or more
+    # the prompt, over keys that nothing has rounded: the softmax's intervals, from rows that see a page or more (the last, of less)
     prompt = clear.prompt_attention(queries[:tokens], keys[:tokens], values[:tokens], ranges=True)
-    rows = slice(clear.PAGE_TOKENS - 1, None)
+    rows = slice(min(clear.PAGE_TOKENS, tokens) - 1, None)
     ranges = clear.softmax_ranges(prompt.low[rows], prompt.high[rows], prompt.lse[rows])
 
     # its keys and values in 4-bit pages, and what every cached token was given
@@ -60,7 +60,7 @@ def run(tokens: int = 4096, keep: int = 256, recent: int = 64, seed: int = 0) ->
     weights = pool.weigh(queries[:tokens], table, lengths, cached.lse, starts=starts, most=tokens)
 
     # every key head's heaviest tokens, and the last ones
-    kept = pool.evict(table, lengths, weights, window, keep, recent=recent)
+    kept = pool.evict(table, lengths, weights, window, keep, recent=min(recent, keep))
     held = pool.read(slots(window, 0, min(keep, tokens)), torch.float32)
 
     # the next token over the whole prompt and over what was kept
