@@ -5,7 +5,8 @@
 One attention layer of the decode step's shape (32 query heads over 8 key heads of 128) with random weights runs in the
 clear: queries and keys get their rotary positions, the prompt's attention over the keys as they came gives the softmax's
 shift and intervals, the keys and values go into 4-bit pages, and every key head keeps the tokens to which its queries gave
-most, beside the last ones: two pages, as the encrypted step holds them.  The next token's attention over those is compared
+most, beside the last ones: two pages, as the encrypted step holds them.  Their keys and values as they came, from before the 4
+bits, are the history that ``encrypt_kv_history`` encrypts for it.  The next token's attention over the pages that are kept is compared
 with the one over the whole prompt.  Random weights attend almost evenly, so what is kept here is not much of the whole; a model's
 is.
 """
@@ -63,11 +64,15 @@ def run(tokens: int = 4096, keep: int = 256, recent: int = 64, seed: int = 0) ->
     kept = pool.evict(table, lengths, weights, window, keep, recent=min(recent, keep))
     held = pool.read(slots(window, 0, min(keep, tokens)), torch.float32)
 
+    # the same tokens as they came, as ``encrypt_kv_history`` takes them: [tokens][kv_heads * head_dim], each head's its own
+    at = kept.kept[0, :, :min(keep, tokens)].T.long()[..., None].expand(-1, -1, dim)
+    history = keys[:tokens].gather(0, at).flatten(1), values[:tokens].gather(0, at).flatten(1)
+
     # the next token over the whole prompt and over what was kept
     whole = pool.attend(queries[tokens:], table, lengths)
     part = pool.attend(queries[tokens:], window, kept.lengths)
     after = pool.weigh(queries[tokens:], window, kept.lengths, part.lse, prior=kept.weights)
-    return {"ranges": ranges, "weights": weights, "kept": kept, "held": held, "whole": whole, "part": part, "after": after,
+    return {"ranges": ranges, "weights": weights, "kept": kept, "held": held, "history": history, "whole": whole, "part": part, "after": after,
             "queries": queries, "keys": keys, "values": values, "prompt": prompt, "cached": cached}
 
 

@@ -11,8 +11,8 @@ operators here run that model's attention over real prompts at their full length
 * ``ClearKVPages``: a key/value cache in 4 bits on the GPU, in pages of 128 tokens like the encrypted
   cache's; ``append`` quantises keys and values as they are written, ``read`` gives back what is held,
   ``attend`` is the attention of queries over it, with the same numbers of every row; ``weigh`` sums what attention has
-  given each cached token, and ``evict`` brings a sequence down to its heaviest ones, as the few pages of the encrypted
-  layer's cache want it;
+  given each cached token, and ``evict`` brings a sequence down to its heaviest ones and says which they are, for
+  the few pages of the encrypted layer's cache;
 * ``softmax_ranges``: the encrypted softmax's shift and intervals from those, and ``score_rounding`` what the keys'
   4 bits can have moved them by;
 * ``token_logprobs``: log probabilities of given tokens, entropy and top alternatives of logits.
