@@ -162,11 +162,12 @@ int launch(RotaryArgs A, int rotated, bool interleaved, hipStream_t s) {
   A.units = A.turned + (A.dim - rotated) / v;
   const int heads = A.heads[0] + A.heads[1];
   A.by_units = inverse_of(A.units), A.by_heads = inverse_of(heads);
-  // tokens of a workgroup: up to 600 units (32768 tokens of 320 units: one 113 us, two 120, four 126; 6001 of 144: two 8.8, four
-  // 8.0, five 8.1), what the angles have room for, and no more than leave 1024 workgroups
-  const int64_t many = 600 / ((int64_t)heads * A.units);
+  // Tokens of a workgroup: about 8 KB of values, what the angles have room for, and no more than leave 1024 workgroups.  (Tokens of
+  // 128 bytes to 40 KB, 2500 to 32768 of them, both kinds of pairs, all of a head and half, any alignment, 1 to 32 tokens
+  // a workgroup: this is off the best by 2 % on average and 13 at the most; by 16 KB 3 and 14, by 6 KB 3 and 19.  32768
+  // tokens of 1280 bytes: one 27.4 us, two 22.1, six 17.4, twelve 17.9; of 10 KB: one 106, two 114.)
+  const int64_t size = (int64_t)heads * A.dim * sizeof(T), many = ((8 << 10) + size / 2) / size;
   A.per = (int)std::max<int64_t>(1, std::min({many, (int64_t)kAngles / A.pairs, A.tokens / 1024}));
-  if ((int64_t)A.per * heads * A.units >= 1 << 16 && A.per > 1) A.per = 1;
   const int64_t groups = (A.tokens + A.per - 1) / A.per;
   if (!fits_grid(groups, kThreads)) return HCK_ERR_ARG;
   const dim3 grid((unsigned)groups);
