@@ -25,7 +25,7 @@ struct EvictArgs {
   int *kept, *new_lengths;
   float* new_weights;
   int64_t pages, table_stride, into_stride, w_seq, w_head;
-  int cols, heads, seqs, width, into_cols, keep, recent;
+  int cols, heads, seqs, width, keep, recent;
   int *counts, segs;  // of long rows: Counts of each row, and its segments
 };
 
@@ -450,7 +450,7 @@ extern "C" int hck_kv4_evict(void* pool, int64_t pages, int kv_heads, int head_d
   A.kept = kept, A.new_lengths = new_lengths, A.new_weights = new_weights;
   A.pages = pages, A.table_stride = table_stride, A.into_stride = into_stride, A.w_seq = weight_seq_stride,
   A.w_head = weight_head_stride, A.cols = table_columns, A.heads = kv_heads, A.seqs = seqs, A.width = weight_places,
-  A.into_cols = into_columns, A.keep = keep, A.recent = recent;
+  A.keep = keep, A.recent = recent;
   A.segs = hck::segments(table_columns), A.counts = (int*)workspace;
   const size_t bytes = hck_kv4_evict_workspace_bytes(seqs, kv_heads, table_columns);
   if (bytes && (!workspace || workspace_bytes < bytes)) return HCK_ERR_WORKSPACE;
