@@ -218,7 +218,10 @@ class ClearKVPages:
         those of the largest ``weights`` [sequences][kv_heads][places] (float32; 0 behind the last place, NaN above
         all, the earlier one where they tie).  They are copied, in their order, to the pages ``into`` (int32
         [sequences][at least keep / 128]), of which each head then holds tokens of its own choice; the pages of ``table`` stay as they are.
-        A sequence of fewer tokens keeps all.  A token whose page is outside the pool is not kept, and a page of ``into``
+        A sequence of fewer tokens keeps all.  How a call is run goes by the table's columns, not by the lengths, which are on the
+        device: a view without spare columns (``table[:, :columns]``) saves work, and beyond 128 columns a workspace of 24.6 KB for
+        every 64 of them, sequence and head (32 sequences of 384 tokens to 256, 8 heads: 10 us through 3 columns, 14 through 128, 39 and 19 MB
+        through 129, 211 and 101 MB through 1024).  A token whose page is outside the pool is not kept, and a page of ``into``
         outside it takes nothing.  The pages of ``into`` must be none of the tables' and differ (else what they hold is undefined);
         places in them behind the kept tokens stay as they were."""
 
@@ -286,7 +289,9 @@ class RotaryPositions:
     """Rotary positions: of the first ``rotated`` dims of a head (default: all), pairs (i, i + rotated / 2), or, with
     ``interleaved``, (2 i, 2 i + 1), are turned by position * base^(-2 i / rotated) radians; the dims behind stay.  The
     default is what ``DecodeSpec`` and ``PrefillSpec`` take (pairs of halves, rope_theta 500000).  ``scaling``: for long
-    contexts.  The angle of any position below 2^31 is exact to 2^-34 turns."""
+    contexts.  Frequencies are held as float64 (``frequencies``) and turned into whole units of 2^-64 turns a token, which
+    adds 2^-34 turns to an angle at position 2^31; the float64's own rounding is up to 2^-25 turns there.  Sine, cosine and
+    products are of 32 bits."""
 
     def __init__(self, head_dim: int = 128, *, base: float = 500000.0, rotated: int | None = None,
                  interleaved: bool = False, scaling: RotaryScaling | None = None, device="cuda"):
@@ -329,7 +334,8 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     Sequence b is the tokens ``starts[b] .. starts[b + 1]`` (int32 [sequences + 1], not decreasing; without ``starts`` there
     is one of all tokens), and query i of it sees its tokens up to i, or, with ``causal`` off, all.  ``most`` bounds the queries
     of one sequence (default: all) and only saves work; a longer one has the rest left unwritten, as has any row that no sequence
-    covers.  ``scale`` and ``ranges`` as for ``ClearKVPages.attend``: the ranges here are those of keys that nothing has
+    covers.  Scores, statistics and sums are of 32 bits; a probability goes into its product with the values in their 16 bits (in two
+    parts where a row sees few tokens), which adds less to an output's error than its own rounding.  ``scale`` and ``ranges`` as for ``ClearKVPages.attend``: the ranges here are those of keys that nothing has
     rounded, so ``softmax_ranges`` needs no ``rounding`` for them."""
 
     got = _window().prompt(queries, keys, values, starts, most, causal, scale, ranges)

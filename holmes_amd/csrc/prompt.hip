@@ -13,14 +13,16 @@
 // four tokens by 16 dims at a time through the transposing LDS read, at piece ^ 4 (token % 4).  What lies behind a
 // sequence's end is out of the loads' bounds and becomes zeros.
 //
-// Probabilities are rounded to the values' type for the second product: half a step each, so that an output's error is that of a
-// sum of rounded terms, of the size of its own rounding where there are many.  Rows of few tokens, where it would be half as
+// Probabilities are rounded to the values' type for the second product, for every caller: one part of 16 bits, which halves that
+// product's matrix instructions against two.  Half a step each, so that an output's error is that of a
+// sum of rounded terms, of the size of its own rounding where there are many (against 64 bits, relative to the outputs: 8192 tokens in
+// bf16 1.70e-3, where probabilities of 32 bits leave 1.66e-3).  Rows of few tokens, where it would be half as
 // much again, see them in units that others of their tile see in part: there the rounding's rest goes in as well, by a second
 // product.  l, and with it lse, is the sum of the unrounded ones.
 //
 // What bounds it: per 64 tokens and 32 rows 32 matrix instructions (1024 of the SIMD's cycles at D = 128) and some 150 vector ones, 32 of
 // them exponentials (730), of two waves that share a SIMD.  8192 tokens, 32 query heads over 8 key heads of 128, bf16: 555 GFLOP in
-// 541 to 567 us on different cards, 0.98 to 1.03 PFLOP/s at the 1.95 GHz that the clock falls to; a bf16 8192^3 product runs at 1.23.  References of the
+// 524 to 571 us on different cards, 0.97 to 1.06 PFLOP/s at the 1.95 GHz that the clock falls to; a bf16 8192^3 product runs at 1.23.  References of the
 // exponentials are multiples of 8 in units of log 2, so that going over to another is an exact power of two and seldom done.
 #include "prompt_way.hpp"
 

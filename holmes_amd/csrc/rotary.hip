@@ -5,9 +5,10 @@
 // The pairs are (i, i + rotated / 2), or, interleaved, (2 i, 2 i + 1); dims behind `rotated` are copied.
 //
 // A frequency is held as turns per token in units of 2^-64, so position * frequency modulo 2^64 is the angle's part of a
-// turn with nothing lost but the frequency's own rounding (position * 2^-65 turns): no reduction of a large angle, and no
-// cosine of one.  What is left, within an eighth of a turn of a multiple of a quarter, goes through double into float, and
-// sine and cosine are their Taylor polynomials there (terms up to x^9 and x^10: off by less than 2^-26).
+// turn with nothing lost but the frequency's rounding to whole units (position * 2^-65 turns): no reduction of a large angle,
+// and no cosine of one.  What is left, within an eighth of a turn of a multiple of a quarter, goes through double into float, and
+// sine and cosine are their Taylor polynomials there (terms up to x^9 and x^10: off by less than 2^-26), in 32 bits, as are their
+// products with the amount: half a step of float each, which only fp32 outputs can show.
 //
 // Bound by the bytes.  A workgroup takes all heads of a few tokens, so that each angle is made once, into LDS, for queries
 // and keys together.  32768 tokens, 32 query heads and 8 key heads of 128 in bf16, 671 MB: 108 us, 6.2 TB/s (a large copy
