@@ -335,8 +335,9 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     is one of all tokens), and query i of it sees its tokens up to i, or, with ``causal`` off, all.  ``most`` bounds the queries
     of one sequence (default: all) and only saves work; a longer one has the rest left unwritten, as has any row that no sequence
     covers.  Scores, statistics and sums are of 32 bits; a probability goes into its product with the values in their 16 bits (in two
-    parts where a row sees few tokens), which adds less to an output's error than its own rounding.  ``scale`` and ``ranges`` as for ``ClearKVPages.attend``: the ranges here are those of keys that nothing has
-    rounded, so ``softmax_ranges`` needs no ``rounding`` for them."""
+    parts where a row sees few tokens), which can add as much to an output's error as its own rounding does; in fp16 those below 2^-32 of
+    the row's largest may count as 0.  An infinite value makes its dim infinite or NaN in all rows that see it.  ``scale`` and ``ranges`` as
+    for ``ClearKVPages.attend``: the ranges here are those of keys that nothing has rounded, so ``softmax_ranges`` needs no ``rounding`` for them."""
 
     got = _window().prompt(queries, keys, values, starts, most, causal, scale, ranges)
     if type(got) is int:

@@ -194,7 +194,8 @@ __device__ __forceinline__ void write_row(const PromptArgs& A, int64_t at, int h
   if constexpr (RANGE) A.low[at] = l != l ? l : low * kLn2, A.high[at] = l != l ? l : m * kLn2;
 }
 
-// Exponentials are taken times 2^lift.  fp16: the largest up to 2^15, so that those down to 2^-29 of it keep all bits.  bf16:
+// Exponentials are taken times 2^lift.  fp16: the largest is between 2^7 and 2^15, so that those down to 2^-21 of it at the least, and
+// 2^-29 at the most, keep all bits, and those below 2^-32 may become 0.  bf16:
 // such that their sum over n tokens is at most 1, and no sum of values overflows (by eights: references, which are multiples of
 // 8, stay exact to 2^27).
 template <typename T>
