@@ -213,8 +213,6 @@ inline bool batches_overlap(const uint64_t* p, int64_t p_stride, int64_t p_len, 
   const uint64_t* q_end = q + (int64_t)(n - 1) * q_stride + q_len;
   return p < q_end && q < p_end;
 }
-// Whether so many workgroups can be launched along x: their threads are counted in 32 bits.
-inline bool fits_grid(int64_t groups, int threads) { return groups <= 0xffffffffll / threads; }
 }  // namespace hck
 
 #define HCK_CHECK_LAUNCH()                         \

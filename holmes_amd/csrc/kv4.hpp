@@ -49,6 +49,9 @@ struct Kv4 {
 
 constexpr int64_t kL2s = 32 << 20;  // bytes of the XCDs' L2 caches together
 
+// Whether so many workgroups can be launched along x: their threads are counted in 32 bits.
+inline bool fits_grid(int64_t groups, int threads) { return groups <= 0xffffffffll / threads; }
+
 // Bytes of one head's part of a page (host side; 0: no such head dimension).
 inline int kv4_bytes(int head_dim) {
   return head_dim == 128 ? Kv4<128>::kBytes : head_dim == 64 ? Kv4<64>::kBytes : 0;
