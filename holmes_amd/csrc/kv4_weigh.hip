@@ -21,7 +21,7 @@ struct WeighArgs {
 
 // A row's share of the exponents: what comes off, in units of log 2, and a factor, near 1 for scores of ordinary size, for what
 // rounding took from that and from scale log2 e (counted where the score is the row's lse, near which weights are large).  Its
-// exponent is within 38 up to |lse| = 2^28, and kept within 64 beyond, where half a step of lse itself is e^16 or more: so
+// exponent is within 45 up to |lse| = 2^28, and kept within 64 beyond, where half a step of lse itself is e^16 or more: so
 // that no row's share is negative, or 0 times an infinity.
 struct RowTerm {
   float off, factor;

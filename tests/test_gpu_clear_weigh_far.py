@@ -1,8 +1,8 @@
 """Weights of rows whose scores are far from 0 (ClearKVPages.weigh), against float64 and the lse that is given.
 
 Scores here are exact in 32 bits, and what is left is the kernel's arithmetic.  At |lse| = 2^27 what rounding took from lse log2 e
-is below 8 + 2.6 and from scale log2 e below 7 units of log 2, each known to 2^-23 of itself and rounded twice by 2^-24 of
-their sum: 2^-18.5, times log 2 a relative 2^-19 of the weight, and two exponentials and their product 2^-22.  The exponent's
+is below 8 + 2.6 and from scale log2 e below 12 units of log 2, the last known to 2^-23 of itself and their sums rounded by 2^-24: 2^-18.1,
+times log 2 a relative 2^-18.6 of the weight, and two exponentials and their product 2^-22.  The exponent's
 difference rounds by 2^-24 of itself, and scale's part is counted where the score is lse: taken together as 2^-18 + 2^-21 |s - lse|."""
 
 import math
